@@ -586,6 +586,103 @@ int plx_swifttd_apply(plx_ctx* ctx, uint64_t n_features, float* const* fields,
                       uint32_t n_active, plx_td_globals* globals, void* scratch,
                       uint64_t scratch_bytes);
 
+/* ---- the read-out: rows of unit activations ------------------------------ */
+
+/* Operators over `rows` rows (samples, or steps of a stream) of n units each,
+ * the many-row, many-output counterparts of the per-unit steps above and of
+ * the losses of traits.hpp:185-240. A row's values are contiguous; row r
+ * starts at element r * ld (the stride of a single row is not used). Values
+ * are of one of three types, everything between load and store is in 32
+ * bits. rows < 2^31, n < 2^31; rows = 0 does nothing. An output array may be
+ * the input array of the same shape with the same row stride; no other
+ * overlap is allowed. Rows of which the start is 16-byte aligned are the
+ * fastest. The calls enqueue kernels and nothing else: they can be captured,
+ * and calls on several streams can run at once where their arrays (and
+ * scratch) are their own. */
+#define PLX_F32 0
+#define PLX_BF16 1
+#define PLX_F16 2
+
+/* Layer norm: y = (x - mean) * rstd * weight + bias, with the row's mean,
+ * rstd = 1 / sqrt(variance + eps). weight and bias are [n] of type
+ * param_dtype (PLX_F32 or dtype), or NULL for 1 and 0; mean and rstd [rows]
+ * are written where not NULL (the backward call reads them). */
+int plx_layer_norm(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* x,
+                   int64_t ldx, int param_dtype, const void* weight, const void* bias, float eps,
+                   void* y, int64_t ldy, float* mean, float* rstd);
+
+/* Scratch of plx_layer_norm_backward when it writes dweight or dbias. */
+size_t plx_layer_norm_scratch_bytes(uint64_t rows, uint32_t n);
+
+/* Gradients of layer norm: dx [rows, n] and, of type param_dtype, dweight and
+ * dbias [n], each written where not NULL (dweight and dbias are the sums over
+ * all rows, added in an order that rows, n and the types alone set: the same
+ * bits on every call; zero for rows = 0). scratch is 16-byte aligned and may
+ * hold anything; calls that run at once need scratch of their own. */
+int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* dy,
+                            int64_t lddy, const void* x, int64_t ldx, const float* mean,
+                            const float* rstd, int param_dtype, const void* weight, void* dx,
+                            int64_t lddx, void* dweight, void* dbias, void* scratch,
+                            size_t scratch_bytes);
+
+/* Most alternatives a call of plx_log_probs can return. */
+#define PLX_TOP_MAX 64
+
+/* What the softmax of scale * logits answers in each row (scale > 0, the
+ * inverse temperature; cf. SoftmaxCrossEntropyLoss, traits.hpp:222-240, whose
+ * loss against a single target is -logp):
+ *   lse      [rows]  log of the sum of exp(scale * x)
+ *   logp     [rows]  log probability of target[row]; 0 for target -1 (none).
+ *                    target and logp are both given or both NULL. A target
+ *                    outside [-1, n) counts as none and makes plx_ctx_sync
+ *                    report PLX_ERR_ARG
+ *   entropy  [rows]  or NULL
+ *   top_ids, top_logp [rows, top]: the `top` outputs with the largest logits
+ *                    and their log probabilities, largest first, the lower
+ *                    index first among equals; top <= min(n, PLX_TOP_MAX)
+ * Logits of -inf are masked: probability 0. In a row that is masked whole
+ * lse, logp and top_logp are -inf, entropy is 0 and top_ids the lowest
+ * indexes. A NaN or +inf makes the row's lse, entropy and log probabilities
+ * NaN (NaN ranks above every value in top_ids). */
+int plx_log_probs(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* logits,
+                  int64_t ld, const int32_t* target, float scale, uint32_t top, float* logp,
+                  float* lse, float* entropy, int32_t* top_ids, float* top_logp);
+
+/* Gradient of sum over rows of grad_logp * logp + grad_entropy * entropy with
+ * respect to the logits. lse and entropy are those of plx_log_probs with the
+ * same arguments; grad_logp (needs target) or grad_entropy (needs entropy)
+ * may be NULL, not both. A row without a target (or with one outside [0, n))
+ * has no gradient from grad_logp. */
+int plx_log_probs_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype,
+                           const void* logits, int64_t ld, const int32_t* target, float scale,
+                           const float* lse, const float* entropy, const float* grad_logp,
+                           const float* grad_entropy, void* dlogits, int64_t ldd);
+
+/* Most teacher entries a row of plx_distill can have. */
+#define PLX_DISTILL_MAX_K 64
+/* What teacher_values hold: the teacher's logits of the listed outputs
+ * (q = softmax(values / temperature) over the row's list), or their log
+ * probabilities at the temperature of the call (q = exp(values): the listed
+ * outputs keep the mass the teacher gave them, the rest is left out). */
+#define PLX_TEACHER_LOGITS 0
+#define PLX_TEACHER_LOG_PROBS 1
+
+/* Distillation from a teacher's top outputs, loss and gradient in one call.
+ * With p = softmax(logits / temperature) over all n outputs and the teacher's
+ * entries (teacher_ids[row, j], q_j), j < k <= PLX_DISTILL_MAX_K:
+ *   loss[row] = row_weight[row] * temperature^2 * sum_j q_j (log q_j - log p_j)
+ *   dlogits   = gradient of the sum of loss over the rows, written unless NULL
+ * row_weight [rows] may be NULL (1). An id of -1 is an empty entry; the same
+ * id twice is two entries, both of which count; an id outside [-1, n) counts
+ * as empty and makes plx_ctx_sync report PLX_ERR_ARG. Where row_weight is 0,
+ * or no entry has q > 0, loss and gradient are 0 whatever the logits hold.
+ * Masked logits (-inf) have p = 0: an entry with q > 0 there makes the loss
+ * +inf and its gradient -row_weight * temperature * q. */
+int plx_distill(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* logits,
+                int64_t ld, uint32_t k, const int32_t* teacher_ids, const float* teacher_values,
+                int teacher_kind, float temperature, const float* row_weight, float* loss,
+                void* dlogits, int64_t ldd);
+
 #ifdef __cplusplus
 }
 #endif

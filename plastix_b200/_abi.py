@@ -6,7 +6,7 @@ fails with an ImportError-style exception when the shared library is missing.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_float, c_int, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libplastix_b200.so")
@@ -73,6 +73,14 @@ KEEP_ABS_GE = 2
 FIELD_INC_SAT_U8 = 1
 COUNT_UNKNOWN = 0xFFFFFFFF
 MAX_FIELDS = 16
+
+F32 = 0
+BF16 = 1
+F16 = 2
+TOP_MAX = 64
+DISTILL_MAX_K = 64
+TEACHER_LOGITS = 0
+TEACHER_LOG_PROBS = 1
 
 # name -> (restype, argtypes)
 _SIGNATURES = {
@@ -169,6 +177,23 @@ _SIGNATURES = {
                                                  c_void_p, c_uint32, c_void_p, c_void_p,
                                                  c_float, c_float, c_void_p, c_void_p,
                                                  c_uint32, c_uint32, c_uint32]),
+    "plx_layer_norm": (c_int, [c_void_p, c_uint64, c_uint32, c_int, c_void_p, c_int64, c_int,
+                               c_void_p, c_void_p, c_float, c_void_p, c_int64, c_void_p,
+                               c_void_p]),
+    "plx_layer_norm_scratch_bytes": (ctypes.c_size_t, [c_uint64, c_uint32]),
+    "plx_layer_norm_backward": (c_int, [c_void_p, c_uint64, c_uint32, c_int, c_void_p, c_int64,
+                                        c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p,
+                                        c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                        ctypes.c_size_t]),
+    "plx_log_probs": (c_int, [c_void_p, c_uint64, c_uint32, c_int, c_void_p, c_int64, c_void_p,
+                              c_float, c_uint32, c_void_p, c_void_p, c_void_p, c_void_p,
+                              c_void_p]),
+    "plx_log_probs_backward": (c_int, [c_void_p, c_uint64, c_uint32, c_int, c_void_p, c_int64,
+                                       c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_int64]),
+    "plx_distill": (c_int, [c_void_p, c_uint64, c_uint32, c_int, c_void_p, c_int64, c_uint32,
+                            c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p, c_void_p,
+                            c_int64]),
 }
 
 _lib = None

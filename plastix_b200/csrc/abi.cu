@@ -119,6 +119,9 @@ extern "C" int plx_ctx_sync(plx_ctx* ctx) {
                                     "the activation array");
     if (st == kStatusBadPlan)
       return set_error(PLX_ERR_ARG, "a sweep was given an invalid plan");
+    if (st == kStatusBadOutput)
+      return set_error(PLX_ERR_ARG, "a target or teacher entry named an output "
+                                    "outside its row");
     return set_error(PLX_ERR_ARG, "device status %d", st);
   }
   return PLX_OK;

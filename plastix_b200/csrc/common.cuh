@@ -44,6 +44,7 @@ enum DeviceStatus : int32_t {
   kStatusTimeout = 1,   // a bounded wait expired
   kStatusBadIndex = 2,  // a connection named a unit outside the given array
   kStatusBadPlan = 3,   // a sweep was given an invalid plan
+  kStatusBadOutput = 4,  // a target or teacher entry named an output outside its row
 };
 
 // ---------------------------------------------------------------------------

@@ -1,0 +1,110 @@
+// Shared pieces of the row operators (norm.cu, readout.cu): element types,
+// 16-byte row access and block-wide reductions in a fixed order.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace plx {
+
+inline bool valid_dtype(int dtype) {
+  return dtype == PLX_F32 || dtype == PLX_BF16 || dtype == PLX_F16;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// Runs f with a value of the C++ type that `dtype` names.
+template <typename F>
+int with_dtype(int dtype, F f) {
+  if (dtype == PLX_F32) return f(float{});
+  if (dtype == PLX_BF16) return f(__nv_bfloat16{});
+  return f(__half{});
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+// NaN wins, as in the arithmetic that follows it.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+
+// Block-wide sum / maximum, the same value in every thread, added in a fixed
+// order. `red` holds one float per warp; the barrier at the head lets it be
+// used again at once.
+template <int WARPS>
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = warp_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = red[0];
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) s = __fadd_rn(s, red[w]);
+  return s;
+}
+template <int WARPS>
+__device__ __forceinline__ float block_max(float v, float* red) {
+  v = warp_max(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = red[0];
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) s = max_nan(s, red[w]);
+  return s;
+}
+
+// 2^x by the special-function unit (relative error about 2^-22; 0 for
+// arguments below -126).
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+}  // namespace plx
+
+// Makes a context's device current for one call and puts the caller's back.
+struct DeviceGuard {
+  int before = -1;
+  cudaError_t err;
+  explicit DeviceGuard(int device) {
+    err = cudaGetDevice(&before);
+    if (err == cudaSuccess && before != device)
+      err = cudaSetDevice(device);
+    else
+      before = -1;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
