@@ -303,6 +303,20 @@ def test_log_probs_of_masked_and_non_finite_rows(ctx, n):
     assert abs(float(r.logp[5]) + np.log(n)) <= U * (depth(n) + 8 * np.log(n))
 
 
+def test_entropy_of_rows_as_wide_as_the_type(ctx):
+    # the running maximum moves from the type's lowest value upwards, masked values in between
+    low, inf = torch.finfo(torch.float32).min, float("inf")
+    x = torch.full((3, 50000), low, device="cuda")
+    x[0, ::3] = -inf
+    x[0, 40000] = 5.0
+    x[1, :25000] = -inf
+    x[2, 100:] = 1.0
+    r = readout.log_probs(ctx, x, top=1, entropy=True)
+    ctx.sync()
+    for row, ways in ((0, 1), (1, 25000), (2, 49900)):
+        assert abs(float(r.entropy[row]) - np.log(ways)) <= U * (depth(50000) + 8 * np.log(50000))
+
+
 def test_a_target_outside_its_row_is_reported(ctx):
     x = torch.randn(3, 50, device="cuda")
     for bad in (50, -2, 2 ** 31 - 1):
@@ -414,6 +428,15 @@ def test_distill_edge_rows(ctx):
     with pytest.raises(_abi.PlxError, match="outside its row"):
         ctx.sync()
     ctx.sync()
+
+
+@pytest.mark.parametrize("kind", ["logits", "log_probs"])
+def test_distill_where_the_teacher_masks_all_it_lists(ctx, kind):
+    x = torch.randn(2, 90, device="cuda")
+    ids = torch.tensor([[4, 5], [4, -1]], dtype=torch.int32, device="cuda")
+    loss, dx = readout.distill(ctx, x, ids, torch.full((2, 2), -float("inf"), device="cuda"), kind=kind)
+    ctx.sync()
+    assert not loss.any() and not dx.any()
 
 
 def test_distill_gradient_against_differences_of_the_loss(ctx):
