@@ -4,124 +4,178 @@
 //   dx_i = w tau (Q p_i - sum_{j: id_j = i} q_j)
 //
 // Bound by memory: logits read once, gradient written once. The gradient needs
-// the row's sum first, so the row is gone over twice: once for maximum and sum
-// (logits.cuh), once, out of L2, for the gradient. The few outputs the teacher
-// lists are put right after that.
+// the row's sum first, so the row is gone over twice: for maximum and sum
+// (logits.cuh) and for the gradient. In between it stays in shared memory, up
+// to kKeepBytes a block, a long row spread over the blocks of a cluster; what
+// does not fit is read again out of L2. The first warp takes care of the
+// teacher's entries; the outputs they name are put right at the end.
 #include "logits.cuh"
 
 namespace plx {
 namespace {
 
+// Of a row in a block's shared memory: three blocks an SM fit, so that one's
+// loads run beside another's stores.
+constexpr uint32_t kKeepBytes = 72 * 1024;
+
+// THREADS threads go over the row; one more warp takes care of the teacher.
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS)
-k_distill(uint32_t n, const T* x, int64_t ld, uint32_t k, const int32_t* __restrict__ ids,
-          const float* __restrict__ values, int kind, float tau, float inv_tau,
-          const float* __restrict__ weight, float* __restrict__ loss, T* dx, int64_t ldd,
-          int32_t* __restrict__ status) {
-  constexpr int WARPS = THREADS / 32, V = Piece<T>::V;
-  static_assert(THREADS >= PLX_DISTILL_MAX_K, "one thread an entry");
-  __shared__ float red[WARPS];
+__global__ void __launch_bounds__(THREADS + 32, 1536 / (THREADS < 256 ? THREADS + 32 : THREADS))
+k_distill(uint32_t n, uint32_t each, const T* x, int64_t ld, uint32_t k,
+          const int32_t* __restrict__ ids, const float* __restrict__ values, int kind, float tau,
+          float inv_tau, const float* __restrict__ weight, float* __restrict__ loss, T* dx,
+          int64_t ldd, uint32_t keep_pieces, int32_t* __restrict__ status) {
+  constexpr int WARPS = THREADS / 32, V = Piece<T>::V, E = PLX_DISTILL_MAX_K / 32;
+  extern __shared__ uint4 keep[];
+  __shared__ Sums all[WARPS], mine;
   __shared__ int32_t sid[PLX_DISTILL_MAX_K];
-  __shared__ float sq[PLX_DISTILL_MAX_K];
-  __shared__ Sums mine;
+  __shared__ float sq[PLX_DISTILL_MAX_K], qsum_of;
   cg::cluster_group cl = cg::this_cluster();
   const uint32_t parts = cl.num_blocks(), part = cl.block_rank();
-  const int64_t r = blockIdx.x / parts;
+  const int64_t r = cluster_row();
   const T* xr = x + r * ld;
-  const Share<T> share(xr, n, part, parts);
+  const Share<T> share(xr, n, part, each);
   T* out = dx ? dx + r * ldd + share.start : nullptr;
-  const bool whole = (reinterpret_cast<uintptr_t>(out + share.head) & 15u) == 0;
-  auto store = [&](uint32_t i, const uint4& o) {
-    const uint32_t first = share.piece_at(i);
-    if (whole) {
-      *reinterpret_cast<uint4*>(out + first) = o;
-    } else {
-      const T* e = reinterpret_cast<const T*>(&o);
-#pragma unroll
-      for (int j = 0; j < V; ++j) out[first + j] = e[j];
-    }
-  };
-
-  // The teacher's row: one thread an entry.
-  const uint32_t j = threadIdx.x;
-  int32_t id = j < k ? ids[r * k + j] : -1;
-  if (id < -1 || id >= (int64_t)n) {
-    record_status(status, kStatusBadOutput);
-    id = -1;
-  }
-  float lq = id < 0 ? -INFINITY : values[r * k + j];
-  const float x_at = id < 0 ? 0.0f : to_f32(xr[id]);  // before any gradient takes its place
-  if (kind == PLX_TEACHER_LOGITS) {
-    const float most = block_max<WARPS>(lq, red);
-    if (most != -INFINITY) lq = (lq - most) * inv_tau;
-    const float sum = block_sum<WARPS>(expf(lq), red);
-    if (most != -INFINITY) lq -= logf(sum);
-  }
-  const float q = id < 0 || lq == -INFINITY ? 0.0f : expf(lq);
-  if (j < k) {
-    sid[j] = id;
-    sq[j] = q;
-  }
-  const float qsum = block_sum<WARPS>(q, red);
-  const float w = weight ? weight[r] : 1.0f;
-  if (w == 0.0f || qsum == 0.0f) {  // the row does not count, whatever it holds
+  const bool teacher = threadIdx.x >= THREADS;
+  const uint32_t lane = threadIdx.x & 31;
+  auto clear = [&] {  // the row does not count, whatever it holds
     if (part == 0 && threadIdx.x == 0) loss[r] = 0.0f;
-    if (out) {
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      if (threadIdx.x < share.head) out[threadIdx.x] = from_f32<T>(0.0f);
-      for (uint32_t i = threadIdx.x; i < share.pieces; i += THREADS) store(i, zero);
-      if (threadIdx.x < share.tail) out[share.tail_at() + threadIdx.x] = from_f32<T>(0.0f);
-    }
-    return;  // every block of the row's cluster does
+    if (!out || teacher) return;
+    if (threadIdx.x < share.head) out[threadIdx.x] = from_f32<T>(0.0f);
+    share.with_whole(out, [&](auto whole) {
+      for (uint32_t i = threadIdx.x; i < share.pieces; i += THREADS)
+        share.template put_piece<decltype(whole)::value>(out, i, make_uint4(0, 0, 0, 0));
+    });
+    if (threadIdx.x < share.tail) out[share.tail_at() + threadIdx.x] = from_f32<T>(0.0f);
+  };
+  const float w = weight ? weight[r] : 1.0f;
+  if (w == 0.0f) {  // so says every block of the row's cluster
+    clear();
+    return;
   }
 
   const float c = inv_tau * kLog2e;
-  uint32_t pos;
-  Sums v = join_block<false, WARPS>(scan_share<T, false, false, THREADS>(share, c, pos), c, red);
+  const uint32_t kept = out ? min(share.pieces, keep_pieces) : 0;
+  Sums v{-INFINITY, 0.0f, 0.0f};
+  // The teacher's row, E entries a lane: of an output named twice the first
+  // entry has the sum, `all_q`, and is the one that writes.
+  int32_t id[E];
+  float lq[E], q[E], all_q[E], x_at[E], qsum = 0.0f;
+  if (!teacher) {
+    v = scan_share<T, false, false, true, THREADS>(share, c, nullptr, keep, kept);
+  } else {
+    float most = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint32_t j = lane + 32 * e;
+      id[e] = j < k ? ids[r * k + j] : -1;
+      lq[e] = j < k ? values[r * k + j] : -INFINITY;
+      if (id[e] < -1 || id[e] >= (int64_t)n) {
+        record_status(status, kStatusBadOutput);
+        id[e] = -1;
+      }
+      if (id[e] < 0) lq[e] = -INFINITY;
+      x_at[e] = id[e] < 0 ? 0.0f : to_f32(xr[id[e]]);  // before a gradient takes its place
+      most = max_nan(most, lq[e]);
+    }
+    if (kind == PLX_TEACHER_LOGITS) {
+      most = warp_max(most);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (most != -INFINITY) lq[e] = (lq[e] - most) * inv_tau;
+        sum += expf(lq[e]);
+      }
+      sum = warp_sum(sum);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (kind == PLX_TEACHER_LOGITS && most != -INFINITY) lq[e] -= logf(sum);
+      q[e] = lq[e] == -INFINITY ? 0.0f : expf(lq[e]);
+      qsum += q[e];
+      sid[lane + 32 * e] = id[e];
+      sq[lane + 32 * e] = q[e];
+    }
+    qsum = warp_sum(qsum);
+    if (lane == 0) qsum_of = qsum;
+    __syncwarp();
+    if (out) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        all_q[e] = 0.0f;
+        bool first = true;
+        for (uint32_t j = 0; j < k; ++j)
+          if (sid[j] == id[e]) {
+            all_q[e] += sq[j];
+            first = first && j >= lane + 32 * e;
+          }
+        if (!first || (uint32_t)id[e] - share.start >= share.count) id[e] = -1;  // not written here
+      }
+    }
+  }
+  v = join_block<false, WARPS>(v, c, all);
   if (parts > 1) {
-    v = join_cluster<false>(cl, &mine, v, c);
+    if (threadIdx.x == 0) mine = v;
+    cl.sync();
+    v = join_parts<false>(cl, &mine, c);
     cl.barrier_arrive();  // done with the others' memory; waited for before leaving
   }
-  const bool none = v.m == -INFINITY;  // the student masks every output
-  const float ls = logf(v.s);
-  const float logp = none ? -INFINITY : (x_at - v.m) * inv_tau - ls;
-  if (part == 0) {
-    const float term = block_sum<WARPS>(q != 0.0f ? q * (lq - logp) : 0.0f, red);
-    if (threadIdx.x == 0) loss[r] = w * tau * tau * term;
+  qsum = qsum_of;
+  if (qsum == 0.0f) {
+    clear();
+    if (parts > 1) cl.barrier_wait();
+    return;
   }
-  if (out) {
-    const float a = w * tau, f = none ? 0.0f : a * qsum / v.s;
+  const bool none = v.m == -INFINITY;  // the student masks every output
+  const float a = w * tau, f = none ? 0.0f : a * qsum / v.s;
+  float fixed[E];  // the gradients at the teacher's outputs
+  if (teacher) {
+    const float ls = logf(v.s);
+    float term = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float logp = none ? -INFINITY : (x_at[e] - v.m) * inv_tau - ls;
+      if (q[e] != 0.0f) term += q[e] * (lq[e] - logp);
+      fixed[e] = a * (qsum * expf(logp) - all_q[e]);
+    }
+    term = warp_sum(term);
+    if (part == 0 && lane == 0) loss[r] = w * tau * tau * term;
+  } else if (out) {
     const float m = none ? INFINITY : v.m;  // 2^-inf = 0
     auto single = [&](uint32_t i) {
       out[i] = from_f32<T>(f * exp2_approx((to_f32(share.p[i]) - m) * c));
     };
     if (threadIdx.x < share.head) single(threadIdx.x);
-    const F2 minus = pack2(-m, -m), c2 = pack2(c, c), f2 = pack2(f, f);
-    for (uint32_t i = threadIdx.x; i < share.pieces; i += THREADS) {
-      const uint4 p = share.piece(i);
-      uint4 o;
-#pragma unroll
-      for (int e = 0; e < V / 2; ++e) {
-        float a0, a1;
-        unpack2(mul2(add2(Piece<T>::pair(p, e), minus), c2), a0, a1);
-        unpack2(mul2(pack2(exp2_approx(a0), exp2_approx(a1)), f2), a0, a1);
-        Piece<T>::put(o, e, a0, a1);
-      }
-      store(i, o);
-    }
     if (threadIdx.x < share.tail) single(share.tail_at() + threadIdx.x);
-    __syncthreads();
-    // An output named twice is written by its first entry.
-    if (id >= 0 && (uint32_t)id - share.start < share.count) {
-      float both = 0.0f;
-      bool first = true;
-      for (uint32_t i = 0; i < k; ++i)
-        if (sid[i] == id) {
-          both += sq[i];
-          if (i < j) first = false;
+    const F2 minus = pack2(-m, -m), c2 = pack2(c, c), f2 = pack2(f, f);
+    share.with_whole(out, [&](auto whole) {
+      auto piece = [&](uint32_t i, const uint4& p) {
+        uint4 o;
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) {
+          const F2 d = mul2(add2(Piece<T>::pair(p, e), minus), c2);
+          const F2 g = mul2(pack2(exp2_approx(d.x), exp2_approx(d.y)), f2);
+          Piece<T>::put(o, e, g.x, g.y);
         }
-      if (first) out[(uint32_t)id - share.start] = from_f32<T>(a * (qsum * expf(logp) - both));
-    }
+        share.template put_piece<decltype(whole)::value>(out, i, o);
+      };
+      uint32_t i = threadIdx.x;
+      for (; i < kept; i += THREADS) piece(i, keep[i]);
+      for (; i + 3 * THREADS < share.pieces; i += 4 * THREADS) {
+        uint4 q4[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) q4[u] = share.piece(i + u * THREADS);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) piece(i + u * THREADS, q4[u]);
+      }
+      for (; i < share.pieces; i += THREADS) piece(i, share.piece(i));
+    });
+  }
+  if (out) {
+    __syncthreads();
+    if (teacher)
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (id[e] >= 0) out[(uint32_t)id[e] - share.start] = from_f32<T>(fixed[e]);
   }
   if (parts > 1) cl.barrier_wait();
 }
@@ -155,13 +209,30 @@ extern "C" int plx_distill(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, c
   if (rows == 1) ld = ldd = 0;
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
+    constexpr uint32_t V = Piece<T>::V;
+    // A row that has to stay is split until half of a part fits: what is read
+    // again of 444 parts at once is then still in L2.
+    uint32_t parts = row_parts(rows, n);
+    if (dlogits)
+      while (parts < 8 && (uint64_t)n * sizeof(T) > (uint64_t)parts * 2 * kKeepBytes) parts *= 2;
     auto go = [&](auto kernel, uint32_t threads) {
-      PLX_TRY_CUDA(launch_rows(kernel, rows, row_parts(rows, n, 4096), threads, ctx->stream, n,
-                               (const T*)logits, ld, k, teacher_ids, teacher_values, teacher_kind,
+      uint32_t pieces = 0;
+      if (dlogits) {
+        pieces = std::min<uint32_t>((n + parts - 1) / parts / V + 1, kKeepBytes / 16);
+        if (pieces * 16 > 47 * 1024)
+          PLX_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            kKeepBytes));
+      }
+      PLX_TRY_CUDA(launch_rows(kernel, rows, parts, threads + 32, (size_t)pieces * 16, ctx->stream, n,
+                               part_length(n, parts, V), (const T*)logits, ld, k, teacher_ids, teacher_values, teacher_kind,
                                temperature, 1.0f / temperature, row_weight, loss, (T*)dlogits, ldd,
-                               ctx->d_status));
+                               pieces, ctx->d_status));
       return PLX_OK;
     };
-    return n < 128 * 4 * Piece<T>::V ? go(k_distill<T, 128>, 128) : go(k_distill<T, 512>, 512);
+    switch (row_threads(n / parts)) {
+      case 64: return go(k_distill<T, 64>, 64);
+      case 128: return go(k_distill<T, 128>, 128);
+      default: return go(k_distill<T, 256>, 256);
+    }
   });
 }

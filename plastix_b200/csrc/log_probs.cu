@@ -8,117 +8,195 @@
 //
 // Bound by memory: the forward pass reads a row once (running maximum and
 // sums, logits.cuh) and finds the alternatives from what the threads saw: of
-// the threads' own maxima the `top` best are a threshold, only the threads at
-// or above it can hold an alternative, and only those look at their share
-// again (out of L2, a few kilobytes a row).
+// the threads' own maxima the `top` best are a threshold, only threads at or
+// above it can hold an alternative, and of those only the runs of pieces whose
+// maximum reaches it are looked at again (a few kilobytes a row, out of L2).
 #include "logits.cuh"
 
 namespace plx {
 namespace {
 
-// A number that orders values: larger for larger ones, NaN above all, -0 as 0.
-__device__ __forceinline__ uint32_t order_of(float v) {
-  const uint32_t b = __float_as_uint(v + 0.0f);
-  return v != v ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float value_of(uint32_t o) {
-  return __uint_as_float(o == 0xffffffffu ? 0x7fffffffu : (o & 0x80000000u) ? o ^ 0x80000000u : ~o);
-}
-// With its index: the lower one first among equals. 0 is no element.
+// A value's order with its index: the lower one first among equals. 0 is no
+// element.
 __device__ __forceinline__ uint64_t rank_key(float v, uint32_t i) {
   return (uint64_t)order_of(v) << 32 | (0xffffffffu - i);
 }
 
 constexpr uint32_t kCandidates = 1024;
+constexpr uint32_t kSpare = 32;  // threads more than asked for that may reach the threshold
 
 template <int THREADS>
 struct TopShared {
-  uint64_t red[THREADS / 32];
   uint64_t keys[kCandidates];
-  uint64_t best[PLX_TOP_MAX];
-  uint32_t count;
+  uint64_t best[PLX_TOP_MAX];  // best first, 0 where there are fewer
+  uint64_t red[THREADS / 32];
+  uint32_t most[THREADS];      // each thread's maximum, as a number that orders
+  Slots<THREADS> slots;
+  uint16_t runs[(PLX_TOP_MAX + kSpare) * kSlots];  // that can hold an alternative
+  uint32_t listed, count, threshold, reached;
 };
 
-// The block's `top` best elements into sh.best, best first, 0 where there are
-// fewer. m, pos: the thread's maximum and the first unit that attains it.
-template <typename T, int THREADS>
-__device__ void block_top(const Share<T>& share, float m, uint32_t pos, uint32_t top,
-                          TopShared<THREADS>& sh) {
-  const uint32_t tid = threadIdx.x;
-  const uint32_t mine = pos == 0xffffffffu ? 0u : order_of(m);
-  // The largest value that at least `top` threads' maxima reach.
-  uint64_t lo = 1, hi = 1ull << 32;
-  uint32_t at_lo = (uint32_t)__syncthreads_count(mine >= 1u), above = 0;
-  if (at_lo > top)
-    while (hi - lo > 1) {
-      const uint64_t mid = (lo + hi) / 2;
-      const uint32_t n = (uint32_t)__syncthreads_count(mine >= mid);
-      if (n >= top) {
-        lo = mid;
-        at_lo = n;
-        if (n == top) break;
-      } else {
-        hi = mid;
-        above = n;
-      }
-    }
-  // Among equals at the threshold the units that come first are enough.
-  uint32_t last = 0xfffffffeu;
-  auto narrow = [&] {
-    uint32_t a = 0, b = share.start + share.count - 1;
-    while (a < b) {
-      const uint32_t mid = a + (b - a) / 2;
-      if ((uint32_t)__syncthreads_count(mine == lo && pos <= mid) >= top - above) b = mid;
-      else a = mid + 1;
-    }
-    last = a;
-  };
-  bool narrowed = at_lo <= top;
-  if (at_lo > top + 32) {
-    narrow();
-    narrowed = true;
+// A value that at least `top` threads' maxima reach, and (in `reached`) by how
+// many: a few more than `top`, unless many are equal to it; then it is the
+// largest such value. At least `top` elements are at or above it, so no element
+// below it counts, and no other thread's. By one warp; most[i] is of thread
+// lane + 32 i.
+template <int K>
+__device__ __forceinline__ uint32_t find_threshold(uint32_t top, const uint32_t (&most)[K],
+                                                   uint32_t& reached) {
+  static_assert(PLX_TOP_MAX <= 64 && K >= 2, "two of each lane are enough");
+  uint32_t a = 0, b = 0;  // the lane's two best
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    b = max(b, min(a, most[i]));
+    a = max(a, most[i]);
   }
-  // Calls f(value, index) for every element of this thread that can count.
-  auto candidates = [&](auto f) {
-    if (mine < lo || (mine == lo && pos > last)) return;
-    auto unit = [&](uint32_t first, uint32_t n) {
-      for (uint32_t k = 0; k < n; ++k) {
-        const float x = to_f32(share.p[first + k]);
-        const uint32_t o = order_of(x);
-        if (o > lo || (o == lo && share.start + first <= last)) f(x, share.start + first + k);
-      }
-    };
-    constexpr int V = Piece<T>::V;
-    if (tid < share.head) unit(tid, 1);
-    for (uint32_t i = tid; i < share.pieces; i += THREADS) {
-      const uint4 q = share.piece(i);
-      const float most = Piece<T>::most(q);
-      if (order_of(most) >= lo) unit(share.piece_at(i), V);
-    }
-    if (tid < share.tail) unit(share.tail_at() + tid, 1);
+  auto reach = [&](uint32_t v) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) n += most[i] >= v;
+    return __reduce_add_sync(0xffffffffu, n);
   };
-  for (;;) {
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-    candidates([&](float x, uint32_t i) {
-      const uint32_t k = atomicAdd(&sh.count, 1u);
-      if (k < kCandidates) sh.keys[k] = rank_key(x, i);
-    });
-    __syncthreads();
-    if (sh.count <= kCandidates || narrowed) break;
-    narrow();
-    narrowed = true;
+  uint32_t lo = 1;
+  reached = reach(1);
+  if (reached <= top) return lo;
+  // 32 (64) maxima reach the least of the lanes' best (second best) ones. No
+  // more than one reaches the largest.
+  uint32_t hi = __reduce_max_sync(0xffffffffu, a);
+  const uint32_t least = __reduce_min_sync(0xffffffffu, top <= 32 ? a : b);
+  if (least > 1) reached = reach(lo = least);
+  if (const uint32_t n = reach(hi); n >= top) {
+    reached = n;
+    return hi;
+  }
+  while (hi - lo > 1 && reached > top + kSpare / 4) {
+    const uint32_t mid = lo + (hi - lo) / 2, n = reach(mid);
+    if (n >= top) {
+      lo = mid;
+      reached = n;
+    } else {
+      hi = mid;
+    }
+  }
+  return lo;
+}
+
+// Places of `count` different keys (0 is none) by the number of better ones; put(place, key)
+// for the places below `top`. By `threads` threads, of which this is the me-th.
+template <typename F>
+__device__ __forceinline__ void place_keys(const uint64_t* keys, uint32_t count, uint32_t top,
+                                           uint32_t me, uint32_t threads, F put) {
+  for (uint32_t i = me; i < count; i += threads) {
+    const uint64_t key = keys[i];
+    uint32_t place = 0;
+#pragma unroll 8
+    for (uint32_t j = 0; j < count; ++j) place += keys[j] > key;
+    if (key && place < top) put(place, key);
+  }
+}
+
+// A share's `top` best elements into sh.best, from what scan_share left in
+// sh.slots and sh.most (after a barrier).
+template <typename T, int THREADS>
+__device__ __forceinline__ void share_top(const Share<T>& share, uint32_t top,
+                                          TopShared<THREADS>& sh) {
+  constexpr int K = THREADS / 32, SPARE = kSpareBits<T>;
+  constexpr uint32_t V = Piece<T>::V;
+  const uint32_t tid = threadIdx.x;
+  if (tid < 32) {
+    uint32_t most[K], reached;
+#pragma unroll
+    for (int i = 0; i < K; ++i) most[i] = sh.most[tid + 32 * i] >> SPARE;
+    const uint32_t threshold = find_threshold<K>(top, most, reached);
+    if (tid == 0) {
+      sh.threshold = threshold;
+      sh.reached = reached;
+      sh.listed = sh.count = 0;
+    }
   }
   for (uint32_t k = tid; k < top; k += THREADS) sh.best[k] = 0;
-  const uint32_t count = sh.count;
   __syncthreads();
-  if (count <= kCandidates) {  // each candidate's place is the number of better ones
-    for (uint32_t i = tid; i < count; i += THREADS) {
-      const uint64_t key = sh.keys[i];
-      uint32_t place = 0;
-      for (uint32_t j = 0; j < count; ++j) place += sh.keys[j] > key;
-      if (place < top) sh.best[place] = key;
+  const uint32_t threshold = sh.threshold;
+  // Values that very many threads reach at best (a row of few distinct values):
+  // those above are taken first, then ties from the row's start.
+  const bool ties = sh.reached > top + kSpare;
+  const uint32_t bar = ties ? threshold : threshold - 1;  // elements above it
+  auto order = [](float v) { return order_of(v) >> SPARE; };
+  const uint32_t shift = share.slot_shift(THREADS);
+  if (sh.most[tid] >> SPARE > bar) {
+    const uint32_t pieces = share.pieces > tid ? (share.pieces - tid - 1) / THREADS + 1 : 0;
+#pragma unroll
+    for (uint32_t s = 0; s < kSlots; ++s) {
+      if (s << shift >= pieces) break;
+      const uint32_t h = sh.slots.most[s * THREADS + tid];
+      if ((h & 0x8000u ? ~h & 0xffffu : h | 0x8000u) >= bar << SPARE >> 16)
+        sh.runs[atomicAdd(&sh.listed, 1u)] = (uint16_t)(s * THREADS + tid);
     }
+  }
+  __syncthreads();
+  auto elements = [&](const uint4& q, uint32_t first, auto f) {
+#pragma unroll
+    for (uint32_t e = 0; e < V / 2; ++e) {
+      const F2 v = Piece<T>::pair(q, e);
+      f(v.x, first + 2 * e);
+      f(v.y, first + 2 * e + 1);
+    }
+  };
+  // Calls f(value, index) for every element above the bar: of the pieces of
+  // the listed runs, spread over the block, and of the single elements.
+  auto candidates = [&](auto f) {
+    auto element = [&](float x, uint32_t i) {
+      if (order(x) > bar) f(x, share.start + i);
+    };
+    if (tid < share.head) element(to_f32(share.p[tid]), tid);
+    if (tid < share.tail) element(to_f32(share.p[share.tail_at() + tid]), share.tail_at() + tid);
+    const uint32_t pieces = sh.listed << shift;
+    for (uint32_t k = tid; k < pieces; k += THREADS) {
+      const uint32_t run = sh.runs[k >> shift];
+      const uint64_t i = run % THREADS +
+                         (uint64_t)((run / THREADS << shift) + (k & ((1u << shift) - 1))) * THREADS;
+      if (i >= share.pieces) continue;
+      const uint4 q = share.piece((uint32_t)i);
+      if (order(Piece<T>::template most<1>(&q)) > bar)
+        elements(q, share.piece_at((uint32_t)i), element);
+    }
+  };
+  auto keep = [&](float x, uint32_t i) {
+    const uint32_t k = atomicAdd(&sh.count, 1u);
+    if (k < kCandidates) sh.keys[k] = rank_key(x, i);
+  };
+  candidates(keep);
+  __syncthreads();
+  if (ties) {
+    // If fewer than `top` are above, the list holds every one of them and has
+    // room for a step of ties (64 units, at most 512 values) more than it
+    // takes to fill up.
+    const uint32_t units = share.head + share.pieces + share.tail;
+    uint32_t have = sh.count;
+    for (uint32_t u = 0; u < units && have < top; u += 64) {
+      __syncthreads();
+      const uint32_t k = u + tid, i = k - share.head;  // of the pieces
+      auto element = [&](float x, uint32_t at) {
+        if (order(x) == threshold) keep(x, share.start + at);
+      };
+      if (tid < 64 && k < units) {
+        if (k < share.head) {
+          element(to_f32(share.p[k]), k);
+        } else if (i >= share.pieces) {
+          const uint32_t at = share.tail_at() + (i - share.pieces);
+          element(to_f32(share.p[at]), at);
+        } else {
+          elements(share.piece(i), share.piece_at(i), element);
+        }
+      }
+      __syncthreads();
+      have = sh.count;
+    }
+  }
+  const uint32_t count = sh.count;
+  if (count <= kCandidates) {
+    place_keys(sh.keys, count, top, tid, THREADS,
+               [&](uint32_t place, uint64_t key) { sh.best[place] = key; });
   } else {  // a few threads hold very many: one alternative at a time
     uint64_t below = ~0ull;
     for (uint32_t k = 0; k < top; ++k) {
@@ -134,7 +212,7 @@ __device__ void block_top(const Share<T>& share, float m, uint32_t pos, uint32_t
       __syncthreads();
       best = sh.red[0];
 #pragma unroll
-      for (int w = 1; w < THREADS / 32; ++w) best = max(best, sh.red[w]);
+      for (int w = 1; w < K; ++w) best = max(best, sh.red[w]);
       if (tid == 0) sh.best[k] = best;
       below = best;
     }
@@ -142,40 +220,54 @@ __device__ void block_top(const Share<T>& share, float m, uint32_t pos, uint32_t
   __syncthreads();
 }
 
+// A block has a row, or a cluster of blocks a part each.
 template <typename T, bool ENT, bool TOP, int THREADS>
-__global__ void __launch_bounds__(THREADS)
-k_log_probs(uint32_t n, const T* __restrict__ x, int64_t ld, const int32_t* __restrict__ target,
-            float scale, uint32_t top, float* __restrict__ logp, float* __restrict__ lse,
-            float* __restrict__ entropy, int32_t* __restrict__ top_ids,
-            float* __restrict__ top_logp, int32_t* __restrict__ status) {
+__global__ void __launch_bounds__(THREADS, (TOP ? 1024 : 1536) / THREADS)
+k_log_probs(uint32_t n, uint32_t each, const T* __restrict__ x, int64_t ld,
+            const int32_t* __restrict__ target, float scale, uint32_t top,
+            float* __restrict__ logp, float* __restrict__ lse, float* __restrict__ entropy,
+            int32_t* __restrict__ top_ids, float* __restrict__ top_logp,
+            int32_t* __restrict__ status) {
   constexpr int WARPS = THREADS / 32;
-  __shared__ float red[WARPS];
-  __shared__ Sums mine;
+  __shared__ Sums all[WARPS], mine;
+  __shared__ std::conditional_t<TOP, TopShared<THREADS>, char> sh;
   cg::cluster_group cl = cg::this_cluster();
   const uint32_t parts = cl.num_blocks(), part = cl.block_rank();
-  const int64_t r = blockIdx.x / parts;
+  const int64_t r = cluster_row();
   const T* xr = x + r * ld;
-  const Share<T> share(xr, n, part, parts);
+  const Share<T> share(xr, n, part, each);
   const float c = scale * kLog2e;
-  uint32_t pos;
-  const Sums own = scan_share<T, ENT, TOP, THREADS>(share, c, pos);
-  Sums v = join_block<ENT, WARPS>(own, c, red);
-  __shared__ TopShared<TOP ? THREADS : 32> sh;
-  if constexpr (TOP) block_top<T, THREADS>(share, own.m, pos, top, sh);
-  if (parts > 1) v = join_cluster<ENT>(cl, &mine, v, c);
+  // The target's logit is two dependent loads away: both are on their way early.
+  const bool first = part == 0 && threadIdx.x == 0;
+  int32_t at = first && logp ? target[r] : -1;
+  Slots<THREADS>* slots = nullptr;
+  if constexpr (TOP) slots = &sh.slots;
+  Sums v = scan_share<T, ENT, TOP, false, THREADS>(share, c, slots);
+  if (at < -1 || at >= (int64_t)n) {
+    record_status(status, kStatusBadOutput);
+    at = -1;
+  }
+  const float x_at = at < 0 ? 0.0f : to_f32(xr[at]);
+  if constexpr (TOP) {
+    const uint32_t tid = threadIdx.x;
+    const bool any = tid < share.head || tid < share.pieces || tid < share.tail;
+    sh.most[tid] = any ? order_of(v.m) : 0u;
+  }
+  v = join_block<ENT, WARPS>(v, c, all);
+  if constexpr (TOP) share_top<T, THREADS>(share, top, sh);
+  if (parts > 1) {
+    if (threadIdx.x == 0) mine = v;
+    cl.sync();
+    v = join_parts<ENT>(cl, &mine, c);
+  }
   if (part == 0) {
     const bool none = v.m == -INFINITY;  // every output masked
     const float ls = logf(v.s);
-    auto log_p = [&](float at) { return none ? -INFINITY : scale * (at - v.m) - ls; };
-    if (threadIdx.x == 0) {
+    auto log_p = [&](float y) { return none ? -INFINITY : scale * (y - v.m) - ls; };
+    if (first) {
       lse[r] = none ? -INFINITY : fmaf(scale, v.m, ls);
       if (ENT) entropy[r] = none ? 0.0f : ls - scale * (v.t / v.s);
-      if (logp) {
-        const int32_t at = target[r];
-        const bool out = at < -1 || at >= (int64_t)n;
-        if (out) record_status(status, kStatusBadOutput);
-        logp[r] = out || at < 0 ? 0.0f : log_p(to_f32(xr[at]));
-      }
+      if (logp) logp[r] = at < 0 ? 0.0f : log_p(x_at);
     }
     if constexpr (TOP) {
       auto put = [&](uint32_t place, uint64_t key) {
@@ -184,16 +276,11 @@ k_log_probs(uint32_t n, const T* __restrict__ x, int64_t ld, const int32_t* __re
       };
       if (parts == 1) {
         for (uint32_t k = threadIdx.x; k < top; k += THREADS) put(k, sh.best[k]);
-      } else {  // the blocks' lists side by side, each key's place as above
+      } else {  // the blocks' lists side by side
         for (uint32_t i = threadIdx.x; i < parts * top; i += THREADS)
           sh.keys[i] = cl.map_shared_rank(&sh.best[0], i / top)[i % top];
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < parts * top; i += THREADS) {
-          const uint64_t key = sh.keys[i];
-          uint32_t place = 0;
-          for (uint32_t j = 0; j < parts * top; ++j) place += sh.keys[j] > key;
-          if (key && place < top) put(place, key);
-        }
+        place_keys(sh.keys, parts * top, top, threadIdx.x, THREADS, put);
       }
     }
   }
@@ -202,49 +289,80 @@ k_log_probs(uint32_t n, const T* __restrict__ x, int64_t ld, const int32_t* __re
 
 constexpr int kBwdThreads = 256;
 
-template <typename T>
+// dx = p (A l + B) (+ the target's own term), with l = log p, A = -scale h',
+// B = -scale (h' H + g'); h', g': gradients of entropy H and of logp.
+template <typename T, bool ENT>
 __global__ void __launch_bounds__(kBwdThreads)
-k_log_probs_bwd(uint32_t n, uint32_t parts, const T* x, int64_t ld,
+k_log_probs_bwd(uint32_t n, uint32_t parts, uint32_t each, const T* x, int64_t ld,
                 const int32_t* __restrict__ target, float scale, const float* __restrict__ lse,
                 const float* __restrict__ entropy, const float* __restrict__ grad_logp,
                 const float* __restrict__ grad_entropy, T* dx, int64_t ldd) {
-  constexpr int V = Piece<T>::V;
-  const int64_t r = blockIdx.x / parts;
-  const Share<T> sh(x + r * ld, n, blockIdx.x % parts, parts);
+  constexpr int V = Piece<T>::V, U = 4;
+  const int64_t r = parts == 1 ? blockIdx.x : blockIdx.x / parts;
+  const Share<T> sh(x + r * ld, n, blockIdx.x - (uint32_t)r * parts, each);
   T* out = dx + r * ldd + sh.start;
-  const float z = lse[r];
-  const int32_t at = target ? target[r] : -1;
-  const float g = grad_logp && at >= 0 && at < (int64_t)n ? grad_logp[r] : 0.0f;
-  const float gh = grad_entropy ? grad_entropy[r] : 0.0f;
-  const float h = grad_entropy ? entropy[r] : 0.0f;
-  auto one = [&](float v, uint32_t i) {
-    const float l = fmaf(v, scale, -z);
-    const float p = z == -INFINITY ? 0.0f : exp2_approx(l * kLog2e);
-    float d = p == 0.0f ? 0.0f : -p * fmaf(gh, l + h, g);
-    if (sh.start + i == (uint32_t)at) d += g;
-    return d * scale;
+  const float z0 = lse[r];
+  const float z = z0 == -INFINITY ? INFINITY : z0;  // a row masked whole: p = 0
+  const int32_t at = grad_logp ? target[r] : -1;
+  const bool has = at >= 0 && at < (int64_t)n;
+  const float g = has ? grad_logp[r] : 0.0f;
+  const float gh = ENT ? grad_entropy[r] : 0.0f;
+  const float A = -scale * gh, B = -scale * fmaf(gh, ENT ? entropy[r] : 0.0f, g);
+  // Where the target is within this share; no index where it is not.
+  const uint32_t hot = has && (uint32_t)at - sh.start < sh.count ? (uint32_t)at - sh.start : ~0u;
+  const F2 s2 = pack2(scale, scale), z2 = pack2(-z, -z), e2 = pack2(kLog2e, kLog2e);
+  const F2 A2 = pack2(A, A), B2 = pack2(B, B);
+  // Gradients of two values. l is kept off -inf (p is 0 long before): 0 times it would be NaN.
+  auto two = [&](F2 v, float& a, float& b) {
+    F2 l = fma2(v, s2, z2);
+    if (ENT) {
+      unpack2(l, a, b);
+      l = pack2(max_nan(a, -1000.0f), max_nan(b, -1000.0f));
+    }
+    unpack2(mul2(l, e2), a, b);
+    const F2 p = pack2(exp2_approx(a), exp2_approx(b));
+    unpack2(mul2(p, ENT ? fma2(A2, l, B2) : B2), a, b);
   };
-  auto single = [&](uint32_t i) { out[i] = from_f32<T>(one(to_f32(sh.p[i]), i)); };
+  auto single = [&](uint32_t i) {
+    const float v = to_f32(sh.p[i]);
+    float a, b;
+    two(pack2(v, v), a, b);
+    out[i] = from_f32<T>(a);
+  };
+  // The target's own term is added by the thread that has written it.
+  uint32_t owner = hot - sh.head;
+  if (hot < sh.head) owner = hot;
+  else if (hot >= sh.tail_at()) owner = hot - sh.tail_at();
+  else owner = owner / V % kBwdThreads;
+  const bool mine = hot != ~0u && threadIdx.x == owner;
+  const float x_hot = mine ? to_f32(sh.p[hot]) : 0.0f;
   if (threadIdx.x < sh.head) single(threadIdx.x);
   if (threadIdx.x < sh.tail) single(sh.tail_at() + threadIdx.x);
-  const bool whole = (reinterpret_cast<uintptr_t>(out + sh.head) & 15u) == 0;
-  for (uint32_t i = threadIdx.x; i < sh.pieces; i += kBwdThreads) {
-    const uint4 q = sh.piece(i);
-    const uint32_t first = sh.piece_at(i);
-    uint4 o;
+  sh.with_whole(out, [&](auto whole) {
+    auto piece = [&](uint32_t i, const uint4& q) {
+      uint4 o;
 #pragma unroll
-    for (int k = 0; k < V / 2; ++k) {
-      float a, b;
-      unpack2(Piece<T>::pair(q, k), a, b);
-      Piece<T>::put(o, k, one(a, first + 2 * k), one(b, first + 2 * k + 1));
-    }
-    if (whole) {
-      *reinterpret_cast<uint4*>(out + first) = o;
-    } else {
-      const T* e = reinterpret_cast<const T*>(&o);
+      for (int k = 0; k < V / 2; ++k) {
+        float a, b;
+        two(Piece<T>::pair(q, k), a, b);
+        Piece<T>::put(o, k, a, b);
+      }
+      sh.template put_piece<decltype(whole)::value>(out, i, o);
+    };
+    uint32_t i = threadIdx.x;
+    for (; i + (U - 1) * kBwdThreads < sh.pieces; i += U * kBwdThreads) {
+      uint4 q[U];
 #pragma unroll
-      for (int k = 0; k < V; ++k) out[first + k] = e[k];
+      for (int u = 0; u < U; ++u) q[u] = sh.piece(i + u * kBwdThreads);
+#pragma unroll
+      for (int u = 0; u < U; ++u) piece(i + u * kBwdThreads, q[u]);
     }
+    for (; i < sh.pieces; i += kBwdThreads) piece(i, sh.piece(i));
+  });
+  if (mine) {
+    float a, b;
+    two(pack2(x_hot, x_hot), a, b);
+    out[hot] = from_f32<T>(fmaf(g, scale, a));
   }
 }
 
@@ -269,18 +387,26 @@ extern "C" int plx_log_probs(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype,
   PLX_TRY_CUDA(guard.err);
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
+    const uint32_t parts = row_parts(rows, n);
     auto go = [&](auto kernel, uint32_t threads) {
-      PLX_TRY_CUDA(launch_rows(kernel, rows, row_parts(rows, n, 4096), threads, ctx->stream, n,
-                               (const T*)logits, rows == 1 ? (int64_t)0 : ld, target, scale, top,
-                               logp, lse, entropy, top_ids, top_logp, ctx->d_status));
+      PLX_TRY_CUDA(launch_rows(kernel, rows, parts, threads, (size_t)0, ctx->stream, n,
+                               part_length(n, parts, Piece<T>::V), (const T*)logits,
+                               rows == 1 ? (int64_t)0 : ld, target, scale, top, logp, lse, entropy,
+                               top_ids, top_logp, ctx->d_status));
       return PLX_OK;
     };
-    // Blocks of 512 keep enough reads in flight; rows too short for one batch
-    // of pieces each take blocks of 128.
     auto pick = [&](auto ent, auto best) {
       constexpr bool E = decltype(ent)::value, B = decltype(best)::value;
-      return n < 128 * 4 * Piece<T>::V ? go(k_log_probs<T, E, B, 128>, 128)
-                                       : go(k_log_probs<T, E, B, 512>, 512);
+      // With alternatives 128 threads at most (4,096 rows of 65,536 bf16, 8
+      // alternatives: 102 us, with 256 threads 108), but four times as many as
+      // alternatives, or their maxima say too little (64: 143 us, with 256 130).
+      uint32_t threads = row_threads(n / parts);
+      if (B) threads = std::max(std::min(threads, 128u), top > 32 ? 256u : top > 16 ? 128u : 64u);
+      switch (threads) {
+        case 64: return go(k_log_probs<T, E, B, 64>, 64);
+        case 128: return go(k_log_probs<T, E, B, 128>, 128);
+        default: return go(k_log_probs<T, E, B, 256>, 256);
+      }
     };
     using Yes = std::true_type;
     using No = std::false_type;
@@ -306,12 +432,16 @@ extern "C" int plx_log_probs_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, i
   if (rows == 1) ld = ldd = 0;
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    // Four pieces a thread, as far as the grid's size allows.
-    const uint64_t each = kBwdThreads * 4 * Piece<T>::V;
+    // Sixteen pieces a thread hide what a block costs; down to four where that
+    // would leave SMs without blocks. As far as the grid's size allows.
+    uint64_t each = kBwdThreads * 16 * Piece<T>::V;
+    while (each > kBwdThreads * 4 * Piece<T>::V && rows * ((n + each - 1) / each) < 148 * 32)
+      each /= 2;
     const uint32_t parts = (uint32_t)std::max<uint64_t>(
         1, std::min<uint64_t>((n + each - 1) / each, ((1ull << 31) - 1) / rows));
-    k_log_probs_bwd<T><<<(unsigned)(rows * parts), kBwdThreads, 0, ctx->stream>>>(
-        n, parts, (const T*)logits, ld, target, scale, lse, entropy, grad_logp, grad_entropy,
+    auto* kernel = grad_entropy ? k_log_probs_bwd<T, true> : k_log_probs_bwd<T, false>;
+    kernel<<<(unsigned)(rows * parts), kBwdThreads, 0, ctx->stream>>>(
+        n, parts, part_length(n, parts, Piece<T>::V), (const T*)logits, ld, target, scale, lse, entropy, grad_logp, grad_entropy,
         (T*)dlogits, ldd);
     PLX_LAUNCH_CHECK("k_log_probs_bwd");
     return PLX_OK;

@@ -27,6 +27,7 @@ from . import _abi
 from .runtime import Context
 
 _TYPES = {torch.float32: _abi.F32, torch.bfloat16: _abi.BF16, torch.float16: _abi.F16}
+_HERE = nullcontext()
 _KINDS = {"logits": _abi.TEACHER_LOGITS, "log_probs": _abi.TEACHER_LOG_PROBS}
 
 
@@ -77,7 +78,7 @@ def _result(ctx: Context, out: Optional[torch.Tensor], source: torch.Tensor, ld:
     """The tensor of rows that a call writes, and its row stride: ``out``, or
     a new one like ``source``. ``out`` may be the source itself."""
     if out is None:
-        return torch.empty(source.shape, dtype=source.dtype, device=source.device), source.shape[-1]
+        return source.new_empty(source.shape), source.shape[-1]
     if out.shape != source.shape or out.dtype != source.dtype:
         raise ValueError(f"{name} has to be {source.dtype} {tuple(source.shape)}, got {out.dtype} "
                          f"{tuple(out.shape)}")
@@ -92,8 +93,9 @@ def _scope(ctx: Context, *used):
     """The context's stream as the current one, where it is not already, so
     that what a call allocates belongs to it; what the call uses is kept from
     being given out again until that stream is done with it."""
-    if torch.cuda.current_stream(ctx.device) == ctx.stream:
-        return nullcontext()
+    # the handle alone: making a Stream object of it costs more than a small kernel
+    if torch._C._cuda_getCurrentRawStream(ctx.device.index) == ctx.stream.cuda_stream:
+        return _HERE
     for t in used:
         if t is not None:
             t.record_stream(ctx.stream)
@@ -129,7 +131,8 @@ def layer_norm(ctx: Context, x: torch.Tensor, weight: Optional[torch.Tensor] = N
         y, ldy = _result(ctx, out, x, ld, "out")
         mean = rstd = None
         if stats:
-            mean, rstd = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
+            mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+            rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
         _abi.call("plx_layer_norm", ctx.handle, rows, n, _TYPES[x.dtype], x.data_ptr(), ld,
                   _abi.F32 if kind is None else kind, _address(weight), _address(bias), eps,
                   y.data_ptr(), ldy, _address(mean), _address(rstd))
@@ -156,9 +159,9 @@ def layer_norm_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, mean: t
         dw = db = scratch = None
         size = 0
         if weight is not None:
-            dw, db = torch.empty((2, n), dtype=weight.dtype, device=x.device)
+            dw, db = weight.new_empty(n), weight.new_empty(n)
             size = _abi.lib().plx_layer_norm_scratch_bytes(rows, n)
-            scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+            scratch = x.new_empty(size, dtype=torch.uint8)
         _abi.call("plx_layer_norm_backward", ctx.handle, rows, n, _TYPES[x.dtype], dy.data_ptr(),
                   lddy, x.data_ptr(), ld, mean_p, rstd_p, _abi.F32 if kind is None else kind,
                   _address(weight), dx.data_ptr(), lddx, _address(dw), _address(db),
@@ -175,14 +178,13 @@ def log_probs(ctx: Context, logits: torch.Tensor, target: Optional[torch.Tensor]
     lead = logits.shape[:-1]
     target_p = None if target is None else _like(ctx, target, lead, torch.int32, "target")
     with _scope(ctx, logits, target):
-        dev = logits.device
-        lse = torch.empty(lead, dtype=torch.float32, device=dev)
-        logp = None if target is None else torch.empty(lead, dtype=torch.float32, device=dev)
-        ent = torch.empty(lead, dtype=torch.float32, device=dev) if entropy else None
+        lse = logits.new_empty(lead, dtype=torch.float32)
+        logp = None if target is None else logits.new_empty(lead, dtype=torch.float32)
+        ent = logits.new_empty(lead, dtype=torch.float32) if entropy else None
         ids = best = None
         if top:
-            ids = torch.empty(lead + (top,), dtype=torch.int32, device=dev)
-            best = torch.empty(lead + (top,), dtype=torch.float32, device=dev)
+            ids = logits.new_empty(lead + (top,), dtype=torch.int32)
+            best = logits.new_empty(lead + (top,), dtype=torch.float32)
         _abi.call("plx_log_probs", ctx.handle, rows, n, _TYPES[logits.dtype], logits.data_ptr(),
                   ld, target_p, scale, top, _address(logp), lse.data_ptr(), _address(ent),
                   _address(ids), _address(best))
@@ -245,7 +247,7 @@ def distill(ctx: Context, logits: torch.Tensor, teacher_ids: torch.Tensor,
     if out is not None and not grad:
         raise ValueError("out is for the gradient: it needs grad=True")
     with _scope(ctx, logits, teacher_ids, teacher_values, weight, out):
-        loss = torch.empty(lead, dtype=torch.float32, device=logits.device)
+        loss = logits.new_empty(lead, dtype=torch.float32)
         dx, ldd = _result(ctx, out, logits, ld, "out") if grad else (None, 0)
         _abi.call("plx_distill", ctx.handle, rows, n, _TYPES[logits.dtype], logits.data_ptr(), ld,
                   k, ids_p, values_p, _KINDS[kind], temperature, _address(weight),

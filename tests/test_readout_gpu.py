@@ -249,8 +249,28 @@ def test_alternatives_among_equals_take_the_lowest_index(ctx, dtype, n):
                   r.integers(0, 3, n).astype(float),  # long runs of equals
                   np.full(n, -np.inf), np.arange(n) % 2.0,
                   np.minimum(np.arange(n), 2000.0),  # the best at the end, equal there
-                  -np.arange(n, dtype=float).clip(0, 2000)])
+                  -np.arange(n, dtype=float).clip(0, 2000),
+                  np.full(n, np.nan), np.where(np.arange(n) % 3 == 2, np.nan, np.inf),
+                  np.where(np.arange(n) % 5 == 4, -0.0, -1.0),  # the best are zeros below zero
+                  np.where(np.arange(n) >= n - 3, 1.0, 0.0)])
     a[3, n // 2:] = np.where(np.arange(n - n // 2) % 7 == 1, -5.0, -np.inf)  # fewer finite than asked for
+    x, _ = rows_tensor(a, dtype)
+    got = readout.log_probs(ctx, x, top=top)
+    ctx.sync()
+    np.testing.assert_array_equal(got.top_ids.cpu().numpy(), F.order(f64(x))[:, :top])
+
+
+@pytest.mark.parametrize("rows", [1, 600])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_alternatives_of_few_distinct_values(ctx, rows, dtype):
+    # many threads tie at the threshold, with few or many elements above it, at any place
+    n, top = 33333, 64
+    r = np.random.default_rng(rows)
+    a = r.integers(0, 40, (rows, n)) / 4.0
+    a[:, :n // 2] = np.minimum(a[:, :n // 2], 9.0)
+    a[::2] = np.minimum(a[::2], r.integers(1, 40, (len(a[::2]), 1)) / 4.0)
+    for row in range(0, rows, 3):
+        a[row, r.integers(0, n, 50)] = 30.0
     x, _ = rows_tensor(a, dtype)
     got = readout.log_probs(ctx, x, top=top)
     ctx.sync()
