@@ -18,17 +18,6 @@ namespace plx {
 
 namespace cg = cooperative_groups;
 
-// ---- two 32-bit values at once (one instruction each) ----------------------
-using F2 = float2;
-__device__ __forceinline__ F2 pack2(float a, float b) { return make_float2(a, b); }
-__device__ __forceinline__ void unpack2(F2 v, float& a, float& b) {
-  a = v.x;
-  b = v.y;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) { return __fadd2_rn(a, b); }
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) { return __fmul2_rn(a, b); }
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { return __ffma2_rn(a, b, c); }
-
 // ---- sixteen bytes of a row ----------------------------------------------
 template <typename T>
 struct Piece;
@@ -207,17 +196,6 @@ __device__ __forceinline__ void rebase(Sums& v, float b, float c) {
   v.m = b;
 }
 
-// 16 bytes from global to shared memory without a register in between.
-__device__ __forceinline__ void copy_async16(void* dst_smem, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst_smem)), "l"(src)
-               : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // A thread's share of a row. RUNS: also the maxima of its runs of pieces, into
 // `slots`. KEEP: the first `kept` pieces stay in `keep` (shared memory), piece i
 // at keep[i], where the thread that scanned them can read them again.
@@ -232,9 +210,9 @@ __device__ __forceinline__ Sums scan_share(const Share<T>& sh, float c, Slots<TH
     const uint32_t rounds = (kept + THREADS - 1) / THREADS;
     half = tid + (rounds + 1) / 2 * THREADS;
     uint32_t i = tid;
-    for (; i < min(kept, half); i += THREADS) copy_async16(keep + i, sh.p + sh.piece_at(i));
+    for (; i < min(kept, half); i += THREADS) copy_async<16>(keep + i, sh.p + sh.piece_at(i));
     copy_commit();
-    for (; i < kept; i += THREADS) copy_async16(keep + i, sh.p + sh.piece_at(i));
+    for (; i < kept; i += THREADS) copy_async<16>(keep + i, sh.p + sh.piece_at(i));
     copy_commit();
   }
   auto single = [&](uint32_t at) {

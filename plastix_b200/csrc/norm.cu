@@ -24,50 +24,83 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
   const uint32_t r = blockIdx.x * ROWS + threadIdx.x / TPR;
   if (ROWS > 1 && r >= rows) return;
   const T* xr = x + r * ldx;
+  constexpr int E = NV * V, H = E / 2;  // a thread's columns, as H pairs
+  static_assert(E % 2 == 0, "columns in pairs");
   Pack<T, V> q[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const uint32_t i = (j * TPR + lane) * V;
-    if (i < n) q[j] = load_pack<T, V>(xr + i);
-  }
-  float v[NV][V];
-  float s[1] = {0.0f};
+    if (i < n) {
+      q[j] = load_pack<T, V>(xr + i);
+    } else {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const bool in = (j * TPR + lane) * V < n;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      v[j][e] = in ? to_f32(q[j].v[e]) : 0.0f;
-      s[0] += v[j][e];
+      for (int e = 0; e < V; ++e) q[j].v[e] = from_f32<T>(0.0f);
     }
+  }
+  float f[E];
+  widen<NV, V>(q, f);
+  F2 v[H], s2 = pack2(0.0f, 0.0f);
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    v[h] = pack2(f[2 * h], f[2 * h + 1]);
+    s2 = add2(s2, v[h]);
   }
   int turn = 0;
+  float s[1] = {s2.x + s2.y};
   row_sum<TPR>(s, red, turn);
   const float mu = s[0] / (float)n;
-  s[0] = 0.0f;
+  const F2 minus = pack2(-mu, -mu);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const bool in = (j * TPR + lane) * V < n;
+  for (int h = 0; h < H; ++h) v[h] = add2(v[h], minus);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      v[j][e] -= mu;
-      if (in) s[0] = fmaf(v[j][e], v[j][e], s[0]);
-    }
-  }
+  for (int j = 0; j < NV; ++j)  // columns past the row's end have no deviation
+    if ((j * TPR + lane) * V >= n)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int k = j * V + e;
+        (k & 1 ? v[k / 2].y : v[k / 2].x) = 0.0f;
+      }
+  s2 = pack2(0.0f, 0.0f);
+#pragma unroll
+  for (int h = 0; h < H; ++h) s2 = fma2(v[h], v[h], s2);
+  s[0] = s2.x + s2.y;
   row_sum<TPR>(s, red, turn);
   const float rs = 1.0f / sqrtf(s[0] / (float)n + eps);
+  const F2 rs2 = pack2(rs, rs);
+#pragma unroll
+  for (int h = 0; h < H; ++h) v[h] = mul2(v[h], rs2);
+  float g[E];
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    f[2 * h] = v[h].x;
+    f[2 * h + 1] = v[h].y;
+  }
+  // Weights one after the other: they come out of L1.
+  if (w) {
+    Pack<P, V> p[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if ((j * TPR + lane) * V < n) p[j] = load_pack<P, V>(w + (j * TPR + lane) * V);
+    widen<NV, V>(p, g);
+#pragma unroll
+    for (int k = 0; k < E; ++k) f[k] *= g[k];
+  }
+  if (b) {
+    Pack<P, V> p[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if ((j * TPR + lane) * V < n) p[j] = load_pack<P, V>(b + (j * TPR + lane) * V);
+    widen<NV, V>(p, g);
+#pragma unroll
+    for (int k = 0; k < E; ++k) f[k] += g[k];
+  }
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const uint32_t i = (j * TPR + lane) * V;
     if (i < n) {
-      Pack<P, V> pw, pb;
-      if (w) pw = load_pack<P, V>(w + i);
-      if (b) pb = load_pack<P, V>(b + i);
       Pack<T, V> out;
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        out.v[e] = from_f32<T>(fmaf(v[j][e] * rs, w ? to_f32(pw.v[e]) : 1.0f,
-                                    b ? to_f32(pb.v[e]) : 0.0f));
+      for (int e = 0; e < V; ++e) out.v[e] = from_f32<T>(f[j * V + e]);
       *reinterpret_cast<Pack<T, V>*>(y + r * ldy + i) = out;
     }
   }
@@ -133,7 +166,13 @@ extern "C" int plx_layer_norm(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype
                                                 mean, rstd);
       };
       const unsigned one = (unsigned)rows, eighth = (unsigned)((rows + 7) / 8);
-      if (whole_pieces(n, sizeof(T), {x, y, weight, bias}, {ldx, ldy})) {
+      const uint32_t v = piece_values(n, sizeof(T), {x, y}, {ldx, ldy}, weight, bias, sizeof(P));
+      auto loops = [&] {
+        k_norm_long<T, P><<<one, 1024, 0, ctx->stream>>>(n, (const T*)x, ldx, (const P*)weight,
+                                                         (const P*)bias, eps, (T*)y, ldy, mean,
+                                                         rstd);
+      };
+      if (v == V) {
         const uint32_t pieces = n / V;
         if (pieces <= 32) launch(k_norm<T, P, V, 1, 32>, eighth, 256);
         else if (pieces <= 64) launch(k_norm<T, P, V, 2, 32>, eighth, 256);
@@ -143,20 +182,21 @@ extern "C" int plx_layer_norm(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype
         else if (pieces <= 1024) launch(k_norm<T, P, V, 4, 256>, one, 256);
         else if (pieces <= 2048) launch(k_norm<T, P, V, 4, 512>, one, 512);
         else if (pieces <= 4096) launch(k_norm<T, P, V, 4, 1024>, one, 1024);
-        else
-          k_norm_long<T, P><<<one, 1024, 0, ctx->stream>>>(n, (const T*)x, ldx, (const P*)weight,
-                                                           (const P*)bias, eps, (T*)y, ldy, mean,
-                                                           rstd);
+        else loops();
+      } else if (sizeof(T) == 2 && v >= 2) {
+        const uint32_t pieces = n / 2;
+        if (pieces <= 256) launch(k_norm<T, P, 2, 8, 32>, eighth, 256);
+        else if (pieces <= 1024) launch(k_norm<T, P, 2, 8, 128>, one, 128);
+        else if (pieces <= 2048) launch(k_norm<T, P, 2, 8, 256>, one, 256);
+        else if (pieces <= 4096) launch(k_norm<T, P, 2, 8, 512>, one, 512);
+        else loops();
       } else if (n <= 128) launch(k_norm<T, P, 1, 4, 32>, eighth, 256);
       else if (n <= 256) launch(k_norm<T, P, 1, 8, 32>, eighth, 256);
       else if (n <= 1024) launch(k_norm<T, P, 1, 8, 128>, one, 128);
-      else if (n <= 2048) launch(k_norm<T, P, 1, 8, 256>, one, 256);
-      else if (n <= 4096) launch(k_norm<T, P, 1, 8, 512>, one, 512);
-      else if (n <= 8192) launch(k_norm<T, P, 1, 8, 1024>, one, 1024);
-      else
-        k_norm_long<T, P><<<one, 1024, 0, ctx->stream>>>(n, (const T*)x, ldx, (const P*)weight,
-                                                         (const P*)bias, eps, (T*)y, ldy, mean,
-                                                         rstd);
+      else if (n <= 2048) launch(k_norm<T, P, 1, 16, 128>, one, 128);
+      else if (n <= 4096) launch(k_norm<T, P, 1, 16, 256>, one, 256);
+      else if (n <= 8192) launch(k_norm<T, P, 1, 16, 512>, one, 512);
+      else loops();
       PLX_LAUNCH_CHECK("k_norm");
       return PLX_OK;
     };

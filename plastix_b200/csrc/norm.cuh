@@ -12,6 +12,15 @@ struct alignas(V * sizeof(T) >= 16 ? 16 : V * sizeof(T)) Pack {
   T v[V];
 };
 
+// All a thread's values of a row at once, in 32 bits.
+template <int NV, int V, typename T>
+__device__ __forceinline__ void widen(const Pack<T, V> (&q)[NV], float (&f)[NV * V]) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[j * V + e] = to_f32(q[j].v[e]);
+}
+
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   return *reinterpret_cast<const Pack<T, V>*>(p);
@@ -41,6 +50,33 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* red, int& turn) {
   }
 }
 
+// Two sums at once: half of the warp carries each, so that they cost five
+// exchanges and not ten. Else as row_sum.
+template <int TPR>
+__device__ __forceinline__ F2 row_sum2(F2 v, float* red, int& turn) {
+  const uint32_t lane = threadIdx.x & 31;
+  const bool upper = lane & 16;
+  float a = upper ? v.y : v.x;
+  a += __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, 16);
+#pragma unroll
+  for (int d = 8; d; d >>= 1) a += __shfl_xor_sync(0xffffffffu, a, d);
+  if constexpr (TPR > 32) {
+    constexpr int W = TPR / 32;  // 4 to 32
+    float* r = red + turn * W * 2;
+    turn ^= 1;
+    if ((lane & 15) == 0) r[(upper ? W : 0) + (threadIdx.x >> 5)] = a;
+    __syncthreads();
+    const uint32_t k = lane & 15;
+    a = k < W ? r[(upper ? W : 0) + k] : 0.0f;
+    if (W > 16) a += r[(upper ? W : 0) + 16 + k];
+#pragma unroll
+    for (int d = W < 16 ? W / 2 : 8; d; d >>= 1) a += __shfl_xor_sync(0xffffffffu, a, d);
+    if (W < 16) a = __shfl_sync(0xffffffffu, a, lane & 16);
+  }
+  const float b = __shfl_xor_sync(0xffffffffu, a, 16);
+  return upper ? pack2(b, a) : pack2(a, b);
+}
+
 inline int check_norm(const plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, int param_dtype) {
   PLX_CHECK_ARG(ctx, "ctx is required");
   PLX_CHECK_ARG(valid_dtype(dtype), "dtype %d is none of PLX_F32, PLX_BF16, PLX_F16", dtype);
@@ -53,16 +89,20 @@ inline int check_norm(const plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, 
   return PLX_OK;
 }
 
-// Whether rows can be read in 16-byte pieces: no piece crosses a row's end.
-inline bool whole_pieces(uint32_t n, size_t elem, std::initializer_list<const void*> ptrs,
-                         std::initializer_list<int64_t> strides) {
-  const uint32_t v = 16 / (uint32_t)elem;
-  if (n % v) return false;
-  for (const void* p : ptrs)
-    if (!aligned16(p)) return false;
-  for (int64_t s : strides)
-    if (s % v) return false;
-  return true;
+// How many values, of 16 bytes down to one value, can be read together: no
+// piece crosses a row's end, and every one is aligned. The weights may be of
+// another size.
+inline uint32_t piece_values(uint32_t n, size_t elem, std::initializer_list<const void*> rows,
+                             std::initializer_list<int64_t> strides, const void* weight,
+                             const void* bias, size_t param) {
+  uint64_t all = n;
+  for (int64_t s : strides) all |= (uint64_t)s;
+  uint64_t at = 0, wat = 0;
+  for (const void* p : rows) at |= reinterpret_cast<uintptr_t>(p);
+  wat |= reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(bias);
+  uint32_t v = 16 / (uint32_t)elem;
+  while (v > 1 && (all % v || at % (v * elem) || wat % std::min<size_t>(16, v * param))) v /= 2;
+  return v;
 }
 
 }  // namespace plx

@@ -4,11 +4,12 @@
 //
 // Bound by memory (x and dy read once, dx written once), so the sums over rows
 // are taken in the same pass: a thread owns the same columns of every row its
-// block visits and carries their two sums in registers (32 bits), the next
-// row's values being loaded while the current one is worked on. Blocks leave
+// block visits and carries their two sums in registers (32 bits), while the
+// next rows are on their way into shared memory. Blocks leave
 // their sums in scratch and a second kernel adds them in a fixed order: no
 // atomics, the same bits on every call.
 #include <initializer_list>
+#include <type_traits>
 
 #include "norm.cuh"
 
@@ -16,87 +17,151 @@ namespace plx {
 namespace {
 
 constexpr uint32_t kSms = 148;                // of a B200; fixes the order of the sums
-constexpr uint32_t kMaxGroups = kSms * 4;     // blocks that leave column sums
+constexpr uint32_t kMaxGroups = kSms * 8;     // blocks that leave column sums
 
-template <typename T, typename P, int V, int NV, int TPR>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR)
-k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x,
-           int64_t ldx, const float* __restrict__ mean, const float* __restrict__ rstd,
+// Rows under way at once, in shared memory: enough of them to keep memory busy
+// beside one barrier a row. A thread reads what it copied itself. (Copies are
+// of 4 bytes at least; single 16-bit values go through registers, one row
+// ahead.)
+template <typename T, int V, int NV, int TPR>
+struct Ring {
+  static constexpr int piece = V * sizeof(T);
+  static constexpr bool on = piece >= 4;
+  static constexpr int block = TPR == 32 ? 256 : TPR;
+  static constexpr int row_bytes = 2 * NV * block * piece;
+  static constexpr int stages = !on ? 1 : row_bytes <= 16384 ? 4 : 3;
+  static constexpr int bytes = on ? stages * row_bytes : 0;
+};
+
+template <typename T, typename P, int V, int NV, int TPR, int EACH>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, EACH)
+k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x, int64_t ldx,
+           const float* __restrict__ mean, const float* __restrict__ rstd,
            const P* __restrict__ w, T* dx, int64_t lddx, float* __restrict__ partial) {
-  constexpr int ROWS = TPR == 32 ? 8 : 1;
-  __shared__ float red[4 * (TPR / 32)];
-  const uint32_t lane = threadIdx.x % TPR;
+  using R = Ring<T, V, NV, TPR>;
+  constexpr int ROWS = TPR == 32 ? 8 : 1, S = R::stages, BLOCK = R::block;
+  extern __shared__ uint4 ring_bytes[];
+  auto* ring = reinterpret_cast<Pack<T, V>*>(ring_bytes);  // [stage][x, dy][piece][thread]
+  __shared__ float red[4 * (TPR / 32)], stats[S][BLOCK / 32][2];
+  constexpr int E = NV * V, H = E / 2;  // a thread's columns, as H pairs
+  static_assert(E % 2 == 0, "columns in pairs");
+  const uint32_t lane = threadIdx.x % TPR, warp = threadIdx.x / 32, wl = threadIdx.x & 31;
   const uint32_t step = gridDim.x * ROWS;
   uint32_t r = blockIdx.x * ROWS + threadIdx.x / TPR;
-  float wv[NV][V], aw[NV][V], ab[NV][V];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const uint32_t i = (j * TPR + lane) * V;
-    Pack<P, V> pw;
-    if (w && i < n) pw = load_pack<P, V>(w + i);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      wv[j][e] = w && i < n ? to_f32(pw.v[e]) : 1.0f;
-      aw[j][e] = ab[j][e] = 0.0f;
-    }
-  }
+  auto slot = [&](uint32_t stage, int array, int j) {
+    return ring + ((stage * 2 + array) * NV + j) * BLOCK + threadIdx.x;
+  };
+  // Columns past the row's end: weight and values are 0 and stay so.
   Pack<T, V> qx[NV], qg[NV];
-  float mu = 0.0f, rs = 0.0f;
-  auto fetch = [&](uint32_t row) {
-    if (row >= rows) return;
+  F2 wv[H], aw[H], ab[H];
+  {
+    float f[E];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const uint32_t i = (j * TPR + lane) * V;
-      if (i < n) {
-        qx[j] = load_pack<T, V>(x + row * ldx + i);
-        qg[j] = load_pack<T, V>(dy + row * lddy + i);
+      Pack<P, V> pw;
+      if (w && i < n) pw = load_pack<P, V>(w + i);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[j * V + e] = i >= n ? 0.0f : w ? to_f32(pw.v[e]) : 1.0f;
+        qx[j].v[e] = qg[j].v[e] = from_f32<T>(0.0f);
+      }
+      if (R::on && i >= n)
+        for (int s = 0; s < S; ++s) *slot(s, 0, j) = *slot(s, 1, j) = qx[j];
+    }
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      wv[h] = pack2(f[2 * h], f[2 * h + 1]);
+      aw[h] = ab[h] = pack2(0.0f, 0.0f);
+    }
+  }
+  float mu = 0.0f, rs = 0.0f;
+  // Starts the loads of a row: into the ring, or into registers.
+  auto fetch = [&](uint64_t row, uint32_t stage) {
+    if (row < rows) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const uint32_t i = (j * TPR + lane) * V;
+        if (i >= n) continue;
+        if constexpr (R::on) {
+          copy_async<R::piece>(slot(stage, 0, j), x + row * ldx + i);
+          copy_async<R::piece>(slot(stage, 1, j), dy + row * lddy + i);
+        } else {
+          qx[j] = load_pack<T, V>(x + row * ldx + i);
+          qg[j] = load_pack<T, V>(dy + row * lddy + i);
+        }
+      }
+      if constexpr (R::on) {
+        if (wl < 2) copy_async<4>(&stats[stage][warp][wl], (wl ? rstd : mean) + row);
+      } else {
+        mu = mean[row];
+        rs = rstd[row];
       }
     }
-    mu = mean[row];
-    rs = rstd[row];
+    if (R::on) copy_commit();
   };
-  fetch(r);
+#pragma unroll
+  for (int s = 0; s < (R::on ? S - 1 : 1); ++s) fetch(r + (uint64_t)s * step, s);
   int turn = 0;
+  uint32_t stage = 0;
   const float inv_n = 1.0f / (float)n;
   // Rows of a block-wide row end for the whole block at once; those of a warp
   // for the warp (no barrier inside).
   for (; r < rows; r += step) {
-    Pack<T, V> cx[NV], cg[NV];
-    const float m = mu, s = rs;
+    float m, s, fx[E], fg[E];
+    if constexpr (R::on) {
+      fetch(r + (uint64_t)(S - 1) * step, stage == 0 ? S - 1 : stage - 1);
+      copy_wait<S - 1>();
+      __syncwarp();  // the statistics are two lanes' copies
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      cx[j] = qx[j];
-      cg[j] = qg[j];
+      for (int j = 0; j < NV; ++j) {
+        qx[j] = *slot(stage, 0, j);
+        qg[j] = *slot(stage, 1, j);
+      }
+      m = stats[stage][warp][0];
+      s = stats[stage][warp][1];
+      __syncwarp();
+      stage = stage == S - 1 ? 0 : stage + 1;
+    } else {
+      m = mu;
+      s = rs;
     }
-    fetch(r + step);
-    float c[2] = {0.0f, 0.0f};
+    widen<NV, V>(qx, fx);
+    widen<NV, V>(qg, fg);
+    if (!R::on) fetch((uint64_t)r + step, 0);
+    // With d = dy, t = d (x - mu): g = w d, g h = rstd w t, dy h = rstd t.
+    F2 xm[H], c0 = pack2(0.0f, 0.0f), c1 = c0;
+    const F2 minus = pack2(-m, -m), s2 = pack2(s, s);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if ((j * TPR + lane) * V < n)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float d = to_f32(cg[j].v[e]), h = (to_f32(cx[j].v[e]) - m) * s;
-          const float g = d * wv[j][e];
-          aw[j][e] = fmaf(d, h, aw[j][e]);
-          ab[j][e] += d;
-          c[0] += g;
-          c[1] = fmaf(g, h, c[1]);
-        }
+    for (int h = 0; h < H; ++h) {
+      const F2 d = pack2(fg[2 * h], fg[2 * h + 1]);
+      xm[h] = add2(pack2(fx[2 * h], fx[2 * h + 1]), minus);
+      const F2 t = mul2(d, xm[h]);
+      aw[h] = fma2(t, s2, aw[h]);
+      ab[h] = add2(d, ab[h]);
+      c0 = fma2(d, wv[h], c0);
+      c1 = fma2(t, wv[h], c1);
     }
     if (dx) {
-      row_sum<TPR>(c, red, turn);
-      c[0] *= inv_n;
-      c[1] *= inv_n;
+      const F2 c = row_sum2<TPR>(pack2(c0.x + c0.y, c1.x + c1.y), red, turn);
+      // dx = s g + ((x - mu) a + b), a = -s^2 mean(g h), b = -s mean g
+      const float a = -s * s * (c.y * s * inv_n), b = -s * (c.x * inv_n);
+      const F2 a2 = pack2(a, a), b2 = pack2(b, b);
+      float o[E];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const F2 g = mul2(pack2(fg[2 * h], fg[2 * h + 1]), wv[h]);
+        const F2 v = fma2(g, s2, fma2(xm[h], a2, b2));
+        o[2 * h] = v.x;
+        o[2 * h + 1] = v.y;
+      }
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const uint32_t i = (j * TPR + lane) * V;
         if (i < n) {
           Pack<T, V> out;
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float h = (to_f32(cx[j].v[e]) - m) * s;
-            out.v[e] = from_f32<T>(s * fmaf(-h, c[1], fmaf(to_f32(cg[j].v[e]), wv[j][e], -c[0])));
-          }
+          for (int e = 0; e < V; ++e) out.v[e] = from_f32<T>(o[j * V + e]);
           *reinterpret_cast<Pack<T, V>*>(dx + r * lddx + i) = out;
         }
       }
@@ -104,6 +169,10 @@ k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x,
   }
   if (!partial) return;
   float* out = partial + (uint64_t)blockIdx.x * 2 * n;
+  auto column = [&](int half, int e) {
+    const F2 v = half ? ab[e / 2] : aw[e / 2];
+    return e & 1 ? v.y : v.x;
+  };
   if constexpr (ROWS == 1) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -111,19 +180,20 @@ k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x,
       if (i < n)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          out[i + e] = aw[j][e];
-          out[n + i + e] = ab[j][e];
+          out[i + e] = column(0, j * V + e);
+          out[n + i + e] = column(1, j * V + e);
         }
     }
   } else {  // the eight warps' sums, added in their order
-    __shared__ float joined[8][32 * NV * V];
+    __shared__ float joined[8][32 * E];
+#pragma unroll
     for (int half = 0; half < 2; ++half) {
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          joined[threadIdx.x / 32][(j * 32 + lane) * V + e] = half ? ab[j][e] : aw[j][e];
+          joined[threadIdx.x / 32][(j * 32 + lane) * V + e] = column(half, j * V + e);
       __syncthreads();
       for (uint32_t i = threadIdx.x; i < n; i += 256) {
         float s = joined[0][i];
@@ -245,13 +315,22 @@ extern "C" int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
     auto go = [&](auto p) {
       using P = decltype(p);
       uint32_t groups = 0;
-      // `each` blocks an SM; a block visits rows of the same remainder.
-      auto launch = [&](auto kernel, uint32_t block, uint32_t per_block, uint32_t each) {
-        groups = (uint32_t)std::min<uint64_t>((rows + per_block - 1) / per_block, kSms * each);
-        if (groups == 0) return;
-        kernel<<<groups, block, 0, ctx->stream>>>((uint32_t)rows, n, (const T*)dy, lddy,
-                                                  (const T*)x, ldx, mean, rstd, (const P*)weight,
-                                                  (T*)dx, lddx, partial);
+      // EACH blocks an SM; a block visits rows of the same remainder.
+      auto launch = [&](auto nv_c, auto tpr_c, auto each_c, auto v_c) -> int {
+        constexpr int NV = decltype(nv_c)::value, TPR = decltype(tpr_c)::value;
+        constexpr int EACH = decltype(each_c)::value, VV = decltype(v_c)::value;
+        using R = Ring<T, VV, NV, TPR>;
+        auto* kernel = k_norm_bwd<T, P, VV, NV, TPR, EACH>;
+        const uint32_t per_block = TPR == 32 ? 8 : 1;
+        groups = (uint32_t)std::min<uint64_t>((rows + per_block - 1) / per_block, kSms * EACH);
+        if (groups == 0) return PLX_OK;
+        if (R::bytes > 32 * 1024)
+          PLX_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            R::bytes));
+        kernel<<<groups, R::block, R::bytes, ctx->stream>>>(
+            (uint32_t)rows, n, (const T*)dy, lddy, (const T*)x, ldx, mean, rstd, (const P*)weight,
+            (T*)dx, lddx, partial);
+        return PLX_OK;
       };
       auto loops = [&] {
         if (sums && rows) {
@@ -263,22 +342,39 @@ extern "C" int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
           k_norm_dx_long<T, P><<<(unsigned)rows, 1024, 0, ctx->stream>>>(
               n, (const T*)dy, lddy, (const T*)x, ldx, mean, rstd, (const P*)weight, (T*)dx, lddx);
       };
-      if (whole_pieces(n, sizeof(T), {dy, x, dx, weight}, {lddy, ldx, lddx})) {
+      using std::integral_constant;
+#define PLX_C(v) integral_constant<int, v>{}
+      int rc = PLX_OK;
+      const uint32_t v = piece_values(n, sizeof(T), {dy, x, dx}, {lddy, ldx, lddx}, weight,
+                                      nullptr, sizeof(P));
+      if (v == V) {
         const uint32_t pieces = n / V;
-        if (pieces <= 32) launch(k_norm_bwd<T, P, V, 1, 32>, 256, 8, 4);
-        else if (pieces <= 64) launch(k_norm_bwd<T, P, V, 2, 32>, 256, 8, 2);
-        else if (pieces <= 256) launch(k_norm_bwd<T, P, V, 2, 128>, 128, 1, 4);
-        else if (pieces <= 512) launch(k_norm_bwd<T, P, V, 2, 256>, 256, 1, 2);
-        else if (pieces <= 1024) launch(k_norm_bwd<T, P, V, 2, 512>, 512, 1, 1);
-        else if (pieces <= 2048) launch(k_norm_bwd<T, P, V, 2, 1024>, 1024, 1, 1);
+        if (pieces <= 32) rc = launch(PLX_C(1), PLX_C(32), PLX_C(4), PLX_C(V));
+        else if (pieces <= 64) rc = launch(PLX_C(2), PLX_C(32), PLX_C(2), PLX_C(V));
+        else if (pieces <= 128) rc = launch(PLX_C(1), PLX_C(128), PLX_C(8), PLX_C(V));
+        else if (pieces <= 256) rc = launch(PLX_C(2), PLX_C(128), PLX_C(4), PLX_C(V));
+        else if (pieces <= 512) rc = launch(PLX_C(2), PLX_C(256), PLX_C(2), PLX_C(V));
+        else if (pieces <= 1024) rc = launch(PLX_C(2), PLX_C(512), PLX_C(1), PLX_C(V));
+        else if (pieces <= 2048) rc = launch(PLX_C(2), PLX_C(1024), PLX_C(1), PLX_C(V));
         else loops();
-      } else if (n <= 128) launch(k_norm_bwd<T, P, 1, 4, 32>, 256, 8, 4);
-      else if (n <= 256) launch(k_norm_bwd<T, P, 1, 8, 32>, 256, 8, 4);
-      else if (n <= 1024) launch(k_norm_bwd<T, P, 1, 8, 128>, 128, 1, 4);
-      else if (n <= 2048) launch(k_norm_bwd<T, P, 1, 8, 256>, 256, 1, 4);
-      else if (n <= 4096) launch(k_norm_bwd<T, P, 1, 8, 512>, 512, 1, 2);
-      else if (n <= 8192) launch(k_norm_bwd<T, P, 1, 8, 1024>, 1024, 1, 1);
+      } else if (sizeof(T) == 2 && v >= 2) {
+        const uint32_t pieces = n / 2;
+        if (pieces <= 128) rc = launch(PLX_C(4), PLX_C(32), PLX_C(4), PLX_C(2));
+        else if (pieces <= 512) rc = launch(PLX_C(4), PLX_C(128), PLX_C(6), PLX_C(2));
+        else if (pieces <= 1024) rc = launch(PLX_C(4), PLX_C(256), PLX_C(3), PLX_C(2));
+        else if (pieces <= 2048) rc = launch(PLX_C(4), PLX_C(512), PLX_C(2), PLX_C(2));
+        else if (pieces <= 4096) rc = launch(PLX_C(4), PLX_C(1024), PLX_C(1), PLX_C(2));
+        else loops();
+      } else if (n <= 128) rc = launch(PLX_C(4), PLX_C(32), PLX_C(4), PLX_C(1));
+      else if (n <= 256) rc = launch(PLX_C(8), PLX_C(32), PLX_C(4), PLX_C(1));
+      else if (n <= 1024) rc = launch(PLX_C(8), PLX_C(128), PLX_C(6), PLX_C(1));
+      else if (n <= 2048) rc = launch(PLX_C(8), PLX_C(256), PLX_C(3), PLX_C(1));
+      else if (n <= 4096) rc = launch(PLX_C(8), PLX_C(512), PLX_C(2), PLX_C(1));
+      else if (n <= 5120) rc = launch(PLX_C(10), PLX_C(512), PLX_C(2), PLX_C(1));
+      else if (n <= 8192) rc = launch(PLX_C(8), PLX_C(1024), PLX_C(1), PLX_C(1));
       else loops();
+#undef PLX_C
+      if (rc != PLX_OK) return rc;
       PLX_LAUNCH_CHECK("k_norm_bwd");
       if (sums) {
         k_norm_join<P><<<(unsigned)((2ull * n + 31) / 32), 1024, 0, ctx->stream>>>(

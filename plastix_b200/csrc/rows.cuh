@@ -44,6 +44,17 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int d = 16; d; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, d));
   return v;
 }
+// ---- two 32-bit values at once (one instruction each) ----------------------
+using F2 = float2;
+__device__ __forceinline__ F2 pack2(float a, float b) { return make_float2(a, b); }
+__device__ __forceinline__ void unpack2(F2 v, float& a, float& b) {
+  a = v.x;
+  b = v.y;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { return __ffma2_rn(a, b, c); }
+
 // NaN wins, as in the arithmetic that follows it.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -80,6 +91,23 @@ __device__ __forceinline__ float block_max(float v, float* red) {
 #pragma unroll
   for (int w = 1; w < WARPS; ++w) s = max_nan(s, red[w]);
   return s;
+}
+
+// From global to shared memory without a register in between.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst_smem, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst_smem)), "l"(src)
+                 : "memory");
+  else  // 4 or 8
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_addr(dst_smem)), "l"(src),
+                 "n"(BYTES)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // 2^x by the special-function unit (relative error about 2^-22; 0 for
