@@ -215,24 +215,24 @@ extern "C" int plx_distill(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, c
     uint32_t parts = row_parts(rows, n);
     if (dlogits)
       while (parts < 8 && (uint64_t)n * sizeof(T) > (uint64_t)parts * 2 * kKeepBytes) parts *= 2;
-    auto go = [&](auto kernel, uint32_t threads) {
+    auto go = [&](auto threads_c) {
+      constexpr int THREADS = decltype(threads_c)::value;
+      constexpr auto kernel = k_distill<T, THREADS>;
       uint32_t pieces = 0;
       if (dlogits) {
         pieces = std::min<uint32_t>((n + parts - 1) / parts / V + 1, kKeepBytes / 16);
-        if (pieces * 16 > 47 * 1024)
-          PLX_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            kKeepBytes));
+        if (pieces * 16 > 47 * 1024) PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, kKeepBytes));
       }
-      PLX_TRY_CUDA(launch_rows(kernel, rows, parts, threads + 32, (size_t)pieces * 16, ctx->stream, n,
-                               part_length(n, parts, V), (const T*)logits, ld, k, teacher_ids, teacher_values, teacher_kind,
-                               temperature, 1.0f / temperature, row_weight, loss, (T*)dlogits, ldd,
-                               pieces, ctx->d_status));
+      PLX_TRY_CUDA(launch_rows(kernel, rows, parts, THREADS + 32, (size_t)pieces * 16, ctx->stream,
+                               n, part_length(n, parts, V), (const T*)logits, ld, k, teacher_ids,
+                               teacher_values, teacher_kind, temperature, 1.0f / temperature,
+                               row_weight, loss, (T*)dlogits, ldd, pieces, ctx->d_status));
       return PLX_OK;
     };
     switch (row_threads(n / parts)) {
-      case 64: return go(k_distill<T, 64>, 64);
-      case 128: return go(k_distill<T, 128>, 128);
-      default: return go(k_distill<T, 256>, 256);
+      case 64: return go(std::integral_constant<int, 64>{});
+      case 128: return go(std::integral_constant<int, 128>{});
+      default: return go(std::integral_constant<int, 256>{});
     }
   });
 }

@@ -320,13 +320,12 @@ extern "C" int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
         constexpr int NV = decltype(nv_c)::value, TPR = decltype(tpr_c)::value;
         constexpr int EACH = decltype(each_c)::value, VV = decltype(v_c)::value;
         using R = Ring<T, VV, NV, TPR>;
-        auto* kernel = k_norm_bwd<T, P, VV, NV, TPR, EACH>;
+        constexpr auto kernel = k_norm_bwd<T, P, VV, NV, TPR, EACH>;
         const uint32_t per_block = TPR == 32 ? 8 : 1;
         groups = (uint32_t)std::min<uint64_t>((rows + per_block - 1) / per_block, kSms * EACH);
         if (groups == 0) return PLX_OK;
         if (R::bytes > 32 * 1024)
-          PLX_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            R::bytes));
+          PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, R::bytes));
         kernel<<<groups, R::block, R::bytes, ctx->stream>>>(
             (uint32_t)rows, n, (const T*)dy, lddy, (const T*)x, ldx, mean, rstd, (const P*)weight,
             (T*)dx, lddx, partial);

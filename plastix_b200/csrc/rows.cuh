@@ -2,6 +2,8 @@
 // 16-byte row access and block-wide reductions in a fixed order.
 #pragma once
 
+#include <atomic>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -120,6 +122,19 @@ __device__ __forceinline__ float exp2_approx(float x) {
 constexpr float kLog2e = 1.4426950408889634f;
 
 }  // namespace plx
+
+// Lets a kernel use `bytes` of dynamic shared memory, asking the driver once a
+// device. `KERNEL` makes the memory of that the kernel's own.
+template <auto KERNEL>
+cudaError_t allow_shared(int device, int bytes) {
+  static std::atomic<uint64_t> asked{0};
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (asked.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  const cudaError_t e =
+      cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 // Makes a context's device current for one call and puts the caller's back.
 struct DeviceGuard {

@@ -40,35 +40,40 @@ class LogProbs(NamedTuple):
 
 
 def _rows(ctx: Context, t: torch.Tensor, name: str):
-    """(rows, n, row stride) of a tensor of rows on the context's device."""
+    """(rows, n, row stride, type number) of a tensor of rows on the context's
+    device."""
     if t.device != ctx.device:
         raise ValueError(f"{name} is on {t.device}, the context on {ctx.device}")
-    if t.dtype not in _TYPES:
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
         raise ValueError(f"{name} is {t.dtype}: float32, bfloat16 and float16 are supported")
-    if t.dim() == 0 or t.shape[-1] == 0:
-        raise ValueError(f"{name} needs a last dimension of units, got shape {tuple(t.shape)}")
-    n = t.shape[-1]
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) == 0 or shape[-1] == 0:
+        raise ValueError(f"{name} needs a last dimension of units, got shape {tuple(shape)}")
+    n = shape[-1]
+    if len(shape) != 2:
         try:
             t = t.view(-1, n) if t.numel() else t.reshape(-1, n)
         except RuntimeError:
             raise ValueError(f"the dimensions of {name} before the last do not collapse into "
                              f"rows of one stride (strides {t.stride()})") from None
-    rows, ld = t.shape[0], t.stride(0)
-    if n > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name} needs a stride of 1 in its last dimension, got {t.stride(1)}")
+        shape = t.shape
+    rows = shape[0]
+    ld, one = t.stride()
+    if one != 1 and n > 1:
+        raise ValueError(f"{name} needs a stride of 1 in its last dimension, got {one}")
     if rows <= 1:
         ld = n
     elif ld < n:
         raise ValueError(f"the rows of {name} overlap (row stride {ld}, {n} units)")
-    return rows, n, ld
+    return rows, n, ld, kind
 
 
 def _like(ctx: Context, t: torch.Tensor, shape, dtype, name: str) -> int:
     """Address of a contiguous tensor of the given shape and type."""
-    if t.device != ctx.device:
-        raise ValueError(f"{name} is on {t.device}, the context on {ctx.device}")
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or t.device != ctx.device or not t.is_contiguous():
+        if t.device != ctx.device:
+            raise ValueError(f"{name} is on {t.device}, the context on {ctx.device}")
         raise ValueError(f"{name} has to be a contiguous {dtype} tensor of shape {tuple(shape)}, "
                          f"got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
@@ -78,12 +83,14 @@ def _result(ctx: Context, out: Optional[torch.Tensor], source: torch.Tensor, ld:
     """The tensor of rows that a call writes, and its row stride: ``out``, or
     a new one like ``source``. ``out`` may be the source itself."""
     if out is None:
-        return source.new_empty(source.shape), source.shape[-1]
+        return (torch.empty_like(source) if source.is_contiguous() else
+                source.new_empty(source.shape)), source.shape[-1]
     if out.shape != source.shape or out.dtype != source.dtype:
         raise ValueError(f"{name} has to be {source.dtype} {tuple(source.shape)}, got {out.dtype} "
                          f"{tuple(out.shape)}")
     ldo = _rows(ctx, out, name)[2]
-    if (out.untyped_storage().data_ptr() == source.untyped_storage().data_ptr()
+    if (out is not source
+            and out.untyped_storage().data_ptr() == source.untyped_storage().data_ptr()
             and not (out.data_ptr() == source.data_ptr() and ldo == ld)):
         raise ValueError(f"{name} shares memory with the input and is not the input itself")
     return out, ldo
@@ -106,17 +113,12 @@ def _address(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _param(ctx: Context, t: Optional[torch.Tensor], n: int, x: torch.Tensor, other, name: str):
-    """The type number of an affine parameter (None: that of ``other``)."""
-    if t is None:
-        return other
-    if t.dtype != torch.float32 and t.dtype != x.dtype:
-        raise ValueError(f"{name} is {t.dtype}: float32 or the rows' {x.dtype} is supported")
+def _param(ctx: Context, t: torch.Tensor, n: int, dtype, name: str) -> int:
+    """The type number of an affine parameter of rows of the given type."""
+    if t.dtype != torch.float32 and t.dtype != dtype:
+        raise ValueError(f"{name} is {t.dtype}: float32 or the rows' {dtype} is supported")
     _like(ctx, t, (n,), t.dtype, name)
-    kind = _TYPES[t.dtype]
-    if other is not None and other != kind:
-        raise ValueError("weight and bias have different types")
-    return kind
+    return _TYPES[t.dtype]
 
 
 def layer_norm(ctx: Context, x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -125,17 +127,23 @@ def layer_norm(ctx: Context, x: torch.Tensor, weight: Optional[torch.Tensor] = N
     """Rows of ``x`` with mean 0 and variance 1 (plus ``eps``), times
     ``weight`` plus ``bias`` ([n], float32 or x's type). With ``stats`` returns
     (y, mean, rstd), which ``layer_norm_backward`` takes. ``out`` may be x."""
-    rows, n, ld = _rows(ctx, x, "x")
-    kind = _param(ctx, bias, n, x, _param(ctx, weight, n, x, None, "weight"), "bias")
+    rows, n, ld, dtype = _rows(ctx, x, "x")
+    kind = _abi.F32
+    if bias is not None:
+        kind = _param(ctx, bias, n, x.dtype, "bias")
+    if weight is not None:
+        other, kind = kind, _param(ctx, weight, n, x.dtype, "weight")
+        if bias is not None and other != kind:
+            raise ValueError("weight and bias have different types")
     with _scope(ctx, x, weight, bias, out):
         y, ldy = _result(ctx, out, x, ld, "out")
         mean = rstd = None
         if stats:
             mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
-            rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
-        _abi.call("plx_layer_norm", ctx.handle, rows, n, _TYPES[x.dtype], x.data_ptr(), ld,
-                  _abi.F32 if kind is None else kind, _address(weight), _address(bias), eps,
-                  y.data_ptr(), ldy, _address(mean), _address(rstd))
+            rstd = torch.empty_like(mean)
+        _abi.call("plx_layer_norm", ctx.handle, rows, n, dtype, x.data_ptr(), ld, kind,
+                  _address(weight), _address(bias), eps, y.data_ptr(), ldy, _address(mean),
+                  _address(rstd))
     return (y, mean, rstd) if stats else y
 
 
@@ -145,7 +153,7 @@ def layer_norm_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, mean: t
     """(dx, dweight, dbias) for the rows and statistics of ``layer_norm``;
     dweight and dbias have weight's type and are None without a weight. The
     same bits on every call. ``out`` (for dx) may be dy."""
-    rows, n, ld = _rows(ctx, x, "x")
+    rows, n, ld, dtype = _rows(ctx, x, "x")
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError(f"dy has to be {x.dtype} {tuple(x.shape)}, got {dy.dtype} "
                          f"{tuple(dy.shape)}")
@@ -153,19 +161,18 @@ def layer_norm_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, mean: t
     lead = x.shape[:-1]
     mean_p = _like(ctx, mean, lead, torch.float32, "mean")
     rstd_p = _like(ctx, rstd, lead, torch.float32, "rstd")
-    kind = _param(ctx, weight, n, x, None, "weight")
+    kind = _abi.F32 if weight is None else _param(ctx, weight, n, x.dtype, "weight")
     with _scope(ctx, dy, x, mean, rstd, weight, out):
         dx, lddx = _result(ctx, out, dy, lddy, "out")
         dw = db = scratch = None
         size = 0
         if weight is not None:
-            dw, db = weight.new_empty(n), weight.new_empty(n)
+            dw, db = torch.empty_like(weight), torch.empty_like(weight)
             size = _abi.lib().plx_layer_norm_scratch_bytes(rows, n)
             scratch = x.new_empty(size, dtype=torch.uint8)
-        _abi.call("plx_layer_norm_backward", ctx.handle, rows, n, _TYPES[x.dtype], dy.data_ptr(),
-                  lddy, x.data_ptr(), ld, mean_p, rstd_p, _abi.F32 if kind is None else kind,
-                  _address(weight), dx.data_ptr(), lddx, _address(dw), _address(db),
-                  _address(scratch), size)
+        _abi.call("plx_layer_norm_backward", ctx.handle, rows, n, dtype, dy.data_ptr(), lddy,
+                  x.data_ptr(), ld, mean_p, rstd_p, kind, _address(weight), dx.data_ptr(), lddx,
+                  _address(dw), _address(db), _address(scratch), size)
     return dx, dw, db
 
 
@@ -174,19 +181,19 @@ def log_probs(ctx: Context, logits: torch.Tensor, target: Optional[torch.Tensor]
     """Softmax of ``scale * logits`` in each row: log probability of
     ``target`` (int32, -1 = none), entropy, and the ``top`` best alternatives
     with theirs. See plx_log_probs for masked and non-finite rows."""
-    rows, n, ld = _rows(ctx, logits, "logits")
+    rows, n, ld, dtype = _rows(ctx, logits, "logits")
     lead = logits.shape[:-1]
     target_p = None if target is None else _like(ctx, target, lead, torch.int32, "target")
     with _scope(ctx, logits, target):
         lse = logits.new_empty(lead, dtype=torch.float32)
-        logp = None if target is None else logits.new_empty(lead, dtype=torch.float32)
-        ent = logits.new_empty(lead, dtype=torch.float32) if entropy else None
+        logp = None if target is None else torch.empty_like(lse)
+        ent = torch.empty_like(lse) if entropy else None
         ids = best = None
         if top:
             ids = logits.new_empty(lead + (top,), dtype=torch.int32)
-            best = logits.new_empty(lead + (top,), dtype=torch.float32)
-        _abi.call("plx_log_probs", ctx.handle, rows, n, _TYPES[logits.dtype], logits.data_ptr(),
-                  ld, target_p, scale, top, _address(logp), lse.data_ptr(), _address(ent),
+            best = torch.empty_like(ids, dtype=torch.float32)
+        _abi.call("plx_log_probs", ctx.handle, rows, n, dtype, logits.data_ptr(), ld,
+                  target_p, scale, top, _address(logp), lse.data_ptr(), _address(ent),
                   _address(ids), _address(best))
     return LogProbs(logp, lse, ent, ids, best)
 
@@ -200,15 +207,17 @@ def log_probs_backward(ctx: Context, logits: torch.Tensor, lse: torch.Tensor,
     """Gradient of sum(grad_logp * logp) + sum(grad_entropy * entropy) with
     respect to the logits; lse and entropy as ``log_probs`` returned them for
     the same logits and scale. ``out`` may be logits."""
-    rows, n, ld = _rows(ctx, logits, "logits")
+    rows, n, ld, dtype = _rows(ctx, logits, "logits")
     lead = logits.shape[:-1]
     lse_p = _like(ctx, lse, lead, torch.float32, "lse")
     if target is not None:
         _like(ctx, target, lead, torch.int32, "target")
-    for t, name in ((grad_logp, "grad_logp"), (entropy, "entropy"),
-                    (grad_entropy, "grad_entropy")):
-        if t is not None:
-            _like(ctx, t, lead, torch.float32, name)
+    if grad_logp is not None:
+        _like(ctx, grad_logp, lead, torch.float32, "grad_logp")
+    if entropy is not None:
+        _like(ctx, entropy, lead, torch.float32, "entropy")
+    if grad_entropy is not None:
+        _like(ctx, grad_entropy, lead, torch.float32, "grad_entropy")
     if grad_logp is None and grad_entropy is None:
         raise ValueError("grad_logp or grad_entropy is required")
     if grad_logp is not None and target is None:
@@ -217,8 +226,8 @@ def log_probs_backward(ctx: Context, logits: torch.Tensor, lse: torch.Tensor,
         raise ValueError("grad_entropy needs entropy")
     with _scope(ctx, logits, lse, target, grad_logp, entropy, grad_entropy, out):
         dx, ldd = _result(ctx, out, logits, ld, "out")
-        _abi.call("plx_log_probs_backward", ctx.handle, rows, n, _TYPES[logits.dtype],
-                  logits.data_ptr(), ld, _address(target), scale, lse_p, _address(entropy),
+        _abi.call("plx_log_probs_backward", ctx.handle, rows, n, dtype, logits.data_ptr(), ld,
+                  _address(target), scale, lse_p, _address(entropy),
                   _address(grad_logp), _address(grad_entropy), dx.data_ptr(), ldd)
     return dx
 
@@ -233,7 +242,7 @@ def distill(ctx: Context, logits: torch.Tensor, teacher_ids: torch.Tensor,
     temperature), and the gradient of its sum over the rows (None without
     ``grad``). ``kind``: what the values are, the teacher's "logits" or its
     "log_probs" at this temperature. ``out`` (for dlogits) may be logits."""
-    rows, n, ld = _rows(ctx, logits, "logits")
+    rows, n, ld, dtype = _rows(ctx, logits, "logits")
     lead = logits.shape[:-1]
     if kind not in _KINDS:
         raise ValueError(f"kind {kind!r} is neither 'logits' nor 'log_probs'")
@@ -247,9 +256,9 @@ def distill(ctx: Context, logits: torch.Tensor, teacher_ids: torch.Tensor,
     if out is not None and not grad:
         raise ValueError("out is for the gradient: it needs grad=True")
     with _scope(ctx, logits, teacher_ids, teacher_values, weight, out):
-        loss = logits.new_empty(lead, dtype=torch.float32)
+        loss = teacher_values.new_empty(lead)
         dx, ldd = _result(ctx, out, logits, ld, "out") if grad else (None, 0)
-        _abi.call("plx_distill", ctx.handle, rows, n, _TYPES[logits.dtype], logits.data_ptr(), ld,
+        _abi.call("plx_distill", ctx.handle, rows, n, dtype, logits.data_ptr(), ld,
                   k, ids_p, values_p, _KINDS[kind], temperature, _address(weight),
                   loss.data_ptr(), _address(dx), ldd)
     return loss, dx
