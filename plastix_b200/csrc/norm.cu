@@ -27,15 +27,27 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
   constexpr int E = NV * V, H = E / 2;  // a thread's columns, as H pairs
   static_assert(E % 2 == 0, "columns in pairs");
   Pack<T, V> q[NV];
+  if constexpr (V * sizeof(T) >= 4) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const uint32_t i = (j * TPR + lane) * V;
-    if (i < n) {
-      q[j] = load_pack<T, V>(xr + i);
-    } else {
+    for (int j = 0; j < NV; ++j) {
+      const uint32_t i = (j * TPR + lane) * V;
+      if (i < n) {
+        q[j] = load_pack<T, V>(xr + i);
+      } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) q[j].v[e] = from_f32<T>(0.0f);
+        for (int e = 0; e < V; ++e) q[j].v[e] = from_f32<T>(0.0f);
+      }
     }
+  } else {
+    using St = Staged<T, TPR, NV>;
+    __shared__ uint4 stage[ROWS * St::bytes / 16];
+    char* at = reinterpret_cast<char*>(stage) + threadIdx.x / TPR * St::bytes;
+    St::fetch(at, xr, n, lane, r == 0, r == rows - 1);
+    copy_commit();
+    copy_wait<0>();
+    if (TPR == 32) __syncwarp();
+    else __syncthreads();
+    St::read(at, xr, n, lane, q);
   }
   float f[E];
   widen<NV, V>(q, f);
@@ -193,8 +205,10 @@ extern "C" int plx_layer_norm(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype
       } else if (n <= 128) launch(k_norm<T, P, 1, 4, 32>, eighth, 256);
       else if (n <= 256) launch(k_norm<T, P, 1, 8, 32>, eighth, 256);
       else if (n <= 1024) launch(k_norm<T, P, 1, 8, 128>, one, 128);
-      else if (n <= 2048) launch(k_norm<T, P, 1, 16, 128>, one, 128);
-      else if (n <= 4096) launch(k_norm<T, P, 1, 16, 256>, one, 256);
+      else if (n <= 2048) launch(k_norm<T, P, 1, 8, 256>, one, 256);
+      else if (n <= 2560) launch(k_norm<T, P, 1, 10, 256>, one, 256);
+      else if (n <= 4096) launch(k_norm<T, P, 1, 8, 512>, one, 512);
+      else if (n <= 5120) launch(k_norm<T, P, 1, 10, 512>, one, 512);
       else if (n <= 8192) launch(k_norm<T, P, 1, 16, 512>, one, 512);
       else loops();
       PLX_LAUNCH_CHECK("k_norm");

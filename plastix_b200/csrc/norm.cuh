@@ -26,6 +26,47 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   return *reinterpret_cast<const Pack<T, V>*>(p);
 }
 
+// Rows of 16-bit values of which not even two can be read together: sixteen-byte
+// chunks go to shared memory whole and the values are read from there. A
+// chunk's bytes outside its row are of the rows beside it; those before the
+// first row and behind the last are not touched.
+template <typename T, int TPR, int NV>
+struct Staged {
+  static_assert(sizeof(T) == 2, "for 16-bit values");
+  static constexpr int bytes = (TPR * NV * 2 + 31) / 16 * 16;  // a row, at any offset
+
+  static __device__ __forceinline__ uint32_t offset(const T* row) {
+    return (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15u);
+  }
+  // Starts the copies of this thread's chunks of a row.
+  static __device__ __forceinline__ void fetch(char* to, const T* row, uint32_t n, uint32_t lane,
+                                               bool first, bool last) {
+    const uint32_t off = offset(row), end = off + 2 * n;
+    const char* from = reinterpret_cast<const char*>(row) - off;
+    for (uint32_t c = lane * 16; c < end; c += TPR * 16) {
+      if (c == 0 && off && first) {
+        for (uint32_t e = off; e < min(end, 16u); e += 2)
+          *reinterpret_cast<T*>(to + e) = *reinterpret_cast<const T*>(from + e);
+      } else {
+        const uint32_t have = last ? min(16u, end - c) : 16u;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(to + c)),
+                     "l"(from + c), "r"(have)
+                     : "memory");
+      }
+    }
+  }
+  // This thread's values (0 past the row's end).
+  static __device__ __forceinline__ void read(const char* at, const T* row, uint32_t n,
+                                              uint32_t lane, Pack<T, 1> (&q)[NV]) {
+    const T* v = reinterpret_cast<const T*>(at + offset(row));
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const uint32_t i = j * TPR + lane;
+      q[j].v[0] = i < n ? v[i] : from_f32<T>(0.0f);
+    }
+  }
+};
+
 // Sum over the TPR threads that share a row, the same in each of them. `red`
 // holds two halves used in turn, so one barrier a sum is enough.
 template <int TPR, int K>

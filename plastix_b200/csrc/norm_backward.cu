@@ -20,17 +20,18 @@ constexpr uint32_t kSms = 148;                // of a B200; fixes the order of t
 constexpr uint32_t kMaxGroups = kSms * 8;     // blocks that leave column sums
 
 // Rows under way at once, in shared memory: enough of them to keep memory busy
-// beside one barrier a row. A thread reads what it copied itself. (Copies are
-// of 4 bytes at least; single 16-bit values go through registers, one row
-// ahead.)
+// beside one barrier a row. A thread reads what it copied itself, except where
+// the values are too small for that (staged).
 template <typename T, int V, int NV, int TPR>
 struct Ring {
   static constexpr int piece = V * sizeof(T);
-  static constexpr bool on = piece >= 4;
+  static constexpr bool staged = piece < 4;
   static constexpr int block = TPR == 32 ? 256 : TPR;
-  static constexpr int row_bytes = 2 * NV * block * piece;
-  static constexpr int stages = !on ? 1 : row_bytes <= 16384 ? 4 : 3;
-  static constexpr int bytes = on ? stages * row_bytes : 0;
+  static constexpr int array_bytes =
+      staged ? (TPR * NV * 2 + 31) / 16 * 16 * (block / TPR) : NV * block * piece;
+  static constexpr int stage_bytes = 2 * array_bytes;  // x, dy
+  static constexpr int stages = stage_bytes <= 17408 ? 4 : 3;
+  static constexpr int bytes = stages * stage_bytes;
 };
 
 template <typename T, typename P, int V, int NV, int TPR, int EACH>
@@ -40,16 +41,25 @@ k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x, int
            const P* __restrict__ w, T* dx, int64_t lddx, float* __restrict__ partial) {
   using R = Ring<T, V, NV, TPR>;
   constexpr int ROWS = TPR == 32 ? 8 : 1, S = R::stages, BLOCK = R::block;
-  extern __shared__ uint4 ring_bytes[];
-  auto* ring = reinterpret_cast<Pack<T, V>*>(ring_bytes);  // [stage][x, dy][piece][thread]
+  extern __shared__ uint4 ring_bytes[];  // [stage][x, dy]
+  char* ring = reinterpret_cast<char*>(ring_bytes);
   __shared__ float red[4 * (TPR / 32)], stats[S][BLOCK / 32][2];
   constexpr int E = NV * V, H = E / 2;  // a thread's columns, as H pairs
   static_assert(E % 2 == 0, "columns in pairs");
   const uint32_t lane = threadIdx.x % TPR, warp = threadIdx.x / 32, wl = threadIdx.x & 31;
   const uint32_t step = gridDim.x * ROWS;
   uint32_t r = blockIdx.x * ROWS + threadIdx.x / TPR;
-  auto slot = [&](uint32_t stage, int array, int j) {
-    return ring + ((stage * 2 + array) * NV + j) * BLOCK + threadIdx.x;
+  auto slot = [&](uint32_t stage, int array, int j) {  // a piece of this thread's
+    char* at = ring + stage * R::stage_bytes + array * R::array_bytes;
+    return reinterpret_cast<Pack<T, V>*>(at) + j * BLOCK + threadIdx.x;
+  };
+  auto staged_row = [&](uint32_t stage, int array) {  // or the row that it shares
+    return ring + stage * R::stage_bytes + array * R::array_bytes +
+           threadIdx.x / TPR * (R::array_bytes / ROWS);
+  };
+  auto rows_barrier = [] {
+    if (TPR == 32) __syncwarp();
+    else __syncthreads();
   };
   // Columns past the row's end: weight and values are 0 and stay so.
   Pack<T, V> qx[NV], qg[NV];
@@ -66,7 +76,7 @@ k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x, int
         f[j * V + e] = i >= n ? 0.0f : w ? to_f32(pw.v[e]) : 1.0f;
         qx[j].v[e] = qg[j].v[e] = from_f32<T>(0.0f);
       }
-      if (R::on && i >= n)
+      if (!R::staged && i >= n)
         for (int s = 0; s < S; ++s) *slot(s, 0, j) = *slot(s, 1, j) = qx[j];
     }
 #pragma unroll
@@ -75,60 +85,56 @@ k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x, int
       aw[h] = ab[h] = pack2(0.0f, 0.0f);
     }
   }
-  float mu = 0.0f, rs = 0.0f;
-  // Starts the loads of a row: into the ring, or into registers.
+  // Starts the copies of a row.
   auto fetch = [&](uint64_t row, uint32_t stage) {
     if (row < rows) {
+      const T *xr = x + row * ldx, *gr = dy + row * lddy;
+      if constexpr (R::staged) {
+        const bool one = row == 0, end = row == rows - 1;
+        Staged<T, TPR, NV>::fetch(staged_row(stage, 0), xr, n, lane, one, end);
+        Staged<T, TPR, NV>::fetch(staged_row(stage, 1), gr, n, lane, one, end);
+      } else {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const uint32_t i = (j * TPR + lane) * V;
-        if (i >= n) continue;
-        if constexpr (R::on) {
-          copy_async<R::piece>(slot(stage, 0, j), x + row * ldx + i);
-          copy_async<R::piece>(slot(stage, 1, j), dy + row * lddy + i);
-        } else {
-          qx[j] = load_pack<T, V>(x + row * ldx + i);
-          qg[j] = load_pack<T, V>(dy + row * lddy + i);
+        for (int j = 0; j < NV; ++j) {
+          const uint32_t i = (j * TPR + lane) * V;
+          if (i >= n) continue;
+          copy_async<R::piece>(slot(stage, 0, j), xr + i);
+          copy_async<R::piece>(slot(stage, 1, j), gr + i);
         }
       }
-      if constexpr (R::on) {
-        if (wl < 2) copy_async<4>(&stats[stage][warp][wl], (wl ? rstd : mean) + row);
-      } else {
-        mu = mean[row];
-        rs = rstd[row];
-      }
+      if (wl < 2) copy_async<4>(&stats[stage][warp][wl], (wl ? rstd : mean) + row);
     }
-    if (R::on) copy_commit();
+    copy_commit();
   };
 #pragma unroll
-  for (int s = 0; s < (R::on ? S - 1 : 1); ++s) fetch(r + (uint64_t)s * step, s);
+  for (int s = 0; s < S - 1; ++s) fetch(r + (uint64_t)s * step, s);
   int turn = 0;
   uint32_t stage = 0;
   const float inv_n = 1.0f / (float)n;
   // Rows of a block-wide row end for the whole block at once; those of a warp
   // for the warp (no barrier inside).
   for (; r < rows; r += step) {
-    float m, s, fx[E], fg[E];
-    if constexpr (R::on) {
-      fetch(r + (uint64_t)(S - 1) * step, stage == 0 ? S - 1 : stage - 1);
-      copy_wait<S - 1>();
-      __syncwarp();  // the statistics are two lanes' copies
+    float fx[E], fg[E];
+    copy_wait<S - 2>();
+    // Staged rows are everybody's, the statistics two lanes' of every warp; and
+    // what is written next has been read by all.
+    if (R::staged) rows_barrier();
+    else __syncwarp();
+    fetch(r + (uint64_t)(S - 1) * step, stage == 0 ? S - 1 : stage - 1);
+    if constexpr (R::staged) {
+      Staged<T, TPR, NV>::read(staged_row(stage, 0), x + (int64_t)r * ldx, n, lane, qx);
+      Staged<T, TPR, NV>::read(staged_row(stage, 1), dy + (int64_t)r * lddy, n, lane, qg);
+    } else {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         qx[j] = *slot(stage, 0, j);
         qg[j] = *slot(stage, 1, j);
       }
-      m = stats[stage][warp][0];
-      s = stats[stage][warp][1];
-      __syncwarp();
-      stage = stage == S - 1 ? 0 : stage + 1;
-    } else {
-      m = mu;
-      s = rs;
     }
+    const float m = stats[stage][warp][0], s = stats[stage][warp][1];
+    stage = stage == S - 1 ? 0 : stage + 1;
     widen<NV, V>(qx, fx);
     widen<NV, V>(qg, fg);
-    if (!R::on) fetch((uint64_t)r + step, 0);
     // With d = dy, t = d (x - mu): g = w d, g h = rstd w t, dy h = rstd t.
     F2 xm[H], c0 = pack2(0.0f, 0.0f), c1 = c0;
     const F2 minus = pack2(-m, -m), s2 = pack2(s, s);
