@@ -204,6 +204,8 @@ extern "C" int plx_distill(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, c
                 "teacher_ids, teacher_values and loss are required");
   PLX_CHECK_ARG(!dlogits || rows == 1 || ldd >= (int64_t)n,
                 "the gradient's row stride is less than n");
+  if (int rc = check_aligned(dtype_bytes(dtype), {dlogits})) return rc;
+  if (int rc = check_aligned(4, {teacher_ids, teacher_values, row_weight, loss})) return rc;
   DeviceGuard guard(ctx->device);
   PLX_TRY_CUDA(guard.err);
   if (rows == 1) ld = ldd = 0;

@@ -368,7 +368,7 @@ inline int check_logits(const plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype
   PLX_CHECK_ARG(rows == 0 || logits, "logits is required");
   PLX_CHECK_ARG(rows <= 1 || ld >= (int64_t)n, "the logits' row stride %lld is less than n",
                 (long long)ld);
-  return PLX_OK;
+  return check_aligned(dtype_bytes(dtype), {logits});
 }
 
 // Threads that go over a row (part) of n values: 256, or fewer where each would

@@ -6,7 +6,6 @@
 // Bound by memory (each value read once, written once): a row is held in
 // registers by the threads that share it, a warp for rows of up to 128
 // sixteen-byte pieces (no barrier), a block of 128 to 1,024 threads above.
-#include <initializer_list>
 
 #include "norm.cuh"
 
@@ -164,6 +163,9 @@ extern "C" int plx_layer_norm(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype
   PLX_CHECK_ARG(x && y, "x and y are required");
   PLX_CHECK_ARG(ldx >= (int64_t)n || rows == 1, "ldx = %lld is less than n", (long long)ldx);
   PLX_CHECK_ARG(ldy >= (int64_t)n || rows == 1, "ldy = %lld is less than n", (long long)ldy);
+  if (int rc = check_aligned(dtype_bytes(dtype), {x, y})) return rc;
+  if (int rc = check_aligned(dtype_bytes(param_dtype), {weight, bias})) return rc;
+  if (int rc = check_aligned(4, {mean, rstd})) return rc;
   DeviceGuard guard(ctx->device);
   PLX_TRY_CUDA(guard.err);
   if (rows == 1) ldx = ldy = 0;

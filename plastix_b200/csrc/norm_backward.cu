@@ -8,7 +8,6 @@
 // next rows are on their way into shared memory. Blocks leave
 // their sums in scratch and a second kernel adds them in a fixed order: no
 // atomics, the same bits on every call.
-#include <initializer_list>
 #include <type_traits>
 
 #include "norm.cuh"
@@ -17,7 +16,9 @@ namespace plx {
 namespace {
 
 constexpr uint32_t kSms = 148;                // of a B200; fixes the order of the sums
-constexpr uint32_t kMaxGroups = kSms * 8;     // blocks that leave column sums
+// Blocks that leave column sums, at most: as many an SM as the launches below
+// take for rows of this length.
+constexpr uint32_t max_groups(uint32_t n) { return kSms * (n <= 1024 ? 8 : 4); }
 
 // Rows under way at once, in shared memory: enough of them to keep memory busy
 // beside one barrier a row. A thread reads what it copied itself, except where
@@ -266,6 +267,7 @@ k_norm_join(uint32_t groups, uint32_t n, const float* __restrict__ partial, P* _
   const uint32_t col = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t i = (uint64_t)blockIdx.x * 32 + col;  // of the 2 n columns of a group
   float s = 0.0f;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the kernel before is done
   if (i < 2ull * n)
     for (uint32_t g = warp; g < groups; g += 32) s += partial[(uint64_t)g * 2 * n + i];
   part[warp][col] = s;
@@ -281,8 +283,8 @@ k_norm_join(uint32_t groups, uint32_t n, const float* __restrict__ partial, P* _
   }
 }
 
-uint32_t most_groups(uint64_t rows) {
-  return (uint32_t)std::min<uint64_t>(std::max<uint64_t>(rows, 1), kMaxGroups);
+uint32_t most_groups(uint64_t rows, uint32_t n) {
+  return (uint32_t)std::min<uint64_t>(std::max<uint64_t>(rows, 1), max_groups(n));
 }
 
 }  // namespace
@@ -291,7 +293,7 @@ uint32_t most_groups(uint64_t rows) {
 using namespace plx;
 
 extern "C" size_t plx_layer_norm_scratch_bytes(uint64_t rows, uint32_t n) {
-  return (size_t)most_groups(rows) * 2 * n * sizeof(float);
+  return (size_t)most_groups(rows, n) * 2 * n * sizeof(float);
 }
 
 extern "C" int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype,
@@ -310,6 +312,9 @@ extern "C" int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
     PLX_CHECK_ARG(rows == 1 || (ldx >= (int64_t)n && lddy >= (int64_t)n && (!dx || lddx >= (int64_t)n)),
                   "a row stride is less than n");
   }
+  if (int rc = check_aligned(dtype_bytes(dtype), {dy, x, dx})) return rc;
+  if (int rc = check_aligned(dtype_bytes(param_dtype), {weight, dweight, dbias})) return rc;
+  if (int rc = check_aligned(4, {mean, rstd})) return rc;
   if (!sums && (!rows || !dx)) return PLX_OK;
   DeviceGuard guard(ctx->device);
   PLX_TRY_CUDA(guard.err);
@@ -328,7 +333,12 @@ extern "C" int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
         using R = Ring<T, VV, NV, TPR>;
         constexpr auto kernel = k_norm_bwd<T, P, VV, NV, TPR, EACH>;
         const uint32_t per_block = TPR == 32 ? 8 : 1;
-        groups = (uint32_t)std::min<uint64_t>((rows + per_block - 1) / per_block, kSms * EACH);
+        // Eight rows a block or more, if that leaves a block an SM: what a block
+        // leaves to be joined costs as much as a few rows.
+        const uint64_t by_rows = (rows + per_block - 1) / per_block;
+        const uint32_t most = std::min<uint32_t>(kSms * EACH, max_groups(n));
+        groups = (uint32_t)std::min<uint64_t>(
+            std::min<uint64_t>(by_rows, std::max<uint64_t>(kSms, (by_rows + 7) / 8)), most);
         if (groups == 0) return PLX_OK;
         if (R::bytes > 32 * 1024)
           PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, R::bytes));
@@ -382,9 +392,18 @@ extern "C" int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
       if (rc != PLX_OK) return rc;
       PLX_LAUNCH_CHECK("k_norm_bwd");
       if (sums) {
-        k_norm_join<P><<<(unsigned)((2ull * n + 31) / 32), 1024, 0, ctx->stream>>>(
-            groups, n, partial, (P*)dweight, (P*)dbias);
-        PLX_LAUNCH_CHECK("k_norm_join");
+        // Launched while the sums are still being made; it waits for them itself.
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)((2ull * n + 31) / 32));
+        cfg.blockDim = dim3(1024);
+        cfg.stream = ctx->stream;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = groups ? 1 : 0;
+        PLX_TRY_CUDA(cudaLaunchKernelEx(&cfg, k_norm_join<P>, groups, n, (const float*)partial,
+                                        (P*)dweight, (P*)dbias));
       }
       return PLX_OK;
     };

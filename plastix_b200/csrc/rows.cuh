@@ -3,6 +3,7 @@
 #pragma once
 
 #include <atomic>
+#include <initializer_list>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -13,6 +14,16 @@ namespace plx {
 
 inline bool valid_dtype(int dtype) {
   return dtype == PLX_F32 || dtype == PLX_BF16 || dtype == PLX_F16;
+}
+
+inline size_t dtype_bytes(int dtype) { return dtype == PLX_F32 ? 4 : 2; }
+
+// Arrays start at a multiple of their elements' size.
+inline int check_aligned(size_t elem, std::initializer_list<const void*> arrays) {
+  for (const void* p : arrays)
+    PLX_CHECK_ARG(reinterpret_cast<uintptr_t>(p) % elem == 0,
+                  "array %p is not aligned to its elements of %zu bytes", p, elem);
+  return PLX_OK;
 }
 
 template <typename T>

@@ -79,6 +79,19 @@ def _like(ctx: Context, t: torch.Tensor, shape, dtype, name: str) -> int:
     return t.data_ptr()
 
 
+def _apart(a: torch.Tensor, lda: int, b: torch.Tensor, ldb: int) -> bool:
+    """Whether two tensors of rows of the same shape and type share no element."""
+    if a.numel() == 0:
+        return True
+    n, size = a.shape[-1], a.element_size()
+    rows = a.numel() // n
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa + ((rows - 1) * lda + n) * size <= pb or pb + ((rows - 1) * ldb + n) * size <= pa:
+        return True
+    # side by side in rows of the same stride
+    return lda == ldb and n <= (pb - pa) // size % lda <= lda - n
+
+
 def _result(ctx: Context, out: Optional[torch.Tensor], source: torch.Tensor, ld: int, name: str):
     """The tensor of rows that a call writes, and its row stride: ``out``, or
     a new one like ``source``. ``out`` may be the source itself."""
@@ -89,11 +102,14 @@ def _result(ctx: Context, out: Optional[torch.Tensor], source: torch.Tensor, ld:
         raise ValueError(f"{name} has to be {source.dtype} {tuple(source.shape)}, got {out.dtype} "
                          f"{tuple(out.shape)}")
     ldo = _rows(ctx, out, name)[2]
-    if (out is not source
-            and out.untyped_storage().data_ptr() == source.untyped_storage().data_ptr()
-            and not (out.data_ptr() == source.data_ptr() and ldo == ld)):
-        raise ValueError(f"{name} shares memory with the input and is not the input itself")
+    _check_result(out, ldo, source, ld, name)
     return out, ldo
+
+
+def _check_result(out, ldo, source, ld, name) -> None:
+    if out is not source and not (out.data_ptr() == source.data_ptr() and ldo == ld) \
+            and not _apart(out, ldo, source, ld):
+        raise ValueError(f"{name} overlaps an input and is not the input itself")
 
 
 def _scope(ctx: Context, *used):
@@ -152,7 +168,7 @@ def layer_norm_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, mean: t
                         out: Optional[torch.Tensor] = None):
     """(dx, dweight, dbias) for the rows and statistics of ``layer_norm``;
     dweight and dbias have weight's type and are None without a weight. The
-    same bits on every call. ``out`` (for dx) may be dy."""
+    same bits on every call. ``out`` (for dx) may be dy or x."""
     rows, n, ld, dtype = _rows(ctx, x, "x")
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError(f"dy has to be {x.dtype} {tuple(x.shape)}, got {dy.dtype} "
@@ -164,6 +180,8 @@ def layer_norm_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, mean: t
     kind = _abi.F32 if weight is None else _param(ctx, weight, n, x.dtype, "weight")
     with _scope(ctx, dy, x, mean, rstd, weight, out):
         dx, lddx = _result(ctx, out, dy, lddy, "out")
+        if out is not None:
+            _check_result(dx, lddx, x, ld, "out")
         dw = db = scratch = None
         size = 0
         if weight is not None:

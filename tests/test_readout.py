@@ -86,6 +86,21 @@ def test_distill_refuses(change, code, text):
     refused(code, text, "plx_distill", *{**DISTILL, **change}.values())
 
 
+ODD = ctypes.c_void_p(0x2002)  # aligned to 16-bit values, not to 32-bit ones
+
+
+@pytest.mark.parametrize("name, args, arrays", [
+    ("plx_layer_norm", NORM, "x y w b mean rstd"),
+    ("plx_layer_norm_backward", NORM_BWD, "dy x mean rstd w dx dw db"),
+    ("plx_log_probs", SCORE, "x target logp lse entropy ids best"),
+    ("plx_log_probs_backward", SCORE_BWD, "x target lse entropy gl ge dx"),
+    ("plx_distill", DISTILL, "x ids values w loss dx")])
+def test_arrays_off_their_elements_are_refused(name, args, arrays):
+    for a in arrays.split():
+        refused(1, b"not aligned", name, *{**args, a: ODD}.values())
+    refused(1, b"not aligned", name, *{**args, "dtype": 1, "x": ctypes.c_void_p(0x2001)}.values())
+
+
 def test_no_rows_are_no_work():
     lib = _abi.lib()
     assert lib.plx_layer_norm(*{**NORM, "rows": 0, "x": None, "y": None}.values()) == 0
@@ -140,8 +155,14 @@ def test_python_layer_refuses():
 def test_result_of_a_call_is_new_or_the_input_itself():
     c, x = FakeContext(), torch.zeros(8, 8)
     assert readout._result(c, x, x, 8, "out") == (x, 8)
-    with pytest.raises(ValueError, match="shares memory"):
-        readout._result(c, x[1:5], x[0:4], 8, "out")
+    for other in (x[1:5], x[0:8:2]):
+        with pytest.raises(ValueError, match="overlaps"):
+            readout._result(c, other, x[0:4], 8, "out")
+    readout._result(c, x[4:], x[:4], 8, "out")
+    readout._result(c, x[:, 4:], x[:, :4], 8, "out")  # side by side
+    readout._result(c, x[:, :4], x[:, 4:], 8, "out")
+    with pytest.raises(ValueError, match="overlaps"):
+        readout._result(c, x[:, 3:7], x[:, :4], 8, "out")
     with pytest.raises(ValueError):
         readout._result(c, x[:4].bfloat16(), x[:4], 8, "out")
 

@@ -71,6 +71,14 @@ NORM_CASES = [  # rows, n, type, type of the weights, row stride beyond n, eleme
     (600, 4096, "bf16", "bf16", 0, 0), (50, 4097, "f16", "f16", 0, 0), (37, 8192, "bf16", "f32", 0, 0),
     (20, 8200, "f32", "f32", 0, 4), (9, 20001, "bf16", "bf16", 0, 0), (3, 65536, "f32", "f32", 0, 0),
     (2500, 40, "f16", "f16", 0, 0), (700, 520, "f32", "f32", 3, 1),
+    (21, 512, "bf16", "bf16", 0, 0), (19, 200, "f32", "f32", 0, 0), (13, 1536, "bf16", "f32", 0, 0),
+    (7, 16384, "bf16", "bf16", 0, 0), (5, 4096, "f32", "f32", 0, 0), (5, 8192, "f32", "f32", 0, 0),
+    (11, 254, "bf16", "bf16", 0, 0), (11, 1002, "f16", "f32", 0, 2), (9, 2050, "bf16", "bf16", 0, 0),
+    (6, 5002, "f16", "f16", 0, 0), (4, 9002, "bf16", "bf16", 0, 0), (9, 129, "f16", "f16", 0, 0),
+    (9, 777, "bf16", "bf16", 0, 0), (9, 1501, "bf16", "f32", 0, 0), (9, 2301, "f16", "f16", 0, 3),
+    (9, 3333, "f16", "f16", 0, 0), (9, 5001, "bf16", "bf16", 0, 0), (9, 7777, "f32", "f32", 0, 0),
+    (6000, 255, "bf16", "bf16", 0, 0), (5000, 128, "f32", "f32", 0, 0), (700, 4097, "f16", "f16", 0, 0),
+    (1, 8191, "bf16", "bf16", 0, 1), (2, 3, "bf16", "bf16", 0, 0), (1200, 1024, "f32", "f32", 0, 0),
 ]
 
 
@@ -187,6 +195,7 @@ SCORE_CASES = [  # rows, n, type, top, scale, row stride beyond n, elements befo
     (1, 32000, "bf16", 64, 1.0, 0, 0), (8, 32003, "bf16", 5, 1.0, 0, 0), (3, 50001, "f32", 1, 1.0, 5, 2),
     (700, 2048, "bf16", 2, 1.0, 0, 0), (2, 131072, "f32", 20, 1.0, 0, 0), (1, 300007, "f16", 10, 1.0, 0, 0),
     (300, 20000, "f32", 8, 1.0, 0, 0), (170, 40010, "f16", 33, 0.25, 6, 0), (5, 1 << 20, "bf16", 16, 1.0, 0, 0),
+    (200, 12000, "bf16", 4, 1.0, 0, 0), (150, 9001, "f32", 64, 1.0, 0, 1), (151, 70003, "f16", 17, 1.0, 0, 0),
 ]
 
 
@@ -359,7 +368,7 @@ DISTILL_CASES = [  # rows, n, type, k, temperature, kind, row stride beyond n, e
     (40, 20011, "f16", 50, 2.0, "logits", 0, 0), (9, 65536, "bf16", 32, 2.0, "log_probs", 0, 0),
     (2, 131072, "f32", 64, 1.0, "logits", 0, 0), (1, 300007, "bf16", 20, 1.0, "log_probs", 0, 1),
     (160, 40000, "f32", 4, 1.0, "logits", 0, 0), (3, 1 << 20, "f16", 12, 1.5, "logits", 8, 0),
-    (2, 1000003, "f32", 7, 1.0, "logits", 0, 0), (300, 12345, "bf16", 33, 1.0, "logits", 0, 0),
+    (2, 1000003, "f32", 7, 1.0, "logits", 0, 0), (300, 20001, "f16", 12, 1.0, "logits", 0, 0), (300, 12345, "bf16", 33, 1.0, "logits", 0, 0),
 ]
 
 
@@ -520,6 +529,56 @@ def test_calls_are_captured_and_replayed():
             assert torch.equal(a, b)
     del graph
     c.close()
+
+
+def test_first_calls_of_a_process_can_be_captured():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from plastix_b200 import readout
+from plastix_b200.runtime import Context
+s = torch.cuda.Stream()
+c = Context(0, s)
+x = torch.randn(40, 40960, device="cuda"); w = torch.ones(40960, device="cuda")
+t = torch.zeros(40, dtype=torch.int32, device="cuda"); one = torch.ones(40, device="cuda")
+torch.cuda.synchronize()
+def calls():
+    y, m, r = readout.layer_norm(c, x[:, :2048], w[:2048], stats=True)
+    d = readout.layer_norm_backward(c, y, x[:, :2048], m, r, w[:2048])
+    p = readout.log_probs(c, x, t, top=3, entropy=True)
+    return [y, *d, *p, readout.log_probs_backward(c, x, p.lse, t, one, p.entropy, one),
+            *readout.distill(c, x, p.top_ids, p.top_logp, kind="log_probs")]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    got = calls()
+with torch.cuda.stream(s):
+    g.replay()
+    want = calls()
+c.sync()
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("captured")
+"""
+    root = Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stdout + done.stderr
+
+
+def test_results_beside_their_input_in_one_buffer(ctx):
+    buf = torch.randn(9, 2 * 1001, device="cuda").bfloat16()
+    x, out = buf[:, :1001], buf[:, 1001:]
+    keep = x.clone()
+    assert torch.equal(readout.layer_norm(ctx, x, out=out), readout.layer_norm(ctx, keep))
+    y, mean, rstd = readout.layer_norm(ctx, keep, stats=True)
+    want = readout.layer_norm_backward(ctx, y, keep, mean, rstd)[0]
+    got = readout.layer_norm_backward(ctx, y, x, mean, rstd, out=x)[0]  # dx takes x's place
+    ctx.sync()
+    assert got is x and torch.equal(got, want)
+    with pytest.raises(ValueError, match="overlaps"):
+        readout.layer_norm_backward(ctx, y, x, mean, rstd, out=buf[:, 500:1501])
 
 
 def test_two_contexts_on_two_streams_at_once(ctx):
