@@ -184,12 +184,21 @@ k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x, int
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const uint32_t i = (j * TPR + lane) * V;
-      if (i < n)
+      if (i >= n) continue;
+      if constexpr (V >= 4) {  // n and i are multiples of four
+#pragma unroll
+        for (int e = 0; e < V; e += 4)
+          for (int half = 0; half < 2; ++half)
+            *reinterpret_cast<float4*>(out + half * (uint64_t)n + i + e) =
+                make_float4(column(half, j * V + e), column(half, j * V + e + 1),
+                            column(half, j * V + e + 2), column(half, j * V + e + 3));
+      } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           out[i + e] = column(0, j * V + e);
           out[n + i + e] = column(1, j * V + e);
         }
+      }
     }
   } else {  // the eight warps' sums, added in their order
     __shared__ float joined[8][32 * E];
@@ -206,7 +215,7 @@ k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x, int
         float s = joined[0][i];
 #pragma unroll
         for (int k = 1; k < 8; ++k) s += joined[k][i];
-        out[half * n + i] = s;
+        out[half * (uint64_t)n + i] = s;
       }
     }
   }
@@ -269,6 +278,7 @@ k_norm_join(uint32_t groups, uint32_t n, const float* __restrict__ partial, P* _
   float s = 0.0f;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the kernel before is done
   if (i < 2ull * n)
+#pragma unroll 8
     for (uint32_t g = warp; g < groups; g += 32) s += partial[(uint64_t)g * 2 * n + i];
   part[warp][col] = s;
   __syncthreads();
