@@ -99,16 +99,24 @@ k_distill(uint32_t n, uint32_t each, const T* x, int64_t ld, uint32_t k,
     if (lane == 0) qsum_of = qsum;
     __syncwarp();
     if (out) {
+      // Mostly no output is named twice, which 32 entries tell at once.
+      const uint32_t same = __match_any_sync(0xffffffffu, id[0]);
+      const bool search =
+          k > 32 || __any_sync(0xffffffffu, id[0] >= 0 && (same & (same - 1)) != 0);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        all_q[e] = 0.0f;
-        bool first = true;
-        for (uint32_t j = 0; j < k; ++j)
-          if (sid[j] == id[e]) {
-            all_q[e] += sq[j];
-            first = first && j >= lane + 32 * e;
-          }
-        if (!first || (uint32_t)id[e] - share.start >= share.count) id[e] = -1;  // not written here
+        all_q[e] = q[e];
+        if (search) {
+          all_q[e] = 0.0f;
+          bool first = true;
+          for (uint32_t j = 0; j < k; ++j)
+            if (sid[j] == id[e]) {
+              all_q[e] += sq[j];
+              first = first && j >= lane + 32 * e;
+            }
+          if (!first) id[e] = -1;  // not written here
+        }
+        if ((uint32_t)id[e] - share.start >= share.count) id[e] = -1;
       }
     }
   }
