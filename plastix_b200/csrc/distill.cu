@@ -242,7 +242,7 @@ extern "C" int plx_distill(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, c
     // Where three blocks an SM have all the shared memory, they are large: 512
     // threads (4,096 rows of 65,536 bf16 205 us, with 256 threads 212).
     const bool large = dlogits && (uint64_t)n * sizeof(T) > (uint64_t)parts * 48 * 1024;
-    switch (large ? 512 : row_threads(n / parts)) {
+    switch (large ? 512 : row_threads(rows * parts, n / parts)) {
       case 512: return go(std::integral_constant<int, 512>{});
       case 64: return go(std::integral_constant<int, 64>{});
       case 128: return go(std::integral_constant<int, 128>{});

@@ -399,8 +399,9 @@ extern "C" int plx_log_probs(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype,
       // With alternatives 128 threads at most (4,096 rows of 65,536 bf16, 8
       // alternatives: 102 us, with 256 threads 108), but four times as many as
       // alternatives, or their maxima say too little (64: 143 us, with 256 130).
-      uint32_t threads = row_threads(n / parts);
-      if (B) threads = std::max(std::min(threads, 128u), top > 32 ? 256u : top > 16 ? 128u : 64u);
+      uint32_t threads = row_threads(rows * parts, n / parts);
+      if (B && rows * parts > 2 * 148) threads = std::min(threads, 128u);
+      if (B) threads = std::max(threads, top > 32 ? 256u : top > 16 ? 128u : 64u);
       switch (threads) {
         case 64: return go(k_log_probs<T, E, B, 64>, 64);
         case 128: return go(k_log_probs<T, E, B, 128>, 128);

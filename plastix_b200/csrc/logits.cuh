@@ -376,7 +376,12 @@ inline int check_logits(const plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype
 // 64. Measured on 8,192 rows of 4,096 bf16: 64 threads 18.9 us, 128 20.6, 256
 // 33.1; on 2,047 of 20,011: 23.5, 23.6, 25.2 (with gradient 58, 52, 40); on
 // 4,096 of 65,536: 101, 93, 89.
-inline uint32_t row_threads(uint32_t n) { return n < 64 * 128 ? 64 : n < 64 * 256 ? 128 : 256; }
+// Where `blocks` leave SMs with two blocks at most, latency counts, and 16 are
+// enough.
+inline uint32_t row_threads(uint64_t blocks, uint32_t n) {
+  const uint32_t each = blocks <= 2 * 148 ? 16 : 64;
+  return n < each * 128 ? 64 : n < each * 256 ? 128 : 256;
+}
 
 // Launches one row a cluster of `parts` blocks (no cluster for one).
 template <typename... Params, typename... Args>
