@@ -227,4 +227,6 @@ def check(code: int, where: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args), name)
+    code = getattr(_lib or lib(), name)(*args)
+    if code != PLX_OK:
+        check(code, name)

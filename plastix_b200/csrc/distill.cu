@@ -156,7 +156,7 @@ k_distill(uint32_t n, uint32_t each, const T* x, int64_t ld, uint32_t k,
     if (threadIdx.x < share.tail) single(share.tail_at() + threadIdx.x);
     const F2 minus = pack2(-m, -m), c2 = pack2(c, c), f2 = pack2(f, f);
     share.with_whole(out, [&](auto whole) {
-      auto piece = [&](uint32_t i, const uint4& p) {
+      auto piece = [&](uint32_t i, const uint4& p, int on = 0) {
         uint4 o;
 #pragma unroll
         for (int e = 0; e < V / 2; ++e) {
@@ -164,16 +164,16 @@ k_distill(uint32_t n, uint32_t each, const T* x, int64_t ld, uint32_t k,
           const F2 g = mul2(pack2(exp2_approx(d.x), exp2_approx(d.y)), f2);
           Piece<T>::put(o, e, g.x, g.y);
         }
-        share.template put_piece<decltype(whole)::value>(out, i, o);
+        share.template put_piece<decltype(whole)::value>(out, i, o, on);
       };
       uint32_t i = threadIdx.x;
       for (; i < kept; i += THREADS) piece(i, keep[i]);
       for (; i + 3 * THREADS < share.pieces; i += 4 * THREADS) {
         uint4 q4[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) q4[u] = share.piece(i + u * THREADS);
+        for (int u = 0; u < 4; ++u) q4[u] = share.piece(i, u * THREADS);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) piece(i + u * THREADS, q4[u]);
+        for (int u = 0; u < 4; ++u) piece(i, q4[u], u * THREADS);
       }
       for (; i < share.pieces; i += THREADS) piece(i, share.piece(i));
     });
@@ -239,14 +239,15 @@ extern "C" int plx_distill(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, c
                                row_weight, loss, (T*)dlogits, ldd, pieces, ctx->d_status));
       return PLX_OK;
     };
-    // Where three blocks an SM have all the shared memory, they are large: 512
-    // threads (4,096 rows of 65,536 bf16 205 us, with 256 threads 212).
+    // Where three blocks an SM have all the shared memory they are the largest
+    // (4,096 rows of 65,536 bf16: 512 threads 191 us, 256 205; 480, for 40
+    // registers each and not 32, 220: the last of a row's rounds is mostly idle).
     const bool large = dlogits && (uint64_t)n * sizeof(T) > (uint64_t)parts * 48 * 1024;
     switch (large ? 512 : row_threads(rows * parts, n / parts)) {
       case 512: return go(std::integral_constant<int, 512>{});
-      case 64: return go(std::integral_constant<int, 64>{});
+      case 256: return go(std::integral_constant<int, 256>{});
       case 128: return go(std::integral_constant<int, 128>{});
-      default: return go(std::integral_constant<int, 256>{});
+      default: return go(std::integral_constant<int, 64>{});
     }
   });
 }

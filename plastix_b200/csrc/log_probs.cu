@@ -337,7 +337,7 @@ k_log_probs_bwd(uint32_t n, uint32_t parts, uint32_t each, const T* x, int64_t l
   if (threadIdx.x < sh.head) single(threadIdx.x);
   if (threadIdx.x < sh.tail) single(sh.tail_at() + threadIdx.x);
   sh.with_whole(out, [&](auto whole) {
-    auto piece = [&](uint32_t i, const uint4& q) {
+    auto piece = [&](uint32_t i, const uint4& q, int on = 0) {
       uint4 o;
 #pragma unroll
       for (int k = 0; k < V / 2; ++k) {
@@ -345,15 +345,15 @@ k_log_probs_bwd(uint32_t n, uint32_t parts, uint32_t each, const T* x, int64_t l
         two(Piece<T>::pair(q, k), a, b);
         Piece<T>::put(o, k, a, b);
       }
-      sh.template put_piece<decltype(whole)::value>(out, i, o);
+      sh.template put_piece<decltype(whole)::value>(out, i, o, on);
     };
     uint32_t i = threadIdx.x;
     for (; i + (U - 1) * THREADS < sh.pieces; i += U * THREADS) {
       uint4 q[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) q[u] = sh.piece(i + u * THREADS);
+      for (int u = 0; u < U; ++u) q[u] = sh.piece(i, u * THREADS);
 #pragma unroll
-      for (int u = 0; u < U; ++u) piece(i + u * THREADS, q[u]);
+      for (int u = 0; u < U; ++u) piece(i, q[u], u * THREADS);
     }
     for (; i < sh.pieces; i += THREADS) piece(i, sh.piece(i));
   });

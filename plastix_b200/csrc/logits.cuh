@@ -137,18 +137,20 @@ struct Share {
     else f(std::false_type{});
   }
   template <bool WHOLE>
-  __device__ __forceinline__ void put_piece(T* out, uint32_t i, const uint4& o) const {
-    T* to = out + piece_at(i);
+  __device__ __forceinline__ void put_piece(T* out, uint32_t i, const uint4& o, int on = 0) const {
     if (WHOLE) {
-      *reinterpret_cast<uint4*>(to) = o;
+      (reinterpret_cast<uint4*>(out + head) + i)[on] = o;
     } else {
+      T* to = out + piece_at(i + on);
       const T* e = reinterpret_cast<const T*>(&o);
 #pragma unroll
       for (int k = 0; k < Piece<T>::V; ++k) to[k] = e[k];
     }
   }
-  __device__ __forceinline__ uint4 piece(uint32_t i) const {
-    return *reinterpret_cast<const uint4*>(p + piece_at(i));
+  // Piece i, and one a constant further on: as pointer and constant, which a
+  // load takes without arithmetic.
+  __device__ __forceinline__ uint4 piece(uint32_t i, int on = 0) const {
+    return (reinterpret_cast<const uint4*>(p + head) + i)[on];
   }
 };
 
@@ -267,36 +269,41 @@ __device__ __forceinline__ Sums scan_share(const Share<T>& sh, float c, Slots<TH
       uint4 q[U], next[U];
       if (i + (U - 1) * THREADS < end)
 #pragma unroll
-        for (int u = 0; u < U; ++u) next[u] = get(i + u * THREADS);
+        for (int u = 0; u < U; ++u) next[u] = get(i, u * THREADS);
       for (; i + (U - 1) * THREADS < end; i += U * THREADS) {
 #pragma unroll
         for (int u = 0; u < U; ++u) q[u] = next[u];
         if (i + (2 * U - 1) * THREADS < end)
 #pragma unroll
-          for (int u = 0; u < U; ++u) next[u] = get(i + (U + u) * THREADS);
+          for (int u = 0; u < U; ++u) next[u] = get(i, (U + u) * THREADS);
         batch(q, std::integral_constant<int, U>{});
       }
     } else {
       for (; i + (U - 1) * THREADS < end; i += U * THREADS) {
         uint4 q[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) q[u] = get(i + u * THREADS);
+        for (int u = 0; u < U; ++u) q[u] = get(i, u * THREADS);
         batch(q, std::integral_constant<int, U>{});
       }
     }
-    for (; i < end; i += THREADS) {
-      const uint4 q = get(i);
-      batch(&q, std::integral_constant<int, 1>{});
-    }
+    if (i >= end) return;
+    uint4 q[U];  // the rest, loaded together
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+      if (i + u * THREADS < end) q[u] = get(i, u * THREADS);
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+      if (i + u * THREADS < end) batch(q + u, std::integral_constant<int, 1>{});
+    i += (end - i + THREADS - 1) / THREADS * THREADS;
   };
   if (KEEP) {  // a thread reads what it copied itself: no barrier
-    auto get = [&](uint32_t k) { return keep[k]; };
+    auto get = [&](uint32_t k, int on) { return (keep + k)[on]; };
     copy_wait<1>();
     go(min(kept, half), get);
     copy_wait<0>();
     go(kept, get);
   }
-  go(sh.pieces, [&](uint32_t k) { return sh.piece(k); });
+  go(sh.pieces, [&](uint32_t k, int on) { return sh.piece(k, on); });
   return v;
 }
 
@@ -318,14 +325,16 @@ __device__ __forceinline__ Sums join_lanes(Sums v, float c, int from) {
 // every thread, in a fixed order. One barrier: `all` is used once a launch.
 template <bool ENT, int WARPS>
 __device__ __forceinline__ Sums join_block(Sums v, float c, Sums* all) {
-  static_assert((WARPS & (WARPS - 1)) == 0 && WARPS <= 32, "a power of two");
+  static_assert(WARPS <= 32, "one lane a warp");
+  constexpr int HALF = WARPS > 16 ? 16 : WARPS > 8 ? 8 : WARPS > 4 ? 4 : WARPS > 2 ? 2 : 1;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (warp < WARPS) {
     v = join_lanes<ENT>(v, c, 16);
     if (lane == 0) all[warp] = v;
   }
   __syncthreads();
-  return join_lanes<ENT>(all[lane & (WARPS - 1)], c, WARPS / 2);
+  const uint32_t k = lane & (2 * HALF - 1);
+  return join_lanes<ENT>(k < WARPS ? all[k] : Sums{-INFINITY, 0.0f, 0.0f}, c, HALF);
 }
 
 // The row's sums from its cluster's blocks', in rank order: `mine` of each, in

@@ -23,15 +23,19 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
   const uint32_t r = blockIdx.x * ROWS + threadIdx.x / TPR;
   if (ROWS > 1 && r >= rows) return;
   const T* xr = x + r * ldx;
+  // This thread's first column; the others are constants further on. A column j
+  // pieces on is within the row where j * STEP < left.
+  constexpr int STEP = TPR * V;
+  const int left = (int)n - (int)(lane * V);
+  const T* xl = xr + lane * V;
   constexpr int E = NV * V, H = E / 2;  // a thread's columns, as H pairs
   static_assert(E % 2 == 0, "columns in pairs");
   Pack<T, V> q[NV];
   if constexpr (V * sizeof(T) >= 4) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const uint32_t i = (j * TPR + lane) * V;
-      if (i < n) {
-        q[j] = load_pack<T, V>(xr + i);
+      if (j * STEP < left) {
+        q[j] = load_pack<T, V>(xl + j * STEP);
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) q[j].v[e] = from_f32<T>(0.0f);
@@ -65,7 +69,7 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
   for (int h = 0; h < H; ++h) v[h] = add2(v[h], minus);
 #pragma unroll
   for (int j = 0; j < NV; ++j)  // columns past the row's end have no deviation
-    if ((j * TPR + lane) * V >= n)
+    if (j * STEP >= left)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const int k = j * V + e;
@@ -91,7 +95,7 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
     Pack<P, V> p[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if ((j * TPR + lane) * V < n) p[j] = load_pack<P, V>(w + (j * TPR + lane) * V);
+      if (j * STEP < left) p[j] = load_pack<P, V>(w + lane * V + j * STEP);
     widen<NV, V>(p, g);
 #pragma unroll
     for (int k = 0; k < E; ++k) f[k] *= g[k];
@@ -100,19 +104,19 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
     Pack<P, V> p[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if ((j * TPR + lane) * V < n) p[j] = load_pack<P, V>(b + (j * TPR + lane) * V);
+      if (j * STEP < left) p[j] = load_pack<P, V>(b + lane * V + j * STEP);
     widen<NV, V>(p, g);
 #pragma unroll
     for (int k = 0; k < E; ++k) f[k] += g[k];
   }
+  T* yl = y + r * ldy + lane * V;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const uint32_t i = (j * TPR + lane) * V;
-    if (i < n) {
+    if (j * STEP < left) {
       Pack<T, V> out;
 #pragma unroll
       for (int e = 0; e < V; ++e) out.v[e] = from_f32<T>(f[j * V + e]);
-      *reinterpret_cast<Pack<T, V>*>(y + r * ldy + i) = out;
+      *reinterpret_cast<Pack<T, V>*>(yl + j * STEP) = out;
     }
   }
   if (lane == 0) {

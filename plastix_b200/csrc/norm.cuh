@@ -58,12 +58,10 @@ struct Staged {
   // This thread's values (0 past the row's end).
   static __device__ __forceinline__ void read(const char* at, const T* row, uint32_t n,
                                               uint32_t lane, Pack<T, 1> (&q)[NV]) {
-    const T* v = reinterpret_cast<const T*>(at + offset(row));
+    const T* v = reinterpret_cast<const T*>(at + offset(row)) + lane;
+    const int left = (int)n - (int)lane;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const uint32_t i = j * TPR + lane;
-      q[j].v[0] = i < n ? v[i] : from_f32<T>(0.0f);
-    }
+    for (int j = 0; j < NV; ++j) q[j].v[0] = j * TPR < left ? v[j * TPR] : from_f32<T>(0.0f);
   }
 };
 

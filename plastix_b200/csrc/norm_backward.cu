@@ -49,6 +49,10 @@ k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x, int
   static_assert(E % 2 == 0, "columns in pairs");
   const uint32_t lane = threadIdx.x % TPR, warp = threadIdx.x / 32, wl = threadIdx.x & 31;
   const uint32_t step = gridDim.x * ROWS;
+  // A column j pieces on from this thread's first one is within the row where
+  // j * STEP < left.
+  constexpr int STEP = TPR * V;
+  const int left = (int)n - (int)(lane * V);
   uint32_t r = blockIdx.x * ROWS + threadIdx.x / TPR;
   auto slot = [&](uint32_t stage, int array, int j) {  // a piece of this thread's
     char* at = ring + stage * R::stage_bytes + array * R::array_bytes;
@@ -97,10 +101,9 @@ k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x, int
       } else {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const uint32_t i = (j * TPR + lane) * V;
-          if (i >= n) continue;
-          copy_async<R::piece>(slot(stage, 0, j), xr + i);
-          copy_async<R::piece>(slot(stage, 1, j), gr + i);
+          if (j * STEP >= left) continue;
+          copy_async<R::piece>(slot(stage, 0, j), xr + lane * V + j * STEP);
+          copy_async<R::piece>(slot(stage, 1, j), gr + lane * V + j * STEP);
         }
       }
       if (wl < 2) copy_async<4>(&stats[stage][warp][wl], (wl ? rstd : mean) + row);
@@ -162,14 +165,14 @@ k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x, int
         o[2 * h] = v.x;
         o[2 * h + 1] = v.y;
       }
+      T* dl = dx + r * lddx + lane * V;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const uint32_t i = (j * TPR + lane) * V;
-        if (i < n) {
+        if (j * STEP < left) {
           Pack<T, V> out;
 #pragma unroll
           for (int e = 0; e < V; ++e) out.v[e] = from_f32<T>(o[j * V + e]);
-          *reinterpret_cast<Pack<T, V>*>(dx + r * lddx + i) = out;
+          *reinterpret_cast<Pack<T, V>*>(dl + j * STEP) = out;
         }
       }
     }
