@@ -7,15 +7,18 @@
 // the row's sum first, so the row is gone over twice: for maximum and sum
 // (logits.cuh) and for the gradient. In between it stays in shared memory, up
 // to kKeepBytes a block, a long row spread over the blocks of a cluster; what
-// does not fit is read again out of L2. The first warp takes care of the
-// teacher's entries; the outputs they name are put right at the end.
+// does not fit is read again out of L2. A warp of its own takes care of the
+// teacher's entries meanwhile; the outputs they name are put right at the end.
+// Measured, 4,096 rows of 65,536 bf16: loss 84 us, 6.4 TB/s; with gradient 191
+// us, 5.6 TB/s (special functions and issue slots are more than half busy);
+// second read out of L2 alone 244. 2,048 rows of 65,536 f32: 80, 202.
 #include "logits.cuh"
 
 namespace plx {
 namespace {
 
 // Of a row in a block's shared memory: three blocks an SM fit, so that one's
-// loads run beside another's stores.
+// loads run beside another's stores (110 KB and two blocks: 220 us, 54 KB: 242).
 constexpr uint32_t kKeepBytes = 72 * 1024;
 
 // THREADS threads go over the row; one more warp takes care of the teacher.
@@ -224,7 +227,9 @@ extern "C" int plx_distill(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, c
     // again of 444 parts at once is then still in L2.
     uint32_t parts = row_parts(rows, n);
     if (dlogits)
-      while (parts < 8 && (uint64_t)n * sizeof(T) > (uint64_t)parts * 2 * kKeepBytes) parts *= 2;
+      while (parts < 8 && (uint64_t)n * sizeof(T) > (uint64_t)parts * 2 * kKeepBytes &&
+             rows * parts < (1ull << 30))
+        parts *= 2;
     auto go = [&](auto threads_c) {
       constexpr int THREADS = decltype(threads_c)::value;
       constexpr auto kernel = k_distill<T, THREADS>;

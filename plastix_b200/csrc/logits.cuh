@@ -172,7 +172,8 @@ struct Sums {
 
 // Low bits of a value of type T that say nothing once it is 32 bits wide.
 template <typename T>
-constexpr int kSpareBits = std::is_same_v<T, __nv_bfloat16> ? 16 : std::is_same_v<T, __half> ? 13 : 0;
+constexpr int kSpareBits =
+    std::is_same_v<T, __nv_bfloat16> ? 16 : std::is_same_v<T, __half> ? 13 : 0;
 
 // A number that orders values: larger for larger ones, NaN above all, -0 as 0.
 __device__ __forceinline__ uint32_t order_of(float v) {

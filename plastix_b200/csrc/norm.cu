@@ -5,15 +5,19 @@
 //
 // Bound by memory (each value read once, written once): a row is held in
 // registers by the threads that share it, a warp for rows of up to 128
-// sixteen-byte pieces (no barrier), a block of 128 to 1,024 threads above.
-
+// sixteen-byte pieces (no barrier), a block of 128 to 1,024 threads above. Few
+// threads with many values each do best: the two sums' exchanges cost the
+// same for every thread (32,768 rows of 4,096 bf16: 128 threads 95 us, 256 107,
+// 512 147). Measured: those rows 95 us, 5.6 TB/s; 16,384 rows of 4,096 f32 79
+// us, 6.8 TB/s (half of it out of L2); 65,536 rows of 1,024 bf16 52 us, 5.2
+// TB/s.
 #include "norm.cuh"
 
 namespace plx {
 namespace {
 
 template <typename T, typename P, int V, int NV, int TPR>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR)
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 512 && V >= 4 ? 2 : 1)
 k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__ w,
        const P* __restrict__ b, float eps, T* y, int64_t ldy, float* __restrict__ mean,
        float* __restrict__ rstd) {
@@ -125,7 +129,9 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
   }
 }
 
-// Rows too long for registers: three passes, the later two out of L2.
+// Rows too long for registers: three passes, the later two out of L2 (one value
+// a thread at a time, for any alignment; 4,096 rows of 32,768 bf16 in registers
+// take 178 us, longer rows are rarer still).
 template <typename T, typename P>
 __global__ void __launch_bounds__(1024)
 k_norm_long(uint32_t n, const T* x, int64_t ldx, const P* __restrict__ w,
