@@ -6,11 +6,13 @@
 // Bound by memory (each value read once, written once): a row is held in
 // registers by the threads that share it, a warp for rows of up to 128
 // sixteen-byte pieces (no barrier), a block of 128 to 1,024 threads above. Few
-// threads with many values each do best: the two sums' exchanges cost the
-// same for every thread (32,768 rows of 4,096 bf16: 128 threads 95 us, 256 107,
-// 512 147). Measured: those rows 95 us, 5.6 TB/s; 16,384 rows of 4,096 f32 79
-// us, 6.8 TB/s (half of it out of L2); 65,536 rows of 1,024 bf16 52 us, 5.2
-// TB/s.
+// threads with many values each do best, since the two sums' exchanges cost the
+// same for every thread (32,768 rows of 4,096 bf16, before the last step: 128
+// threads 95 us, 256 107, 512 147), and weights that are read, applied, rounded
+// and stored piece by piece (95 to 87 us: fewer registers, more blocks an SM).
+// Measured: those rows 87 us, 6.2 TB/s; 8,192 rows of 16,384 bf16 94 us, 5.7
+// TB/s; 65,536 rows of 1,024 bf16 49 us, 5.5 TB/s; 16,384 rows of 2,049 f32 (one
+// value a load) 53 us, 5.1 TB/s; of 4,097 bf16 (staged) 117 us, 2.3 TB/s.
 #include "norm.cuh"
 
 namespace plx {
@@ -19,8 +21,8 @@ namespace {
 template <typename T, typename P, int V, int NV, int TPR>
 __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 512 && V >= 4 ? 2 : 1)
 k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__ w,
-       const P* __restrict__ b, float eps, T* y, int64_t ldy, float* __restrict__ mean,
-       float* __restrict__ rstd) {
+       const P* __restrict__ b, float eps, float inv_n, T* y, int64_t ldy,
+       float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int ROWS = TPR == 32 ? 8 : 1;
   __shared__ float red[2 * (TPR / 32)];
   const uint32_t lane = threadIdx.x % TPR;
@@ -67,13 +69,14 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
   int turn = 0;
   float s[1] = {s2.x + s2.y};
   row_sum<TPR>(s, red, turn);
-  const float mu = s[0] / (float)n;
+  const float mu = s[0] * inv_n;
   const F2 minus = pack2(-mu, -mu);
 #pragma unroll
   for (int h = 0; h < H; ++h) v[h] = add2(v[h], minus);
+  if (n < (uint32_t)(NV * STEP))  // columns past the row's end have no deviation
 #pragma unroll
-  for (int j = 0; j < NV; ++j)  // columns past the row's end have no deviation
-    if (j * STEP >= left)
+    for (int j = 0; j < NV; ++j)
+      if (j * STEP >= left)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const int k = j * V + e;
@@ -84,45 +87,46 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
   for (int h = 0; h < H; ++h) s2 = fma2(v[h], v[h], s2);
   s[0] = s2.x + s2.y;
   row_sum<TPR>(s, red, turn);
-  const float rs = 1.0f / sqrtf(s[0] / (float)n + eps);
+  const float rs = rsqrtf(fmaf(s[0], inv_n, eps));  // two units in the last place at most
   const F2 rs2 = pack2(rs, rs);
 #pragma unroll
   for (int h = 0; h < H; ++h) v[h] = mul2(v[h], rs2);
-  float g[E];
-#pragma unroll
-  for (int h = 0; h < H; ++h) {
-    f[2 * h] = v[h].x;
-    f[2 * h + 1] = v[h].y;
-  }
-  // Weights one after the other: they come out of L1.
-  if (w) {
-    Pack<P, V> p[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (j * STEP < left) p[j] = load_pack<P, V>(w + lane * V + j * STEP);
-    widen<NV, V>(p, g);
-#pragma unroll
-    for (int k = 0; k < E; ++k) f[k] *= g[k];
-  }
-  if (b) {
-    Pack<P, V> p[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (j * STEP < left) p[j] = load_pack<P, V>(b + lane * V + j * STEP);
-    widen<NV, V>(p, g);
-#pragma unroll
-    for (int k = 0; k < E; ++k) f[k] += g[k];
-  }
+  // Weights (out of L1), rounding and storing piece by piece: few of them are
+  // live at once.
   T* yl = y + r * ldy + lane * V;
+  const P *wl = w + lane * V, *bl = b + lane * V;
+  auto finish = [&](auto has_w, auto has_b) {
+    constexpr bool W = decltype(has_w)::value, B = decltype(has_b)::value;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    if (j * STEP < left) {
+    for (int j = 0; j < NV; ++j) {
+      if (j * STEP >= left) continue;
+      Pack<P, V> pw, pb;
+      if (W) pw = load_pack<P, V>(wl + j * STEP);
+      if (B) pb = load_pack<P, V>(bl + j * STEP);
       Pack<T, V> out;
+      if constexpr (V == 1) {
+        const float a = j & 1 ? v[j / 2].y : v[j / 2].x;
+        out.v[0] = from_f32<T>(fmaf(a, W ? to_f32(pw.v[0]) : 1.0f, B ? to_f32(pb.v[0]) : 0.0f));
+      } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) out.v[e] = from_f32<T>(f[j * V + e]);
+        for (int e = 0; e < V; e += 2) {
+          const F2 a = v[(j * V + e) / 2];
+          put_pair(out, e,
+                   W && B ? fma2(a, pair_of(pw, e), pair_of(pb, e))
+                   : W    ? mul2(a, pair_of(pw, e))
+                   : B    ? add2(a, pair_of(pb, e))
+                          : a);
+        }
+      }
       *reinterpret_cast<Pack<T, V>*>(yl + j * STEP) = out;
     }
-  }
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  if (w && b) finish(Yes{}, Yes{});
+  else if (w) finish(Yes{}, No{});
+  else if (b) finish(No{}, Yes{});
+  else finish(No{}, No{});
   if (lane == 0) {
     if (mean) mean[r] = mu;
     if (rstd) rstd[r] = rs;
@@ -130,8 +134,7 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
 }
 
 // Rows too long for registers: three passes, the later two out of L2 (one value
-// a thread at a time, for any alignment; 4,096 rows of 32,768 bf16 in registers
-// take 178 us, longer rows are rarer still).
+// a thread at a time, for any alignment: rows this long are rare).
 template <typename T, typename P>
 __global__ void __launch_bounds__(1024)
 k_norm_long(uint32_t n, const T* x, int64_t ldx, const P* __restrict__ w,
@@ -186,8 +189,8 @@ extern "C" int plx_layer_norm(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype
       using P = decltype(p);
       auto launch = [&](auto kernel, unsigned grid, unsigned block) {
         kernel<<<grid, block, 0, ctx->stream>>>((uint32_t)rows, n, (const T*)x, ldx,
-                                                (const P*)weight, (const P*)bias, eps, (T*)y, ldy,
-                                                mean, rstd);
+                                                (const P*)weight, (const P*)bias, eps,
+                                                1.0f / (float)n, (T*)y, ldy, mean, rstd);
       };
       const unsigned one = (unsigned)rows, eighth = (unsigned)((rows + 7) / 8);
       const uint32_t v = piece_values(n, sizeof(T), {x, y}, {ldx, ldy}, weight, bias, sizeof(P));

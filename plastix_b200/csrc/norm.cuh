@@ -1,6 +1,8 @@
 // Shared by norm.cu (layer norm forward) and norm_backward.cu.
 #pragma once
 
+#include <type_traits>
+
 #include "rows.cuh"
 
 namespace plx {
@@ -19,6 +21,41 @@ __device__ __forceinline__ void widen(const Pack<T, V> (&q)[NV], float (&f)[NV *
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int e = 0; e < V; ++e) f[j * V + e] = to_f32(q[j].v[e]);
+}
+
+// Values e and e + 1 of a piece, rounded together.
+template <typename T, int V>
+__device__ __forceinline__ void put_pair(Pack<T, V>& q, int e, F2 v) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    *reinterpret_cast<__nv_bfloat162*>(&q.v[e]) = __floats2bfloat162_rn(v.x, v.y);
+  } else if constexpr (std::is_same_v<T, __half>) {
+    *reinterpret_cast<__half2*>(&q.v[e]) = __floats2half2_rn(v.x, v.y);
+  } else {
+    q.v[e] = v.x;
+    q.v[e + 1] = v.y;
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ F2 pair_of(const Pack<T, V>& q, int e) {
+  return pack2(to_f32(q.v[e]), to_f32(q.v[e + 1]));
+}
+
+// H pairs of results as NV pieces of a row: piece j goes j * STEP values on
+// from `to`, where that is less than `left`.
+template <int STEP, int NV, int V, typename T>
+__device__ __forceinline__ void store_row(T* to, int left, const F2 (&v)[NV * V / 2]) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (j * STEP >= left) continue;
+    Pack<T, V> out;
+    if constexpr (V == 1) {
+      out.v[0] = from_f32<T>(j & 1 ? v[j / 2].y : v[j / 2].x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) put_pair(out, e, v[(j * V + e) / 2]);
+    }
+    *reinterpret_cast<Pack<T, V>*>(to + j * STEP) = out;
+  }
 }
 
 template <typename T, int V>

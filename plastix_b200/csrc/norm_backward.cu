@@ -160,24 +160,12 @@ k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x, int
       // dx = s g + ((x - mu) a + b), a = -s^2 mean(g h), b = -s mean g
       const float a = -s * s * (c.y * s * inv_n), b = -s * (c.x * inv_n);
       const F2 a2 = pack2(a, a), b2 = pack2(b, b);
-      float o[E];
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         const F2 g = mul2(pack2(fg[2 * h], fg[2 * h + 1]), wv[h]);
-        const F2 v = fma2(g, s2, fma2(xm[h], a2, b2));
-        o[2 * h] = v.x;
-        o[2 * h + 1] = v.y;
+        xm[h] = fma2(g, s2, fma2(xm[h], a2, b2));
       }
-      T* dl = dx + r * lddx + lane * V;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (j * STEP < left) {
-          Pack<T, V> out;
-#pragma unroll
-          for (int e = 0; e < V; ++e) out.v[e] = from_f32<T>(o[j * V + e]);
-          *reinterpret_cast<Pack<T, V>*>(dl + j * STEP) = out;
-        }
-      }
+      store_row<STEP, NV, V>(dx + r * lddx + lane * V, left, xm);
     }
   }
   if (!partial) return;
