@@ -19,9 +19,13 @@ namespace plx {
 namespace {
 
 constexpr uint32_t kSms = 148;                // of a B200; fixes the order of the sums
-// Blocks that leave column sums, at most: as many an SM as the launches below
+constexpr uint32_t kLongest = 16384;          // row of any type that stays in registers
+constexpr uint32_t kLongGroups = 64;          // runs of longer rows
+// Groups of column sums, at most: as many blocks an SM as the launches below
 // take for rows of this length.
-constexpr uint32_t max_groups(uint32_t n) { return kSms * (n <= 1024 ? 8 : 4); }
+constexpr uint32_t max_groups(uint32_t n) {
+  return n > kLongest ? kLongGroups : kSms * (n <= 1024 ? 8 : 4);
+}
 
 // Rows under way at once, in shared memory: enough of them to keep memory busy
 // beside one barrier a row. A thread reads what it copied itself, except where
@@ -337,6 +341,7 @@ extern "C" int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
         constexpr int NV = decltype(nv_c)::value, TPR = decltype(tpr_c)::value;
         constexpr int EACH = decltype(each_c)::value, VV = decltype(v_c)::value;
         using R = Ring<T, VV, NV, TPR>;
+        static_assert(NV * TPR * VV <= kLongest, "max_groups");
         constexpr auto kernel = k_norm_bwd<T, P, VV, NV, TPR, EACH>;
         const uint32_t per_block = TPR == 32 ? 8 : 1;
         // Eight rows a block or more, if that leaves a block an SM: what a block
@@ -355,7 +360,7 @@ extern "C" int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
       };
       auto loops = [&] {
         if (sums && rows) {
-          groups = std::min<uint32_t>((uint32_t)rows, 64);
+          groups = std::min<uint32_t>((uint32_t)rows, kLongGroups);
           k_norm_dw_long<T><<<dim3((n + 255) / 256, groups), 256, 0, ctx->stream>>>(
               (uint32_t)rows, n, (const T*)dy, lddy, (const T*)x, ldx, mean, rstd, partial);
         }

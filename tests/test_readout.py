@@ -53,6 +53,14 @@ def test_layer_norm_backward_refuses(change, code, text):
     refused(code, text, "plx_layer_norm_backward", *{**NORM_BWD, **change}.values())
 
 
+@pytest.mark.parametrize("rows", [600, 100_000])
+@pytest.mark.parametrize("n", [16_385, 65_536, 1_000_003])
+def test_layer_norm_scratch_of_long_rows_is_less_than_600_rows(rows, n):
+    """Column sums of many long rows take a fraction of what 600 of them take."""
+    size = _abi.lib().plx_layer_norm_scratch_bytes(rows, n)
+    assert 2 * 4 * n <= size < 600 * n * 2
+
+
 @pytest.mark.parametrize("change, code, text", [
     (dict(ctx=None), 1, b"ctx"), (dict(dtype=3), 1, b"dtype"), (dict(n=0), 1, b"n = 0"),
     (dict(rows=1 << 31), 3, b"fewer than 2^31"), (dict(x=None), 1, b"logits"),

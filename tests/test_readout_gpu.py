@@ -79,6 +79,7 @@ NORM_CASES = [  # rows, n, type, type of the weights, row stride beyond n, eleme
     (9, 3333, "f16", "f16", 0, 0), (9, 5001, "bf16", "bf16", 0, 0), (9, 7777, "f32", "f32", 0, 0),
     (6000, 255, "bf16", "bf16", 0, 0), (5000, 128, "f32", "f32", 0, 0), (700, 4097, "f16", "f16", 0, 0),
     (1, 8191, "bf16", "bf16", 0, 1), (2, 3, "bf16", "bf16", 0, 0), (1200, 1024, "f32", "f32", 0, 0),
+    (150, 17000, "bf16", "bf16", 0, 0), (70, 16385, "f32", "f32", 0, 0), (130, 16384, "f16", "f16", 0, 1),
 ]
 
 
