@@ -616,8 +616,8 @@ size_t plx_layer_norm_scratch_bytes(uint64_t rows, uint32_t n);
 
 /* Gradients of layer norm: dx [rows, n] and, of type param_dtype, dweight and
  * dbias [n], each written where not NULL (dweight and dbias are the sums over
- * all rows, added in an order that rows, n and the types alone set: the same
- * bits on every call; zero for rows = 0). scratch is 16-byte aligned and may
+ * all rows, added in an order that rows, n, the types and the arrays'
+ * alignment set: the same bits on every call; zero for rows = 0). scratch is 16-byte aligned and may
  * hold anything; calls that run at once need scratch of their own. */
 int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* dy,
                             int64_t lddy, const void* x, int64_t ldx, const float* mean,

@@ -1,5 +1,6 @@
-// Shared pieces of the row operators (norm.cu, readout.cu): element types,
-// 16-byte row access and block-wide reductions in a fixed order.
+// Shared pieces of the row operators (norm.cu, norm_backward.cu, log_probs.cu,
+// distill.cu): element types, pairs of values, reductions in a fixed order and
+// asynchronous copies.
 #pragma once
 
 #include <atomic>
@@ -84,9 +85,8 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// Block-wide sum / maximum, the same value in every thread, added in a fixed
-// order. `red` holds one float per warp; the barrier at the head lets it be
-// used again at once.
+// Block-wide sum, the same value in every thread, added in a fixed order. `red`
+// holds one float per warp; the barrier at the head lets it be used again at once.
 template <int WARPS>
 __device__ __forceinline__ float block_sum(float v, float* red) {
   v = warp_sum(v);
@@ -96,17 +96,6 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   float s = red[0];
 #pragma unroll
   for (int w = 1; w < WARPS; ++w) s = __fadd_rn(s, red[w]);
-  return s;
-}
-template <int WARPS>
-__device__ __forceinline__ float block_max(float v, float* red) {
-  v = warp_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = red[0];
-#pragma unroll
-  for (int w = 1; w < WARPS; ++w) s = max_nan(s, red[w]);
   return s;
 }
 

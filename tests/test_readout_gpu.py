@@ -63,6 +63,20 @@ def norm_tolerance(x, w, b, eps, rstd, half):
         (np.abs(w) * h_err + 3 * U * (np.abs(h * w) + np.abs(b))) * (1 + half) + half * np.abs(y)
 
 
+def gradient_tolerance(dy, x, mean, rstd, w, dx, dw, db, half, ph):
+    """Of dx, dw and db with the statistics that the call was given."""
+    rows, n = x.shape
+    h, g = (x - mean[:, None]) * rstd[:, None], dy * w
+    e1 = (depth(n) + 2) * U * np.abs(g).mean(1, keepdims=True)
+    e2 = (depth(n) + 6) * U * np.abs(g * h).mean(1, keepdims=True)
+    c1, c2 = g.mean(1, keepdims=True), (g * h).mean(1, keepdims=True)
+    err = rstd[:, None] * (e1 + np.abs(h) * e2 + 6 * U * (np.abs(g) + np.abs(c1) + np.abs(h * c2)))
+    down = (min(rows, rows / 16 + 700) + 8) * U
+    return err * (1 + half) + half * np.abs(dx), \
+        down * np.abs(dy * h).sum(0) * (1 + ph) + ph * np.abs(dw), \
+        down * np.abs(dy).sum(0) * (1 + ph) + ph * np.abs(db)
+
+
 NORM_CASES = [  # rows, n, type, type of the weights, row stride beyond n, elements before the first row
     (1, 1, "f32", "f32", 0, 0), (5, 1, "bf16", "bf16", 0, 1), (3, 2, "f16", "f16", 1, 1),
     (7, 33, "f32", "f32", 0, 0), (1, 1024, "bf16", "bf16", 0, 0), (33, 1024, "f16", "f32", 0, 0),
@@ -108,16 +122,55 @@ def test_layer_norm_and_its_gradient(ctx, rows, n, dtype, pdtype, pad, shift):
     # the gradient's formula with the statistics that the call was given
     M, R = f64(mean), f64(rstd)
     DX, DW, DB = F.layer_norm_backward(DY, X, M, R, W)
-    h, g = (X - M[:, None]) * R[:, None], DY * W
-    e1 = (depth(n) + 2) * U * np.abs(g).mean(1, keepdims=True)
-    e2 = (depth(n) + 6) * U * np.abs(g * h).mean(1, keepdims=True)
-    c1, c2 = g.mean(1, keepdims=True), (g * h).mean(1, keepdims=True)
-    err = R[:, None] * (e1 + np.abs(h) * e2 + 6 * U * (np.abs(g) + np.abs(c1) + np.abs(h * c2)))
-    within(f64(dx), DX, err * (1 + half) + half * np.abs(DX) + TINY[dtype], "dx")
-    down = (min(rows, rows / 16 + 700) + 8) * U
-    ph = HALF_STEP[pdtype]
-    within(f64(dw), DW, down * np.abs(DY * h).sum(0) * (1 + ph) + ph * np.abs(DW) + TINY[pdtype], "dw")
-    within(f64(db), DB, down * np.abs(DY).sum(0) * (1 + ph) + ph * np.abs(DB) + TINY[pdtype], "db")
+    tx, tw, tb = gradient_tolerance(DY, X, M, R, W, DX, DW, DB, half, HALF_STEP[pdtype])
+    within(f64(dx), DX, tx + TINY[dtype], "dx")
+    within(f64(dw), DW, tw + TINY[pdtype], "dw")
+    within(f64(db), DB, tb + TINY[pdtype], "db")
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("rows, n, pdtype", [
+    (5, 1, "f32"), (5, 2, "bf16"), (5, 7, "f32"), (5, 8, "bf16"), (5, 9, "f32"), (5, 23, "bf16"),
+    (5, 250, "bf16"), (5, 249, "f32"), (5, 256, "bf16"), (5, 257, "f32"), (5, 505, "bf16"),
+    (5, 513, "f32"), (5, 1000, "bf16"), (5, 1027, "f32"), (5, 2046, "bf16"), (5, 2055, "f32"),
+    (5, 4098, "bf16"), (5, 8190, "f32"), (5, 16377, "bf16"), (310, 1001, "bf16"), (400, 5001, "bf16"),
+    (2500, 77, "f32"), (1, 1001, "bf16"), (170, 9003, "bf16")])
+def test_layer_norm_at_every_offset_writes_its_own_columns_only(ctx, rows, n, pdtype, apart):
+    """Rows that start anywhere (`apart`: x, dy, y and dx each elsewhere), weights anywhere, y
+    and dx in the middle of something else."""
+    r = np.random.default_rng(n)
+    ax, ad = r.normal(size=(rows, n)) + 0.5, r.normal(size=(rows, n))
+    weight = torch.from_numpy(1 + 0.3 * r.normal(size=n)).to("cuda", TYPES[pdtype])
+    half, ph = HALF_STEP["bf16"], HALF_STEP[pdtype]
+    for shift in range(8) if rows < 100 else (0, 3):
+        def place(a, k):
+            return rows_tensor(a, "bf16", n + (9 + 2 * k if apart else 9), (shift + 3 * k * apart) % 8)
+        (x, _), (dy, _), (out, guard), (dx, dguard) = (place(a, k) for k, a in
+                                                       enumerate((ax, ad, ad * 0, ad * 0)))
+        w = torch.empty(n + 8, device="cuda", dtype=weight.dtype)[shift:shift + n].copy_(weight)
+        y, mean, rstd = readout.layer_norm(ctx, x, w, w, stats=True, out=out)
+        _, dw, db = readout.layer_norm_backward(ctx, dy, x, mean, rstd, w, out=dx)
+        ctx.sync()
+        for t, g in ((out, guard), (dx, dguard)):
+            rest = g.clone()
+            rest.as_strided(t.shape, t.stride(), t.storage_offset()).fill_(7.0)
+            assert torch.equal(rest, torch.full_like(rest, 7.0))
+        W, X, DY = f64(w), f64(x), f64(dy)
+        Y, M, R = F.layer_norm(X, W, W, 1e-5)
+        tm, tr, ty = norm_tolerance(X, W, W, 1e-5, R, half)
+        within(f64(mean), M, tm, "mean")
+        within(f64(rstd), R, tr, "rstd")
+        within(f64(out), Y, ty + TINY["bf16"], "y")
+        M, R = f64(mean), f64(rstd)
+        DX, DW, DB = F.layer_norm_backward(DY, X, M, R, W)
+        tx, tw, tb = gradient_tolerance(DY, X, M, R, W, DX, DW, DB, half, ph)
+        within(f64(dx), DX, tx + TINY["bf16"], "dx")
+        within(f64(dw), DW, tw + TINY[pdtype], "dw")
+        within(f64(db), DB, tb + TINY[pdtype], "db")
+        if not apart:  # in place, the same kernels
+            readout.layer_norm_backward(ctx, dy, x, mean, rstd, w, out=dy)
+            readout.layer_norm(ctx, x, w, w, out=x)
+            assert torch.equal(dy, dx) and torch.equal(x, out)
 
 
 def test_layer_norm_without_weights_in_place_and_without_rows(ctx):
