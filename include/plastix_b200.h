@@ -652,7 +652,9 @@ int plx_log_probs(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void
  * respect to the logits. lse and entropy are those of plx_log_probs with the
  * same arguments; grad_logp (needs target) or grad_entropy (needs entropy)
  * may be NULL, not both. A row without a target (or with one outside [0, n))
- * has no gradient from grad_logp. */
+ * has no gradient from grad_logp. Where |lse| is above 32 (or lse is -inf or
+ * NaN) the row's sum is made anew from its logits, because lse in 32 bits
+ * does not hold enough of it: such rows cost a second pass. */
 int plx_log_probs_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype,
                            const void* logits, int64_t ld, const int32_t* target, float scale,
                            const float* lse, const float* entropy, const float* grad_logp,

@@ -6,6 +6,15 @@
 // M is subtracted before scaling, which is exact near M, so large common
 // offsets cost no accuracy. All sums are in 32 bits.
 //
+// The gradient needs log p_i = scale x_i - lse, and lse in 32 bits is off by up
+// to |lse| 2^-24, which every p_i takes over: 2^-20 for |lse| up to 32, as much
+// as a dozen other roundings; a thousandth around 30,000; and in a row of the
+// type's lowest values log s is gone altogether and every p_i comes out as 1.
+// So rows above 32 (and those of lse -inf or NaN) take M and log s from the row
+// itself: one block reads it, and once more to write its gradient. 4,096 rows
+// of 65,536 bf16: 164 us for ordinary rows, 239 if all are far from zero; one
+// row of 131,072 f32 2.3 and 24 (one block instead of 32).
+//
 // Bound by memory: the forward pass reads a row once (running maximum and
 // sums, logits.cuh) and finds the alternatives from what the threads saw: of
 // the threads' own maxima the `top` best are a threshold, only threads at or
@@ -292,8 +301,12 @@ k_log_probs(uint32_t n, uint32_t each, const T* __restrict__ x, int64_t ld,
   if (parts > 1) cl.sync();  // no block leaves while another reads its memory
 }
 
+// Rows of which |lse| is above this have their sum made anew.
+constexpr float kLseExact = 32.0f;
+
 // dx = p (A l + B) (+ the target's own term), with l = log p, A = -scale h',
-// B = -scale (h' H + g'); h', g': gradients of entropy H and of logp.
+// B = -scale (h' H + g'); h', g': gradients of entropy H and of logp. l is
+// scale x - lse, or scale (x - m) - ls where that would lose too much.
 template <typename T, bool ENT, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 k_log_probs_bwd(uint32_t n, uint32_t parts, uint32_t each, const T* x, int64_t ld,
@@ -302,71 +315,100 @@ k_log_probs_bwd(uint32_t n, uint32_t parts, uint32_t each, const T* x, int64_t l
                 const float* __restrict__ grad_entropy, T* dx, int64_t ldd) {
   constexpr int V = Piece<T>::V, U = 4;
   const int64_t r = parts == 1 ? blockIdx.x : blockIdx.x / parts;
-  const Share<T> sh(x + r * ld, n, blockIdx.x - (uint32_t)r * parts, each);
-  T* out = dx + r * ldd + sh.start;
-  const float z0 = lse[r];
-  const float z = z0 == -INFINITY ? INFINITY : z0;  // a row masked whole: p = 0
+  const uint32_t part = blockIdx.x - (uint32_t)r * parts;
+  const T* xr = x + r * ld;
   const int32_t at = grad_logp ? target[r] : -1;
   const bool has = at >= 0 && at < (int64_t)n;
-  const float g = has ? grad_logp[r] : 0.0f;
+  const float z = lse[r], g = has ? grad_logp[r] : 0.0f;
   const float gh = ENT ? grad_entropy[r] : 0.0f;
   const float A = -scale * gh, B = -scale * fmaf(gh, ENT ? entropy[r] : 0.0f, g);
-  // Where the target is within this share; no index where it is not.
-  const uint32_t hot = has && (uint32_t)at - sh.start < sh.count ? (uint32_t)at - sh.start : ~0u;
-  const F2 s2 = pack2(scale, scale), z2 = pack2(-z, -z), e2 = pack2(kLog2e, kLog2e);
+  const F2 s2 = pack2(scale, scale), e2 = pack2(kLog2e, kLog2e);
   const F2 A2 = pack2(A, A), B2 = pack2(B, B);
-  // Gradients of two values. l is kept off -inf (p is 0 long before): 0 times it would be NaN.
-  auto two = [&](F2 v, float& a, float& b) {
-    F2 l = fma2(v, s2, z2);
-    if (ENT) {
-      unpack2(l, a, b);
-      l = pack2(max_nan(a, -1000.0f), max_nan(b, -1000.0f));
-    }
-    unpack2(mul2(l, e2), a, b);
-    const F2 p = pack2(exp2_approx(a), exp2_approx(b));
-    unpack2(mul2(p, ENT ? fma2(A2, l, B2) : B2), a, b);
-  };
-  auto single = [&](uint32_t i) {
-    const float v = to_f32(sh.p[i]);
-    float a, b;
-    two(pack2(v, v), a, b);
-    out[i] = from_f32<T>(a);
-  };
-  // The target's own term is added by the thread that has written it.
-  uint32_t owner = hot - sh.head;
-  if (hot < sh.head) owner = hot;
-  else if (hot >= sh.tail_at()) owner = hot - sh.tail_at();
-  else owner = owner / V % THREADS;
-  const bool mine = hot != ~0u && threadIdx.x == owner;
-  const float x_hot = mine ? to_f32(sh.p[hot]) : 0.0f;
-  if (threadIdx.x < sh.head) single(threadIdx.x);
-  if (threadIdx.x < sh.tail) single(sh.tail_at() + threadIdx.x);
-  sh.with_whole(out, [&](auto whole) {
-    auto piece = [&](uint32_t i, const uint4& q, int on = 0) {
-      uint4 o;
-#pragma unroll
-      for (int k = 0; k < V / 2; ++k) {
-        float a, b;
-        two(Piece<T>::pair(q, k), a, b);
-        Piece<T>::put(o, k, a, b);
+  // A share's gradient: `first` holds the thread's first U pieces already
+  // (FROM_LSE), or each is loaded where it is needed.
+  auto write = [&](auto from_lse, const Share<T>& sh, const uint4 (&first)[U], float m, float ls) {
+    constexpr bool FROM_LSE = decltype(from_lse)::value;
+    T* out = dx + r * ldd + sh.start;
+    // Where the target is within this share; no index where it is not.
+    const uint32_t hot = has && (uint32_t)at - sh.start < sh.count ? (uint32_t)at - sh.start : ~0u;
+    const F2 m2 = pack2(-m, -m), z2 = pack2(-ls, -ls);
+    // Gradients of two values. l is kept off -inf (p is 0 long before): 0 times it would be NaN.
+    auto two = [&](F2 v, float& a, float& b) {
+      F2 l = fma2(FROM_LSE ? v : add2(v, m2), s2, z2);
+      if (ENT) {
+        unpack2(l, a, b);
+        l = pack2(max_nan(a, -1000.0f), max_nan(b, -1000.0f));
       }
-      sh.template put_piece<decltype(whole)::value>(out, i, o, on);
+      unpack2(mul2(l, e2), a, b);
+      const F2 p = pack2(exp2_approx(a), exp2_approx(b));
+      unpack2(mul2(p, ENT ? fma2(A2, l, B2) : B2), a, b);
     };
-    uint32_t i = threadIdx.x;
-    for (; i + (U - 1) * THREADS < sh.pieces; i += U * THREADS) {
-      uint4 q[U];
+    auto single = [&](uint32_t i) {
+      const float v = to_f32(sh.p[i]);
+      float a, b;
+      two(pack2(v, v), a, b);
+      out[i] = from_f32<T>(a);
+    };
+    // The target's own term is added by the thread that has written it.
+    uint32_t owner = hot - sh.head;
+    if (hot < sh.head) owner = hot;
+    else if (hot >= sh.tail_at()) owner = hot - sh.tail_at();
+    else owner = owner / V % THREADS;
+    const bool mine = hot != ~0u && threadIdx.x == owner;
+    const float x_hot = mine ? to_f32(sh.p[hot]) : 0.0f;
+    if (threadIdx.x < sh.head) single(threadIdx.x);
+    if (threadIdx.x < sh.tail) single(sh.tail_at() + threadIdx.x);
+    sh.with_whole(out, [&](auto whole) {
+      auto piece = [&](uint32_t i, const uint4& q, int on = 0) {
+        uint4 o;
 #pragma unroll
-      for (int u = 0; u < U; ++u) q[u] = sh.piece(i, u * THREADS);
+        for (int k = 0; k < V / 2; ++k) {
+          float a, b;
+          two(Piece<T>::pair(q, k), a, b);
+          Piece<T>::put(o, k, a, b);
+        }
+        sh.template put_piece<decltype(whole)::value>(out, i, o, on);
+      };
+      uint32_t i = threadIdx.x;
+      if (FROM_LSE) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) piece(i, q[u], u * THREADS);
+        for (int u = 0; u < U; ++u)
+          if (i + u * THREADS < sh.pieces) piece(i, first[u], u * THREADS);
+        i += U * THREADS;
+      }
+      for (; i + (U - 1) * THREADS < sh.pieces; i += U * THREADS) {
+        uint4 q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = sh.piece(i, u * THREADS);
+#pragma unroll
+        for (int u = 0; u < U; ++u) piece(i, q[u], u * THREADS);
+      }
+      for (; i < sh.pieces; i += THREADS) piece(i, sh.piece(i));
+    });
+    if (mine) {
+      float a, b;
+      two(pack2(x_hot, x_hot), a, b);
+      out[hot] = from_f32<T>(fmaf(g, scale, a));
     }
-    for (; i < sh.pieces; i += THREADS) piece(i, sh.piece(i));
-  });
-  if (mine) {
-    float a, b;
-    two(pack2(x_hot, x_hot), a, b);
-    out[hot] = from_f32<T>(fmaf(g, scale, a));
+  };
+  const Share<T> own(xr, n, part, each);
+  uint4 first[U];  // on their way while lse is
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (threadIdx.x + u * THREADS < own.pieces) first[u] = own.piece(threadIdx.x, u * THREADS);
+  if (fabsf(z) <= kLseExact) {
+    write(std::true_type{}, own, first, 0.0f, z);
+    return;
   }
+  // The whole row is the first block's: others may not write while it is read.
+  if (part != 0) return;
+  __shared__ Sums all[THREADS / 32];
+  const float c = scale * kLog2e;
+  const Share<T> row(xr, n, 0, n);
+  const Sums v = join_block<false, THREADS / 32>(
+      scan_share<T, false, false, false, THREADS>(row, c, nullptr), c, all);
+  const bool none = v.m == -INFINITY;  // masked whole: p = 0
+  write(std::false_type{}, row, first, none ? 0.0f : v.m, none ? INFINITY : logf(v.s));
 }
 
 }  // namespace

@@ -1,0 +1,78 @@
+"""The read-out operators on the device where 32 bits are tight or an array ends: rows far from
+zero, rows of one value, single values of long rows, results and scratch between guards.
+
+Bounds count the kernels' own roundings (U = 2^-24 each) on the inputs as rounded to their type."""
+import numpy as np
+import pytest
+import torch
+
+import readout_formulas as F
+from plastix_b200 import readout
+from test_readout_gpu import HALF_STEP, TINY, TYPES, U, f64, rows_tensor, within
+
+pytestmark = pytest.mark.gpu
+
+
+def batches(n):
+    """Steps of sixteen values or more in which a thread goes over its share of a row: 64 threads
+    have fewer than 8,192 values between them, 128 or more take the longer rows."""
+    return 8 + n / 2048
+
+
+def sum_error(n, spread):
+    """Relative error of sum exp(d): a value is added within its step (16), over the steps, a
+    warp (5), a block (5) and a cluster (8); the sum is moved to a new maximum once a step and
+    twelve times while it is joined at most, at 6 U each (2^x to 4 U and a product); 2^x has 4 U, and its
+    argument four roundings of its size (`spread`: the mean of |d| under the softmax)."""
+    return U * (40 + batches(n) + 6 * (batches(n) + 12) + 4 * spread)
+
+
+# ------------------------------------------------------------------- gradients far from zero
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [100, 4099, 70000, 300007])
+@pytest.mark.parametrize("scale", [1.0, 2.0])
+def test_gradient_of_log_probs_far_from_zero(ctx, dtype, n, scale):
+    """Rows around large values, and rows of the type's lowest value, have the gradient of the
+    same row around zero: no bound below depends on the offset."""
+    r = np.random.default_rng(n)
+    low = float(torch.finfo(TYPES[dtype]).min)
+    a = r.normal(size=(10, n)) * 2.5
+    a += np.array([0.0, 25.0, 40.0, 1000.0, -1000.0, 30000.0, -30000.0, 0.0, 0.0, 0.0])[:, None]
+    a[7] = low
+    a[8] = np.where(np.arange(n) % 3 == 1, low, -np.inf)
+    a[9] = -np.inf
+    x, _ = rows_tensor(a, dtype)
+    target = torch.from_numpy(r.integers(0, n, 10)).int().cuda()
+    target[8] = 1
+    gl = torch.from_numpy(r.normal(size=10)).float().cuda()
+    ge = torch.from_numpy(r.normal(size=10)).float().cuda()
+    s = readout.log_probs(ctx, x, target, scale=scale, entropy=True)
+    both = readout.log_probs_backward(ctx, x, s.lse, target, gl, s.entropy, ge, scale=scale)
+    alone = readout.log_probs_backward(ctx, x, s.lse, target, gl, scale=scale)
+    into = x.clone()
+    assert readout.log_probs_backward(ctx, into, s.lse, target, gl, scale=scale, out=into) is into
+    ctx.sync()
+    assert torch.equal(into, alone)
+    X, at, GL, GE = f64(x), target.cpu().numpy(), f64(gl), f64(ge)
+    # an offset changes nothing, and the lowest value would take log n with it in 64 bits too
+    X -= np.where(np.isfinite(X.max(1, keepdims=True)), X.max(1, keepdims=True), 0.0)
+    logs, lse = F.log_softmax(X * scale)
+    p = np.exp(logs)
+    l = np.where(p > 0, np.abs(logs), 0.0)  # noqa: E741
+    with np.errstate(invalid="ignore"):
+        d = np.where(p > 0, np.abs(scale * X), 0.0)
+    ls = np.where(np.isfinite(lse), lse, 0.0)  # log of the sum
+    entropy, spread = (p * l).sum(1), (p * d).sum(1)
+    e = sum_error(n, spread)
+    # log p: the argument and its difference (3 |l| + 2 |d|), the logarithm (2 |ls|), lse rounded below
+    # 32 (16), 2^x and the products (12)
+    pe = e[:, None] + U * (28 + 3 * l + 2 * d + 2 * ls[:, None])
+    # entropy: log s, and sum e d / s whose terms are off by twice what the sum is
+    he = (e + 4 * U * ls + spread * (2 * e + 6 * U) + U * entropy)[:, None]
+    half = HALF_STEP[dtype]
+    for got, ge_ in ((alone, None), (both, GE)):
+        want = F.log_probs_backward(X, at, scale, GL, ge_)
+        g, h = np.abs(GL)[:, None], 0.0 if ge_ is None else np.abs(GE)[:, None]
+        inner = g + h * (l + entropy[:, None])
+        err = scale * (p * (pe * (inner + h) + h * he + 6 * U * inner) + 2 * U * g)
+        within(f64(got), want, err * (1 + half) + half * np.abs(want) + 2 * TINY[dtype], "gradient")
