@@ -1,7 +1,11 @@
 // Layer norm of rows of unit activations.
 //   mu = mean x; rstd = 1/sqrt(mean (x-mu)^2 + eps); y = (x-mu) rstd w + b
-// Everything between load and store is in 32 bits; the variance is taken of
-// x - mu, so a large common offset costs no accuracy.
+// Everything between load and store is in 32 bits. The mean is off by its sum's
+// roundings, which around a large value are as large as the deviations; so the
+// deviations d from that first mean are summed along with their squares, and
+// what they have of a mean is taken away: mu = first + mean d, variance =
+// mean d^2 - (mean d)^2. A large common offset costs no accuracy (rows of one
+// value come out below 1e-5), and the second sum rides along with the first.
 //
 // Bound by memory (each value read once, written once): a row is held in
 // registers by the threads that share it, a warp for rows of up to 128
@@ -10,13 +14,27 @@
 // same for every thread (32,768 rows of 4,096 bf16, before the last step: 128
 // threads 95 us, 256 107, 512 147), and weights that are read, applied, rounded
 // and stored piece by piece (95 to 87 us: fewer registers, more blocks an SM).
-// Measured: those rows 87 us, 6.2 TB/s; 8,192 rows of 16,384 bf16 94 us, 5.7
-// TB/s; 65,536 rows of 1,024 bf16 49 us, 5.5 TB/s; 16,384 rows of 2,049 f32 (one
-// value a load) 53 us, 5.1 TB/s; of 4,097 bf16 (staged) 117 us, 2.3 TB/s.
+// The sum of d costs two to four per cent of a long row's time (those rows 88 us
+// without). Measured: those rows 90 us, 5.9 TB/s; 8,192 rows of 16,384 bf16 98
+// us, 5.5 TB/s; 65,536 rows of 1,024 bf16 50 us, 5.3 TB/s; 16,384 rows of 2,049
+// f32 (one value a load) 52 us, 5.2 TB/s; of 4,097 bf16 (staged) 117 us, 2.3
+// TB/s; 1,024 rows of 65,536 bf16 (too long for registers) 118 us, 2.3 TB/s.
 #include "norm.cuh"
 
 namespace plx {
 namespace {
+
+struct RowStats {
+  float mean, rstd, shift;  // h = d rstd + shift
+};
+// From the first mean and the sums of d and d^2. rsqrtf is two units in the last
+// place off at most; max_nan: a variance that rounds below 0 is 0, NaN stays.
+__device__ __forceinline__ RowStats row_stats(float first, float d, float d2, float inv_n,
+                                              float eps) {
+  const float e = d * inv_n;
+  const float rs = rsqrtf(max_nan(fmaf(-e, e, d2 * inv_n), 0.0f) + eps);
+  return {first + e, rs, -e * rs};
+}
 
 template <typename T, typename P, int V, int NV, int TPR>
 __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 512 && V >= 4 ? 2 : 1)
@@ -24,7 +42,7 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
        const P* __restrict__ b, float eps, float inv_n, T* y, int64_t ldy,
        float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int ROWS = TPR == 32 ? 8 : 1;
-  __shared__ float red[2 * (TPR / 32)];
+  __shared__ float red[4 * (TPR / 32)];
   const uint32_t lane = threadIdx.x % TPR;
   const uint32_t r = blockIdx.x * ROWS + threadIdx.x / TPR;
   if (ROWS > 1 && r >= rows) return;
@@ -82,15 +100,18 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
         const int k = j * V + e;
         (k & 1 ? v[k / 2].y : v[k / 2].x) = 0.0f;
       }
-  s2 = pack2(0.0f, 0.0f);
+  F2 d2 = pack2(0.0f, 0.0f);
+  s2 = d2;
 #pragma unroll
-  for (int h = 0; h < H; ++h) s2 = fma2(v[h], v[h], s2);
-  s[0] = s2.x + s2.y;
-  row_sum<TPR>(s, red, turn);
-  const float rs = rsqrtf(fmaf(s[0], inv_n, eps));  // two units in the last place at most
-  const F2 rs2 = pack2(rs, rs);
+  for (int h = 0; h < H; ++h) {
+    d2 = add2(v[h], d2);
+    s2 = fma2(v[h], v[h], s2);
+  }
+  const F2 sums = row_sum2<TPR>(pack2(d2.x + d2.y, s2.x + s2.y), red, turn);
+  const RowStats st = row_stats(mu, sums.x, sums.y, inv_n, eps);
+  const F2 rs2 = pack2(st.rstd, st.rstd), shift2 = pack2(st.shift, st.shift);
 #pragma unroll
-  for (int h = 0; h < H; ++h) v[h] = mul2(v[h], rs2);
+  for (int h = 0; h < H; ++h) v[h] = fma2(v[h], rs2, shift2);
   // Weights (out of L1), rounding and storing piece by piece: few of them are
   // live at once.
   T* yl = y + r * ldy + lane * V;
@@ -128,8 +149,8 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
   else if (b) finish(No{}, Yes{});
   else finish(No{}, No{});
   if (lane == 0) {
-    if (mean) mean[r] = mu;
-    if (rstd) rstd[r] = rs;
+    if (mean) mean[r] = st.mean;
+    if (rstd) rstd[r] = st.rstd;
   }
 }
 
@@ -138,27 +159,30 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
 template <typename T, typename P>
 __global__ void __launch_bounds__(1024)
 k_norm_long(uint32_t n, const T* x, int64_t ldx, const P* __restrict__ w,
-            const P* __restrict__ b, float eps, T* y, int64_t ldy, float* __restrict__ mean,
-            float* __restrict__ rstd) {
+            const P* __restrict__ b, float eps, float inv_n, T* y, int64_t ldy,
+            float* __restrict__ mean, float* __restrict__ rstd) {
   __shared__ float red[32];
   const int64_t r = blockIdx.x;
   const T* xr = x + r * ldx;
   T* yr = y + r * ldy;
   float s = 0.0f;
   for (uint32_t i = threadIdx.x; i < n; i += 1024) s += to_f32(xr[i]);
-  const float mu = block_sum<32>(s, red) / (float)n;
+  const float mu = block_sum<32>(s, red) * inv_n;
   s = 0.0f;
+  float e = 0.0f;
   for (uint32_t i = threadIdx.x; i < n; i += 1024) {
     const float d = to_f32(xr[i]) - mu;
+    e += d;
     s = fmaf(d, d, s);
   }
-  const float rs = 1.0f / sqrtf(block_sum<32>(s, red) / (float)n + eps);
+  e = block_sum<32>(e, red);
+  const RowStats st = row_stats(mu, e, block_sum<32>(s, red), inv_n, eps);
   for (uint32_t i = threadIdx.x; i < n; i += 1024)
-    yr[i] = from_f32<T>(fmaf((to_f32(xr[i]) - mu) * rs, w ? to_f32(w[i]) : 1.0f,
+    yr[i] = from_f32<T>(fmaf(fmaf(to_f32(xr[i]) - mu, st.rstd, st.shift), w ? to_f32(w[i]) : 1.0f,
                              b ? to_f32(b[i]) : 0.0f));
   if (threadIdx.x == 0) {
-    if (mean) mean[r] = mu;
-    if (rstd) rstd[r] = rs;
+    if (mean) mean[r] = st.mean;
+    if (rstd) rstd[r] = st.rstd;
   }
 }
 
@@ -196,8 +220,8 @@ extern "C" int plx_layer_norm(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype
       const uint32_t v = piece_values(n, sizeof(T), {x, y}, {ldx, ldy}, weight, bias, sizeof(P));
       auto loops = [&] {
         k_norm_long<T, P><<<one, 1024, 0, ctx->stream>>>(n, (const T*)x, ldx, (const P*)weight,
-                                                         (const P*)bias, eps, (T*)y, ldy, mean,
-                                                         rstd);
+                                                         (const P*)bias, eps, 1.0f / (float)n,
+                                                         (T*)y, ldy, mean, rstd);
       };
       if (v == V) {
         const uint32_t pieces = n / V;

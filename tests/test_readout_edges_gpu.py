@@ -76,3 +76,55 @@ def test_gradient_of_log_probs_far_from_zero(ctx, dtype, n, scale):
         inner = g + h * (l + entropy[:, None])
         err = scale * (p * (pe * (inner + h) + h * he + 6 * U * inner) + 2 * U * g)
         within(f64(got), want, err * (1 + half) + half * np.abs(want) + 2 * TINY[dtype], "gradient")
+
+
+# --------------------------------------------------------------------- layer norm far from zero
+def norm_depth(n):
+    """Additions a value goes through: pairs of up to 16 values a thread and two sums' exchange
+    over a block, or, in rows too long for registers, n / 1,024 a thread and two steps of 32."""
+    return 80 + n / 1024
+
+
+@pytest.mark.parametrize("n", [3, 100, 513, 1000, 1001, 2049, 4096, 5001, 8190, 16384, 20001])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_layer_norm_of_rows_of_one_value(ctx, dtype, n):
+    """The mean may be a rounding off, delta <= (depth + 2) U |x|; the deviations, all delta, have a
+    mean of their own, which is off by (depth + 2) U of it and is taken away."""
+    r = np.random.default_rng(n)
+    a = np.repeat(r.uniform(-1000, 1000, (40, 1)), n, 1)
+    x, _ = rows_tensor(a, dtype)
+    y, mean, rstd = readout.layer_norm(ctx, x, eps=1e-5, stats=True)
+    ctx.sync()
+    X = f64(x)
+    k = (norm_depth(n) + 4) * U
+    delta = k * np.abs(X[:, :1])
+    root = 1e5 ** 0.5
+    within(f64(y), X * 0, np.broadcast_to(1.01 * root * k * delta, X.shape), "y")
+    within(f64(mean), X[:, 0], U * np.abs(X[:, 0]) + 2 * k * delta[:, 0], "mean")
+    # the variance left is 3 k delta^2 at most; eps in 32 bits, its root and two more roundings
+    within(f64(rstd), np.full(40, root), root * (2 * k * delta[:, 0] ** 2 / 1e-5 + 6 * U), "rstd")
+
+
+@pytest.mark.parametrize("rows, n, dtype", [(50, 1000, "f32"), (50, 1001, "f32"), (30, 4096, "f32"),
+                                            (20, 16384, "f32"), (20, 20000, "f32"), (50, 4096, "f16"),
+                                            (50, 1001, "f16")])
+def test_layer_norm_around_a_large_value(ctx, rows, n, dtype):
+    """Deviations of about one around 1e6 (f32) or 1,000 (f16): x - mean is exact there, so only
+    the deviations' own mean, variance and products round."""
+    r = np.random.default_rng(n)
+    x, _ = rows_tensor((1e6 if dtype == "f32" else 1000.0) + 2 * r.normal(size=(rows, n)), dtype)
+    y, mean, rstd = readout.layer_norm(ctx, x, eps=1e-5, stats=True)
+    ctx.sync()
+    X = f64(x)
+    Y, M, R = F.layer_norm(X, np.ones(n), np.zeros(n), 1e-5)
+    k = norm_depth(n) * U
+    delta = (k + 2 * U) * np.abs(M)  # of the first mean
+    shift = (k + 3 * U) * (delta + np.abs(X - M[:, None]).mean(1))  # what is left of it
+    # variance: sums of squares (deviation^2 + delta^2) to k, less the square of the shift
+    rel = (k + 6 * U) * (1 + 2 * (delta * R) ** 2) + 2 * shift * delta * R * R + (shift * R) ** 2
+    h = np.abs(Y) + (delta * R)[:, None]
+    half = HALF_STEP[dtype]
+    tol = (shift * R)[:, None] + h * rel[:, None] + 4 * U * h
+    within(f64(y), Y, tol * (1 + half) + half * np.abs(Y) + TINY[dtype], "y")
+    within(f64(mean), M, U * np.abs(M) + 2 * shift, "mean")
+    within(f64(rstd), R, R * (rel + 4 * U), "rstd")
