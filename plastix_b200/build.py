@@ -40,7 +40,8 @@ FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--fmad=false", "-Xcompiler", "-fPIC"
 
 
 def _headers() -> list[Path]:
-    return sorted(CSRC.glob("*.cuh")) + sorted((ROOT / "include").glob("*.h"))
+    return sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + \
+        sorted((ROOT / "include").glob("*.h"))
 
 
 def _stale(target: Path, deps: list[Path]) -> bool:

@@ -69,7 +69,7 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
     using St = Staged<T, TPR, NV>;
     __shared__ uint4 stage[ROWS * St::bytes / 16];
     char* at = reinterpret_cast<char*>(stage) + threadIdx.x / TPR * St::bytes;
-    St::fetch(at, xr, n, lane, r == 0, r == rows - 1);
+    St::fetch(at, x, ldx, rows, n, r, lane);
     copy_commit();
     copy_wait<0>();
     if (TPR == 32) __syncwarp();

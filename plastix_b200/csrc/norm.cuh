@@ -3,6 +3,7 @@
 
 #include <type_traits>
 
+#include "chunk_copy.h"
 #include "rows.cuh"
 
 namespace plx {
@@ -65,8 +66,8 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
 
 // Rows of 16-bit values of which not even two can be read together: sixteen-byte
 // chunks go to shared memory whole and the values are read from there. A
-// chunk's bytes outside its row are of the rows beside it; those before the
-// first row and behind the last are not touched.
+// chunk's bytes outside its row are of the rows beside it or of what lies
+// between them and are not used; nothing outside the array is touched.
 template <typename T, int TPR, int NV>
 struct Staged {
   static_assert(sizeof(T) == 2, "for 16-bit values");
@@ -75,20 +76,28 @@ struct Staged {
   static __device__ __forceinline__ uint32_t offset(const T* row) {
     return (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15u);
   }
-  // Starts the copies of this thread's chunks of a row.
-  static __device__ __forceinline__ void fetch(char* to, const T* row, uint32_t n, uint32_t lane,
-                                               bool first, bool last) {
+  // Starts the copies of this thread's chunks of row r of an array.
+  static __device__ __forceinline__ void fetch(char* to, const T* array, int64_t ld, uint32_t rows,
+                                               uint32_t n, uint32_t r, uint32_t lane) {
+    const T* row = array + r * ld;
     const uint32_t off = offset(row), end = off + 2 * n;
     const char* from = reinterpret_cast<const char*>(row) - off;
+    const bool near = near_edge(r, rows);
     for (uint32_t c = lane * 16; c < end; c += TPR * 16) {
-      if (c == 0 && off && first) {
-        for (uint32_t e = off; e < min(end, 16u); e += 2)
-          *reinterpret_cast<T*>(to + e) = *reinterpret_cast<const T*>(from + e);
-      } else {
-        const uint32_t have = last ? min(16u, end - c) : 16u;
+      ChunkCopy k{0u, 16u, true};
+      if (near) {
+        const uint64_t at = reinterpret_cast<uintptr_t>(row);
+        const uint64_t first = reinterpret_cast<uintptr_t>(array);
+        k = chunk_copy(at - off + c, at, at + 2 * n, first,
+                       first + ((rows - 1) * ld + n) * sizeof(T));
+      }
+      if (k.whole) {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(to + c)),
-                     "l"(from + c), "r"(have)
+                     "l"(from + c), "r"(k.to)
                      : "memory");
+      } else {
+        for (uint32_t e = c + k.from; e < c + k.to; e += 2)
+          *reinterpret_cast<T*>(to + e) = *reinterpret_cast<const T*>(from + e);
       }
     }
   }

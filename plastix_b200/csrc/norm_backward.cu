@@ -100,12 +100,12 @@ k_norm_bwd(uint32_t rows, uint32_t n, const T* dy, int64_t lddy, const T* x, int
   // Starts the copies of a row.
   auto fetch = [&](uint64_t row, uint32_t stage) {
     if (row < rows) {
-      const T *xr = x + row * ldx, *gr = dy + row * lddy;
       if constexpr (R::staged) {
-        const bool one = row == 0, end = row == rows - 1;
-        Staged<T, TPR, NV>::fetch(staged_row(stage, 0), xr, n, lane, one, end);
-        Staged<T, TPR, NV>::fetch(staged_row(stage, 1), gr, n, lane, one, end);
+        using St = Staged<T, TPR, NV>;
+        St::fetch(staged_row(stage, 0), x, ldx, rows, n, (uint32_t)row, lane);
+        St::fetch(staged_row(stage, 1), dy, lddy, rows, n, (uint32_t)row, lane);
       } else {
+        const T *xr = x + row * ldx, *gr = dy + row * lddy;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           if (j * STEP >= left) continue;

@@ -1,0 +1,49 @@
+"""The read-out operators without a device: where copies begin and end, sizes and scales that
+32 bits do not hold, scratch sizes, and the streams of the measured cases."""
+import subprocess
+from pathlib import Path
+
+CSRC = Path(__file__).resolve().parents[1] / "plastix_b200" / "csrc"
+
+CHUNKS = r"""
+#include <cstdio>
+#include <vector>
+#include "chunk_copy.h"
+// Every row of every small array of 16-bit values, copied as the kernels do: chunk by chunk into
+// zeros, every byte read inside the array, every value of the row there in the end.
+int main() {
+  long read = 0;
+  for (uint64_t base = 64; base < 80; base += 2)
+    for (uint64_t n = 1; n <= 20; ++n)
+      for (uint64_t ld = n; ld <= n + 9; ++ld)
+        for (uint64_t rows = 1; rows <= 20; ++rows) {
+          const uint64_t end = base + 2 * ((rows - 1) * ld + n);
+          for (uint64_t r = 0; r < rows; ++r) {
+            const uint64_t row = base + 2 * r * ld, row_end = row + 2 * n;
+            const bool near = plx::near_edge((uint32_t)r, (uint32_t)rows);
+            std::vector<bool> have(row_end + 16);
+            for (uint64_t c = row / 16 * 16; c < row_end; c += 16) {
+              const plx::ChunkCopy k = near ? plx::chunk_copy(c, row, row_end, base, end)
+                                             : plx::ChunkCopy{0, 16, true};
+              if (k.to > 16 || k.from > k.to || k.from % 2 || k.to % 2 || (k.whole && k.from)) return 1;
+              for (uint64_t b = c + k.from; b < c + k.to; ++b, ++read) {
+                if (b < base || b >= end) return 2;
+                have[b] = true;
+              }
+            }
+            for (uint64_t b = row; b < row_end; ++b)
+              if (!have[b]) return 3;
+          }
+        }
+  std::printf("%ld bytes\n", read);
+  return 0;
+}
+"""
+
+
+def test_chunks_of_odd_rows_stay_inside_their_array(tmp_path):
+    (tmp_path / "chunks.cpp").write_text(CHUNKS)
+    subprocess.run(["g++", "-std=c++17", "-O2", f"-I{CSRC}", str(tmp_path / "chunks.cpp"), "-o",
+                    str(tmp_path / "chunks")], check=True, capture_output=True, text=True)
+    done = subprocess.run([str(tmp_path / "chunks")], capture_output=True, text=True, timeout=60)
+    assert done.returncode == 0, f"a chunk is wrong ({done.returncode})"
