@@ -39,6 +39,12 @@ class LogProbs(NamedTuple):
     top_logp: Optional[torch.Tensor]
 
 
+def _check_count(count: int, name: str) -> None:
+    """Counts are 32-bit arguments of the library, which would take 2^32 + 8 as 8."""
+    if not 0 <= count < 1 << 31:
+        raise ValueError(f"{name} is {count}: 0 to fewer than 2^31 are supported")
+
+
 def _rows(ctx: Context, t: torch.Tensor, name: str):
     """(rows, n, row stride, type number) of a tensor of rows on the context's
     device."""
@@ -51,6 +57,7 @@ def _rows(ctx: Context, t: torch.Tensor, name: str):
     if len(shape) == 0 or shape[-1] == 0:
         raise ValueError(f"{name} needs a last dimension of units, got shape {tuple(shape)}")
     n = shape[-1]
+    _check_count(n, f"the last dimension of {name}")
     if len(shape) != 2:
         try:
             t = t.view(-1, n) if t.numel() else t.reshape(-1, n)
@@ -202,6 +209,7 @@ def log_probs(ctx: Context, logits: torch.Tensor, target: Optional[torch.Tensor]
     rows, n, ld, dtype = _rows(ctx, logits, "logits")
     lead = logits.shape[:-1]
     target_p = None if target is None else _like(ctx, target, lead, torch.int32, "target")
+    _check_count(top, "top")
     with _scope(ctx, logits, target):
         lse = logits.new_empty(lead, dtype=torch.float32)
         logp = None if target is None else torch.empty_like(lse)
@@ -267,6 +275,7 @@ def distill(ctx: Context, logits: torch.Tensor, teacher_ids: torch.Tensor,
     if teacher_ids.dim() == 0:
         raise ValueError("teacher_ids needs a last dimension of entries")
     k = teacher_ids.shape[-1]
+    _check_count(k, "the last dimension of teacher_ids")
     ids_p = _like(ctx, teacher_ids, lead + (k,), torch.int32, "teacher_ids")
     values_p = _like(ctx, teacher_values, lead + (k,), torch.float32, "teacher_values")
     if weight is not None:

@@ -3,6 +3,11 @@
 import subprocess
 from pathlib import Path
 
+import pytest
+import torch
+
+from plastix_b200 import readout
+
 CSRC = Path(__file__).resolve().parents[1] / "plastix_b200" / "csrc"
 
 CHUNKS = r"""
@@ -47,3 +52,29 @@ def test_chunks_of_odd_rows_stay_inside_their_array(tmp_path):
                     str(tmp_path / "chunks")], check=True, capture_output=True, text=True)
     done = subprocess.run([str(tmp_path / "chunks")], capture_output=True, text=True, timeout=60)
     assert done.returncode == 0, f"a chunk is wrong ({done.returncode})"
+
+
+class MetaContext:
+    """A context of tensors without memory: every call here is refused before its handle counts."""
+    device = torch.device("meta")
+    handle = None
+
+
+@pytest.mark.parametrize("n", [1 << 31, (1 << 32) + 8])
+def test_sizes_that_no_32_bit_argument_holds_are_refused(n):
+    # 2^32 + 8 would arrive as 8
+    c = MetaContext()
+    x = torch.empty(1, n, dtype=torch.bfloat16, device="meta")
+    small, one = torch.empty(1, 8, device="meta"), torch.empty(1, device="meta")
+    ids, values = (torch.empty(1, n, dtype=t, device="meta") for t in (torch.int32, torch.float32))
+    for call in (lambda: readout.layer_norm(c, x),
+                 lambda: readout.layer_norm_backward(c, x, x, one, one),
+                 lambda: readout.log_probs(c, x),
+                 lambda: readout.log_probs_backward(c, x, one, one.int(), one),
+                 lambda: readout.distill(c, x, ids[:, :4], values[:, :4]),
+                 lambda: readout.log_probs(c, small, top=n),
+                 lambda: readout.distill(c, small, ids, values)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()
+    with pytest.raises(ValueError, match="top"):
+        readout.log_probs(c, small, top=-1)
