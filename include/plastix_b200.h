@@ -629,7 +629,7 @@ int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, 
 #define PLX_TOP_MAX 64
 
 /* What the softmax of scale * logits answers in each row (scale > 0, the
- * inverse temperature; cf. SoftmaxCrossEntropyLoss, traits.hpp:222-240, whose
+ * inverse temperature, below 2.3e38; cf. SoftmaxCrossEntropyLoss, traits.hpp:222-240, whose
  * loss against a single target is -logp):
  *   lse      [rows]  log of the sum of exp(scale * x)
  *   logp     [rows]  log probability of target[row]; 0 for target -1 (none).

@@ -202,7 +202,7 @@ extern "C" int plx_distill(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, c
                            const float* row_weight, float* loss, void* dlogits, int64_t ldd) {
   if (int rc = check_logits(ctx, rows, n, dtype, logits, ld, temperature, "temperature"))
     return rc;
-  PLX_CHECK_ARG(1.0f / temperature < INFINITY, "temperature = %g is too small", temperature);
+  PLX_CHECK_ARG(1.0f / temperature * kLog2e < INFINITY, "temperature = %g is too small", temperature);
   PLX_CHECK_ARG(teacher_kind == PLX_TEACHER_LOGITS || teacher_kind == PLX_TEACHER_LOG_PROBS,
                 "teacher_kind %d is neither PLX_TEACHER_LOGITS nor PLX_TEACHER_LOG_PROBS",
                 teacher_kind);

@@ -411,6 +411,13 @@ k_log_probs_bwd(uint32_t n, uint32_t parts, uint32_t each, const T* x, int64_t l
   write(std::false_type{}, row, first, none ? 0.0f : v.m, none ? INFINITY : logf(v.s));
 }
 
+int check_scores(const plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* logits,
+                 int64_t ld, float scale) {
+  if (int rc = check_logits(ctx, rows, n, dtype, logits, ld, scale, "scale")) return rc;
+  PLX_CHECK_ARG(scale * kLog2e < INFINITY, "scale = %g is too large", scale);
+  return PLX_OK;
+}
+
 }  // namespace
 }  // namespace plx
 
@@ -420,7 +427,7 @@ extern "C" int plx_log_probs(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype,
                              const void* logits, int64_t ld, const int32_t* target, float scale,
                              uint32_t top, float* logp, float* lse, float* entropy,
                              int32_t* top_ids, float* top_logp) {
-  if (int rc = check_logits(ctx, rows, n, dtype, logits, ld, scale, "scale")) return rc;
+  if (int rc = check_scores(ctx, rows, n, dtype, logits, ld, scale)) return rc;
   PLX_CHECK_ARG(top <= n, "top = %u exceeds the %u outputs of a row", top, n);
   if (top > PLX_TOP_MAX)
     return set_error(PLX_ERR_CAPACITY, "top = %u: at most %d are supported", top, PLX_TOP_MAX);
@@ -470,7 +477,7 @@ extern "C" int plx_log_probs_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, i
                                       float scale, const float* lse, const float* entropy,
                                       const float* grad_logp, const float* grad_entropy,
                                       void* dlogits, int64_t ldd) {
-  if (int rc = check_logits(ctx, rows, n, dtype, logits, ld, scale, "scale")) return rc;
+  if (int rc = check_scores(ctx, rows, n, dtype, logits, ld, scale)) return rc;
   if (rows == 0) return PLX_OK;
   PLX_CHECK_ARG(grad_logp || grad_entropy, "grad_logp or grad_entropy is required");
   PLX_CHECK_ARG(!grad_logp || target, "grad_logp needs target");

@@ -6,7 +6,8 @@ from pathlib import Path
 import pytest
 import torch
 
-from plastix_b200 import readout
+from plastix_b200 import _abi, readout
+from test_readout import DISTILL, SCORE, SCORE_BWD, refused
 
 CSRC = Path(__file__).resolve().parents[1] / "plastix_b200" / "csrc"
 
@@ -78,3 +79,18 @@ def test_sizes_that_no_32_bit_argument_holds_are_refused(n):
             call()
     with pytest.raises(ValueError, match="top"):
         readout.log_probs(c, small, top=-1)
+
+
+def test_scales_that_leave_the_range_of_32_bits_are_refused():
+    """Exponents are taken to base 2: scale * log2 e (or log2 e / temperature) has to be finite,
+    or the largest logit's difference of 0 times it would be NaN."""
+    for scale in (2.4e38, 3.4e38):
+        refused(1, b"scale", "plx_log_probs", *{**SCORE, "scale": scale}.values())
+        refused(1, b"scale", "plx_log_probs_backward", *{**SCORE_BWD, "scale": scale}.values())
+    for tau in (3e-39, 4e-39):  # 1 / tau is finite
+        refused(1, b"too small", "plx_distill", *{**DISTILL, "tau": tau}.values())
+    # large, and fine: no rows, so that nothing more is asked of the pointers
+    lib = _abi.lib()
+    assert lib.plx_log_probs(*{**SCORE, "rows": 0, "scale": 2.3e38}.values()) == 0
+    assert lib.plx_distill(*{**DISTILL, "rows": 0, "tau": 3.4e38}.values()) == 0
+    assert lib.plx_distill(*{**DISTILL, "rows": 0, "tau": 5e-39}.values()) == 0
