@@ -144,6 +144,18 @@ def _param(ctx: Context, t: torch.Tensor, n: int, dtype, name: str) -> int:
     return _TYPES[t.dtype]
 
 
+def _params(ctx: Context, weight, bias, n: int, dtype) -> int:
+    """The type number of a weight and a bias, either of which may be None."""
+    kind = _abi.F32
+    if bias is not None:
+        kind = _param(ctx, bias, n, dtype, "bias")
+    if weight is not None:
+        other, kind = kind, _param(ctx, weight, n, dtype, "weight")
+        if bias is not None and other != kind:
+            raise ValueError("weight and bias have different types")
+    return kind
+
+
 def layer_norm(ctx: Context, x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None, *, eps: float = 1e-5, stats: bool = False,
                out: Optional[torch.Tensor] = None):
@@ -151,13 +163,7 @@ def layer_norm(ctx: Context, x: torch.Tensor, weight: Optional[torch.Tensor] = N
     ``weight`` plus ``bias`` ([n], float32 or x's type). With ``stats`` returns
     (y, mean, rstd), which ``layer_norm_backward`` takes. ``out`` may be x."""
     rows, n, ld, dtype = _rows(ctx, x, "x")
-    kind = _abi.F32
-    if bias is not None:
-        kind = _param(ctx, bias, n, x.dtype, "bias")
-    if weight is not None:
-        other, kind = kind, _param(ctx, weight, n, x.dtype, "weight")
-        if bias is not None and other != kind:
-            raise ValueError("weight and bias have different types")
+    kind = _params(ctx, weight, bias, n, x.dtype)
     with _scope(ctx, x, weight, bias, out):
         y, ldy = _result(ctx, out, x, ld, "out")
         mean = rstd = None
@@ -172,10 +178,13 @@ def layer_norm(ctx: Context, x: torch.Tensor, weight: Optional[torch.Tensor] = N
 
 def layer_norm_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor,
                         rstd: torch.Tensor, weight: Optional[torch.Tensor] = None, *,
+                        bias: Optional[torch.Tensor] = None,
                         out: Optional[torch.Tensor] = None):
-    """(dx, dweight, dbias) for the rows and statistics of ``layer_norm``;
-    dweight and dbias have weight's type and are None without a weight. The
-    same bits on every call. ``out`` (for dx) may be dy or x."""
+    """(dx, dweight, dbias) for the rows and statistics of ``layer_norm``.
+    dweight is None without a weight; dbias comes with a weight or with
+    ``bias``, which only a call without a weight needs to give. Both have the
+    parameters' type and the same bits on every call. ``out`` (for dx) may be
+    dy or x."""
     rows, n, ld, dtype = _rows(ctx, x, "x")
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError(f"dy has to be {x.dtype} {tuple(x.shape)}, got {dy.dtype} "
@@ -184,15 +193,17 @@ def layer_norm_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, mean: t
     lead = x.shape[:-1]
     mean_p = _like(ctx, mean, lead, torch.float32, "mean")
     rstd_p = _like(ctx, rstd, lead, torch.float32, "rstd")
-    kind = _abi.F32 if weight is None else _param(ctx, weight, n, x.dtype, "weight")
-    with _scope(ctx, dy, x, mean, rstd, weight, out):
+    kind = _params(ctx, weight, bias, n, x.dtype)
+    with _scope(ctx, dy, x, mean, rstd, weight, bias, out):
         dx, lddx = _result(ctx, out, dy, lddy, "out")
         if out is not None:
             _check_result(dx, lddx, x, ld, "out")
         dw = db = scratch = None
         size = 0
         if weight is not None:
-            dw, db = torch.empty_like(weight), torch.empty_like(weight)
+            dw = torch.empty_like(weight)
+        if weight is not None or bias is not None:
+            db = torch.empty_like(weight if bias is None else bias)
             size = _abi.lib().plx_layer_norm_scratch_bytes(rows, n)
             scratch = x.new_empty(size, dtype=torch.uint8)
         _abi.call("plx_layer_norm_backward", ctx.handle, rows, n, dtype, dy.data_ptr(), lddy,

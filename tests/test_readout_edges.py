@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from plastix_b200 import _abi, readout
-from test_readout import DISTILL, SCORE, SCORE_BWD, refused
+from test_readout import DISTILL, SCORE, SCORE_BWD, FakeContext, refused
 
 CSRC = Path(__file__).resolve().parents[1] / "plastix_b200" / "csrc"
 
@@ -94,3 +94,13 @@ def test_scales_that_leave_the_range_of_32_bits_are_refused():
     assert lib.plx_log_probs(*{**SCORE, "rows": 0, "scale": 2.3e38}.values()) == 0
     assert lib.plx_distill(*{**DISTILL, "rows": 0, "tau": 3.4e38}.values()) == 0
     assert lib.plx_distill(*{**DISTILL, "rows": 0, "tau": 5e-39}.values()) == 0
+
+
+def test_a_bias_in_the_backward_call_is_checked():
+    c, x, one = FakeContext(), torch.zeros(4, 8), torch.zeros(4)
+    for weight, bias in ((None, torch.zeros(7)), (None, torch.zeros(8).bfloat16()), (None, torch.zeros(8, 2)[:, 0])):
+        with pytest.raises(ValueError, match="bias"):
+            readout.layer_norm_backward(c, x, x, one, one, weight, bias=bias)
+    h = x.bfloat16()
+    with pytest.raises(ValueError, match="different types"):
+        readout.layer_norm_backward(c, h, h, one, one, torch.zeros(8), bias=torch.zeros(8).bfloat16())

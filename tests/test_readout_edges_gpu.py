@@ -128,3 +128,24 @@ def test_layer_norm_around_a_large_value(ctx, rows, n, dtype):
     within(f64(y), Y, tol * (1 + half) + half * np.abs(Y) + TINY[dtype], "y")
     within(f64(mean), M, U * np.abs(M) + 2 * shift, "mean")
     within(f64(rstd), R, R * (rel + 4 * U), "rstd")
+
+
+# ----------------------------------------------------------------------------- the bias' gradient
+@pytest.mark.parametrize("rows, n, dtype, btype", [(37, 513, "f32", "f32"), (300, 1024, "bf16", "bf16"),
+                                                   (9, 20001, "f16", "f32"), (0, 40, "f32", "f32")])
+def test_gradient_of_a_bias_without_a_weight(ctx, rows, n, dtype, btype):
+    r = np.random.default_rng(n)
+    x, dy = (rows_tensor(r.normal(size=(rows, n)), dtype)[0] for _ in range(2))
+    b = torch.from_numpy(r.normal(size=n)).to("cuda", TYPES[btype])
+    y, mean, rstd = readout.layer_norm(ctx, x, None, b, stats=True)
+    dx, dw, db = readout.layer_norm_backward(ctx, dy, x, mean, rstd, bias=b)
+    want = readout.layer_norm_backward(ctx, dy, x, mean, rstd)
+    one = torch.ones_like(b)
+    full = readout.layer_norm_backward(ctx, dy, x, mean, rstd, one, bias=b)
+    ctx.sync()
+    assert dw is None and want[1] is None and want[2] is None and torch.equal(dx, want[0])
+    assert db.dtype == b.dtype and torch.equal(db, full[2]) and torch.equal(dx, full[0])
+    DY = f64(dy)
+    half = HALF_STEP[btype]
+    tol = (rows + 8) * U * np.abs(DY).sum(0)  # every sum, whatever its order
+    within(f64(db), DY.sum(0), tol * (1 + half) + half * np.abs(DY.sum(0)) + TINY[btype], "db")
