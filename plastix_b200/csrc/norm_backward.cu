@@ -22,9 +22,18 @@ constexpr uint32_t kSms = 148;                // of a B200; fixes the order of t
 constexpr uint32_t kLongest = 16384;          // row of any type that stays in registers
 constexpr uint32_t kLongGroups = 64;          // runs of longer rows
 // Groups of column sums, at most: as many blocks an SM as the launches below
-// take for rows of this length.
+// take for the rows of this length that have the most, whatever their type and
+// alignment (each launch checks that for the longest row it is used for).
 constexpr uint32_t max_groups(uint32_t n) {
-  return n > kLongest ? kLongGroups : kSms * (n <= 1024 ? 8 : 4);
+  return n > kLongest ? kLongGroups : kSms * (n <= 1024 ? 8 : n <= 2048 ? 4 : n <= 5120 ? 2 : 1);
+}
+// Groups that `rows` rows leave, a block with `per_block` of them at a time and
+// `most` blocks: eight rows a block or more, if that leaves a block an SM; what
+// a block leaves to be joined costs as much as a few rows.
+uint32_t groups_of(uint64_t rows, uint32_t per_block, uint32_t most) {
+  const uint64_t by_rows = (rows + per_block - 1) / per_block;
+  return (uint32_t)std::min<uint64_t>(
+      std::min<uint64_t>(by_rows, std::max<uint64_t>(kSms, (by_rows + 7) / 8)), most);
 }
 
 // Rows under way at once, in shared memory: enough of them to keep memory busy
@@ -292,17 +301,14 @@ k_norm_join(uint32_t groups, uint32_t n, const float* __restrict__ partial, P* _
   }
 }
 
-uint32_t most_groups(uint64_t rows, uint32_t n) {
-  return (uint32_t)std::min<uint64_t>(std::max<uint64_t>(rows, 1), max_groups(n));
-}
-
 }  // namespace
 }  // namespace plx
 
 using namespace plx;
 
 extern "C" size_t plx_layer_norm_scratch_bytes(uint64_t rows, uint32_t n) {
-  return (size_t)most_groups(rows, n) * 2 * n * sizeof(float);
+  // One row a block: no launch leaves more groups. At least one, of no rows.
+  return (size_t)std::max(1u, groups_of(rows, 1, max_groups(n))) * 2 * n * sizeof(float);
 }
 
 extern "C" int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype,
@@ -341,15 +347,9 @@ extern "C" int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
         constexpr int NV = decltype(nv_c)::value, TPR = decltype(tpr_c)::value;
         constexpr int EACH = decltype(each_c)::value, VV = decltype(v_c)::value;
         using R = Ring<T, VV, NV, TPR>;
-        static_assert(NV * TPR * VV <= kLongest, "max_groups");
+        static_assert(kSms * EACH <= max_groups(NV * TPR * VV), "max_groups");
         constexpr auto kernel = k_norm_bwd<T, P, VV, NV, TPR, EACH>;
-        const uint32_t per_block = TPR == 32 ? 8 : 1;
-        // Eight rows a block or more, if that leaves a block an SM: what a block
-        // leaves to be joined costs as much as a few rows.
-        const uint64_t by_rows = (rows + per_block - 1) / per_block;
-        const uint32_t most = std::min<uint32_t>(kSms * EACH, max_groups(n));
-        groups = (uint32_t)std::min<uint64_t>(
-            std::min<uint64_t>(by_rows, std::max<uint64_t>(kSms, (by_rows + 7) / 8)), most);
+        groups = groups_of(rows, TPR == 32 ? 8 : 1, kSms * EACH);
         if (groups == 0) return PLX_OK;
         if (R::bytes > 32 * 1024)
           PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, R::bytes));

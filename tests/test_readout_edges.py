@@ -104,3 +104,14 @@ def test_a_bias_in_the_backward_call_is_checked():
     h = x.bfloat16()
     with pytest.raises(ValueError, match="different types"):
         readout.layer_norm_backward(c, h, h, one, one, torch.zeros(8), bias=torch.zeros(8).bfloat16())
+
+
+@pytest.mark.parametrize("n, most", [(8192, 148), (12288, 148), (16384, 148), (4096, 296), (5120, 296), (2048, 592),
+                                     (1024, 1184), (16385, 64)])
+def test_layer_norm_scratch_is_what_the_launches_leave(n, most):
+    """Column sums of at most as many blocks as run at once with rows this long, two rows of
+    32-bit values each; few rows leave a block an SM, of a row or more."""
+    size = lambda rows: _abi.lib().plx_layer_norm_scratch_bytes(rows, n) / (8 * n)  # noqa: E731
+    assert size(0) == size(1) == 1
+    assert size(100) == min(100, most) and size(600) == min(148, most)
+    assert size(1 << 20) == most

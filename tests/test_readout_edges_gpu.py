@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import readout_formulas as F
-from plastix_b200 import readout
+from plastix_b200 import _abi, readout
 from test_readout_gpu import HALF_STEP, TINY, TYPES, U, f64, rows_tensor, within
 
 pytestmark = pytest.mark.gpu
@@ -149,3 +149,30 @@ def test_gradient_of_a_bias_without_a_weight(ctx, rows, n, dtype, btype):
     half = HALF_STEP[btype]
     tol = (rows + 8) * U * np.abs(DY).sum(0)  # every sum, whatever its order
     within(f64(db), DY.sum(0), tol * (1 + half) + half * np.abs(DY.sum(0)) + TINY[btype], "db")
+
+
+# -------------------------------------------------------------------------- scratch between guards
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 120, 128, 250, 256, 510, 512, 1000, 1001, 1024, 1030, 2048, 2049, 2050,
+                               4096, 4098, 5001, 5120, 8190, 8192, 8193, 9000, 16384, 16392])
+def test_layer_norm_backward_keeps_to_its_scratch(ctx, dtype, n):
+    for rows in (1, 100, 1300, 20000):
+        if rows * n > 1 << 25:
+            continue
+        x = torch.randn(rows, n, device="cuda").to(TYPES[dtype])
+        w = torch.randn(n, device="cuda")
+        _, mean, rstd = readout.layer_norm(ctx, x, w, stats=True)
+        size = _abi.lib().plx_layer_norm_scratch_bytes(rows, n)
+        room = torch.full((size + 8192,), 0x5A, dtype=torch.uint8, device="cuda")
+        scratch = room[4096:4096 + size]
+        assert scratch.data_ptr() % 16 == 0
+        dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(w)
+        _abi.call("plx_layer_norm_backward", ctx.handle, rows, n, readout._TYPES[x.dtype], x.data_ptr(), n,
+                  x.data_ptr(), n, mean.data_ptr(), rstd.data_ptr(), _abi.F32, w.data_ptr(), dx.data_ptr(), n,
+                  dw.data_ptr(), db.data_ptr(), scratch.data_ptr(), size)
+        ctx.sync()
+        assert (room[:4096] == 0x5A).all() and (room[4096 + size:] == 0x5A).all()
+        # every sum of `rows` terms, in whatever order
+        want = x.double().sum(0)
+        off = (db.double() - want).abs()
+        assert bool((off <= (rows + 2) * U * x.double().abs().sum(0)).all())
