@@ -240,9 +240,13 @@ def _own(s):
     from plastix_b200 import readout
     from plastix_b200.runtime import Context
 
-    if _context is None:
-        _context = Context(torch.cuda.current_device())
+    device = s["x"].device
+    if _context is None or _context.device != device:
+        _context = Context(device.index)
     ctx = _context
+    # a context works on one stream: here torch's current one (asked for by its handle, which is cheap)
+    if torch._C._cuda_getCurrentRawStream(device.index) != ctx.stream.cuda_stream:
+        ctx.use_stream(torch.cuda.current_stream(device))
     if s["op"] == "norm":
         if not s["train"]:
             return {"y": readout.layer_norm(ctx, s["x"], s["w"], s["b"], eps=_EPS)}
