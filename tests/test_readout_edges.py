@@ -115,3 +115,36 @@ def test_layer_norm_scratch_is_what_the_launches_leave(n, most):
     assert size(0) == size(1) == 1
     assert size(100) == min(100, most) and size(600) == min(148, most)
     assert size(1 << 20) == most
+
+
+def test_measured_cases_run_on_the_current_stream(monkeypatch):
+    """A pass under another current stream, or on another device, uses that one."""
+    from types import SimpleNamespace
+
+    from perf import operators
+    from plastix_b200 import runtime
+
+    now = {}
+
+    class FakeRuntimeContext:
+        def __init__(self, index=0, stream=None):
+            self.device, self.stream = torch.device("cuda", index), stream or now["stream"]
+
+        def use_stream(self, stream):
+            self.stream = stream
+
+    seen = []
+    monkeypatch.setattr(runtime, "Context", FakeRuntimeContext)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: now["stream"])
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: now["stream"].cuda_stream, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now["device"])
+    monkeypatch.setattr(readout, "layer_norm",
+                        lambda ctx, *a, **k: seen.append((ctx.device.index, ctx.stream.cuda_stream)))
+    monkeypatch.setattr(operators, "own", True)
+    monkeypatch.setattr(operators, "_context", None)
+    wanted = [(0, 7), (0, 7), (0, 8), (1, 9), (0, 7)]
+    for device, stream in wanted:
+        now.update(device=device, stream=SimpleNamespace(cuda_stream=stream))
+        x = SimpleNamespace(device=torch.device("cuda", device))
+        operators.run({"op": "norm", "train": False, "x": x, "w": None, "b": None})
+    assert seen == wanted
