@@ -176,3 +176,92 @@ def test_layer_norm_backward_keeps_to_its_scratch(ctx, dtype, n):
         want = x.double().sum(0)
         off = (db.double() - want).abs()
         assert bool((off <= (rows + 2) * U * x.double().abs().sum(0)).all())
+
+
+# ------------------------------------------------------------- every value of a row, every branch
+COUNTED = [1, 7, 64, 1000, 4099, 8191, 20011, 32003, 65536, 131072, 131077, 1 << 20]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 8, 400])
+def test_no_value_of_a_row_is_left_out(ctx, dtype, rows):
+    """n equal values: the sum is n exactly in whatever order (a whole number below 2^24), so lse is
+    off by the logarithm's and two more roundings only, far less than one value of a million."""
+    for n in COUNTED:
+        if rows * n > 1 << 26:
+            continue
+        for shift in (0, 1, 5):
+            room = torch.full((shift + rows * (n + 3) + 8,), 7.0, dtype=TYPES[dtype], device="cuda")
+            x = room.as_strided((rows, n), (n + 3, 1), shift).zero_()
+            want = np.log(n)
+            target = torch.full((rows,), n - 1, dtype=torch.int32, device="cuda")
+            got = [readout.log_probs(ctx, x), readout.log_probs(ctx, x, target, entropy=True),
+                   readout.log_probs(ctx, x, top=min(3, n)),
+                   readout.log_probs(ctx, x, target, entropy=True, top=min(3, n))]
+            ids = torch.zeros(rows, 1, dtype=torch.int32, device="cuda")
+            loss = readout.distill(ctx, x, ids, torch.zeros(rows, 1, device="cuda"))[0]
+            ctx.sync()
+            # logf: one unit in the last place, two half units at most of its size; two more roundings
+            tol = 4 * U * want
+            for r in got:
+                within(f64(r.lse), np.full(rows, want), tol, "lse")
+                if r.entropy is not None:
+                    within(f64(r.entropy), np.full(rows, want), tol, "entropy")
+                    within(f64(r.logp), np.full(rows, -want), tol, "logp")
+            within(f64(loss), np.full(rows, want), tol, "loss")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows, n", [(3, 1), (600, 1), (5, 900), (600, 5000), (400, 9000), (600, 20011),
+                                     (300, 40000), (7, 50001), (2, 300007)])
+def test_entropy_without_alternatives(ctx, rows, n, dtype):
+    r = np.random.default_rng(rows + n)
+    a = r.normal(size=(rows, n)) * 2.5
+    if n > 1:
+        a[::3] = np.where(r.random(a[::3].shape) < 0.3, -np.inf, a[::3])
+        a[::3, n // 2] = 0.5
+        a[-1] = -np.inf
+        a[1, 0] = np.nan
+    x, _ = rows_tensor(a, dtype)
+    target = torch.from_numpy(r.integers(-1, n, rows)).int().cuda()
+    got = readout.log_probs(ctx, x, target, scale=0.75, entropy=True)
+    ctx.sync()
+    assert got.top_ids is None and got.top_logp is None
+    X, at = f64(x), target.cpu().numpy()
+    want = F.log_probs(X, at, 0.75)
+    logs, lse = F.log_softmax(0.75 * X)
+    fine = np.isfinite(lse)
+    top = np.where(fine, np.where(np.isnan(X), -np.inf, X).max(1), 0.0)
+    with np.errstate(invalid="ignore"):
+        ls = np.where(fine, lse - 0.75 * top, 0.0)
+        p = np.where(fine[:, None], np.exp(logs), 0.0)
+        d = np.where(p > 0, np.abs(0.75 * (X - top[:, None])), 0.0)
+    spread = (p * d).sum(1)
+    e = sum_error(n, spread)
+    near = e + 4 * U * np.abs(ls)
+    within(f64(got.lse), want["lse"], near + 4 * U * np.abs(np.where(fine, lse, 0)), "lse")
+    within(f64(got.entropy), want["entropy"],
+           near + spread * (2 * e + 6 * U) + U * np.where(fine, np.abs(want["entropy"]), 0), "entropy")
+    x_at = X[np.arange(rows), np.maximum(at, 0)]
+    with np.errstate(invalid="ignore"):
+        away = np.where(np.isfinite(x_at), np.abs(0.75 * (x_at - top)), 0.0)
+    within(f64(got.logp), want["logp"], near + 4 * U * away, "logp")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [2, 40, 150])
+def test_alternatives_of_rows_whose_best_values_few_threads_hold(ctx, rows, dtype):
+    """In every 16,384 values, 20 threads of 256 hold 1,280 of the best: too many to be ordered at
+    once, and fewer threads than alternatives. Odd rows have equals among them."""
+    n, top = 131072, 64
+    r = np.random.default_rng(rows)
+    a = r.normal(size=(rows, n)).clip(-6, 6)
+    v = 16 // torch.empty(0, dtype=TYPES[dtype]).element_size()
+    at = np.arange(n) // v % 256 < 20
+    best = r.uniform(10, 20, (rows, int(at.sum())))
+    best[1::2] = np.floor(best[1::2] * 4) / 4
+    a[:, at] = best
+    x, _ = rows_tensor(a, dtype)
+    got = readout.log_probs(ctx, x, top=top)
+    ctx.sync()
+    np.testing.assert_array_equal(got.top_ids.cpu().numpy(), F.order(f64(x))[:, :top])
