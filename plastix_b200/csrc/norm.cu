@@ -1,11 +1,13 @@
 // Layer norm of rows of unit activations.
 //   mu = mean x; rstd = 1/sqrt(mean (x-mu)^2 + eps); y = (x-mu) rstd w + b
 // Everything between load and store is in 32 bits. The mean is off by its sum's
-// roundings, which around a large value are as large as the deviations; so the
-// deviations d from that first mean are summed along with their squares, and
-// what they have of a mean is taken away: mu = first + mean d, variance =
-// mean d^2 - (mean d)^2. A large common offset costs no accuracy (rows of one
-// value come out below 1e-5), and the second sum rides along with the first.
+// roundings, which around a large value are as large as the deviations. In rows
+// whose mean is more than four deviations from zero the deviations d from that
+// first mean are therefore summed as well, and what they have of a mean is taken
+// away: mu = first + mean d, variance = mean d^2 - (mean d)^2. A large common
+// offset then costs no accuracy (rows of one value come out below 1e-5); below
+// four deviations the first mean is within 5 U of a deviation for each of a
+// sum's few dozen steps.
 //
 // Bound by memory (each value read once, written once): a row is held in
 // registers by the threads that share it, a warp for rows of up to 128
@@ -14,15 +16,18 @@
 // same for every thread (32,768 rows of 4,096 bf16, before the last step: 128
 // threads 95 us, 256 107, 512 147), and weights that are read, applied, rounded
 // and stored piece by piece (95 to 87 us: fewer registers, more blocks an SM).
-// The sum of d costs two to four per cent of a long row's time (those rows 88 us
-// without). Measured: those rows 90 us, 5.9 TB/s; 8,192 rows of 16,384 bf16 98
-// us, 5.5 TB/s; 65,536 rows of 1,024 bf16 50 us, 5.3 TB/s; 16,384 rows of 2,049
-// f32 (one value a load) 52 us, 5.2 TB/s; of 4,097 bf16 (staged) 117 us, 2.3
-// TB/s; 1,024 rows of 65,536 bf16 (too long for registers) 118 us, 2.3 TB/s.
+// Measured (in brackets: if all rows are far from zero): those rows 89 us, 6.0
+// TB/s (93; 90 each if every row summed its deviations); 8,192 rows of 16,384
+// bf16 96 us, 5.6 TB/s (103); 65,536 rows of 1,024 bf16 50 us, 5.4 TB/s (52);
+// 16,384 rows of 2,049 f32 (one value a load) 50 us, 5.4 TB/s (54); of 4,097 bf16
+// (staged) 115 us, 2.3 TB/s (127); 1,024 rows of 65,536 bf16 (too long for
+// registers, where all rows sum their deviations) 117 us, 2.3 TB/s.
 #include "norm.cuh"
 
 namespace plx {
 namespace {
+
+constexpr float kFar = 4.0f;  // deviations between a row's mean and zero
 
 struct RowStats {
   float mean, rstd, shift;  // h = d rstd + shift
@@ -42,7 +47,7 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
        const P* __restrict__ b, float eps, float inv_n, T* y, int64_t ldy,
        float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int ROWS = TPR == 32 ? 8 : 1;
-  __shared__ float red[4 * (TPR / 32)];
+  __shared__ float red[2 * (TPR / 32)];
   const uint32_t lane = threadIdx.x % TPR;
   const uint32_t r = blockIdx.x * ROWS + threadIdx.x / TPR;
   if (ROWS > 1 && r >= rows) return;
@@ -100,15 +105,20 @@ k_norm(uint32_t rows, uint32_t n, const T* x, int64_t ldx, const P* __restrict__
         const int k = j * V + e;
         (k & 1 ? v[k / 2].y : v[k / 2].x) = 0.0f;
       }
-  F2 d2 = pack2(0.0f, 0.0f);
-  s2 = d2;
+  s2 = pack2(0.0f, 0.0f);
 #pragma unroll
-  for (int h = 0; h < H; ++h) {
-    d2 = add2(v[h], d2);
-    s2 = fma2(v[h], v[h], s2);
+  for (int h = 0; h < H; ++h) s2 = fma2(v[h], v[h], s2);
+  s[0] = s2.x + s2.y;
+  row_sum<TPR>(s, red, turn);
+  RowStats st = row_stats(mu, 0.0f, s[0], inv_n, eps);
+  if (fabsf(mu) * st.rstd > kFar) {  // so say all threads of the row
+    s2 = pack2(0.0f, 0.0f);
+#pragma unroll
+    for (int h = 0; h < H; ++h) s2 = add2(v[h], s2);
+    float d[1] = {s2.x + s2.y};
+    row_sum<TPR>(d, red, turn);
+    st = row_stats(mu, d[0], s[0], inv_n, eps);
   }
-  const F2 sums = row_sum2<TPR>(pack2(d2.x + d2.y, s2.x + s2.y), red, turn);
-  const RowStats st = row_stats(mu, sums.x, sums.y, inv_n, eps);
   const F2 rs2 = pack2(st.rstd, st.rstd), shift2 = pack2(st.shift, st.shift);
 #pragma unroll
   for (int h = 0; h < H; ++h) v[h] = fma2(v[h], rs2, shift2);
