@@ -24,7 +24,7 @@
 // one of them of the special-function unit. Measured, 4,096 rows of 65,536
 // bf16: 86 us, 6.2 TB/s; with entropy 89; and 8 alternatives 101, 5.3 TB/s; 64
 // 129. 2,048 rows of 65,536 f32: 86, 87, 93, 114. The gradient (read and written
-// once) of 1,024 rows of 131,072 bf16: 85 us, 6.3 TB/s.
+// once) of 1,024 rows of 131,072 bf16: 84 us, 6.4 TB/s.
 #include "logits.cuh"
 
 namespace plx {
@@ -495,7 +495,8 @@ extern "C" int plx_log_probs_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, i
       constexpr int THREADS = decltype(threads_c)::value;
       // Sixteen pieces a thread hide what a block costs; down to four where
       // that would leave SMs without eight blocks. As far as the grid's size
-      // allows. (1,500 rows of 32,003 f16: 37 us; always four: 43 us.)
+      // allows. (1,500 rows of 32,003 f16, before the first pieces were loaded
+      // ahead: 37 us; always four: 43; now 34.)
       uint64_t each = THREADS * 16 * Piece<T>::V;
       while (each > THREADS * 4 * Piece<T>::V && rows * ((n + each - 1) / each) < 148 * 8)
         each /= 2;

@@ -265,3 +265,44 @@ def test_alternatives_of_rows_whose_best_values_few_threads_hold(ctx, rows, dtyp
     got = readout.log_probs(ctx, x, top=top)
     ctx.sync()
     np.testing.assert_array_equal(got.top_ids.cpu().numpy(), F.order(f64(x))[:, :top])
+
+
+# --------------------------------------------------------------------- behind a network's layers
+def test_the_read_out_of_a_network_trained_on_log_probability(ctx):
+    """One sample through a network's layers, the last without a sigmoid: its output units are the
+    logits, the gradient of -log p goes where the layers' backward pass reads, and the weights
+    follow. Against automatic differentiation in 64 bits."""
+    from plastix_b200.runtime import MlpTopoNet, sweep_forward, sweep_update
+
+    sizes, rate = [5, 24, 37], 0.5
+    r = np.random.default_rng(17)
+    w = (r.normal(size=5 * 24 + 24 * 37) * 0.4).astype(np.float32)
+    x = torch.from_numpy(r.normal(size=5)).float().cuda()
+    net = MlpTopoNet(ctx, sizes, w)
+    (i0, i1), (h0, h1), (o0, o1) = ((net.begin[k], net.begin[k + 1]) for k in range(3))
+    net.act[i0:i1] = x
+    sweep_forward(ctx, net.csr[0], net.from_id[0], net.w[0], net.act, net.act[h0:h1], apply=_abi.APPLY_SIGMOID)
+    sweep_forward(ctx, net.csr[1], net.from_id[1], net.w[1], net.act, net.act[o0:o1], apply=_abi.APPLY_IDENTITY)
+    logits, target = net.act[o0:o1], torch.tensor(11, dtype=torch.int32, device="cuda")
+    s = readout.log_probs(ctx, logits, target, top=3)
+    down = torch.tensor(-1.0, device="cuda")
+    readout.log_probs_backward(ctx, logits, s.lse, target, down, out=net.grad[o0:o1])
+    net.bwd[1].refresh_weight(net.w[1])
+    net.bwd[1].backward(net.grad, net.grad[h0:h1], net.act[h0:h1], _abi.APPLY_SIGMOID_GRAD)
+    for k, (b0, b1) in enumerate(((h0, h1), (o0, o1))):
+        sweep_update(ctx, net.csr[k], net.from_id[k], net.act, net.grad[b0:b1], net.w[k], net.w[k],
+                     kind=_abi.UPDATE_GRADIENT, rate=rate)
+    ctx.sync()
+    w1 = torch.from_numpy(w[:120].reshape(24, 5)).double().requires_grad_()
+    w2 = torch.from_numpy(w[120:].reshape(37, 24)).double().requires_grad_()
+    z = w2 @ torch.sigmoid(w1 @ x.cpu().double())
+    z.retain_grad()
+    logp = torch.log_softmax(z, 0)
+    (-logp[11]).backward()
+    # values below 8 go through sums of 5, 24 and 37 terms and some 30 other roundings, forth and back
+    tol = 8 * U * 2 * (5 + 24 + 37 + 30)
+    assert abs(float(s.logp) - float(logp[11].detach())) <= tol
+    assert s.top_ids.tolist() == logp.topk(3).indices.tolist()
+    within(f64(net.grad[o0:o1]), z.grad.numpy(), tol, "gradient of the outputs")
+    within(f64(net.w[0]), (w1 - rate * w1.grad).detach().numpy().reshape(-1), tol, "weights into the hidden layer")
+    within(f64(net.w[1]), (w2 - rate * w2.grad).detach().numpy().reshape(-1), tol, "weights into the outputs")
