@@ -606,12 +606,14 @@ int plx_swifttd_apply(plx_ctx* ctx, uint64_t n_features, float* const* fields,
 /* Layer norm: y = (x - mean) * rstd * weight + bias, with the row's mean,
  * rstd = 1 / sqrt(variance + eps). weight and bias are [n] of type
  * param_dtype (PLX_F32 or dtype), or NULL for 1 and 0; mean and rstd [rows]
- * are written where not NULL (the backward call reads them). */
+ * are written where not NULL (the backward call reads them; mean in 32 bits, so
+ * that its x - mean is off by up to |mean| 2^-24). */
 int plx_layer_norm(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* x,
                    int64_t ldx, int param_dtype, const void* weight, const void* bias, float eps,
                    void* y, int64_t ldy, float* mean, float* rstd);
 
-/* Scratch of plx_layer_norm_backward when it writes dweight or dbias. */
+/* Scratch of plx_layer_norm_backward when it writes dweight or dbias: 8 n bytes
+ * for each of at most 1,184 groups of rows (fewer for few or long rows). */
 size_t plx_layer_norm_scratch_bytes(uint64_t rows, uint32_t n);
 
 /* Gradients of layer norm: dx [rows, n] and, of type param_dtype, dweight and
