@@ -236,8 +236,8 @@ extern "C" int plx_layer_norm(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype
       // A row takes the first launch that holds it: fewest threads, fewest values
       // each. The next one in its place takes (134 MB of rows) 1.05 to 2.0 times as
       // long for aligned rows, 1.9 to 3.1 for pairs, and for single values 1.01
-      // (2,047 f32, 256 threads of 8: 49 us and 50) to 3.1 (193 f32, a warp: 51 and
-      // 154; 2,559 f32, 256 threads of 10: 46 and 74).
+      // (2,047 f32, 256 threads of 8: 49 us and 50) to 3.3 (193 bf16, a warp: 105 and
+      // 348; 2,559 f32, 256 threads of 10: 46 and 74).
       if (v == V) {
         const uint32_t pieces = n / V;
         if (pieces <= 32) launch(k_norm<T, P, V, 1, 32>, eighth, 256);

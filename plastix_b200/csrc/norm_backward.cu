@@ -374,10 +374,11 @@ extern "C" int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
       const uint32_t v = piece_values(n, sizeof(T), {dy, x, dx}, {lddy, ldx, lddx}, weight,
                                       nullptr, sizeof(P));
       // A row takes the first launch that holds it. The next one in its place takes
-      // (134 MB of rows) 1.03 to 4.4 times as long, but for f32 rows of exactly 128 or 512
-      // values (0.92, 0.99). EACH is as many blocks as registers and shared memory
-      // leave room for: half as many take 1.0 to 2.1 times as long for 16-bit rows
-      // (512 values 71 us and 65), for f32 0.9 (1,024 values 70 and 66) to 1.7.
+      // (134 MB of rows) 1.03 to 4.4 times as long, but for f32 rows of exactly 128
+      // or 512 values (0.92, 0.99). EACH is as many blocks as registers and shared
+      // memory leave room for: half as many take up to 1.9 times as long for 16-bit
+      // rows (8,191 values 143 us and 267; least for 512, 71 and 65), for f32 0.9
+      // (1,024 values 70 and 66) to 1.7.
       if (v == V) {
         const uint32_t pieces = n / V;
         if (pieces <= 32) rc = launch(PLX_C(1), PLX_C(32), PLX_C(4), PLX_C(V));
