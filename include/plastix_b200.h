@@ -687,6 +687,134 @@ int plx_distill(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* 
                 int teacher_kind, float temperature, const float* row_weight, float* loss,
                 void* dlogits, int64_t ldd);
 
+/* ---- a block of hidden units on rows -------------------------------------- */
+
+/* What lies between a network's input and its read-out, over many rows at
+ * once: a fully connected layer, the recurrence of its units over the steps of
+ * streams, and the norms around a block. Rows, types, strides, aliasing and
+ * streams as for the read-out above; where more is not allowed it says so. */
+
+/* Activations of plx_dense. */
+#define PLX_ACT_IDENTITY 0
+#define PLX_ACT_SIGMOID 1
+#define PLX_ACT_TANH 2
+#define PLX_ACT_RELU 3
+#define PLX_ACT_SILU 4 /* z sigmoid(z) */
+#define PLX_ACT_GELU 5 /* z Phi(z), by the error function */
+
+/* Scratch of plx_dense, or (backward not 0) of plx_dense_backward. */
+size_t plx_dense_scratch_bytes(uint64_t rows, uint32_t n, uint32_t m, int dtype, int backward);
+
+/* A fully connected layer (the dense form of DoForwardPass, plastix.hpp:132-149,
+ * weights in FullyConnected's destination-major order, layers.hpp:49-77):
+ *   z = x weight^T + bias;  y = act(z) + residual
+ * x [rows, n], weight [m, n] (row stride ldw), y and residual [rows, m] are of
+ * type dtype, bias [m] of param_dtype (PLX_F32 or dtype); bias and residual may
+ * be NULL. pre [rows, m] (rows of m floats, nothing between them) is z, written
+ * where not NULL, for the backward call. y may be residual's array, not x's.
+ * Products are summed in 32 bits. scratch is 16-byte aligned and may hold
+ * anything; calls that run at once need scratch of their own. */
+int plx_dense(plx_ctx* ctx, uint64_t rows, uint32_t n, uint32_t m, int dtype, const void* x,
+              int64_t ldx, const void* weight, int64_t ldw, int param_dtype, const void* bias,
+              int act, const void* residual, int64_t ldr, void* y, int64_t ldy, float* pre,
+              void* scratch, size_t scratch_bytes);
+
+/* Gradients of plx_dense (cf. DoBackwardPass, plastix.hpp:164-211): with
+ * dz = dy act'(pre), rounded to dtype for the products,
+ *   dx = dz weight;  dweight = dz^T x;  dbias = sum of dz over the rows
+ * each written where not NULL (dweight and dbias are zero for rows = 0); x is
+ * not needed without dweight, weight not without dx, pre not for
+ * PLX_ACT_IDENTITY. The residual's gradient is dy. No output may be an input. */
+int plx_dense_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, uint32_t m, int dtype,
+                       const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                       const void* weight, int64_t ldw, int act, const float* pre, void* dx,
+                       int64_t lddx, void* dweight, int64_t lddw, int param_dtype, void* dbias,
+                       void* scratch, size_t scratch_bytes);
+
+#define PLX_NORM_RMS 0   /* v / sqrt(mean v^2 + eps) */
+#define PLX_NORM_LAYER 1 /* the same of v - mean v   */
+#define PLX_BLOCK_GATE_NONE 0
+#define PLX_BLOCK_GATE_UNITS 1  /* a value of every unit, [n] of param_dtype       */
+#define PLX_BLOCK_GATE_VALUES 2 /* of every unit of every row, [rows, n] of dtype  */
+
+typedef struct plx_block_norm_params {
+  int32_t kind;         /* PLX_NORM_*                                          */
+  int32_t post;         /* 0: the block's output is not normalised             */
+  int32_t gate;         /* PLX_BLOCK_GATE_*                                    */
+  int32_t gate_sigmoid; /* not 0: the gate is sigmoid(gate_values)             */
+  int32_t param_dtype;  /* PLX_F32 or the rows' dtype                          */
+  float scale;          /* of the residual                                     */
+  float eps;
+  const void* gate_values;
+  int64_t ldg;
+  const void *post_weight, *post_bias; /* [n], or NULL for 1 and 0 */
+  const void *pre_weight, *pre_bias;
+} plx_block_norm_params;
+
+/* The norm after a block and the one before the next, with gate and residual:
+ *   p = N(o) post_weight + post_bias   (o where post is 0)
+ *   r = scale * x + gate * p;   u = N(r) pre_weight + pre_bias
+ * x (the residual), o (the block's output), r and u are [rows, n]. u is made of
+ * the r that has not been rounded. stats [rows, 4], 16-byte aligned: mean and
+ * rstd of o, mean and rstd of r (0 where not taken), written where not NULL,
+ * for the backward call. */
+int plx_block_norm(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* x, int64_t ldx,
+                   const void* o, int64_t ldo, const plx_block_norm_params* params, void* r,
+                   int64_t ldr, void* u, int64_t ldu, float* stats);
+
+/* Scratch of plx_block_norm_backward. */
+size_t plx_block_norm_scratch_bytes(uint64_t rows, uint32_t n);
+
+/* Gradients of sum(dr * r) + sum(du * u); dr or du may be NULL, not both. dx and
+ * d_o are required; dgate ([n] of param_dtype or [rows, n], as the gate) and the
+ * parameters' gradients ([n] of param_dtype) are written where not NULL (those
+ * of [n] are zero for rows = 0), summed in an order that the arguments set: the
+ * same bits on every call. scratch as for plx_dense. */
+int plx_block_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* dr,
+                            int64_t lddr, const void* du, int64_t lddu, const void* x, int64_t ldx,
+                            const void* o, int64_t ldo, const float* stats,
+                            const plx_block_norm_params* params, void* dx, int64_t lddx, void* d_o,
+                            int64_t lddo, void* dgate, int64_t lddg, void* dpost_weight,
+                            void* dpost_bias, void* dpre_weight, void* dpre_bias, void* scratch,
+                            size_t scratch_bytes);
+
+#define PLX_GATE_DECAY 0   /* a = gate           */
+#define PLX_GATE_SIGMOID 1 /* a = sigmoid(gate)  */
+
+/* Scratch of plx_recurrence and plx_recurrence_backward (0: none is needed);
+ * ragged: offsets are given. */
+size_t plx_recurrence_scratch_bytes(uint32_t n_streams, uint64_t rows, uint32_t n, int ragged);
+
+/* Gated linear recurrence over the steps of streams (the trace e' = d e + x of
+ * HebbianTraceUpdate, of every unit, with a decay of every step):
+ *   h_t = a_t h_{t-1} + x_t,   or, with mix not 0,  a_t h_{t-1} + (1 - a_t) x_t
+ * Rows are steps. Without offsets every stream has rows / n_streams of them,
+ * stream after stream; with offsets (int32 [n_streams + 1], on the device)
+ * stream s has the rows from offsets[s] to before offsets[s + 1], none where
+ * they are equal; rows of no stream are left as they are. Offsets that decrease
+ * or leave [0, rows] make plx_ctx_sync report PLX_ERR_ARG and leave the results
+ * unspecified. state [n_streams, n] is h before the first steps (NULL: 0),
+ * final_state [n_streams, n] h after the last ones (state where there are none),
+ * written where not NULL; it may be state's array. States are in 32 bits, so is
+ * h from step to step. h may be x's or gate's array. Sums are folded in an
+ * order that the arguments set: the same bits on every call. scratch as for
+ * plx_dense. */
+int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n, int dtype,
+                   const int32_t* offsets, const void* x, int64_t ldx, const void* gate,
+                   int64_t ldg, int gate_kind, int mix, const float* state, void* h, int64_t ldh,
+                   float* final_state, void* scratch, size_t scratch_bytes);
+
+/* Gradients of sum(dh * h) + sum(dfinal * final_state): dx, dgate [rows, n] and,
+ * where not NULL, dstate [n_streams, n]. h as plx_recurrence wrote it; x is
+ * needed with mix alone; state and dfinal may be NULL for 0. dx and dgate may be
+ * the arrays of dh, x or gate, not h's; dstate may be dfinal's. */
+int plx_recurrence_backward(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n, int dtype,
+                            const int32_t* offsets, const void* dh, int64_t lddh, const void* x,
+                            int64_t ldx, const void* gate, int64_t ldg, int gate_kind, int mix,
+                            const void* h, int64_t ldh, const float* state, const float* dfinal,
+                            void* dx, int64_t lddx, void* dgate, int64_t lddg, float* dstate,
+                            void* scratch, size_t scratch_bytes);
+
 #ifdef __cplusplus
 }
 #endif

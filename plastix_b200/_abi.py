@@ -82,6 +82,30 @@ DISTILL_MAX_K = 64
 TEACHER_LOGITS = 0
 TEACHER_LOG_PROBS = 1
 
+ACT_IDENTITY = 0
+ACT_SIGMOID = 1
+ACT_TANH = 2
+ACT_RELU = 3
+ACT_SILU = 4
+ACT_GELU = 5
+NORM_RMS = 0
+NORM_LAYER = 1
+BLOCK_GATE_NONE = 0
+BLOCK_GATE_UNITS = 1
+BLOCK_GATE_VALUES = 2
+GATE_DECAY = 0
+GATE_SIGMOID = 1
+
+
+class BlockNormParams(ctypes.Structure):
+    """plx_block_norm_params."""
+    _fields_ = [("kind", ctypes.c_int32), ("post", ctypes.c_int32), ("gate", ctypes.c_int32),
+                ("gate_sigmoid", ctypes.c_int32), ("param_dtype", ctypes.c_int32),
+                ("scale", c_float), ("eps", c_float), ("gate_values", c_void_p), ("ldg", c_int64),
+                ("post_weight", c_void_p), ("post_bias", c_void_p), ("pre_weight", c_void_p),
+                ("pre_bias", c_void_p)]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "plx_version": (c_char_p, []),
@@ -194,6 +218,32 @@ _SIGNATURES = {
     "plx_distill": (c_int, [c_void_p, c_uint64, c_uint32, c_int, c_void_p, c_int64, c_uint32,
                             c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p, c_void_p,
                             c_int64]),
+    "plx_dense_scratch_bytes": (ctypes.c_size_t, [c_uint64, c_uint32, c_uint32, c_int, c_int]),
+    "plx_dense": (c_int, [c_void_p, c_uint64, c_uint32, c_uint32, c_int, c_void_p, c_int64,
+                          c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_int64, c_void_p,
+                          c_int64, c_void_p, c_void_p, ctypes.c_size_t]),
+    "plx_dense_backward": (c_int, [c_void_p, c_uint64, c_uint32, c_uint32, c_int, c_void_p,
+                                   c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p,
+                                   c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p,
+                                   c_void_p, ctypes.c_size_t]),
+    "plx_block_norm": (c_int, [c_void_p, c_uint64, c_uint32, c_int, c_void_p, c_int64, c_void_p,
+                               c_int64, POINTER(BlockNormParams), c_void_p, c_int64, c_void_p,
+                               c_int64, c_void_p]),
+    "plx_block_norm_scratch_bytes": (ctypes.c_size_t, [c_uint64, c_uint32]),
+    "plx_block_norm_backward": (c_int, [c_void_p, c_uint64, c_uint32, c_int, c_void_p, c_int64,
+                                        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                        c_void_p, POINTER(BlockNormParams), c_void_p, c_int64,
+                                        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                        c_void_p, c_void_p, c_void_p, ctypes.c_size_t]),
+    "plx_recurrence_scratch_bytes": (ctypes.c_size_t, [c_uint32, c_uint64, c_uint32, c_int]),
+    "plx_recurrence": (c_int, [c_void_p, c_uint32, c_uint64, c_uint32, c_int, c_void_p, c_void_p,
+                               c_int64, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p,
+                               c_int64, c_void_p, c_void_p, ctypes.c_size_t]),
+    "plx_recurrence_backward": (c_int, [c_void_p, c_uint32, c_uint64, c_uint32, c_int, c_void_p,
+                                        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                        c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p,
+                                        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                        ctypes.c_size_t]),
 }
 
 _lib = None

@@ -122,6 +122,8 @@ extern "C" int plx_ctx_sync(plx_ctx* ctx) {
     if (st == kStatusBadOutput)
       return set_error(PLX_ERR_ARG, "a target or teacher entry named an output "
                                     "outside its row");
+    if (st == kStatusBadOffsets)
+      return set_error(PLX_ERR_ARG, "offsets of streams decrease or leave the rows");
     return set_error(PLX_ERR_ARG, "device status %d", st);
   }
   return PLX_OK;

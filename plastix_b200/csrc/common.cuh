@@ -45,6 +45,7 @@ enum DeviceStatus : int32_t {
   kStatusBadIndex = 2,  // a connection named a unit outside the given array
   kStatusBadPlan = 3,   // a sweep was given an invalid plan
   kStatusBadOutput = 4,  // a target or teacher entry named an output outside its row
+  kStatusBadOffsets = 5,  // offsets of streams decrease or leave the rows
 };
 
 // ---------------------------------------------------------------------------
