@@ -702,8 +702,11 @@ int plx_distill(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* 
 #define PLX_ACT_SILU 4 /* z sigmoid(z) */
 #define PLX_ACT_GELU 5 /* z Phi(z), by the error function */
 
-/* Scratch of plx_dense, or (backward not 0) of plx_dense_backward. */
-size_t plx_dense_scratch_bytes(uint64_t rows, uint32_t n, uint32_t m, int dtype, int backward);
+/* Scratch of plx_dense, or (backward not 0) of plx_dense_backward; aligned: the
+ * rows that a call multiplies (x, weight, dy) all start at, and have strides of,
+ * multiples of 16 bytes (16-bit rows are copied where they do not). */
+size_t plx_dense_scratch_bytes(uint64_t rows, uint32_t n, uint32_t m, int dtype, int backward,
+                               int aligned);
 
 /* A fully connected layer (the dense form of DoForwardPass, plastix.hpp:132-149,
  * weights in FullyConnected's destination-major order, layers.hpp:49-77):

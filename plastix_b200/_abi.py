@@ -218,7 +218,8 @@ _SIGNATURES = {
     "plx_distill": (c_int, [c_void_p, c_uint64, c_uint32, c_int, c_void_p, c_int64, c_uint32,
                             c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p, c_void_p,
                             c_int64]),
-    "plx_dense_scratch_bytes": (ctypes.c_size_t, [c_uint64, c_uint32, c_uint32, c_int, c_int]),
+    "plx_dense_scratch_bytes": (ctypes.c_size_t, [c_uint64, c_uint32, c_uint32, c_int, c_int,
+                                                 c_int]),
     "plx_dense": (c_int, [c_void_p, c_uint64, c_uint32, c_uint32, c_int, c_void_p, c_int64,
                           c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_int64, c_void_p,
                           c_int64, c_void_p, c_void_p, ctypes.c_size_t]),

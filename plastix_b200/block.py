@@ -104,6 +104,15 @@ def _weight(ctx: Context, weight: torch.Tensor, n: int, dtype):
     return m, ld
 
 
+def _aligned(*rows) -> bool:
+    """Whether tensors of rows (tensor, row stride, rows) start at, and have
+    strides of, multiples of 16 bytes."""
+    for t, ld, count in rows:
+        if t.data_ptr() % 16 or (count > 1 and ld * t.element_size() % 16):
+            return False
+    return True
+
+
 def dense(ctx: Context, x: torch.Tensor, weight: torch.Tensor,
           bias: Optional[torch.Tensor] = None, *, apply: str = "identity",
           residual: Optional[torch.Tensor] = None, pre: bool = False,
@@ -138,7 +147,8 @@ def dense(ctx: Context, x: torch.Tensor, weight: torch.Tensor,
         if out is None:
             y = x.new_empty(shape)
         z = x.new_empty(shape, dtype=torch.float32) if pre else None
-        size = _abi.lib().plx_dense_scratch_bytes(rows, n, m, dtype, 0)
+        size = _abi.lib().plx_dense_scratch_bytes(
+            rows, n, m, dtype, 0, _aligned((x, ldx, rows), (weight, ldw, m)))
         scratch = x.new_empty(size, dtype=torch.uint8) if size else None
         _abi.call("plx_dense", ctx.handle, rows, n, m, dtype, x.data_ptr(), ldx,
                   weight.data_ptr(), ldw, kind, _address(bias), act, _address(residual), ldr,
@@ -171,7 +181,8 @@ def dense_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, weight: torc
         dx = x.new_empty(x.shape) if input_grad else None
         dw = weight.new_empty(weight.shape) if weight_grad else None
         db = torch.empty_like(bias) if bias is not None else None
-        size = _abi.lib().plx_dense_scratch_bytes(rows, n, m, dtype, 1)
+        size = _abi.lib().plx_dense_scratch_bytes(
+            rows, n, m, dtype, 1, _aligned((x, ldx, rows), (weight, ldw, m), (dy, lddy, rows)))
         scratch = x.new_empty(size, dtype=torch.uint8)
         _abi.call("plx_dense_backward", ctx.handle, rows, n, m, dtype, dy.data_ptr(), lddy,
                   x.data_ptr(), ldx, weight.data_ptr(), ldw, act, _address(pre), _address(dx), n,

@@ -85,11 +85,54 @@ int check_dense(const plx_ctx* ctx, uint64_t rows, uint32_t n, uint32_t m, int d
   return PLX_OK;
 }
 
-int product(plx_ctx* ctx, int dtype, const Product& p) { return product_f32(ctx, dtype, p); }
-
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
-// dz and the column sums' groups, in scratch.
+// Rows of 16-bit values that the tensor copies do not take (their start or stride
+// is no multiple of 16 bytes) are copied to some that they do.
+__global__ void __launch_bounds__(256)
+k_dense_pack(uint32_t rows, uint32_t n, const uint16_t* __restrict__ from, int64_t ld,
+             uint16_t* __restrict__ to, int64_t ldto) {
+  const uint32_t c = (blockIdx.x * 32 + (threadIdx.x & 31)) * 8;
+  if (c >= n) return;
+  for (uint32_t r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
+    const uint16_t* at = from + r * ld + c;
+    uint16_t v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < n ? at[e] : 0;
+    *reinterpret_cast<uint4*>(to + r * ldto + c) = *reinterpret_cast<const uint4*>(v);
+  }
+}
+
+bool packed(const void* p, int64_t ld, uint64_t rows, int dtype) {
+  return dtype == PLX_F32 || (aligned16(p) && (rows <= 1 || ld % 8 == 0));
+}
+// Bytes of a packed copy, whose rows are round_up(n, 8) apart.
+uint64_t pack_bytes(uint64_t rows, uint32_t n) { return round_up(rows * round_up(n, 8) * 2, 256); }
+
+// Makes rows of values an operand; `at` is where a copy goes, and is moved past it.
+int operand(plx_ctx* ctx, int dtype, const void* p, int64_t ld, uint64_t rows, uint32_t n,
+            bool k_major, char** at, Operand* out) {
+  *out = {p, ld, k_major};
+  if (dtype == PLX_F32) return PLX_OK;
+  if (packed(p, ld, rows, dtype)) {
+    if (rows <= 1) out->ld = (int64_t)round_up(n, 8);
+    return PLX_OK;
+  }
+  out->p = *at;
+  out->ld = (int64_t)round_up(n, 8);
+  const dim3 grid((n + 255) / 256, (unsigned)std::min<uint64_t>((rows + 7) / 8, 4096));
+  k_dense_pack<<<grid, 256, 0, ctx->stream>>>((uint32_t)rows, n, (const uint16_t*)p, ld,
+                                              (uint16_t*)*at, out->ld);
+  PLX_LAUNCH_CHECK("k_dense_pack");
+  *at += pack_bytes(rows, n);
+  return PLX_OK;
+}
+
+int product(plx_ctx* ctx, int dtype, const Product& p) {
+  return dtype == PLX_F32 ? product_f32(ctx, dtype, p) : product_tensor(ctx, dtype, p);
+}
+
+// dz and the column sums' groups, at the head of a backward call's scratch.
 struct BackwardScratch {
   uint64_t lddz, dz_bytes, sums_bytes;
   BackwardScratch(uint64_t rows, uint32_t m, int dtype) {
@@ -105,11 +148,16 @@ struct BackwardScratch {
 using namespace plx;
 
 extern "C" size_t plx_dense_scratch_bytes(uint64_t rows, uint32_t n, uint32_t m, int dtype,
-                                          int backward) {
-  (void)n;
-  if (!backward || !valid_dtype(dtype)) return 0;
-  const BackwardScratch s(rows, m, dtype);
-  return s.dz_bytes + s.sums_bytes;
+                                          int backward, int aligned) {
+  if (!valid_dtype(dtype) || n == 0 || m == 0) return 0;
+  uint64_t bytes = 0;
+  if (backward) {
+    const BackwardScratch s(rows, m, dtype);
+    bytes = s.dz_bytes + s.sums_bytes;
+  }
+  if (!aligned && dtype != PLX_F32)
+    bytes += pack_bytes(rows, n) + pack_bytes(m, n) + (backward ? pack_bytes(rows, m) : 0);
+  return bytes;
 }
 
 extern "C" int plx_dense(plx_ctx* ctx, uint64_t rows, uint32_t n, uint32_t m, int dtype,
@@ -124,7 +172,9 @@ extern "C" int plx_dense(plx_ctx* ctx, uint64_t rows, uint32_t n, uint32_t m, in
   PLX_CHECK_ARG(rows == 1 || (ldx >= (int64_t)n && ldy >= (int64_t)m &&
                               (!residual || ldr >= (int64_t)m)),
                 "a row stride is less than the row");
-  const size_t need = plx_dense_scratch_bytes(rows, n, m, dtype, 0);
+  const size_t need =
+      plx_dense_scratch_bytes(rows, n, m, dtype, 0,
+                              packed(x, ldx, rows, dtype) && packed(weight, ldw, m, dtype));
   PLX_CHECK_ARG(need == 0 || (scratch && scratch_bytes >= need),
                 "%zu bytes of scratch are needed, got %zu", need,
                 scratch ? scratch_bytes : (size_t)0);
@@ -138,8 +188,9 @@ extern "C" int plx_dense(plx_ctx* ctx, uint64_t rows, uint32_t n, uint32_t m, in
   p.rows = (uint32_t)rows;
   p.cols = m;
   p.depth = n;
-  p.a = {x, ldx, true};
-  p.b = {weight, ldw, true};
+  char* at = (char*)scratch;
+  if (int rc = operand(ctx, dtype, x, ldx, rows, n, true, &at, &p.a)) return rc;
+  if (int rc = operand(ctx, dtype, weight, ldw, m, n, true, &at, &p.b)) return rc;
   p.f = {param_dtype, act, bias, residual, ldr, y, ldy, pre};
   return product(ctx, dtype, p);
 }
@@ -162,7 +213,11 @@ extern "C" int plx_dense_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, uint3
   }
   PLX_CHECK_ARG(m == 1 || ((!dx || ldw >= (int64_t)n) && (!dweight || lddw >= (int64_t)n)),
                 "a row stride of weight or dweight is less than n");
-  const size_t need = plx_dense_scratch_bytes(rows, n, m, dtype, 1);
+  const bool own = act != PLX_ACT_IDENTITY && (dx || dweight);  // dz is not dy
+  const size_t need = plx_dense_scratch_bytes(
+      rows, n, m, dtype, 1,
+      (!dweight || packed(x, ldx, rows, dtype)) && (!dx || packed(weight, ldw, m, dtype)) &&
+          (own || !(dx || dweight) || packed(dy, lddy, rows, dtype)));
   PLX_CHECK_ARG(scratch && scratch_bytes >= need, "%zu bytes of scratch are needed, got %zu", need,
                 scratch ? scratch_bytes : (size_t)0);
   PLX_CHECK_ARG(aligned16(scratch), "scratch has to be 16-byte aligned");
@@ -174,7 +229,6 @@ extern "C" int plx_dense_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, uint3
   const BackwardScratch s(rows, m, dtype);
   void* dz = scratch;
   float* partial = (float*)((char*)scratch + s.dz_bytes);
-  const bool own = act != PLX_ACT_IDENTITY && (dx || dweight);  // dz is not dy
   uint32_t groups = 0;
   if (rows && (own || dbias)) {
     const uint32_t run = (uint32_t)std::max<uint64_t>(8, (rows + kGroups - 1) / kGroups);
@@ -208,25 +262,31 @@ extern "C" int plx_dense_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, uint3
     };
     if (int rc = param_dtype == PLX_F32 ? join(float{}) : with_dtype(dtype, join)) return rc;
   }
-  const void* d = own ? dz : dy;
-  const int64_t ldd = own ? (int64_t)s.lddz : lddy;
+  char* at = (char*)scratch + s.dz_bytes + s.sums_bytes;
+  Operand d = {dz, (int64_t)s.lddz, true};
+  if (!own && rows && (dx || dweight))
+    if (int rc = operand(ctx, dtype, dy, lddy, rows, m, true, &at, &d)) return rc;
   if (dx && rows) {
     Product p = {};
     p.rows = (uint32_t)rows;
     p.cols = n;
     p.depth = m;
-    p.a = {d, ldd, true};
-    p.b = {weight, ldw, false};
+    p.a = d;
+    if (int rc = operand(ctx, dtype, weight, ldw, m, n, false, &at, &p.b)) return rc;
     p.f = {dtype, PLX_ACT_IDENTITY, nullptr, nullptr, 0, dx, lddx, nullptr};
     if (int rc = product(ctx, dtype, p)) return rc;
   }
-  if (dweight) {
+  if (dweight && rows == 0) {
+    PLX_TRY_CUDA(cudaMemset2DAsync(dweight, (size_t)(m > 1 ? lddw : n) * dtype_bytes(dtype), 0,
+                                   (size_t)n * dtype_bytes(dtype), m, ctx->stream));
+  } else if (dweight) {
     Product p = {};
     p.rows = m;
     p.cols = n;
     p.depth = (uint32_t)rows;
-    p.a = {d, ldd, false};
-    p.b = {x, ldx, false};
+    d.k_major = false;
+    p.a = d;
+    if (int rc = operand(ctx, dtype, x, ldx, rows, n, false, &at, &p.b)) return rc;
     p.f = {dtype, PLX_ACT_IDENTITY, nullptr, nullptr, 0, dweight, lddw, nullptr};
     if (int rc = product(ctx, dtype, p)) return rc;
   }

@@ -90,5 +90,7 @@ struct Product {
 };
 
 int product_f32(plx_ctx* ctx, int dtype, const Product& p);
+// 16-bit types; operands start at, and have strides of, multiples of 16 bytes.
+int product_tensor(plx_ctx* ctx, int dtype, const Product& p);
 
 }  // namespace plx
