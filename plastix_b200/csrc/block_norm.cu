@@ -175,6 +175,7 @@ BlockNorm block_norm_of(uint64_t rows, uint32_t n, const plx_block_norm_params* 
   a.post = p->post != 0;
   a.gate = p->gate;
   a.sigmoid = p->gate_sigmoid != 0;
+  a.param_f32 = p->param_dtype == PLX_F32;
   a.scale = p->scale;
   a.eps = p->eps;
   a.gate_values = p->gate == PLX_BLOCK_GATE_NONE ? nullptr : p->gate_values;

@@ -9,7 +9,7 @@ struct BlockNorm {
   uint32_t rows, n;
   float inv_n, scale, eps;
   int gate;
-  bool layer, post, sigmoid;
+  bool layer, post, sigmoid, param_f32;
   const void *x, *o, *gate_values;
   int64_t ldx, ldo, ldg;
   const void *post_weight, *post_bias, *pre_weight, *pre_bias;

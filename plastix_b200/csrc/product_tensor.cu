@@ -12,6 +12,7 @@
 // are units of the layer.
 #include <atomic>
 
+#include "cluster.cuh"
 #include "dense.cuh"
 #include "tensor.cuh"
 
