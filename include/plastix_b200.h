@@ -810,7 +810,7 @@ int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n, 
 /* Gradients of sum(dh * h) + sum(dfinal * final_state): dx, dgate [rows, n] and,
  * where not NULL, dstate [n_streams, n]. h as plx_recurrence wrote it; x is
  * needed with mix alone; state and dfinal may be NULL for 0. dx and dgate may be
- * the arrays of dh, x or gate, not h's; dstate may be dfinal's. */
+ * the arrays of dh, x or gate, not h's; dstate is not dfinal's. */
 int plx_recurrence_backward(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n, int dtype,
                             const int32_t* offsets, const void* dh, int64_t lddh, const void* x,
                             int64_t ldx, const void* gate, int64_t ldg, int gate_kind, int mix,

@@ -20,9 +20,12 @@
 namespace plx {
 namespace {
 
-constexpr int kWarps = 16;   // runs of a tile
+// Runs of a tile, forwards and backwards, which has more values in registers: two
+// blocks an SM either way.
+__host__ __device__ constexpr int warps_of(bool back) { return back ? 12 : 16; }
 constexpr int kRun = 8;      // steps of a run
-constexpr uint32_t kTileSteps = kWarps * kRun;
+__host__ __device__ constexpr uint32_t tile_steps(bool back) { return warps_of(back) * kRun; }
+constexpr uint32_t kLook = 32;  // tiles that one looks back over
 
 // How rows are cut: `parts` parts of `part_rows` rows (the last may be shorter),
 // each of `chunks` tiles of `chunk_rows` rows (a multiple of the runs' length
@@ -31,16 +34,17 @@ struct Cut {
   uint32_t parts, part_rows, chunks, chunk_rows;
 };
 
-Cut cut_rows(uint32_t streams, uint64_t rows, bool ragged) {
+Cut cut_rows(uint32_t streams, uint64_t rows, bool ragged, bool back) {
   Cut c;
   const uint64_t steps = ragged ? rows : rows / streams;
-  if (steps <= kTileSteps && !ragged) {  // whole streams in a tile
-    c.chunk_rows = c.part_rows = (uint32_t)(kTileSteps / steps * steps);
+  const uint32_t tile = tile_steps(back);
+  if (steps <= tile && !ragged) {  // whole streams in a tile
+    c.chunk_rows = c.part_rows = (uint32_t)(tile / steps * steps);
     c.chunks = 1;
   } else {
     c.part_rows = (uint32_t)steps;
-    c.chunks = (uint32_t)((steps + kTileSteps - 1) / kTileSteps);
-    c.chunk_rows = kTileSteps;
+    c.chunks = (uint32_t)((steps + tile - 1) / tile);
+    c.chunk_rows = tile;
   }
   c.parts = (uint32_t)((rows + c.part_rows - 1) / c.part_rows);
   return c;
@@ -80,41 +84,67 @@ __device__ __forceinline__ void st_release(uint32_t* p, uint32_t v) {
   asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
 }
 
-// Waits until a tile's flag is at least `least`; 0 once somebody has given up.
-__device__ __forceinline__ uint32_t wait_flag(const uint32_t* flag, uint32_t least, Scratch* s,
-                                              int32_t* status, uint64_t timeout_ns) {
-  uint32_t v = ld_acquire(flag);
-  if (v >= least) return v;
-  const uint64_t t0 = global_timer_ns();
-  for (uint32_t spin = 1;; ++spin) {
-    v = ld_acquire(flag);
-    if (v >= least) return v;
-    if ((spin & 63u) == 0) {
-      if (*(volatile uint32_t*)&s->gave_up) return 0;
-      if (global_timer_ns() - t0 > timeout_ns) {
-        record_status(status, kStatusTimeout);
-        *(volatile uint32_t*)&s->gave_up = 1;
-        return 0;
-      }
-    }
-  }
+// One or two units at once.
+template <int V>
+using Units = std::conditional_t<V == 2, F2, float>;
+__device__ __forceinline__ float addw(float a, float b) { return __fadd_rn(a, b); }
+__device__ __forceinline__ float mulw(float a, float b) { return __fmul_rn(a, b); }
+__device__ __forceinline__ float fmaw(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ F2 addw(F2 a, F2 b) { return add2(a, b); }
+__device__ __forceinline__ F2 mulw(F2 a, F2 b) { return mul2(a, b); }
+__device__ __forceinline__ F2 fmaw(F2 a, F2 b, F2 c) { return fma2(a, b, c); }
+template <typename W>
+__device__ __forceinline__ W all(float v) {
+  if constexpr (std::is_same_v<W, F2>) return pack2(v, v);
+  else return v;
+}
+template <typename F>
+__device__ __forceinline__ float each(float v, F f) { return f(v); }
+template <typename F>
+__device__ __forceinline__ F2 each(F2 v, F f) { return pack2(f(v.x), f(v.y)); }
+template <typename T, int V>
+__device__ __forceinline__ Units<V> wide(const Pack<T, V>& q) {
+  if constexpr (V == 2) return pair_of(q, 0);
+  else return to_f32(q.v[0]);
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> narrow(Units<V> v) {
+  Pack<T, V> q;
+  if constexpr (V == 2) put_pair(q, 0, v);
+  else q.v[0] = from_f32<T>(v);
+  return q;
 }
 
-// a and 1 - a of a gate, neither by a difference that cancels. The quotient gets
-// one Newton step: what a is off by, a long memory raises to its length.
-template <bool SIGMOID>
-__device__ __forceinline__ void gate_value(float g, float& a, float& keep) {
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
+}
+
+// a and 1 - a of a gate, neither by a difference that cancels: with e = exp(-gate),
+// 1 / (1 + e) and e / (1 + e). The quotient gets one Newton step: what a is off by, a
+// long memory raises to its length. e is at most 2^126 (a gate of -infinity leaves
+// 2^-126 of h).
+template <typename W>
+__device__ __forceinline__ W exp_minus(W g) {
+  return each(mulw(g, all<W>(-kLog2e)), [](float t) { return exp2_approx(min_nan(t, 126.0f)); });
+}
+template <bool SIGMOID, typename W>
+__device__ __forceinline__ void gate_value(W g, W& a, W& keep) {
   if constexpr (SIGMOID) {
-    const float e = exp2_approx(-fabsf(g) * kLog2e), d = 1.0f + e;
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-    r = fmaf(r, fmaf(-d, r, 1.0f), r);
-    const float er = e * r;
-    a = g < 0.0f ? er : r;
-    keep = g < 0.0f ? r : er;
+    const W e = exp_minus(g);
+    const W d = addw(e, all<W>(1.0f)), minus = each(d, [](float t) { return -t; });
+    const W r = each(d, rcp_approx);
+    a = fmaw(r, fmaw(minus, r, all<W>(1.0f)), r);
+    keep = mulw(e, a);
   } else {
     a = g;
-    keep = 1.0f - g;
+    keep = each(g, [](float t) { return __fsub_rn(1.0f, t); });
   }
 }
 
@@ -148,13 +178,67 @@ __device__ __forceinline__ Place place_of(const Args& p, uint64_t row) {
   return q;
 }
 
+// A step's values as both walks use them: forwards a and b (h = a h + b), where a
+// stream begins with its state in b; backwards a, dh and what g is multiplied by.
 template <typename T, int V, bool SIGMOID, bool MIX, bool BACK>
-__global__ void __launch_bounds__(kWarps * 32, 2) k_recurrence(const __grid_constant__ Args p) {
-  constexpr uint32_t C = 32 * V;
-  __shared__ float run_a[kWarps][C], run_h[kWarps][C];
-  __shared__ float look_a[kWarps][C], look_h[kWarps][C];
-  __shared__ uint32_t run_shut[kWarps], look_kind[kWarps], ticket;
+struct Step {
+  using W = Units<V>;
+  using P = Pack<T, V>;
+  W a, b;     // b: forwards
+  P dh;       // backwards
+  W slope;    // dgate = g slope
+  P gate;     // with a, 1 - a
+  __device__ __forceinline__ void forward(P gate, P x) {
+    W k;
+    gate_value<SIGMOID>(wide<T, V>(gate), a, k);
+    b = wide<T, V>(x);
+    if (MIX) b = mulw(b, k);
+  }
+  __device__ __forceinline__ void backward(P gate_, P d, W before, P x) {
+    gate = gate_;
+    W k;
+    gate_value<SIGMOID>(wide<T, V>(gate), a, k);
+    dh = d;
+    slope = before;
+    if (MIX) slope = addw(slope, each(wide<T, V>(x), [](float t) { return -t; }));
+    if (SIGMOID) slope = mulw(slope, mulw(a, k));
+  }
+  __device__ __forceinline__ W dx(W g) const {
+    if (!MIX) return g;
+    if (SIGMOID) return mulw(g, mulw(exp_minus(wide<T, V>(gate)), a));
+    return mulw(g, each(a, [](float t) { return __fsub_rn(1.0f, t); }));
+  }
+};
+
+template <int V>
+__device__ __forceinline__ Units<V> load_units(const float* p, bool in) {
+  if constexpr (V == 2) return in ? pack2(p[0], p[1]) : pack2(0.0f, 0.0f);
+  else return in ? p[0] : 0.0f;
+}
+template <int V>
+__device__ __forceinline__ void store_units(float* p, Units<V> v) {
+  if constexpr (V == 2) {
+    p[0] = v.x;
+    p[1] = v.y;
+  } else {
+    p[0] = v;
+  }
+}
+
+template <typename T, int V, bool SIGMOID, bool MIX, bool BACK>
+__global__ void __launch_bounds__(warps_of(BACK) * 32, 2)
+k_recurrence(const __grid_constant__ Args p) {
+  constexpr int kWarps = warps_of(BACK);
+  using W = Units<V>;
+  using P = Pack<T, V>;
+  struct alignas(8 * V) Pair {
+    W a, h;
+  };
+  __shared__ Pair runs[kWarps][32], look[kLook][32];
+  __shared__ W look_end[32];
+  __shared__ uint32_t run_shut[kWarps], ticket, near;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const W zero = all<W>(0.0f);
 
   if (p.offsets) {  // offsets that no rows have; streams without steps hand their state on
     for (uint32_t s = blockIdx.x; s < p.streams; s += gridDim.x) {
@@ -183,173 +267,166 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_recurrence(const __grid_cons
   const uint64_t part_end = min((uint64_t)(part + 1) * p.cut.part_rows, p.rows);
   const uint64_t row0 = (uint64_t)part * p.cut.part_rows + (uint64_t)chunk * p.cut.chunk_rows;
   const uint64_t row1 = min(row0 + p.cut.chunk_rows, part_end);
-  const uint32_t unit = across * C + lane * V;
+  const uint32_t unit = (across * 32 + lane) * V;
   const bool in = unit < p.n;  // V divides n
   // This warp's run, in the order that it is walked.
   const uint32_t run = BACK ? kWarps - 1 - warp : warp;
   const uint64_t at = row0 + run * kRun;
   const int len = at < row1 ? (int)min((uint64_t)kRun, row1 - at) : 0;
 
-  using P = Pack<T, V>;
-  P qg[kRun], q1[kRun], q2[kRun], q3[kRun];  // gate; x or dh; backwards h before and x
-  const T zero = from_f32<T>(0.0f);
-  auto load = [&](P(&q)[kRun], const void* array, int64_t ld, int64_t first) {
-    const T* from = (const T*)array + first * ld + unit;
+  P qg[kRun], q1[kRun], q2[BACK ? kRun : 1], q3[BACK && MIX ? kRun : 1];
+  P nothing;
+#pragma unroll
+  for (int e = 0; e < V; ++e) nothing.v[e] = from_f32<T>(0.0f);
+  auto load = [&](P(&q)[kRun], const void* array, int64_t ld) {
+    const T* from = (const T*)array + (int64_t)at * ld + unit;
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) q[i].v[e] = zero;
+      q[i] = nothing;
       if (in && i < len) q[i] = load_pack<T, V>(from + i * ld);
     }
   };
-  load(qg, p.gate, p.ldg, (int64_t)at);
-  load(q1, BACK ? p.dh : p.x, BACK ? p.lddh : p.ldx, (int64_t)at);
-  if (BACK && MIX) load(q3, p.x, p.ldx, (int64_t)at);
+  load(qg, p.gate, p.ldg);
+  load(q1, BACK ? p.dh : p.x, BACK ? p.lddh : p.ldx);
+  if constexpr (BACK && MIX) load(q3, p.x, p.ldx);
   // Where streams begin and end in the run: a row to a lane.
   Place mine = {0, false, false, false};
   if ((int)lane < len) mine = place_of(p, at + lane);
   const uint32_t valid = __ballot_sync(~0u, mine.valid);
   const uint32_t first = __ballot_sync(~0u, mine.first), last = __ballot_sync(~0u, mine.last);
-  auto state_at = [&](const float* states, int i, float (&v)[V]) {
+  auto state_at = [&](const float* states, int i) {
     const uint32_t s = __shfl_sync(~0u, mine.stream, i);
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = states && in ? states[(uint64_t)s * p.n + unit + e] : 0.0f;
+    return states ? load_units<V>(states + (uint64_t)s * p.n + unit, in) : zero;
   };
   if constexpr (BACK) {
     const T* from = (const T*)p.h + ((int64_t)at - 1) * p.ldh + unit;
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) q2[i].v[e] = zero;
+      q2[i] = nothing;
       if (in && (valid >> i & 1) && !(first >> i & 1)) q2[i] = load_pack<T, V>(from + i * p.ldh);
     }
   }
 
   // ---- the run's pair. `stop`: rows at which what was before does not count.
   const uint32_t stop = BACK ? last : first;
-  float A[V], H[V], extra[kRun][V];  // what a stream's state adds where it begins
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    A[e] = 1.0f;
-    H[e] = 0.0f;
-  }
-  // One step: forwards h = a h + b; backwards g = dh + c, c' = a g (h is c).
-  auto forward = [&](int i, int e, float before) {
-    float a, keep;
-    gate_value<SIGMOID>(to_f32(qg[i].v[e]), a, keep);
-    float b = to_f32(q1[i].v[e]);
-    if (MIX) b *= keep;
-    return fmaf(a, before, b);
-  };
+  Step<T, V, SIGMOID, MIX, BACK> steps[kRun];
+  W A = all<W>(1.0f), H = zero;
 #pragma unroll
   for (int k = 0; k < kRun; ++k) {
     const int i = BACK ? kRun - 1 - k : k;
-#pragma unroll
-    for (int e = 0; e < V; ++e) extra[i][e] = 0.0f;
     if (i >= len) continue;
-    if (stop >> i & 1) {  // the same for the whole warp
-      state_at(BACK ? p.dfinal : p.state, i, extra[i]);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        H[e] = extra[i][e];
-        A[e] = 0.0f;
+    auto& st = steps[i];
+    if constexpr (BACK) {
+      W before = wide<T, V>(q2[i]);
+      if (first >> i & 1) before = state_at(p.state, i);
+      st.backward(qg[i], q1[i], before, q3[MIX ? i : 0]);
+      if (stop >> i & 1) {  // the same for the whole warp
+        H = state_at(p.dfinal, i);
+        A = zero;
+      }
+      H = mulw(st.a, addw(wide<T, V>(st.dh), H));
+      A = mulw(A, st.a);
+    } else {
+      st.forward(qg[i], q1[i]);
+      if (stop >> i & 1) {
+        st.b = fmaw(st.a, state_at(p.state, i), st.b);
+        H = st.b;
+        A = zero;
+      } else {
+        H = fmaw(st.a, H, st.b);
+        A = mulw(A, st.a);
       }
     }
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float a, keep;
-      gate_value<SIGMOID>(to_f32(qg[i].v[e]), a, keep);
-      if constexpr (BACK) H[e] = a * (to_f32(q1[i].v[e]) + H[e]);
-      else H[e] = forward(i, e, H[e]);
-      A[e] *= a;
-    }
   }
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    run_a[warp][lane * V + e] = A[e];
-    run_h[warp][lane * V + e] = H[e];
-  }
+  runs[warp][lane] = {A, H};
   if (lane == 0) run_shut[warp] = stop;
   __syncthreads();
 
   // ---- what the tile is given, and what it leaves
-  float carry[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) carry[e] = 0.0f;
+  W carry = zero;
   if (chained) {
-    float ta[V], th[V];
-    bool shut = false;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      ta[e] = 1.0f;
-      th[e] = 0.0f;
-    }
-    for (int w = 0; w < kWarps; ++w) {
-      const bool s = run_shut[w] != 0;
-      shut |= s;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float a = run_a[w][lane * V + e], h = run_h[w][lane * V + e];
-        th[e] = s ? h : fmaf(a, th[e], h);
-        ta[e] = s ? 0.0f : ta[e] * a;
-      }
-    }
     const uint32_t step = p.cut.parts * p.tiles;  // between tiles of a part
-    const uint64_t slot = (uint64_t)id * C + lane * V;
-    auto leave = [&](bool end, const float (&h)[V]) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (end) p.ends[slot + e] = h[e];
-        else p.pairs[slot + e] = make_float2(ta[e], h[e]);
-      }
+    Pair* pairs = reinterpret_cast<Pair*>(p.pairs);
+    W* ends = reinterpret_cast<W*>(p.ends);
+    W ta = all<W>(1.0f), th = zero;
+    bool shut = turn == 0;
+    auto leave = [&](bool end) {
+      if (end) ends[(uint64_t)id * 32 + lane] = th;
+      else pairs[(uint64_t)id * 32 + lane] = {ta, th};
       __threadfence();
       __syncwarp();
       if (lane == 0) st_release(p.flags + id, end ? kEnd : kPair);
     };
-    const bool ready = shut || turn == 0;
-    if (warp == 0) leave(ready, th);
-    if (turn > 0) {
-      uint32_t kind = kEnd;
-      if (warp < turn) {
-        const uint32_t from = id - (warp + 1) * step;
-        // the furthest one is waited for until it has its end value
-        kind = wait_flag(p.flags + from, warp == kWarps - 1 ? kEnd : kPair, p.scratch, p.status,
-                         p.timeout_ns);
-        kind = __reduce_min_sync(~0u, kind);  // what every lane has seen
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const uint64_t s = (uint64_t)from * C + lane * V + e;
-          float2 v = make_float2(0.0f, 0.0f);
-          if (kind == kPair) v = __ldcg(p.pairs + s);
-          else if (kind == kEnd) v.y = __ldcg(p.ends + s);
-          look_a[warp][lane * V + e] = v.x;
-          look_h[warp][lane * V + e] = v.y;
+    if (warp == 0) {
+      for (int w = 0; w < kWarps; ++w) {
+        const Pair v = runs[w][lane];
+        const bool s = run_shut[w] != 0;
+        shut |= s;
+        th = s ? v.h : fmaw(v.a, th, v.h);
+        ta = s ? zero : mulw(ta, v.a);
+      }
+      leave(shut);
+    } else if (warp == 1 && turn > 0) {
+      // The nearest tile before that has its end value, all in between their pairs.
+      const bool there = lane < turn;
+      const uint32_t* flag = p.flags + id - (lane + 1) * (there ? step : 0);
+      const uint64_t t0 = global_timer_ns();
+      uint32_t found = kLook;
+      for (uint32_t spin = 1;; ++spin) {
+        const uint32_t v = there ? ld_acquire(flag) : kPair;
+        const uint32_t ended = __ballot_sync(~0u, v == kEnd);
+        const uint32_t waiting = __ballot_sync(~0u, v == 0);
+        if (ended) {
+          found = __ffs(ended) - 1;
+          if (!(waiting & ((1u << found) - 1))) break;
+        }
+        if ((spin & 63u) == 0) {
+          bool stop_now = *(volatile uint32_t*)&p.scratch->gave_up != 0;
+          if (global_timer_ns() - t0 > p.timeout_ns) {
+            record_status(p.status, kStatusTimeout);
+            *(volatile uint32_t*)&p.scratch->gave_up = 1;
+            stop_now = true;
+          }
+          if (__any_sync(~0u, stop_now)) {
+            found = kLook;
+            break;
+          }
         }
       }
-      if (lane == 0) look_kind[warp] = kind;
-      __syncthreads();
-      int near = 0;
-      while (near < kWarps - 1 && look_kind[near] == kPair) ++near;
-#pragma unroll
-      for (int e = 0; e < V; ++e) carry[e] = look_h[near][lane * V + e];
-      for (int w = near - 1; w >= 0; --w)
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          carry[e] = fmaf(look_a[w][lane * V + e], carry[e], look_h[w][lane * V + e]);
-      if (warp == 0 && !ready) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) th[e] = fmaf(ta[e], carry[e], th[e]);
-        leave(true, th);
+      __threadfence();
+      if (lane == 0) near = found;
+    }
+    __syncthreads();
+    if (turn > 0 && near < kLook) {
+      const uint32_t count = near;
+      for (uint32_t j = warp; j <= count; j += kWarps) {
+        const uint64_t from = (uint64_t)(id - (j + 1) * step) * 32 + lane;
+        if (j == count) {
+          if constexpr (V == 2) look_end[lane] = __ldcg(reinterpret_cast<const float2*>(ends + from));
+          else look_end[lane] = __ldcg(ends + from);
+        } else if constexpr (V == 2) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(pairs + from));
+          look[j][lane] = {pack2(v.x, v.y), pack2(v.z, v.w)};
+        } else {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(pairs + from));
+          look[j][lane] = {v.x, v.y};
+        }
       }
+      __syncthreads();
+      carry = look_end[lane];
+      for (int j = (int)count - 1; j >= 0; --j) {
+        const Pair v = look[j][lane];
+        carry = fmaw(v.a, carry, v.h);
+      }
+    }
+    if (warp == 0 && !shut) {
+      th = fmaw(ta, carry, th);
+      leave(true);
     }
   }
   for (uint32_t w = 0; w < warp; ++w) {
-    const bool s = run_shut[w] != 0;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float a = run_a[w][lane * V + e], h = run_h[w][lane * V + e];
-      carry[e] = s ? h : fmaf(a, carry[e], h);
-    }
+    const Pair v = runs[w][lane];
+    carry = run_shut[w] ? v.h : fmaw(v.a, carry, v.h);
   }
 
   // ---- the run once more, from what it is given
@@ -357,45 +434,24 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_recurrence(const __grid_cons
   for (int k = 0; k < kRun; ++k) {
     const int i = BACK ? kRun - 1 - k : k;
     if (i >= len) continue;
-    if (stop >> i & 1)
-#pragma unroll
-      for (int e = 0; e < V; ++e) carry[e] = extra[i][e];
-    float before[V];
-    if constexpr (BACK) {
-      if (first >> i & 1) {
-        state_at(p.state, i, before);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) before[e] = to_f32(q2[i].v[e]);
-      }
-    }
-    P o1, o2;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      if constexpr (BACK) {
-        float a, keep;
-        gate_value<SIGMOID>(to_f32(qg[i].v[e]), a, keep);
-        const float g = to_f32(q1[i].v[e]) + carry[e];
-        carry[e] = a * g;
-        float da = g * (MIX ? before[e] - to_f32(q3[i].v[e]) : before[e]);
-        if (SIGMOID) da *= a * keep;
-        o1.v[e] = from_f32<T>(MIX ? g * keep : g);
-        o2.v[e] = from_f32<T>(da);
-      } else {
-        carry[e] = forward(i, e, carry[e]);
-        o1.v[e] = from_f32<T>(carry[e]);
-      }
-    }
+    const auto& st = steps[i];
     const int64_t row = (int64_t)(at + i);
-    if (in && (valid >> i & 1)) {
-      *reinterpret_cast<P*>((T*)p.out + row * p.ldo + unit) = o1;
-      if (BACK) *reinterpret_cast<P*>((T*)p.out2 + row * p.ldo2 + unit) = o2;
+    const bool write = in && (valid >> i & 1);
+    if constexpr (BACK) {
+      if (stop >> i & 1) carry = state_at(p.dfinal, i);
+      const W g = addw(wide<T, V>(st.dh), carry);
+      carry = mulw(st.a, g);
+      if (write) {
+        *reinterpret_cast<P*>((T*)p.out + row * p.ldo + unit) = narrow<T, V>(st.dx(g));
+        *reinterpret_cast<P*>((T*)p.out2 + row * p.ldo2 + unit) = narrow<T, V>(mulw(g, st.slope));
+      }
+    } else {
+      carry = stop >> i & 1 ? st.b : fmaw(st.a, carry, st.b);
+      if (write) *reinterpret_cast<P*>((T*)p.out + row * p.ldo + unit) = narrow<T, V>(carry);
     }
     if (p.state_out && ((BACK ? first : last) >> i & 1)) {
       const uint32_t s = __shfl_sync(~0u, mine.stream, i);
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (in) p.state_out[(uint64_t)s * p.n + unit + e] = carry[e];
+      if (in) store_units<V>(p.state_out + (uint64_t)s * p.n + unit, carry);
     }
   }
 }
@@ -445,7 +501,7 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
   }
   if (a.rows == 1) a.ldx = a.ldg = a.ldh = a.lddh = a.ldo = a.ldo2 = a.n;
   a.steps = a.offsets ? 0 : (uint32_t)(a.rows / a.streams);
-  a.cut = cut_rows(a.streams, a.rows, a.offsets != nullptr);
+  a.cut = cut_rows(a.streams, a.rows, a.offsets != nullptr, BACK);
   a.status = ctx->d_status;
   a.timeout_ns = ctx->timeout_ns;
   return with_dtype(dtype, [&](auto t) {
@@ -472,7 +528,7 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
         PLX_TRY_CUDA(cudaMemsetAsync(at, 0, head, ctx->stream));
       }
       k_recurrence<T, V, decltype(sigmoid_c)::value, decltype(mix_c)::value, BACK>
-          <<<(unsigned)blocks, kWarps * 32, 0, ctx->stream>>>(a);
+          <<<(unsigned)blocks, warps_of(BACK) * 32, 0, ctx->stream>>>(a);
       PLX_LAUNCH_CHECK("k_recurrence");
       return PLX_OK;
     };
@@ -496,7 +552,7 @@ using namespace plx;
 extern "C" size_t plx_recurrence_scratch_bytes(uint32_t n_streams, uint64_t rows, uint32_t n,
                                                int ragged) {
   if (n_streams == 0 || rows == 0 || n == 0) return 0;
-  const Cut c = cut_rows(n_streams, rows, ragged != 0);
+  const Cut c = cut_rows(n_streams, rows, ragged != 0, true);  // the shorter tiles
   if (c.chunks == 1) return 0;
   const uint64_t blocks = (uint64_t)c.parts * c.chunks * ((n + 31) / 32);
   return sizeof(Scratch) + (blocks * 4 + 255) / 256 * 256 + blocks * 32 * 12;
