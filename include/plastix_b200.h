@@ -784,9 +784,10 @@ int plx_block_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, 
 #define PLX_GATE_DECAY 0   /* a = gate           */
 #define PLX_GATE_SIGMOID 1 /* a = sigmoid(gate)  */
 
-/* Scratch of plx_recurrence and plx_recurrence_backward (0: none is needed);
- * ragged: offsets are given. */
-size_t plx_recurrence_scratch_bytes(uint32_t n_streams, uint64_t rows, uint32_t n, int ragged);
+/* Scratch of plx_recurrence and plx_recurrence_backward; ragged: offsets are
+ * given. */
+size_t plx_recurrence_scratch_bytes(uint32_t n_streams, uint64_t rows, uint32_t n, int ragged,
+                                    int backward);
 
 /* Gated linear recurrence over the steps of streams (the trace e' = d e + x of
  * HebbianTraceUpdate, of every unit, with a decay of every step):
@@ -810,7 +811,7 @@ int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n, 
 /* Gradients of sum(dh * h) + sum(dfinal * final_state): dx, dgate [rows, n] and,
  * where not NULL, dstate [n_streams, n]. h as plx_recurrence wrote it; x is
  * needed with mix alone; state and dfinal may be NULL for 0. dx and dgate may be
- * the arrays of dh, x or gate, not h's; dstate is not dfinal's. */
+ * the arrays of dh, x or gate, not h's; dstate may be dfinal's. */
 int plx_recurrence_backward(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n, int dtype,
                             const int32_t* offsets, const void* dh, int64_t lddh, const void* x,
                             int64_t ldx, const void* gate, int64_t ldg, int gate_kind, int mix,

@@ -4,15 +4,17 @@
 // Units are independent; steps are folded as pairs (A, H): a run of steps takes
 // what it is given, h, to A h + H, and two runs join to (A1 A2, A2 H1 + H2).
 //
-// Bound by memory: a tile of steps x units is read once, its values stay in
-// registers between the fold of its runs and the second walk that writes its
-// results. A warp has the steps of one run, a lane one or two units; the block's
-// runs are joined through shared memory, tiles of one stream through scratch: a
-// tile leaves its pair, looks back over up to 16 tiles before it to the nearest
-// one that already has its end value, and folds from there on in the order of
-// the steps, which gives the bits that the tile in between gives itself: the
-// result does not depend on who was first. Tiles are handed out in the order of
-// the steps, so those waited for are under way.
+// Bound by memory. Long streams are walked by a block each (32 or 64 units),
+// tile after tile of 64 steps, the next tiles on their way into shared memory: a
+// warp has a run of eight steps, whose pairs are joined behind one barrier a tile. Where that leaves
+// SMs idle (few streams of few units) or streams have lengths that only the device
+// knows, rows are cut into parts: a first kernel leaves every part's pair, the
+// second folds those before its own and walks again with results. Reading twice
+// costs less than parts that wait for one another: tiles that look back over the
+// ones before them took 205 us for 65,536 steps of 512 units.
+// Short streams are taken in tiles, several to a block: a warp has the steps of
+// one run, runs are joined through shared memory, values stay in registers.
+// Everything is folded in an order that the arguments set.
 #include <type_traits>
 
 #include "norm.cuh"
@@ -23,43 +25,15 @@ namespace {
 // Runs of a tile, forwards and backwards, which has more values in registers: two
 // blocks an SM either way.
 __host__ __device__ constexpr int warps_of(bool back) { return back ? 12 : 16; }
-constexpr int kRun = 8;      // steps of a run
+constexpr int kRun = 8;      // steps of a run, and of a stage of a walk
 __host__ __device__ constexpr uint32_t tile_steps(bool back) { return warps_of(back) * kRun; }
-constexpr uint32_t kLook = 32;  // tiles that one looks back over
-
-// How rows are cut: `parts` parts of `part_rows` rows (the last may be shorter),
-// each of `chunks` tiles of `chunk_rows` rows (a multiple of the runs' length
-// but for the last). No stream crosses a part's end.
-struct Cut {
-  uint32_t parts, part_rows, chunks, chunk_rows;
-};
-
-Cut cut_rows(uint32_t streams, uint64_t rows, bool ragged, bool back) {
-  Cut c;
-  const uint64_t steps = ragged ? rows : rows / streams;
-  const uint32_t tile = tile_steps(back);
-  if (steps <= tile && !ragged) {  // whole streams in a tile
-    c.chunk_rows = c.part_rows = (uint32_t)(tile / steps * steps);
-    c.chunks = 1;
-  } else {
-    c.part_rows = (uint32_t)steps;
-    c.chunks = (uint32_t)((steps + tile - 1) / tile);
-    c.chunk_rows = tile;
-  }
-  c.parts = (uint32_t)((rows + c.part_rows - 1) / c.part_rows);
-  return c;
-}
-
-struct Scratch {  // at the head of the scratch; the flags of the tiles follow
-  uint32_t ticket, gave_up, pad[62];
-};
-constexpr uint32_t kPair = 1, kEnd = 2;  // a tile has left its pair, its end value
 
 struct Args {
   uint64_t rows;
   uint32_t n, streams, steps;  // steps of a stream; 0 with offsets
-  Cut cut;
   uint32_t tiles;              // across the units
+  uint32_t tile_rows;          // of short streams: whole ones
+  uint32_t groups, group_rows, parts, part_rows;  // of long ones: no stream crosses a group's end
   const int32_t* offsets;
   const void *x, *gate, *h, *dh;
   int64_t ldx, ldg, ldh, lddh;
@@ -67,22 +41,10 @@ struct Args {
   void *out, *out2;            // h; or dx and dgate
   int64_t ldo, ldo2;
   float* state_out;            // final; or dstate
-  Scratch* scratch;
-  uint32_t* flags;
-  float2* pairs;
-  float* ends;
+  float2* pairs;               // of the parts, [group][part][unit]
+  uint32_t* shut;              // parts in which a stream begins (ends), [group][part]
   int32_t* status;
-  uint64_t timeout_ns;
 };
-
-__device__ __forceinline__ uint32_t ld_acquire(const uint32_t* p) {
-  uint32_t v;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void st_release(uint32_t* p, uint32_t v) {
-  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
 
 // One or two units at once.
 template <int V>
@@ -148,33 +110,33 @@ __device__ __forceinline__ void gate_value(W g, W& a, W& keep) {
   }
 }
 
-// The stream of a row, and whether it begins or ends there.
+// The stream of a row, its rows, and whether it begins or ends there.
 struct Place {
   uint32_t stream;
   bool valid, first, last;
+  int64_t begin, end;
 };
 __device__ __forceinline__ Place place_of(const Args& p, uint64_t row) {
   Place q;
   if (!p.offsets) {
-    q.stream = (uint32_t)(row / p.steps);
-    const uint32_t at = (uint32_t)(row - (uint64_t)q.stream * p.steps);
-    q.valid = true;
-    q.first = at == 0;
-    q.last = at + 1 == p.steps;
-    return q;
+    q.stream = (uint32_t)row / p.steps;  // rows < 2^31
+    q.begin = (int64_t)q.stream * p.steps;
+    q.end = q.begin + p.steps;
+  } else {
+    // the last stream that begins at or before the row (empty ones come before it)
+    uint32_t lo = 0, hi = p.streams;
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if ((int64_t)__ldg(p.offsets + mid) <= (int64_t)row) lo = mid;
+      else hi = mid;
+    }
+    q.stream = lo;
+    q.begin = __ldg(p.offsets + lo);
+    q.end = __ldg(p.offsets + lo + 1);
   }
-  // the last stream that begins at or before the row (empty ones come before it)
-  uint32_t lo = 0, hi = p.streams;  // offsets[lo] <= row where any is
-  while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if ((int64_t)__ldg(p.offsets + mid) <= (int64_t)row) lo = mid;
-    else hi = mid;
-  }
-  const int64_t begin = __ldg(p.offsets + lo), end = __ldg(p.offsets + lo + 1);
-  q.stream = lo;
-  q.valid = begin <= (int64_t)row && (int64_t)row < end;
-  q.first = q.valid && begin == (int64_t)row;
-  q.last = q.valid && end == (int64_t)row + 1;
+  q.valid = q.begin <= (int64_t)row && (int64_t)row < q.end;
+  q.first = q.valid && q.begin == (int64_t)row;
+  q.last = q.valid && q.end == (int64_t)row + 1;
   return q;
 }
 
@@ -225,49 +187,23 @@ __device__ __forceinline__ void store_units(float* p, Units<V> v) {
   }
 }
 
+// Short streams, whole ones in a tile.
 template <typename T, int V, bool SIGMOID, bool MIX, bool BACK>
 __global__ void __launch_bounds__(warps_of(BACK) * 32, 2)
-k_recurrence(const __grid_constant__ Args p) {
+k_recurrence_tile(const __grid_constant__ Args p) {
   constexpr int kWarps = warps_of(BACK);
   using W = Units<V>;
   using P = Pack<T, V>;
   struct alignas(8 * V) Pair {
     W a, h;
   };
-  __shared__ Pair runs[kWarps][32], look[kLook][32];
-  __shared__ W look_end[32];
-  __shared__ uint32_t run_shut[kWarps], ticket, near;
+  __shared__ Pair runs[kWarps][32];
+  __shared__ uint32_t run_shut[kWarps];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const W zero = all<W>(0.0f);
-
-  if (p.offsets) {  // offsets that no rows have; streams without steps hand their state on
-    for (uint32_t s = blockIdx.x; s < p.streams; s += gridDim.x) {
-      const int64_t begin = p.offsets[s], end = p.offsets[s + 1];
-      if (threadIdx.x == 0 && (begin < 0 || begin > end || (uint64_t)end > p.rows))
-        record_status(p.status, kStatusBadOffsets);
-      const float* given = BACK ? p.dfinal : p.state;
-      if (begin == end && p.state_out)
-        for (uint32_t i = threadIdx.x; i < p.n; i += kWarps * 32)
-          p.state_out[(uint64_t)s * p.n + i] = given ? given[(uint64_t)s * p.n + i] : 0.0f;
-    }
-  }
-
-  // Tiles in the order of the steps (backwards: from the last), those of all
-  // parts beside each other.
-  uint32_t id = blockIdx.x;
-  const bool chained = p.cut.chunks > 1;
-  if (chained) {
-    if (threadIdx.x == 0) ticket = atomicAdd(&p.scratch->ticket, 1u);
-    __syncthreads();
-    id = ticket;
-  }
-  const uint32_t across = id % p.tiles, rest = id / p.tiles;
-  const uint32_t part = rest % p.cut.parts, turn = rest / p.cut.parts;
-  const uint32_t chunk = BACK ? p.cut.chunks - 1 - turn : turn;
-  const uint64_t part_end = min((uint64_t)(part + 1) * p.cut.part_rows, p.rows);
-  const uint64_t row0 = (uint64_t)part * p.cut.part_rows + (uint64_t)chunk * p.cut.chunk_rows;
-  const uint64_t row1 = min(row0 + p.cut.chunk_rows, part_end);
-  const uint32_t unit = (across * 32 + lane) * V;
+  const uint64_t row0 = (uint64_t)(blockIdx.x / p.tiles) * p.tile_rows;
+  const uint64_t row1 = min(row0 + p.tile_rows, p.rows);
+  const uint32_t unit = (blockIdx.x % p.tiles * 32 + lane) * V;
   const bool in = unit < p.n;  // V divides n
   // This warp's run, in the order that it is walked.
   const uint32_t run = BACK ? kWarps - 1 - warp : warp;
@@ -290,12 +226,15 @@ k_recurrence(const __grid_constant__ Args p) {
   load(q1, BACK ? p.dh : p.x, BACK ? p.lddh : p.ldx);
   if constexpr (BACK && MIX) load(q3, p.x, p.ldx);
   // Where streams begin and end in the run: a row to a lane.
-  Place mine = {0, false, false, false};
-  if ((int)lane < len) mine = place_of(p, at + lane);
-  const uint32_t valid = __ballot_sync(~0u, mine.valid);
-  const uint32_t first = __ballot_sync(~0u, mine.first), last = __ballot_sync(~0u, mine.last);
+  uint32_t stream = 0, place = 0;
+  if ((int)lane < len) {
+    stream = (uint32_t)(at + lane) / p.steps;
+    place = (uint32_t)(at + lane) - stream * p.steps;
+  }
+  const uint32_t first = __ballot_sync(~0u, (int)lane < len && place == 0);
+  const uint32_t last = __ballot_sync(~0u, (int)lane < len && place + 1 == p.steps);
   auto state_at = [&](const float* states, int i) {
-    const uint32_t s = __shfl_sync(~0u, mine.stream, i);
+    const uint32_t s = __shfl_sync(~0u, stream, i);
     return states ? load_units<V>(states + (uint64_t)s * p.n + unit, in) : zero;
   };
   if constexpr (BACK) {
@@ -303,7 +242,7 @@ k_recurrence(const __grid_constant__ Args p) {
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
       q2[i] = nothing;
-      if (in && (valid >> i & 1) && !(first >> i & 1)) q2[i] = load_pack<T, V>(from + i * p.ldh);
+      if (in && i < len && !(first >> i & 1)) q2[i] = load_pack<T, V>(from + i * p.ldh);
     }
   }
 
@@ -341,89 +280,7 @@ k_recurrence(const __grid_constant__ Args p) {
   runs[warp][lane] = {A, H};
   if (lane == 0) run_shut[warp] = stop;
   __syncthreads();
-
-  // ---- what the tile is given, and what it leaves
   W carry = zero;
-  if (chained) {
-    const uint32_t step = p.cut.parts * p.tiles;  // between tiles of a part
-    Pair* pairs = reinterpret_cast<Pair*>(p.pairs);
-    W* ends = reinterpret_cast<W*>(p.ends);
-    W ta = all<W>(1.0f), th = zero;
-    bool shut = turn == 0;
-    auto leave = [&](bool end) {
-      if (end) ends[(uint64_t)id * 32 + lane] = th;
-      else pairs[(uint64_t)id * 32 + lane] = {ta, th};
-      __threadfence();
-      __syncwarp();
-      if (lane == 0) st_release(p.flags + id, end ? kEnd : kPair);
-    };
-    if (warp == 0) {
-      for (int w = 0; w < kWarps; ++w) {
-        const Pair v = runs[w][lane];
-        const bool s = run_shut[w] != 0;
-        shut |= s;
-        th = s ? v.h : fmaw(v.a, th, v.h);
-        ta = s ? zero : mulw(ta, v.a);
-      }
-      leave(shut);
-    } else if (warp == 1 && turn > 0) {
-      // The nearest tile before that has its end value, all in between their pairs.
-      const bool there = lane < turn;
-      const uint32_t* flag = p.flags + id - (lane + 1) * (there ? step : 0);
-      const uint64_t t0 = global_timer_ns();
-      uint32_t found = kLook;
-      for (uint32_t spin = 1;; ++spin) {
-        const uint32_t v = there ? ld_acquire(flag) : kPair;
-        const uint32_t ended = __ballot_sync(~0u, v == kEnd);
-        const uint32_t waiting = __ballot_sync(~0u, v == 0);
-        if (ended) {
-          found = __ffs(ended) - 1;
-          if (!(waiting & ((1u << found) - 1))) break;
-        }
-        if ((spin & 63u) == 0) {
-          bool stop_now = *(volatile uint32_t*)&p.scratch->gave_up != 0;
-          if (global_timer_ns() - t0 > p.timeout_ns) {
-            record_status(p.status, kStatusTimeout);
-            *(volatile uint32_t*)&p.scratch->gave_up = 1;
-            stop_now = true;
-          }
-          if (__any_sync(~0u, stop_now)) {
-            found = kLook;
-            break;
-          }
-        }
-      }
-      __threadfence();
-      if (lane == 0) near = found;
-    }
-    __syncthreads();
-    if (turn > 0 && near < kLook) {
-      const uint32_t count = near;
-      for (uint32_t j = warp; j <= count; j += kWarps) {
-        const uint64_t from = (uint64_t)(id - (j + 1) * step) * 32 + lane;
-        if (j == count) {
-          if constexpr (V == 2) look_end[lane] = __ldcg(reinterpret_cast<const float2*>(ends + from));
-          else look_end[lane] = __ldcg(ends + from);
-        } else if constexpr (V == 2) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(pairs + from));
-          look[j][lane] = {pack2(v.x, v.y), pack2(v.z, v.w)};
-        } else {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(pairs + from));
-          look[j][lane] = {v.x, v.y};
-        }
-      }
-      __syncthreads();
-      carry = look_end[lane];
-      for (int j = (int)count - 1; j >= 0; --j) {
-        const Pair v = look[j][lane];
-        carry = fmaw(v.a, carry, v.h);
-      }
-    }
-    if (warp == 0 && !shut) {
-      th = fmaw(ta, carry, th);
-      leave(true);
-    }
-  }
   for (uint32_t w = 0; w < warp; ++w) {
     const Pair v = runs[w][lane];
     carry = run_shut[w] ? v.h : fmaw(v.a, carry, v.h);
@@ -436,33 +293,343 @@ k_recurrence(const __grid_constant__ Args p) {
     if (i >= len) continue;
     const auto& st = steps[i];
     const int64_t row = (int64_t)(at + i);
-    const bool write = in && (valid >> i & 1);
     if constexpr (BACK) {
       if (stop >> i & 1) carry = state_at(p.dfinal, i);
       const W g = addw(wide<T, V>(st.dh), carry);
       carry = mulw(st.a, g);
-      if (write) {
+      if (in) {
         *reinterpret_cast<P*>((T*)p.out + row * p.ldo + unit) = narrow<T, V>(st.dx(g));
         *reinterpret_cast<P*>((T*)p.out2 + row * p.ldo2 + unit) = narrow<T, V>(mulw(g, st.slope));
       }
     } else {
       carry = stop >> i & 1 ? st.b : fmaw(st.a, carry, st.b);
-      if (write) *reinterpret_cast<P*>((T*)p.out + row * p.ldo + unit) = narrow<T, V>(carry);
+      if (in) *reinterpret_cast<P*>((T*)p.out + row * p.ldo + unit) = narrow<T, V>(carry);
     }
     if (p.state_out && ((BACK ? first : last) >> i & 1)) {
-      const uint32_t s = __shfl_sync(~0u, mine.stream, i);
+      const uint32_t s = __shfl_sync(~0u, stream, i);
       if (in) store_units<V>(p.state_out + (uint64_t)s * p.n + unit, carry);
     }
   }
 }
 
-__global__ void k_copy_state(uint64_t count, const float* from, float* to) {
-  const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < count) to[i] = from ? from[i] : 0.0f;
+// Stages of a walk under way: a run of every array that it reads, a lane's own
+// values (no other lane reads them, so that no barrier is needed). Values of less
+// than four bytes are read when their turn comes.
+constexpr int kWalkWarps = 8;
+constexpr uint32_t kWalkSteps = kWalkWarps * kRun;  // of a tile
+template <typename T, int V, int ARRAYS>
+struct WalkRing {
+  static constexpr int piece = V * sizeof(T);
+  static constexpr bool used = piece >= 4;
+  static constexpr int row = 32 * piece;
+  static constexpr int warp = ARRAYS * kRun * row;
+  static constexpr int stage = kWalkWarps * warp;
+  static constexpr int stages = stage <= 16 * 1024 ? 4 : stage <= 32 * 1024 ? 3 : 2;
+  static constexpr int bytes = used ? stages * stage : 0;
+};
+
+// A part of a long stream (or of ragged ones behind each other), tile after tile.
+// LEAVE: the part's pair, else its results.
+template <typename T, int V, bool SIGMOID, bool MIX, bool BACK, bool LEAVE>
+__global__ void __launch_bounds__(kWalkWarps * 32, BACK && !LEAVE ? 2 : 4)
+k_recurrence_walk(const __grid_constant__ Args p) {
+  using W = Units<V>;
+  using P = Pack<T, V>;
+  constexpr int ARRAYS = LEAVE || !BACK ? 2 : MIX ? 4 : 3;
+  using R = WalkRing<T, V, ARRAYS>;
+  constexpr int S = R::stages;
+  struct alignas(8 * V) Pair {
+    W a, h;
+  };
+  extern __shared__ uint4 walk_bytes[];
+  __shared__ Pair runs[2][kWalkWarps][32];
+  __shared__ uint32_t run_shut[2][kWalkWarps];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const W zero = all<W>(0.0f);
+
+  if (p.offsets && !LEAVE) {  // offsets that no rows have; streams without steps hand their state on
+    for (uint32_t s = blockIdx.x; s < p.streams; s += gridDim.x) {
+      const int64_t begin = p.offsets[s], end = p.offsets[s + 1];
+      if (threadIdx.x == 0 && (begin < 0 || begin > end || (uint64_t)end > p.rows))
+        record_status(p.status, kStatusBadOffsets);
+      const float* given = BACK ? p.dfinal : p.state;
+      if (begin == end && p.state_out)
+        for (uint32_t i = threadIdx.x; i < p.n; i += kWalkWarps * 32)
+          p.state_out[(uint64_t)s * p.n + i] = given ? given[(uint64_t)s * p.n + i] : 0.0f;
+    }
+  }
+  const uint32_t across = blockIdx.x % p.tiles, rest = blockIdx.x / p.tiles;
+  const uint32_t group = rest / p.parts, part = rest % p.parts;
+  const uint32_t unit = (across * 32 + lane) * V;
+  const bool in = unit < p.n;  // V divides n
+  const int64_t g0 = (int64_t)group * p.group_rows, g1 = min(g0 + p.group_rows, (int64_t)p.rows);
+  const int64_t row0 = min(g0 + (int64_t)part * p.part_rows, g1);
+  const int64_t row1 = min(row0 + p.part_rows, g1);
+  const int tiles = (int)((row1 - row0 + kWalkSteps - 1) / kWalkSteps);
+  // This warp's run of the first tile that is walked; tiles and the steps of a run
+  // follow in the direction `dir`.
+  constexpr int dir = BACK ? -1 : 1;
+  int64_t at = row0 + (BACK ? (int64_t)(tiles - 1) * kWalkSteps + (kWalkWarps - 1 - warp) * kRun
+                            : warp * kRun);
+
+  const T* from[4] = {(const T*)p.gate, (const T*)(BACK ? p.dh : p.x), (const T*)p.h,
+                      (const T*)p.x};
+  const int64_t ld[4] = {p.ldg, BACK ? p.lddh : p.ldx, p.ldh, p.ldx};
+  char* ring = reinterpret_cast<char*>(walk_bytes) + warp * R::warp + lane * R::piece;
+  const T* next[ARRAYS];  // where the run fetched next begins
+#pragma unroll
+  for (int k = 0; k < ARRAYS; ++k) next[k] = from[k] + (at - (k == 2 ? 1 : 0)) * ld[k] + unit;
+  int64_t next_at = at;
+  int fetched = 0;
+  auto fetch = [&](uint32_t stage) {
+    if constexpr (R::used) {
+      if (in && fetched < tiles) {
+        const int left = (int)min((int64_t)kRun, row1 - next_at);
+        char* to = ring + stage * R::stage;
+#pragma unroll
+        for (int k = 0; k < ARRAYS; ++k) {
+          const T* q = next[k];
+#pragma unroll
+          for (int i = 0; i < kRun; ++i) {
+            // h before the first row of all is no row's
+            if (i < left && !(k == 2 && i == 0 && next_at == 0))
+              copy_async<R::piece>(to + (k * kRun + i) * R::row, q);
+            q += ld[k];
+          }
+          next[k] += dir * (int)kWalkSteps * ld[k];
+        }
+      }
+      next_at += dir * (int)kWalkSteps;
+      ++fetched;
+      copy_commit();
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(s);
+
+  W A = all<W>(1.0f), given = zero;  // forwards h; backwards what a step hands to the one before
+  bool shut = false;
+  if constexpr (!LEAVE) {
+    // what the parts walked before leave
+    const uint32_t before = BACK ? p.parts - 1 - part : part;
+    if (before) {
+      if (warp == 0) {
+#pragma unroll 8
+        for (uint32_t j = 0; j < before; ++j) {
+          const uint32_t q = group * p.parts + (BACK ? p.parts - 1 - j : j);
+          const bool s = p.shut[q] != 0;
+          const Pair v = reinterpret_cast<const Pair*>(p.pairs)[((uint64_t)q * p.tiles + across) * 32 + lane];
+          given = s ? v.h : fmaw(v.a, given, v.h);
+        }
+        runs[0][0][lane].h = given;
+      }
+      __syncthreads();
+      given = runs[0][0][lane].h;
+      __syncthreads();
+    }
+  }
+  P nothing;
+#pragma unroll
+  for (int e = 0; e < V; ++e) nothing.v[e] = from_f32<T>(0.0f);
+  int64_t clear0 = 0, clear1 = 0;  // rows in which no stream begins or ends, and all are some stream's
+  uint32_t stage = 0, half = 0;
+  for (int tile = 0; tile < tiles; ++tile, at += dir * (int)kWalkSteps, half ^= 1) {
+    const int len = (int)max((int64_t)0, min((int64_t)kRun, row1 - at));
+    P q[4][kRun];
+    if constexpr (R::used) {
+      copy_wait<S - 2>();
+      const char* to = ring + stage * R::stage;
+#pragma unroll
+      for (int k = 0; k < ARRAYS; ++k)
+#pragma unroll
+        for (int i = 0; i < kRun; ++i)
+          q[k][i] = *reinterpret_cast<const P*>(to + (k * kRun + i) * R::row);
+      fetch(stage == 0 ? S - 1 : stage - 1);
+      stage = stage == S - 1 ? 0 : stage + 1;
+    } else {
+#pragma unroll
+      for (int k = 0; k < ARRAYS; ++k)
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+          q[k][i] = nothing;
+          const int64_t r = at + i - (k == 2 ? 1 : 0);
+          if (in && i < len && r >= 0) q[k][i] = load_pack<T, V>(from[k] + r * ld[k] + unit);
+        }
+    }
+    uint32_t valid = 0xff, first = 0, last = 0;
+    Place mine = {0, false, false, false};
+    if (len && !(clear0 <= at && at + len <= clear1)) {
+      if ((int)lane < len) mine = place_of(p, (uint64_t)(at + lane));
+      valid = __ballot_sync(~0u, mine.valid);
+      first = __ballot_sync(~0u, mine.first);
+      last = __ballot_sync(~0u, mine.last);
+      // the stream that the last of these rows is in goes on
+      clear0 = __shfl_sync(~0u, mine.begin, BACK ? 0 : len - 1) + 1;
+      clear1 = __shfl_sync(~0u, mine.end, BACK ? 0 : len - 1) - 1;
+    }
+    const uint32_t stop = BACK ? last : first;  // rows at which what was before does not count
+    auto state_at = [&](const float* states, int i) {
+      const uint32_t s = __shfl_sync(~0u, mine.stream, i);
+      return states ? load_units<V>(states + (uint64_t)s * p.n + unit, in) : zero;
+    };
+
+    // ---- the run's pair
+    Step<T, V, SIGMOID, MIX, BACK> st[kRun];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      if constexpr (BACK && LEAVE) {
+        W k;
+        gate_value<SIGMOID>(wide<T, V>(q[0][i]), st[i].a, k);
+        st[i].dh = q[1][i];
+      } else if constexpr (BACK) {
+        W before = wide<T, V>(q[2][i]);
+        if (first >> i & 1) before = state_at(p.state, i);
+        st[i].backward(q[0][i], q[1][i], before, q[MIX ? 3 : 2][i]);
+      } else {
+        st[i].forward(q[0][i], q[1][i]);
+      }
+    }
+    W a = all<W>(1.0f), h = zero;
+    if (len == kRun && !stop) {
+#pragma unroll
+      for (int k = 0; k < kRun; ++k) {
+        const int i = BACK ? kRun - 1 - k : k;
+        h = BACK ? mulw(st[i].a, addw(wide<T, V>(st[i].dh), h)) : fmaw(st[i].a, h, st[i].b);
+        a = mulw(a, st[i].a);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kRun; ++k) {
+        const int i = BACK ? kRun - 1 - k : k;
+        if (i >= len) continue;
+        if (stop >> i & 1) {  // the same for the whole warp
+          h = state_at(BACK ? p.dfinal : p.state, i);
+          a = zero;
+        }
+        h = BACK ? mulw(st[i].a, addw(wide<T, V>(st[i].dh), h)) : fmaw(st[i].a, h, st[i].b);
+        a = mulw(a, st[i].a);
+      }
+    }
+    runs[half][warp][lane] = {a, h};
+    if (lane == 0) run_shut[half][warp] = stop;
+    __syncthreads();  // the half is written again after the next tile's barrier
+    W carry = given;
+#pragma unroll
+    for (uint32_t w = 0; w < kWalkWarps; ++w) {
+      const Pair v = runs[half][w][lane];
+      const bool s = run_shut[half][w] != 0;
+      if (w == warp) carry = given;
+      given = s ? v.h : fmaw(v.a, given, v.h);
+      if constexpr (LEAVE) {
+        A = s ? zero : mulw(A, v.a);
+        shut |= s;
+      }
+    }
+    if constexpr (!LEAVE) {
+      // ---- the run once more, from what it is given
+      T *o1 = (T*)p.out + at * p.ldo + unit, *o2 = (T*)p.out2 + at * p.ldo2 + unit;
+      if (BACK) {
+        o1 += (kRun - 1) * p.ldo;
+        o2 += (kRun - 1) * p.ldo2;
+      }
+      auto results = [&](int i) {
+        if constexpr (BACK) {
+          const W g = addw(wide<T, V>(st[i].dh), carry);
+          carry = mulw(st[i].a, g);
+          *reinterpret_cast<P*>(o1) = narrow<T, V>(st[i].dx(g));
+          *reinterpret_cast<P*>(o2) = narrow<T, V>(mulw(g, st[i].slope));
+        } else {
+          carry = fmaw(st[i].a, carry, st[i].b);
+          *reinterpret_cast<P*>(o1) = narrow<T, V>(carry);
+        }
+      };
+      if (len == kRun && valid == 0xff && !first && !last) {
+        if (in)
+#pragma unroll
+          for (int k = 0; k < kRun; ++k) {
+            results(BACK ? kRun - 1 - k : k);
+            o1 += dir * p.ldo;
+            if (BACK) o2 += dir * p.ldo2;
+          }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+          const int i = BACK ? kRun - 1 - k : k;
+          if (i < len) {
+            if (stop >> i & 1) carry = state_at(BACK ? p.dfinal : p.state, i);
+            if (in && (valid >> i & 1)) results(i);
+            if (p.state_out && ((BACK ? first : last) >> i & 1)) {
+              const uint32_t s = __shfl_sync(~0u, mine.stream, i);
+              if (in) store_units<V>(p.state_out + (uint64_t)s * p.n + unit, carry);
+            }
+          }
+          o1 += dir * p.ldo;
+          if (BACK) o2 += dir * p.ldo2;
+        }
+      }
+    }
+  }
+  if constexpr (LEAVE) {
+    if (warp == 0) {
+      const uint32_t q = group * p.parts + part;
+      reinterpret_cast<Pair*>(p.pairs)[((uint64_t)q * p.tiles + across) * 32 + lane] = {A, given};
+      if (across == 0 && lane == 0) p.shut[q] = shut;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256)
+k_copy_state(uint64_t count, const float* from, float* to) {
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += gridDim.x * 256ull)
+    to[i] = from ? from[i] : 0.0f;
+}
+
+// How a call is cut, and what it needs of scratch.
+struct Plan {
+  bool short_streams, states_apart;
+  int units;  // a lane's
+  uint32_t tiles, tile_rows, groups, group_rows, parts, part_rows;
+  uint64_t pair_bytes, shut_bytes;
+};
+
+// Streams of at most this many steps go in tiles.
+constexpr uint32_t kShort = 64;
+// Blocks that keep all SMs busy.
+constexpr uint32_t kWalks = 148 * 3;
+
+Plan plan_of(uint32_t streams, uint64_t rows, uint32_t n, bool ragged, int units, bool back) {
+  Plan c = {};
+  c.units = units;
+  const uint32_t steps = ragged ? (uint32_t)rows : (uint32_t)(rows / streams);
+  c.tiles = (n + 32 * units - 1) / (32 * units);
+  c.short_streams = !ragged && steps <= kShort;
+  if (c.short_streams) {
+    c.tile_rows = tile_steps(back) / steps * steps;
+    c.states_apart = back;
+    return c;
+  }
+  c.group_rows = steps;
+  c.groups = ragged ? 1 : streams;
+  const uint64_t walks = (uint64_t)c.groups * c.tiles;
+  c.parts = walks >= kWalks / 2 ? 1 : (uint32_t)((kWalks + walks - 1) / walks);
+  c.parts = std::max(1u, std::min(c.parts, steps / kShort));
+  c.part_rows = (steps + c.parts - 1) / c.parts;
+  c.part_rows = (c.part_rows + kWalkSteps - 1) / kWalkSteps * kWalkSteps;
+  c.parts = (steps + c.part_rows - 1) / c.part_rows;
+  c.states_apart = c.parts > 1;
+  if (c.parts > 1) {
+    c.pair_bytes = (uint64_t)c.groups * c.parts * c.tiles * 32 * units * 8;
+    c.shut_bytes = ((uint64_t)c.groups * c.parts * 4 + 255) / 256 * 256;
+  }
+  return c;
+}
+
+uint64_t state_bytes(uint32_t streams, uint32_t n) {
+  return ((uint64_t)streams * n * 4 + 255) / 256 * 256;
 }
 
 int check_recurrence(const plx_ctx* ctx, uint32_t streams, uint64_t rows, uint32_t n, int dtype,
-                     const int32_t* offsets, int gate_kind, const void* scratch,
+                     const int32_t* offsets, int gate_kind, bool back, const void* scratch,
                      size_t scratch_bytes) {
   PLX_CHECK_ARG(ctx, "ctx is required");
   PLX_CHECK_ARG(valid_dtype(dtype), "dtype %d is none of PLX_F32, PLX_BF16, PLX_F16", dtype);
@@ -477,7 +644,7 @@ int check_recurrence(const plx_ctx* ctx, uint32_t streams, uint64_t rows, uint32
   PLX_CHECK_ARG(offsets || streams == 0 || rows % streams == 0,
                 "%llu rows are not the same number of steps for each of %u streams",
                 (unsigned long long)rows, streams);
-  const size_t need = plx_recurrence_scratch_bytes(streams, rows, n, offsets != nullptr);
+  const size_t need = plx_recurrence_scratch_bytes(streams, rows, n, offsets != nullptr, back);
   PLX_CHECK_ARG(need == 0 || (scratch && scratch_bytes >= need),
                 "%zu bytes of scratch are needed, got %zu", need,
                 scratch ? scratch_bytes : (size_t)0);
@@ -490,21 +657,21 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
   if (a.streams == 0) return PLX_OK;
   DeviceGuard guard(ctx->device);
   PLX_TRY_CUDA(guard.err);
-  if (a.rows == 0) {
-    const float* from = BACK ? a.dfinal : a.state;
-    const uint64_t count = (uint64_t)a.streams * a.n;
-    if (a.state_out && a.state_out != from)
-      k_copy_state<<<(unsigned)((count + 255) / 256), 256, 0, ctx->stream>>>(count, from,
-                                                                            a.state_out);
+  const float* given = BACK ? a.dfinal : a.state;
+  const uint64_t count = (uint64_t)a.streams * a.n;
+  float* state_out = a.state_out;
+  auto copy_state = [&](const float* from) {
+    k_copy_state<<<(unsigned)std::min<uint64_t>((count + 255) / 256, 1 << 16), 256, 0,
+                   ctx->stream>>>(count, from, state_out);
     PLX_LAUNCH_CHECK("k_copy_state");
     return PLX_OK;
-  }
+  };
+  if (a.rows == 0) return state_out && state_out != given ? copy_state(given) : PLX_OK;
   if (a.rows == 1) a.ldx = a.ldg = a.ldh = a.lddh = a.ldo = a.ldo2 = a.n;
   a.steps = a.offsets ? 0 : (uint32_t)(a.rows / a.streams);
-  a.cut = cut_rows(a.streams, a.rows, a.offsets != nullptr, BACK);
   a.status = ctx->d_status;
-  a.timeout_ns = ctx->timeout_ns;
-  return with_dtype(dtype, [&](auto t) {
+  bool copied = false;
+  const int rc = with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     uint64_t odd = a.n;
     for (int64_t ld : {a.ldx, a.ldg, a.ldh, a.lddh, a.ldo, a.ldo2}) odd |= (uint64_t)ld;
@@ -513,23 +680,48 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
       odd |= reinterpret_cast<uintptr_t>(q);
     auto go = [&](auto v_c, auto sigmoid_c, auto mix_c) -> int {
       constexpr int V = decltype(v_c)::value;
-      a.tiles = (a.n + 32 * V - 1) / (32 * V);
-      const uint64_t blocks = (uint64_t)a.tiles * a.cut.parts * a.cut.chunks;
+      constexpr bool SIGMOID = decltype(sigmoid_c)::value, MIX = decltype(mix_c)::value;
+      const Plan c = plan_of(a.streams, a.rows, a.n, a.offsets != nullptr, V, BACK);
+      a.tiles = c.tiles;
+      a.tile_rows = c.tile_rows;
+      a.groups = c.groups;
+      a.group_rows = c.group_rows;
+      a.parts = c.parts;
+      a.part_rows = c.part_rows;
+      const uint64_t blocks =
+          c.short_streams ? (a.rows + c.tile_rows - 1) / c.tile_rows * c.tiles
+                          : (uint64_t)c.groups * c.parts * c.tiles;
       if (blocks >= (1ull << 31))
         return set_error(PLX_ERR_CAPACITY, "%llu rows of %u units are too many for one call",
                          (unsigned long long)a.rows, a.n);
-      if (a.cut.chunks > 1) {
-        char* at = (char*)scratch;
-        a.scratch = (Scratch*)at;
-        a.flags = (uint32_t*)(at + sizeof(Scratch));
-        const uint64_t head = sizeof(Scratch) + (blocks * 4 + 255) / 256 * 256;
-        a.pairs = (float2*)(at + head);
-        a.ends = (float*)(at + head + blocks * 32 * V * 8);
-        PLX_TRY_CUDA(cudaMemsetAsync(at, 0, head, ctx->stream));
+      char* at = (char*)scratch;
+      if (c.states_apart) {
+        // What is given is read by other warps than those that write the result:
+        // where both are one array, the result goes to scratch first.
+        copied = state_out && state_out == given;
+        if (copied) a.state_out = (float*)at;
+        at += state_bytes(a.streams, a.n);
       }
-      k_recurrence<T, V, decltype(sigmoid_c)::value, decltype(mix_c)::value, BACK>
-          <<<(unsigned)blocks, warps_of(BACK) * 32, 0, ctx->stream>>>(a);
-      PLX_LAUNCH_CHECK("k_recurrence");
+      if (c.short_streams) {
+        k_recurrence_tile<T, V, SIGMOID, MIX, BACK>
+            <<<(unsigned)blocks, warps_of(BACK) * 32, 0, ctx->stream>>>(a);
+        PLX_LAUNCH_CHECK("k_recurrence_tile");
+        return PLX_OK;
+      }
+      if (c.parts > 1) {
+        a.shut = (uint32_t*)at;
+        a.pairs = (float2*)(at + c.shut_bytes);
+        using R = WalkRing<T, V, 2>;
+        constexpr auto leave = k_recurrence_walk<T, V, SIGMOID, MIX, BACK, true>;
+        if (R::bytes > 48 * 1024 - 8192) PLX_TRY_CUDA(allow_shared<leave>(ctx->device, R::bytes));
+        leave<<<(unsigned)blocks, kWalkWarps * 32, R::bytes, ctx->stream>>>(a);
+        PLX_LAUNCH_CHECK("k_recurrence_walk");
+      }
+      using R = WalkRing<T, V, BACK ? (MIX ? 4 : 3) : 2>;
+      constexpr auto kernel = k_recurrence_walk<T, V, SIGMOID, MIX, BACK, false>;
+      if (R::bytes > 48 * 1024 - 8192) PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, R::bytes));
+      kernel<<<(unsigned)blocks, kWalkWarps * 32, R::bytes, ctx->stream>>>(a);
+      PLX_LAUNCH_CHECK("k_recurrence_walk");
       return PLX_OK;
     };
     using std::integral_constant;
@@ -542,6 +734,8 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
     return odd % (2 * sizeof(T)) == 0 ? kinds(integral_constant<int, 2>{})
                                       : kinds(integral_constant<int, 1>{});
   });
+  if (rc != PLX_OK) return rc;
+  return copied ? copy_state(a.state_out) : PLX_OK;
 }
 
 }  // namespace
@@ -550,12 +744,15 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
 using namespace plx;
 
 extern "C" size_t plx_recurrence_scratch_bytes(uint32_t n_streams, uint64_t rows, uint32_t n,
-                                               int ragged) {
-  if (n_streams == 0 || rows == 0 || n == 0) return 0;
-  const Cut c = cut_rows(n_streams, rows, ragged != 0, true);  // the shorter tiles
-  if (c.chunks == 1) return 0;
-  const uint64_t blocks = (uint64_t)c.parts * c.chunks * ((n + 31) / 32);
-  return sizeof(Scratch) + (blocks * 4 + 255) / 256 * 256 + blocks * 32 * 12;
+                                               int ragged, int backward) {
+  if (n_streams == 0 || rows == 0 || n == 0 || rows >= (1ull << 31)) return 0;
+  uint64_t most = 0;  // whatever the arrays' alignment
+  for (int units : {1, 2}) {
+    const Plan c = plan_of(n_streams, rows, n, ragged != 0, units, backward != 0);
+    most = std::max(most, (c.states_apart ? state_bytes(n_streams, n) : 0) + c.pair_bytes +
+                              c.shut_bytes);
+  }
+  return most;
 }
 
 extern "C" int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n,
@@ -563,7 +760,7 @@ extern "C" int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, u
                               const void* gate, int64_t ldg, int gate_kind, int mix,
                               const float* state, void* h, int64_t ldh, float* final_state,
                               void* scratch, size_t scratch_bytes) {
-  if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, scratch,
+  if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, false, scratch,
                                 scratch_bytes))
     return rc;
   if (rows) PLX_CHECK_ARG(x && gate && h, "x, gate and h are required");
@@ -594,7 +791,7 @@ extern "C" int plx_recurrence_backward(plx_ctx* ctx, uint32_t n_streams, uint64_
                                        int64_t ldh, const float* state, const float* dfinal,
                                        void* dx, int64_t lddx, void* dgate, int64_t lddg,
                                        float* dstate, void* scratch, size_t scratch_bytes) {
-  if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, scratch,
+  if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, true, scratch,
                                 scratch_bytes))
     return rc;
   if (rows) {
