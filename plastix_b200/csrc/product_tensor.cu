@@ -10,8 +10,6 @@
 // the order of the blocks.
 // Few rows (at most 64) are the tile's second side, so that the first one's 128
 // are units of the layer.
-#include <atomic>
-
 #include "cluster.cuh"
 #include "dense.cuh"
 #include "tensor.cuh"
@@ -310,45 +308,6 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
   }
 }
 
-// The driver's encoder of tensor maps, found once.
-using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                            const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                            CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                            CUtensorMapFloatOOBfill);
-int encoder(Encode* out) {
-  static std::atomic<void*> found{nullptr};
-  void* f = found.load(std::memory_order_acquire);
-  if (!f) {
-    cudaDriverEntryPointQueryResult q;
-    PLX_TRY_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q));
-    if (q != cudaDriverEntryPointSuccess || !f)
-      return set_error(PLX_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
-    found.store(f, std::memory_order_release);
-  }
-  *out = reinterpret_cast<Encode>(f);
-  return PLX_OK;
-}
-
-// Boxes of 64 values of the contiguous dimension by `other`; outside: 0.
-int tensor_map(CUtensorMap* map, bool bf16, const Operand& o, uint32_t count, uint32_t depth,
-               uint32_t other) {
-  Encode encode;
-  if (int rc = encoder(&encode)) return rc;
-  const uint32_t inner = o.k_major ? depth : count, outer = o.k_major ? count : depth;
-  const cuuint64_t dims[2] = {inner, outer};
-  const cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
-  const cuuint32_t box[2] = {64, other}, elem[2] = {1, 1};
-  const CUresult e = encode(
-      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-      const_cast<void*>(o.p), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (e != CUDA_SUCCESS)
-    return set_error(PLX_ERR_CUDA, "cuTensorMapEncodeTiled: error %d for %u x %u values, stride %lld",
-                     (int)e, inner, outer, (long long)o.ld);
-  return PLX_OK;
-}
-
 template <typename T, int BN>
 int launch(plx_ctx* ctx, TensorProduct& t, const Product& p, const Operand& a, const Operand& b,
            uint32_t parts, bool wide) {
@@ -357,8 +316,12 @@ int launch(plx_ctx* ctx, TensorProduct& t, const Product& p, const Operand& a, c
   t.tiles_a = (t.rows + kTileA - 1) / kTileA;
   t.tiles_b = (t.cols + BN - 1) / BN;
   t.kind = product_kind(bf16, !a.k_major, !b.k_major, BN);
-  if (int rc = tensor_map(&t.a, bf16, a, t.rows, t.depth, a.k_major ? kTileA : kTileK)) return rc;
-  if (int rc = tensor_map(&t.b, bf16, b, t.cols, t.depth, b.k_major ? BN : kTileK)) return rc;
+  auto map = [&](CUtensorMap* m, const Operand& o, uint32_t count, uint32_t tile) {
+    return tensor_map(m, bf16 ? PLX_BF16 : PLX_F16, o.p, o.k_major ? t.depth : count,
+                      o.k_major ? count : t.depth, o.ld, 64, o.k_major ? tile : kTileK, true);
+  };
+  if (int rc = map(&t.a, a, t.rows, kTileA)) return rc;
+  if (int rc = map(&t.b, b, t.cols, BN)) return rc;
   const uint64_t tiles = (uint64_t)t.tiles_a * t.tiles_b;
   if (tiles >= (1ull << 28))
     return set_error(PLX_ERR_CAPACITY, "%u x %u results are too many for one call", p.rows, p.cols);

@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "norm.cuh"
+#include "tensor.cuh"
 
 namespace plx {
 namespace {
@@ -44,6 +45,7 @@ struct Args {
   float2* pairs;               // of the parts, [group][part][unit]
   uint32_t* shut;              // parts in which a stream begins (ends), [group][part]
   int32_t* status;
+  uint64_t timeout_ns;
 };
 
 // One or two units at once.
@@ -77,36 +79,41 @@ __device__ __forceinline__ Pack<T, V> narrow(Units<V> v) {
   return q;
 }
 
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ float rcp_approx(float d) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
   return r;
 }
+// The larger of each value and -87 (NaN stays NaN): e^87 is a 32-bit number.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> at_least_minus_87(Pack<T, V> q) {
+  if constexpr (sizeof(T) == 2 && V == 2) {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    T2 v = *reinterpret_cast<T2*>(&q);
+    if constexpr (std::is_same_v<T, __half>) v = __hmax2_nan(v, __floats2half2_rn(-87.0f, -87.0f));
+    else v = __hmax2_nan(v, __floats2bfloat162_rn(-87.0f, -87.0f));
+    return *reinterpret_cast<Pack<T, V>*>(&v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) q.v[e] = from_f32<T>(max_nan(to_f32(q.v[e]), -87.0f));
+    return q;
+  }
+}
 
 // a and 1 - a of a gate, neither by a difference that cancels: with e = exp(-gate),
-// 1 / (1 + e) and e / (1 + e). The quotient gets one Newton step: what a is off by, a
-// long memory raises to its length. e is at most 2^126 (a gate of -infinity leaves
-// 2^-126 of h).
-template <typename W>
-__device__ __forceinline__ W exp_minus(W g) {
-  return each(mulw(g, all<W>(-kLog2e)), [](float t) { return exp2_approx(min_nan(t, 126.0f)); });
-}
-template <bool SIGMOID, typename W>
-__device__ __forceinline__ void gate_value(W g, W& a, W& keep) {
+// 1 / (1 + e) and e / (1 + e). Gates below -87 count as -87 (which leaves e^-87 of
+// h). The quotient is off by 2^-23 at most.
+template <bool SIGMOID, typename T, int V>
+__device__ __forceinline__ void gate_value(Pack<T, V> gate, Units<V>& a, Units<V>& keep) {
+  using W = Units<V>;
   if constexpr (SIGMOID) {
-    const W e = exp_minus(g);
-    const W d = addw(e, all<W>(1.0f)), minus = each(d, [](float t) { return -t; });
-    const W r = each(d, rcp_approx);
-    a = fmaw(r, fmaw(minus, r, all<W>(1.0f)), r);
+    const W g = wide<T, V>(at_least_minus_87(gate));
+    const W e = each(mulw(g, all<W>(-kLog2e)), exp2_approx);
+    a = each(addw(e, all<W>(1.0f)), rcp_approx);
     keep = mulw(e, a);
   } else {
-    a = g;
-    keep = each(g, [](float t) { return __fsub_rn(1.0f, t); });
+    a = wide<T, V>(gate);
+    keep = addw(all<W>(1.0f), each(a, [](float t) { return -t; }));
   }
 }
 
@@ -141,7 +148,8 @@ __device__ __forceinline__ Place place_of(const Args& p, uint64_t row) {
 }
 
 // A step's values as both walks use them: forwards a and b (h = a h + b), where a
-// stream begins with its state in b; backwards a, dh and what g is multiplied by.
+// stream begins in a tile of several with its state in b; backwards a, dh and what g
+// is multiplied by.
 template <typename T, int V, bool SIGMOID, bool MIX, bool BACK>
 struct Step {
   using W = Units<V>;
@@ -149,27 +157,20 @@ struct Step {
   W a, b;     // b: forwards
   P dh;       // backwards
   W slope;    // dgate = g slope
-  P gate;     // with a, 1 - a
+  W keep;     // dx = g keep
   __device__ __forceinline__ void forward(P gate, P x) {
-    W k;
-    gate_value<SIGMOID>(wide<T, V>(gate), a, k);
+    gate_value<SIGMOID>(gate, a, keep);
     b = wide<T, V>(x);
-    if (MIX) b = mulw(b, k);
+    if (MIX) b = mulw(b, keep);
   }
-  __device__ __forceinline__ void backward(P gate_, P d, W before, P x) {
-    gate = gate_;
-    W k;
-    gate_value<SIGMOID>(wide<T, V>(gate), a, k);
+  __device__ __forceinline__ void backward(P gate, P d, W before, P x) {
+    gate_value<SIGMOID>(gate, a, keep);
     dh = d;
     slope = before;
     if (MIX) slope = addw(slope, each(wide<T, V>(x), [](float t) { return -t; }));
-    if (SIGMOID) slope = mulw(slope, mulw(a, k));
+    if (SIGMOID) slope = mulw(slope, mulw(a, keep));
   }
-  __device__ __forceinline__ W dx(W g) const {
-    if (!MIX) return g;
-    if (SIGMOID) return mulw(g, mulw(exp_minus(wide<T, V>(gate)), a));
-    return mulw(g, each(a, [](float t) { return __fsub_rn(1.0f, t); }));
-  }
+  __device__ __forceinline__ W dx(W g) const { return MIX ? mulw(g, keep) : g; }
 };
 
 template <int V>
@@ -322,17 +323,24 @@ struct WalkRing {
   static constexpr int piece = V * sizeof(T);
   static constexpr bool used = piece >= 4;
   static constexpr int row = 32 * piece;
-  static constexpr int warp = ARRAYS * kRun * row;
-  static constexpr int stage = kWalkWarps * warp;
+  static constexpr int run = kRun * row;
+  static constexpr int array = kWalkWarps * run;
+  static constexpr int stage = ARRAYS * array;
   static constexpr int stages = stage <= 16 * 1024 ? 4 : stage <= 32 * 1024 ? 3 : 2;
   static constexpr int bytes = used ? stages * stage : 0;
 };
 
+struct Maps {
+  CUtensorMap of[4];  // gate; x or dh; h; x
+};
+
 // A part of a long stream (or of ragged ones behind each other), tile after tile.
-// LEAVE: the part's pair, else its results.
-template <typename T, int V, bool SIGMOID, bool MIX, bool BACK, bool LEAVE>
-__global__ void __launch_bounds__(kWalkWarps * 32, BACK && !LEAVE ? 2 : 4)
-k_recurrence_walk(const __grid_constant__ Args p) {
+// LEAVE: the part's pair, else its results. TENSOR: one thread has a tile's arrays
+// copied by tensor copies (rows whose start and stride are multiples of 16 bytes),
+// else every lane has its own values copied, in three times the instructions.
+template <typename T, int V, bool SIGMOID, bool MIX, bool BACK, bool LEAVE, bool TENSOR>
+__global__ void __launch_bounds__(kWalkWarps * 32, BACK && !LEAVE ? 2 : 3)
+k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps maps) {
   using W = Units<V>;
   using P = Pack<T, V>;
   constexpr int ARRAYS = LEAVE || !BACK ? 2 : MIX ? 4 : 3;
@@ -341,7 +349,9 @@ k_recurrence_walk(const __grid_constant__ Args p) {
   struct alignas(8 * V) Pair {
     W a, h;
   };
-  extern __shared__ uint4 walk_bytes[];
+  extern __shared__ __align__(128) uint8_t walk_bytes[];
+  __shared__ uint64_t full[S];
+  __shared__ uint32_t gave_up;
   __shared__ Pair runs[2][kWalkWarps][32];
   __shared__ uint32_t run_shut[2][kWalkWarps];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -375,17 +385,29 @@ k_recurrence_walk(const __grid_constant__ Args p) {
   const T* from[4] = {(const T*)p.gate, (const T*)(BACK ? p.dh : p.x), (const T*)p.h,
                       (const T*)p.x};
   const int64_t ld[4] = {p.ldg, BACK ? p.lddh : p.ldx, p.ldh, p.ldx};
-  char* ring = reinterpret_cast<char*>(walk_bytes) + warp * R::warp + lane * R::piece;
+  // of this warp's run in a tile in the ring, this lane's values
+  const char* ring = reinterpret_cast<const char*>(walk_bytes) + lane * R::piece +
+                     (BACK ? kWalkWarps - 1 - warp : warp) * R::run;
   const T* next[ARRAYS];  // where the run fetched next begins
 #pragma unroll
   for (int k = 0; k < ARRAYS; ++k) next[k] = from[k] + (at - (k == 2 ? 1 : 0)) * ld[k] + unit;
   int64_t next_at = at;
   int fetched = 0;
   auto fetch = [&](uint32_t stage) {
-    if constexpr (R::used) {
+    if constexpr (TENSOR) {  // by one thread
+      if (fetched < tiles) {
+        const int y = (int)(row0 + (BACK ? tiles - 1 - fetched : fetched) * (int64_t)kWalkSteps);
+        mbar_arrive_expect_tx(&full[stage], R::stage);
+#pragma unroll
+        for (int k = 0; k < ARRAYS; ++k)
+          tensor_load(walk_bytes + stage * R::stage + k * R::array, &maps.of[k],
+                      (int)(across * 32 * V), y - (k == 2 ? 1 : 0), &full[stage]);
+      }
+      ++fetched;
+    } else if constexpr (R::used) {
       if (in && fetched < tiles) {
         const int left = (int)min((int64_t)kRun, row1 - next_at);
-        char* to = ring + stage * R::stage;
+        char* to = const_cast<char*>(ring) + stage * R::stage;
 #pragma unroll
         for (int k = 0; k < ARRAYS; ++k) {
           const T* q = next[k];
@@ -393,7 +415,7 @@ k_recurrence_walk(const __grid_constant__ Args p) {
           for (int i = 0; i < kRun; ++i) {
             // h before the first row of all is no row's
             if (i < left && !(k == 2 && i == 0 && next_at == 0))
-              copy_async<R::piece>(to + (k * kRun + i) * R::row, q);
+              copy_async<R::piece>(to + k * R::array + i * R::row, q);
             q += ld[k];
           }
           next[k] += dir * (int)kWalkSteps * ld[k];
@@ -404,8 +426,18 @@ k_recurrence_walk(const __grid_constant__ Args p) {
       copy_commit();
     }
   };
+  if constexpr (TENSOR) {
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < S; ++s) mbar_init(&full[s], 1);
+      mbar_init_fence();
+      gave_up = 0;
+      for (int s = 0; s < S; ++s) fetch(s);
+    }
+    __syncthreads();
+  } else {
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s) fetch(s);
+    for (int s = 0; s < S - 1; ++s) fetch(s);
+  }
 
   W A = all<W>(1.0f), given = zero;  // forwards h; backwards what a step hands to the one before
   bool shut = false;
@@ -432,20 +464,26 @@ k_recurrence_walk(const __grid_constant__ Args p) {
 #pragma unroll
   for (int e = 0; e < V; ++e) nothing.v[e] = from_f32<T>(0.0f);
   int64_t clear0 = 0, clear1 = 0;  // rows in which no stream begins or ends, and all are some stream's
-  uint32_t stage = 0, half = 0;
+  uint32_t stage = 0, half = 0, parity = 0;
   for (int tile = 0; tile < tiles; ++tile, at += dir * (int)kWalkSteps, half ^= 1) {
     const int len = (int)max((int64_t)0, min((int64_t)kRun, row1 - at));
     P q[4][kRun];
     if constexpr (R::used) {
-      copy_wait<S - 2>();
+      if constexpr (!TENSOR) {
+        copy_wait<S - 2>();
+      } else if (!mbar_try_wait(&full[stage], parity) &&
+                 (*(volatile uint32_t*)&gave_up ||
+                  !mbar_wait_bounded(&full[stage], parity, p.timeout_ns))) {
+        *(volatile uint32_t*)&gave_up = 1;
+        record_status(p.status, kStatusTimeout);
+      }
       const char* to = ring + stage * R::stage;
 #pragma unroll
       for (int k = 0; k < ARRAYS; ++k)
 #pragma unroll
         for (int i = 0; i < kRun; ++i)
-          q[k][i] = *reinterpret_cast<const P*>(to + (k * kRun + i) * R::row);
-      fetch(stage == 0 ? S - 1 : stage - 1);
-      stage = stage == S - 1 ? 0 : stage + 1;
+          q[k][i] = *reinterpret_cast<const P*>(to + k * R::array + i * R::row);
+      if constexpr (!TENSOR) fetch(stage == 0 ? S - 1 : stage - 1);
     } else {
 #pragma unroll
       for (int k = 0; k < ARRAYS; ++k)
@@ -479,7 +517,7 @@ k_recurrence_walk(const __grid_constant__ Args p) {
     for (int i = 0; i < kRun; ++i) {
       if constexpr (BACK && LEAVE) {
         W k;
-        gate_value<SIGMOID>(wide<T, V>(q[0][i]), st[i].a, k);
+        gate_value<SIGMOID>(q[0][i], st[i].a, k);
         st[i].dh = q[1][i];
       } else if constexpr (BACK) {
         W before = wide<T, V>(q[2][i]);
@@ -512,16 +550,29 @@ k_recurrence_walk(const __grid_constant__ Args p) {
     }
     runs[half][warp][lane] = {a, h};
     if (lane == 0) run_shut[half][warp] = stop;
-    __syncthreads();  // the half is written again after the next tile's barrier
+    // the half is written again after the next tile's barrier; a stage has been read
+    const bool any = __syncthreads_or(stop != 0);
+    if constexpr (TENSOR) {
+      if (threadIdx.x == 0) fetch(stage);
+    }
+    parity ^= stage == S - 1;
+    stage = stage == S - 1 ? 0 : stage + 1;
     W carry = given;
+    if (!any) {
 #pragma unroll
-    for (uint32_t w = 0; w < kWalkWarps; ++w) {
-      const Pair v = runs[half][w][lane];
-      const bool s = run_shut[half][w] != 0;
-      if (w == warp) carry = given;
-      given = s ? v.h : fmaw(v.a, given, v.h);
-      if constexpr (LEAVE) {
-        A = s ? zero : mulw(A, v.a);
+      for (uint32_t w = 0; w < kWalkWarps; ++w) {
+        const Pair v = runs[half][w][lane];
+        if (w == warp) carry = given;
+        given = fmaw(v.a, given, v.h);
+        if (LEAVE) A = mulw(A, v.a);
+      }
+    } else {
+      for (uint32_t w = 0; w < kWalkWarps; ++w) {
+        const Pair v = runs[half][w][lane];
+        const bool s = run_shut[half][w] != 0;
+        if (w == warp) carry = given;
+        given = s ? v.h : fmaw(v.a, given, v.h);
+        if (LEAVE) A = s ? zero : mulw(A, v.a);
         shut |= s;
       }
     }
@@ -568,6 +619,11 @@ k_recurrence_walk(const __grid_constant__ Args p) {
         }
       }
     }
+  }
+  if constexpr (TENSOR) {
+    if (threadIdx.x == 0 && *(volatile uint32_t*)&gave_up)  // what is still on its way
+      for (int j = max(0, min(fetched, tiles) - S); j < min(fetched, tiles); ++j)
+        mbar_wait_bounded(&full[j % S], (j / S) & 1, p.timeout_ns);
   }
   if constexpr (LEAVE) {
     if (warp == 0) {
@@ -670,6 +726,7 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
   if (a.rows == 1) a.ldx = a.ldg = a.ldh = a.lddh = a.ldo = a.ldo2 = a.n;
   a.steps = a.offsets ? 0 : (uint32_t)(a.rows / a.streams);
   a.status = ctx->d_status;
+  a.timeout_ns = ctx->timeout_ns;
   bool copied = false;
   const int rc = with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
@@ -711,18 +768,40 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
       if (c.parts > 1) {
         a.shut = (uint32_t*)at;
         a.pairs = (float2*)(at + c.shut_bytes);
-        using R = WalkRing<T, V, 2>;
-        constexpr auto leave = k_recurrence_walk<T, V, SIGMOID, MIX, BACK, true>;
-        if (R::bytes > 48 * 1024 - 8192) PLX_TRY_CUDA(allow_shared<leave>(ctx->device, R::bytes));
-        leave<<<(unsigned)blocks, kWalkWarps * 32, R::bytes, ctx->stream>>>(a);
-        PLX_LAUNCH_CHECK("k_recurrence_walk");
       }
-      using R = WalkRing<T, V, BACK ? (MIX ? 4 : 3) : 2>;
-      constexpr auto kernel = k_recurrence_walk<T, V, SIGMOID, MIX, BACK, false>;
-      if (R::bytes > 48 * 1024 - 8192) PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, R::bytes));
-      kernel<<<(unsigned)blocks, kWalkWarps * 32, R::bytes, ctx->stream>>>(a);
-      PLX_LAUNCH_CHECK("k_recurrence_walk");
-      return PLX_OK;
+      auto walk = [&](auto tensor_c) -> int {
+        constexpr bool TENSOR = decltype(tensor_c)::value;
+        constexpr int ARRAYS = BACK ? (MIX ? 4 : 3) : 2;
+        Maps maps;
+        if constexpr (TENSOR) {
+          const void* of[4] = {a.gate, BACK ? a.dh : a.x, a.h, a.x};
+          const int64_t ld[4] = {a.ldg, BACK ? a.lddh : a.ldx, a.ldh, a.ldx};
+          for (int k = 0; k < ARRAYS; ++k)
+            if (int rc = tensor_map(&maps.of[k], dtype, of[k], a.n, a.rows, ld[k], 32 * V,
+                                    kWalkSteps, false))
+              return rc;
+        }
+        if (c.parts > 1) {
+          constexpr auto leave = k_recurrence_walk<T, V, SIGMOID, MIX, BACK, true, TENSOR>;
+          using R = WalkRing<T, V, 2>;
+          PLX_TRY_CUDA(allow_shared<leave>(ctx->device, R::bytes));
+          leave<<<(unsigned)blocks, kWalkWarps * 32, R::bytes, ctx->stream>>>(a, maps);
+          PLX_LAUNCH_CHECK("k_recurrence_walk");
+        }
+        constexpr auto kernel = k_recurrence_walk<T, V, SIGMOID, MIX, BACK, false, TENSOR>;
+        using R = WalkRing<T, V, ARRAYS>;
+        PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, R::bytes));
+        kernel<<<(unsigned)blocks, kWalkWarps * 32, R::bytes, ctx->stream>>>(a, maps);
+        PLX_LAUNCH_CHECK("k_recurrence_walk");
+        return PLX_OK;
+      };
+      if constexpr (V == 2) {
+        bool tensor = true;
+        for (int64_t ld : {a.ldx, a.ldg, a.ldh, a.lddh}) tensor &= ld * sizeof(T) % 16 == 0;
+        for (const void* q : {a.x, a.gate, a.h, a.dh}) tensor &= aligned16(q);
+        if (tensor) return walk(std::true_type{});
+      }
+      return walk(std::false_type{});
     };
     using std::integral_constant;
     auto kinds = [&](auto v) {

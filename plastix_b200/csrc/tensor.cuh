@@ -1,5 +1,5 @@
 // The tensor cores' instructions (tcgen05), their memory (TMEM) and tensor copies
-// (TMA), as far as product_tensor.cu uses them.
+// (TMA), as far as product_tensor.cu and recurrence.cu use them.
 #pragma once
 
 #include <cuda.h>
@@ -9,6 +9,12 @@
 namespace plx {
 
 // ---- tensor copies -----------------------------------------------------------
+// A map of `outer` rows of `inner` values, `ld` apart (start and stride multiples of
+// 16 bytes), for copies of boxes; what is outside reads as 0. swizzle: 16-byte chunks
+// of rows of 128 bytes as the products take them.
+int tensor_map(CUtensorMap* map, int dtype, const void* p, uint64_t inner, uint64_t outer,
+               int64_t ld, uint32_t box_inner, uint32_t box_outer, bool swizzle);
+
 // A box of a two-dimensional array to shared memory; x (values into a row) times
 // their size is a multiple of 16 bytes.
 __device__ __forceinline__ void tensor_load(void* dst_smem, const CUtensorMap* map, int x, int y,
