@@ -376,11 +376,15 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
   const int64_t row0 = min(g0 + (int64_t)part * p.part_rows, g1);
   const int64_t row1 = min(row0 + p.part_rows, g1);
   const int tiles = (int)((row1 - row0 + kWalkSteps - 1) / kWalkSteps);
-  // This warp's run of the first tile that is walked; tiles and the steps of a run
-  // follow in the direction `dir`.
+  // Steps are walked in the direction `dir`, and so are tiles for results. For a
+  // part's pair they are taken the other way round: what is read last is what the
+  // next kernel reads first, out of L2.
   constexpr int dir = BACK ? -1 : 1;
-  int64_t at = row0 + (BACK ? (int64_t)(tiles - 1) * kWalkSteps + (kWalkWarps - 1 - warp) * kRun
-                            : warp * kRun);
+  constexpr bool FROM_END = BACK != LEAVE;
+  constexpr int tile_dir = FROM_END ? -1 : 1;
+  // This warp's run of the first tile.
+  int64_t at = row0 + (FROM_END ? (int64_t)(tiles - 1) * kWalkSteps : 0) +
+               (BACK ? kWalkWarps - 1 - warp : warp) * kRun;
 
   const T* from[4] = {(const T*)p.gate, (const T*)(BACK ? p.dh : p.x), (const T*)p.h,
                       (const T*)p.x};
@@ -396,7 +400,7 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
   auto fetch = [&](uint32_t stage) {
     if constexpr (TENSOR) {  // by one thread
       if (fetched < tiles) {
-        const int y = (int)(row0 + (BACK ? tiles - 1 - fetched : fetched) * (int64_t)kWalkSteps);
+        const int y = (int)(row0 + (FROM_END ? tiles - 1 - fetched : fetched) * (int64_t)kWalkSteps);
         mbar_arrive_expect_tx(&full[stage], R::stage);
 #pragma unroll
         for (int k = 0; k < ARRAYS; ++k)
@@ -408,20 +412,24 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
       if (in && fetched < tiles) {
         const int left = (int)min((int64_t)kRun, row1 - next_at);
         char* to = const_cast<char*>(ring) + stage * R::stage;
+        auto copy = [&](auto whole) {
 #pragma unroll
-        for (int k = 0; k < ARRAYS; ++k) {
-          const T* q = next[k];
+          for (int k = 0; k < ARRAYS; ++k) {
+            const T* q = next[k];
 #pragma unroll
-          for (int i = 0; i < kRun; ++i) {
-            // h before the first row of all is no row's
-            if (i < left && !(k == 2 && i == 0 && next_at == 0))
-              copy_async<R::piece>(to + k * R::array + i * R::row, q);
-            q += ld[k];
+            for (int i = 0; i < kRun; ++i) {
+              // h before the first row of all is no row's
+              if (decltype(whole)::value || (i < left && !(k == 2 && i == 0 && next_at == 0)))
+                copy_async<R::piece>(to + k * R::array + i * R::row, q);
+              q += ld[k];
+            }
+            next[k] += tile_dir * (int)kWalkSteps * ld[k];
           }
-          next[k] += dir * (int)kWalkSteps * ld[k];
-        }
+        };
+        if (left == kRun && next_at > 0) copy(std::true_type{});
+        else copy(std::false_type{});
       }
-      next_at += dir * (int)kWalkSteps;
+      next_at += tile_dir * (int)kWalkSteps;
       ++fetched;
       copy_commit();
     }
@@ -465,7 +473,7 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
   for (int e = 0; e < V; ++e) nothing.v[e] = from_f32<T>(0.0f);
   int64_t clear0 = 0, clear1 = 0;  // rows in which no stream begins or ends, and all are some stream's
   uint32_t stage = 0, half = 0, parity = 0;
-  for (int tile = 0; tile < tiles; ++tile, at += dir * (int)kWalkSteps, half ^= 1) {
+  for (int tile = 0; tile < tiles; ++tile, at += tile_dir * (int)kWalkSteps, half ^= 1) {
     const int len = (int)max((int64_t)0, min((int64_t)kRun, row1 - at));
     P q[4][kRun];
     if constexpr (R::used) {
@@ -501,9 +509,9 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
       valid = __ballot_sync(~0u, mine.valid);
       first = __ballot_sync(~0u, mine.first);
       last = __ballot_sync(~0u, mine.last);
-      // the stream that the last of these rows is in goes on
-      clear0 = __shfl_sync(~0u, mine.begin, BACK ? 0 : len - 1) + 1;
-      clear1 = __shfl_sync(~0u, mine.end, BACK ? 0 : len - 1) - 1;
+      // the stream that the row nearest to the next tile is in goes on
+      clear0 = __shfl_sync(~0u, mine.begin, FROM_END ? 0 : len - 1) + 1;
+      clear1 = __shfl_sync(~0u, mine.end, FROM_END ? 0 : len - 1) - 1;
     }
     const uint32_t stop = BACK ? last : first;  // rows at which what was before does not count
     auto state_at = [&](const float* states, int i) {
@@ -557,23 +565,35 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
     }
     parity ^= stage == S - 1;
     stage = stage == S - 1 ? 0 : stage + 1;
+    if constexpr (LEAVE) {
+      if (warp == 0 && !shut) {  // before a stream's start nothing counts
+        W ta = all<W>(1.0f), th = zero;
+        bool cut = false;
+        for (uint32_t w = 0; w < kWalkWarps; ++w) {
+          const Pair v = runs[half][w][lane];
+          const bool s = any && run_shut[half][w] != 0;
+          th = s ? v.h : fmaw(v.a, th, v.h);
+          ta = s ? zero : mulw(ta, v.a);
+          cut |= s;
+        }
+        given = fmaw(A, th, given);
+        A = mulw(A, ta);
+        shut = cut;
+      }
+    }
     W carry = given;
-    if (!any) {
+    if (!LEAVE && !any) {
 #pragma unroll
       for (uint32_t w = 0; w < kWalkWarps; ++w) {
         const Pair v = runs[half][w][lane];
         if (w == warp) carry = given;
         given = fmaw(v.a, given, v.h);
-        if (LEAVE) A = mulw(A, v.a);
       }
-    } else {
+    } else if (!LEAVE) {
       for (uint32_t w = 0; w < kWalkWarps; ++w) {
         const Pair v = runs[half][w][lane];
-        const bool s = run_shut[half][w] != 0;
         if (w == warp) carry = given;
-        given = s ? v.h : fmaw(v.a, given, v.h);
-        if (LEAVE) A = s ? zero : mulw(A, v.a);
-        shut |= s;
+        given = run_shut[half][w] ? v.h : fmaw(v.a, given, v.h);
       }
     }
     if constexpr (!LEAVE) {
