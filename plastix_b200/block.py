@@ -24,7 +24,8 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _abi
-from .readout import _address, _check_count, _check_result, _like, _param, _rows, _scope
+from .readout import (_TYPES, _address, _check_count, _check_result, _like, _param, _rows,
+                      _scope)
 from .runtime import Context
 
 _ACTS = {"identity": _abi.ACT_IDENTITY, "sigmoid": _abi.ACT_SIGMOID, "tanh": _abi.ACT_TANH,
@@ -51,12 +52,33 @@ def _one_of(table: dict, key: str, name: str) -> int:
     return value
 
 
+def _plain_rows(ctx: Context, t: torch.Tensor, name: str):
+    """(rows, n, row stride, type number), as ``_rows``; quickly for contiguous tensors."""
+    kind, shape = _TYPES.get(t.dtype), t.shape
+    if kind is not None and shape and 0 < shape[-1] < 1 << 31 and t.is_contiguous() \
+            and t.device == ctx.device:
+        n = shape[-1]
+        return t.numel() // n, n, n, kind
+    return _rows(ctx, t, name)
+
+
 def _same_rows(ctx: Context, t: torch.Tensor, like: torch.Tensor, name: str, of: str) -> int:
     """The row stride of a tensor that has to have another one's shape and type."""
+    if t.shape == like.shape and t.dtype is like.dtype and t.is_contiguous() \
+            and t.device == ctx.device:
+        return t.shape[-1]
     if t.shape != like.shape or t.dtype != like.dtype:
         raise ValueError(f"{name} has to be {like.dtype} {tuple(like.shape)} like {of}, got "
                          f"{t.dtype} {tuple(t.shape)}")
     return _rows(ctx, t, name)[2]
+
+
+def _vector(ctx: Context, t: torch.Tensor, n: int, dtype, name: str) -> int:
+    """The type number of a parameter of every unit, as ``_param``."""
+    if t.dtype is dtype and t.dim() == 1 and t.shape[0] == n and t.is_contiguous() \
+            and t.device == ctx.device:
+        return _TYPES[dtype]
+    return _param(ctx, t, n, dtype, name)
 
 
 def _span(t: torch.Tensor, ld: int):
@@ -78,17 +100,20 @@ def _check_apart(out: torch.Tensor, ldo: int, name: str, *others) -> None:
                 raise ValueError(f"{name} overlaps {other}")
 
 
-def _in_place_of(ctx: Context, out: Optional[torch.Tensor], n: int, *inputs):
-    """``out`` and its row stride (None and that of a new one): it may be one of
-    the inputs (tensor, row stride, name) and touches no other. Inputs that are
-    the same tensor count as one."""
-    if out is None:
-        return None, n
+def _new(like: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of another one's shape and type."""
+    return torch.empty_like(like) if like.is_contiguous() else like.new_empty(like.shape)
+
+
+def _in_place_of(ctx: Context, out: torch.Tensor, *inputs) -> int:
+    """The row stride of ``out``, which may be one of the inputs (tensor, row
+    stride, name) and touches no other. Inputs that are the same tensor count as
+    one."""
     ldo = _same_rows(ctx, out, inputs[0][0], "out", inputs[0][2])
     same = [t for t, ld, _ in inputs if t.data_ptr() == out.data_ptr() and ld == ldo]
     _check_apart(out, ldo, "out", *((t, ld, name) for t, ld, name in inputs
                                     if not any(t.data_ptr() == s.data_ptr() for s in same)))
-    return out, ldo
+    return ldo
 
 
 # ------------------------------------------------------------------------------- dense layer
@@ -97,10 +122,9 @@ def _weight(ctx: Context, weight: torch.Tensor, n: int, dtype):
     if weight.dim() != 2 or weight.shape[1] != n or weight.dtype != dtype:
         raise ValueError(f"weight has to be {dtype} [units, {n}], got {weight.dtype} "
                          f"{tuple(weight.shape)}")
-    m, _, ld, _ = _rows(ctx, weight, "weight")
-    if m == 0:
-        raise ValueError("weight has no units")
-    _check_count(m, "the first dimension of weight")
+    m, _, ld, _ = _plain_rows(ctx, weight, "weight")
+    if not 0 < m < 1 << 31:
+        raise ValueError(f"weight has {m} units: 1 to fewer than 2^31 are supported")
     return m, ld
 
 
@@ -123,10 +147,10 @@ def dense(ctx: Context, x: torch.Tensor, weight: torch.Tensor,
     sigmoid(z)) or "gelu" (z Phi(z)). With ``pre`` returns (y, z): z = x
     weight^T + bias in float32, which ``dense_backward`` takes. ``out`` may be
     residual."""
-    rows, n, ldx, dtype = _rows(ctx, x, "x")
+    rows, n, ldx, dtype = _plain_rows(ctx, x, "x")
     m, ldw = _weight(ctx, weight, n, x.dtype)
     act = _one_of(_ACTS, apply, "apply")
-    kind = _abi.F32 if bias is None else _param(ctx, bias, m, x.dtype, "bias")
+    kind = _abi.F32 if bias is None else _vector(ctx, bias, m, x.dtype, "bias")
     shape = x.shape[:-1] + (m,)
     ldr = 0
     if residual is not None:
@@ -143,12 +167,13 @@ def dense(ctx: Context, x: torch.Tensor, weight: torch.Tensor,
         if residual is not None:
             _check_result(out, ldy, residual, ldr, "out")
         _check_apart(out, ldy, "out", (x, ldx, "x"), (weight, ldw, "weight"))
+    # aligned rows need no scratch
+    size = 0 if _aligned((x, ldx, rows), (weight, ldw, m)) else \
+        _abi.lib().plx_dense_scratch_bytes(rows, n, m, dtype, 0, 0)
     with _scope(ctx, x, weight, bias, residual, out):
         if out is None:
             y = x.new_empty(shape)
         z = x.new_empty(shape, dtype=torch.float32) if pre else None
-        size = _abi.lib().plx_dense_scratch_bytes(
-            rows, n, m, dtype, 0, _aligned((x, ldx, rows), (weight, ldw, m)))
         scratch = x.new_empty(size, dtype=torch.uint8) if size else None
         _abi.call("plx_dense", ctx.handle, rows, n, m, dtype, x.data_ptr(), ldx,
                   weight.data_ptr(), ldw, kind, _address(bias), act, _address(residual), ldr,
@@ -164,7 +189,7 @@ def dense_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, weight: torc
     ``pre`` is z as ``dense`` returned it (not needed for "identity"). dx is
     None without ``input_grad``, dweight without ``weight_grad``; dbias, in
     bias's type, comes with ``bias``."""
-    rows, n, ldx, dtype = _rows(ctx, x, "x")
+    rows, n, ldx, dtype = _plain_rows(ctx, x, "x")
     m, ldw = _weight(ctx, weight, n, x.dtype)
     act = _one_of(_ACTS, apply, "apply")
     shape = x.shape[:-1] + (m,)
@@ -176,7 +201,7 @@ def dense_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, weight: torc
         _like(ctx, pre, shape, torch.float32, "pre")
     elif act != _abi.ACT_IDENTITY:
         raise ValueError(f"pre is required for {apply!r}")
-    kind = _abi.F32 if bias is None else _param(ctx, bias, m, x.dtype, "bias")
+    kind = _abi.F32 if bias is None else _vector(ctx, bias, m, x.dtype, "bias")
     with _scope(ctx, dy, x, weight, pre, bias):
         dx = x.new_empty(x.shape) if input_grad else None
         dw = weight.new_empty(weight.shape) if weight_grad else None
@@ -195,28 +220,28 @@ def _block_params(ctx: Context, x, gate, gate_apply, kind, post, scale, eps, pos
                   post_bias, pre_weight, pre_bias):
     """The call's parameters, and what they were made of."""
     n, dtype = x.shape[-1], x.dtype
-    p = _abi.BlockNormParams(kind=_one_of(_NORMS, kind, "kind"), post=int(bool(post)),
-                             gate_sigmoid=_one_of(_GATE_APPLY, gate_apply, "gate_apply"),
-                             scale=scale, eps=eps)
     if not post and (post_weight is not None or post_bias is not None):
         raise ValueError("post_weight and post_bias need post=True")
-    vectors = {"post_weight": post_weight, "post_bias": post_bias, "pre_weight": pre_weight,
-               "pre_bias": pre_bias}
+    how, address, ldg, units = _abi.BLOCK_GATE_NONE, None, 0, None
     if gate is not None:
+        address = gate.data_ptr()
         if gate.dim() == 1 and x.dim() != 1:
-            p.gate = _abi.BLOCK_GATE_UNITS
-            vectors["gate"] = gate
+            how, units = _abi.BLOCK_GATE_UNITS, gate
         else:
-            p.gate = _abi.BLOCK_GATE_VALUES
-            p.ldg = _same_rows(ctx, gate, x, "gate", "x")
-        p.gate_values = gate.data_ptr()
-    kinds = {name: _param(ctx, v, n, dtype, name) for name, v in vectors.items() if v is not None}
-    if len(set(kinds.values())) > 1:
-        raise ValueError(f"{', '.join(kinds)} have different types")
-    p.param_dtype = next(iter(kinds.values()), _abi.F32)
-    for name in ("post_weight", "post_bias", "pre_weight", "pre_bias"):
-        setattr(p, name, _address(vectors[name]))
-    return p
+            how, ldg = _abi.BLOCK_GATE_VALUES, _same_rows(ctx, gate, x, "gate", "x")
+    param = None
+    for name, v in (("gate", units), ("post_weight", post_weight), ("post_bias", post_bias),
+                    ("pre_weight", pre_weight), ("pre_bias", pre_bias)):
+        if v is not None:
+            of = _vector(ctx, v, n, dtype, name)
+            if param is not None and of != param:
+                raise ValueError("the parameters have different types")
+            param = of
+    return _abi.BlockNormParams(
+        _one_of(_NORMS, kind, "kind"), 1 if post else 0, how,
+        _one_of(_GATE_APPLY, gate_apply, "gate_apply"), _abi.F32 if param is None else param, scale,
+        eps, address, ldg, _address(post_weight), _address(post_bias), _address(pre_weight),
+        _address(pre_bias))
 
 
 def block_norm(ctx: Context, x: torch.Tensor, o: torch.Tensor,
@@ -236,18 +261,20 @@ def block_norm(ctx: Context, x: torch.Tensor, o: torch.Tensor,
     so is a gate for an x of one dimension), or None for 1; ``gate_apply``
     "sigmoid" takes its sigmoid. With ``stats`` returns (r, u, stats), which
     ``block_norm_backward`` takes. ``out`` (for r) may be x or o."""
-    rows, n, ldx, dtype = _rows(ctx, x, "x")
+    rows, n, ldx, dtype = _plain_rows(ctx, x, "x")
     ldo = _same_rows(ctx, o, x, "o", "x")
     p = _block_params(ctx, x, gate, gate_apply, kind, post, scale, eps, post_weight, post_bias,
                       pre_weight, pre_bias)
-    inputs = [(x, ldx, "x"), (o, ldo, "o")]
-    if p.gate == _abi.BLOCK_GATE_VALUES:
-        inputs.append((gate, p.ldg, "gate"))
-    r, ldr = _in_place_of(ctx, out, n, *inputs)
+    r, ldr = out, n
+    if out is not None:
+        inputs = [(x, ldx, "x"), (o, ldo, "o")]
+        if p.gate == _abi.BLOCK_GATE_VALUES:
+            inputs.append((gate, p.ldg, "gate"))
+        ldr = _in_place_of(ctx, out, *inputs)
     with _scope(ctx, x, o, gate, post_weight, post_bias, pre_weight, pre_bias, out):
         if out is None:
-            r = x.new_empty(x.shape)
-        u = x.new_empty(x.shape)
+            r = _new(x)
+        u = _new(x)
         st = x.new_empty(x.shape[:-1] + (4,), dtype=torch.float32) if stats else None
         _abi.call("plx_block_norm", ctx.handle, rows, n, dtype, x.data_ptr(), ldx, o.data_ptr(),
                   ldo, byref(p), r.data_ptr(), ldr, u.data_ptr(), n, _address(st))
@@ -266,7 +293,7 @@ def block_norm_backward(ctx: Context, dr: Optional[torch.Tensor], du: Optional[t
     of ``block_norm``; dr or du may be None. Gradients of the parameters and of
     a gate of every unit are summed over the rows, the same bits on every
     call."""
-    rows, n, ldx, dtype = _rows(ctx, x, "x")
+    rows, n, ldx, dtype = _plain_rows(ctx, x, "x")
     ldo = _same_rows(ctx, o, x, "o", "x")
     if dr is None and du is None:
         raise ValueError("dr or du is required")
@@ -276,7 +303,7 @@ def block_norm_backward(ctx: Context, dr: Optional[torch.Tensor], du: Optional[t
     p = _block_params(ctx, x, gate, gate_apply, kind, post, scale, 0.0, post_weight, post_bias,
                       pre_weight, pre_bias)
     with _scope(ctx, dr, du, x, o, stats, gate, post_weight, post_bias, pre_weight, pre_bias):
-        dx, do = x.new_empty(x.shape), x.new_empty(x.shape)
+        dx, do = _new(x), _new(x)
         dgate = None if gate is None else gate.new_empty(gate.shape)
         dw1, db1, dw2, db2 = (None if v is None else torch.empty_like(v)
                               for v in (post_weight, post_bias, pre_weight, pre_bias))
@@ -330,12 +357,14 @@ def recurrence(ctx: Context, x: torch.Tensor, gate: torch.Tensor,
     n] in float32 is h before the first steps (None: 0), ``final`` h after the
     last ones, what ``state`` was for streams without steps. ``out`` may be x
     or gate, ``final_out`` state: a step in place."""
-    rows, n, ldx, dtype = _rows(ctx, x, "x")
+    rows, n, ldx, dtype = _plain_rows(ctx, x, "x")
     ldg = _same_rows(ctx, gate, x, "gate", "x")
     gate_kind = _one_of(_GATES, kind, "kind")
     streams, offsets_p = _streams(ctx, x, offsets)
     state_p = _state(ctx, state, x, streams, "state")
-    h, ldh = _in_place_of(ctx, out, n, (x, ldx, "x"), (gate, ldg, "gate"))
+    h, ldh = out, n
+    if out is not None:
+        ldh = _in_place_of(ctx, out, (x, ldx, "x"), (gate, ldg, "gate"))
     final = final_out
     if final is not None:
         _state(ctx, final, x, streams, "final_out")
@@ -343,7 +372,7 @@ def recurrence(ctx: Context, x: torch.Tensor, gate: torch.Tensor,
             _check_apart(final, n, "final_out", (state, n, "state"))
     with _scope(ctx, x, gate, state, offsets, out, final_out):
         if out is None:
-            h = x.new_empty(x.shape)
+            h = _new(x)
         if final is None:
             final = x.new_empty((streams, n), dtype=torch.float32)
         size = _abi.lib().plx_recurrence_scratch_bytes(streams, rows, n, offsets is not None,
@@ -364,7 +393,7 @@ def recurrence_backward(ctx: Context, dh: torch.Tensor, gate: torch.Tensor, h: t
     the arguments of ``recurrence`` and the h that it returned. ``x`` is needed
     with ``mix`` alone; ``dfinal`` may be None. dstate is None without a state.
     Rows of no stream are left as they are in dx and dgate."""
-    rows, n, ldg, dtype = _rows(ctx, gate, "gate")
+    rows, n, ldg, dtype = _plain_rows(ctx, gate, "gate")
     lddh = _same_rows(ctx, dh, gate, "dh", "gate")
     ldh = _same_rows(ctx, h, gate, "h", "gate")
     if mix and x is None:
@@ -375,7 +404,7 @@ def recurrence_backward(ctx: Context, dh: torch.Tensor, gate: torch.Tensor, h: t
     state_p = _state(ctx, state, gate, streams, "state")
     dfinal_p = _state(ctx, dfinal, gate, streams, "dfinal")
     with _scope(ctx, dh, gate, h, x, state, dfinal, offsets):
-        dx, dgate = gate.new_empty(gate.shape), gate.new_empty(gate.shape)
+        dx, dgate = _new(gate), _new(gate)
         dstate = None if state is None else torch.empty_like(state)
         size = _abi.lib().plx_recurrence_scratch_bytes(streams, rows, n, offsets is not None,
                                                        1)

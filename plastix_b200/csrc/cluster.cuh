@@ -24,10 +24,17 @@ __device__ __forceinline__ uint32_t peer_smem(const void* p, uint32_t rank) {
 __device__ __forceinline__ void st_peer(uint32_t at, float2 v) {
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.x), "f"(v.y) : "memory");
 }
-__device__ __forceinline__ float ld_peer(uint32_t at) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
+__device__ __forceinline__ void st_peer(uint32_t at, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+__device__ __forceinline__ void st_peer(uint32_t at, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y),
+               "f"(v.z), "f"(v.w)
+               : "memory");
+}
+// Arrives at a barrier of another block of the cluster.
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t at) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory");
 }
 
 }  // namespace plx

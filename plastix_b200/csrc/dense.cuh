@@ -25,8 +25,43 @@ __device__ __forceinline__ float act_value(float z) {
   else if constexpr (ACT == PLX_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
   else if constexpr (ACT == PLX_ACT_SILU) return z * squash(z).a;
   else if constexpr (ACT == PLX_ACT_GELU)
-    return z * (0.5f + 0.5f * erff(z * 0.70710678118654752f));
+    return z * (0.5f * erfcf(z * -0.70710678118654752f));
   else return z;
+}
+// The same for results of 16 bits, in fewer instructions: relative errors of a few
+// 2^-22, of GELU's Phi below 4e-6 for |z| < 10 and 1e-4 beyond (where it is below
+// 1e-23).
+template <int ACT>
+__device__ __forceinline__ float act_value16(float z) {
+  auto quotient = [](float d) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    return r;
+  };
+  if constexpr (ACT == PLX_ACT_SIGMOID) {
+    return quotient(1.0f + exp2_approx(z * -kLog2e));
+  } else if constexpr (ACT == PLX_ACT_SILU) {
+    return z * quotient(1.0f + exp2_approx(z * -kLog2e));
+  } else if constexpr (ACT == PLX_ACT_TANH) {
+    // (1 - e) / (1 + e), e = exp(-2 |z|); near 0, where that cancels, z - z^3 / 3
+    const float a = fabsf(z), e = exp2_approx(a * (-2.0f * kLog2e));
+    const float far = copysignf((1.0f - e) * quotient(1.0f + e), z);
+    return a < 0.02f ? fmaf(z * z * z, -1.0f / 3.0f, z) : far;
+  } else if constexpr (ACT == PLX_ACT_GELU) {
+    // Phi(-|z|) = exp(-z^2 / 2) times a polynomial in t = 1 / (1 + 0.3 |z|) without a
+    // constant, fitted for the least relative error over |z| <= 10
+    const float t = quotient(fmaf(fabsf(z), 0.3f, 1.0f));
+    float q = -0.08074618130922318f;
+    q = fmaf(q, t, 0.22719280421733856f);
+    q = fmaf(q, t, -0.029975734651088715f);
+    q = fmaf(q, t, 0.1514199823141098f);
+    q = fmaf(q, t, 0.11184987425804138f);
+    q = fmaf(q, t, 0.1202608123421669f);
+    q *= t * exp2_approx(z * z * (-0.5f * kLog2e));
+    return z * (z < 0.0f ? q : 1.0f - q);
+  } else {
+    return act_value<ACT>(z);
+  }
 }
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
@@ -43,7 +78,7 @@ __device__ __forceinline__ float act_slope(float z) {
     return s.a * fmaf(z, s.keep, 1.0f);
   } else if constexpr (ACT == PLX_ACT_GELU) {
     const float pdf = 0.39894228040143268f * exp2_approx(-0.5f * kLog2e * z * z);
-    return fmaf(z, pdf, 0.5f + 0.5f * erff(z * 0.70710678118654752f));
+    return fmaf(z, pdf, 0.5f * erfcf(z * -0.70710678118654752f));
   } else {
     return 1.0f;
   }

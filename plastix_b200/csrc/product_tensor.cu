@@ -5,9 +5,12 @@
 // stages of 64 values of k, one issues the products on them, eight warps finish
 // the tile before (bias, activation, residual, rounding) out of the other half of
 // TMEM meanwhile. Blocks stay and take every gridDim-th tile.
-// Where tiles are few, a cluster of blocks shares one tile's k: each leaves its
-// sums in shared memory, and all of them add and finish a part of the tile, in
-// the order of the blocks.
+// PAIR: two blocks make a tile of 256 x 256 together, each with half of both
+// operands, so that what a block reads is two thirds of what it reads for 128 x 256
+// (all blocks together read as fast as L2 gives).
+// SPLIT: where tiles are few, a cluster of blocks shares one tile's k: each sends
+// its sums to the blocks' shared memory, and each block adds and finishes the rows
+// of the tile that are its own, in the order of the blocks.
 // Few rows (at most 64) are the tile's second side, so that the first one's 128
 // are units of the layer.
 #include "cluster.cuh"
@@ -21,13 +24,18 @@ constexpr uint32_t kTileA = 128, kTileK = 64;
 constexpr int kFinishWarps = 8, kThreads = 64 + 32 * kFinishWarps;
 constexpr uint32_t kSmem = 232448;  // a block can have
 
-template <int BN>
+enum Mode { ONE, SPLIT, PAIR };
+
+template <int BN, Mode MODE>
 struct Stages {
-  static constexpr uint32_t a_bytes = kTileA * kTileK * 2, b_bytes = BN * kTileK * 2;
+  static constexpr uint32_t b_rows = MODE == PAIR ? BN / 2 : BN;  // a block's
+  static constexpr uint32_t a_bytes = kTileA * kTileK * 2, b_bytes = b_rows * kTileK * 2;
   static constexpr uint32_t bytes = a_bytes + b_bytes;
-  static constexpr uint32_t most = (kSmem - 2048) / bytes;
+  // sums that the blocks of a cluster are sent, of a tile in all
+  static constexpr uint32_t sums = MODE == SPLIT ? (BN + 4) * kTileA * 4 : 0;
+  static constexpr uint32_t most = (kSmem - 2048 - sums) / bytes;
   static constexpr uint32_t count = most < 12 ? most : 12;
-  static constexpr uint32_t smem = count * bytes + 1024;  // to a multiple of 1,024
+  static constexpr uint32_t smem = count * bytes + sums + 1024;  // to a multiple of 1,024
   static constexpr uint32_t columns = 2 * BN < 32 ? 32 : 2 * BN;
 };
 
@@ -56,7 +64,7 @@ template <int C>
 __device__ __forceinline__ void activate(int act, float (&v)[C]) {
   auto all = [&](auto a) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] = act_value<decltype(a)::value>(v[i]);
+    for (int i = 0; i < C; ++i) v[i] = act_value16<decltype(a)::value>(v[i]);
   };
   using std::integral_constant;
   switch (act) {
@@ -111,17 +119,18 @@ __device__ __forceinline__ void finish_row(const Finish& f, uint32_t row, uint32
   T* to = (T*)f.y + (int64_t)row * f.ldy + col;
   const T* res = (const T*)f.residual + (int64_t)row * f.ldr + col;
   if (wide) {
+    constexpr int N = C < 8 ? C : 8;
 #pragma unroll
-    for (int i = 0; i < C; i += 8) {
-      Pack<T, 8> q;
+    for (int i = 0; i < C; i += N) {
+      Pack<T, N> q;
       if (f.residual) {
-        q = load_pack<T, 8>(res + i);
+        q = load_pack<T, N>(res + i);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[i + e] += to_f32(q.v[e]);
+        for (int e = 0; e < N; ++e) v[i + e] += to_f32(q.v[e]);
       }
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) put_pair(q, e, pack2(v[i + e], v[i + e + 1]));
-      *reinterpret_cast<Pack<T, 8>*>(to + i) = q;
+      for (int e = 0; e < N; e += 2) put_pair(q, e, pack2(v[i + e], v[i + e + 1]));
+      *reinterpret_cast<Pack<T, N>*>(to + i) = q;
     }
   } else {
 #pragma unroll
@@ -133,13 +142,17 @@ __device__ __forceinline__ void finish_row(const Finish& f, uint32_t row, uint32
   }
 }
 
-template <typename T, int BN, bool SPLIT>
+template <typename T, int BN, Mode MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
-  using S = Stages<BN>;
-  constexpr uint32_t C = BN < 32 ? 16 : 32;  // columns at a time
-  extern __shared__ uint8_t smem_bytes[];
-  uint8_t* ring = smem_bytes + (1024 - (smem_addr(smem_bytes) & 1023)) % 1024;
+  using S = Stages<BN, MODE>;
+  constexpr bool TWO = MODE == PAIR;
+  constexpr uint32_t C = BN <= 32 ? 16 : 32;  // columns at a time, at most half of a tile's
+  static_assert(BN == 16 || BN % (2 * C) == 0, "halves of a tile");
+  constexpr uint32_t kHigh = TWO ? 2 * kTileA : kTileA;  // of a tile
+  extern __shared__ __align__(128) uint8_t product_bytes[];
+  uint8_t* ring = product_bytes + (1024 - (smem_addr(product_bytes) & 1023)) % 1024;
+  float* sent = reinterpret_cast<float*>(ring + S::count * S::bytes);
   __shared__ uint64_t full[S::count], empty[S::count], done[2], taken[2];
   __shared__ uint32_t tmem, gave_up;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -147,7 +160,7 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
   uint32_t k_first = 0, k_last = blocks, rank = 0, parts = 1;
   uint32_t tile0 = blockIdx.x, step = gridDim.x;
   const uint32_t tiles = p.tiles_a * p.tiles_b;
-  if constexpr (SPLIT) {
+  if constexpr (MODE == SPLIT) {
     rank = cluster_rank();
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(parts));
     tile0 = blockIdx.x / parts;
@@ -155,6 +168,10 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
     const uint32_t each = (blocks + parts - 1) / parts;
     k_first = min(rank * each, blocks);
     k_last = min(k_first + each, blocks);
+  } else if constexpr (TWO) {
+    rank = cluster_rank();
+    tile0 = blockIdx.x / 2;
+    step = gridDim.x / 2;
   }
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < S::count; ++s) {
@@ -163,14 +180,15 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
     }
     for (int h = 0; h < 2; ++h) {
       mbar_init(&done[h], 1);
-      mbar_init(&taken[h], kFinishWarps);
+      mbar_init(&taken[h], TWO ? 2 * kFinishWarps : kFinishWarps);
     }
     mbar_init_fence();
     gave_up = 0;
   }
-  if (warp == 1) tmem_alloc(&tmem, S::columns);
+  if (warp == 1) tmem_alloc<TWO>(&tmem, S::columns);
   tmem_fence_before();
   __syncthreads();
+  if constexpr (MODE != ONE) cluster_barrier();  // the others' barriers are there
   tmem_fence_after();
   const uint32_t sums = *(volatile uint32_t*)&tmem;
   // Tiles in groups of eight along a's side, so that what is under way at one
@@ -188,33 +206,40 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
     for (uint32_t tile = tile0; ok && tile < tiles; tile += step) {
       uint32_t ia, ib;
       place(tile, ia, ib);
+      const int a0 = (int)(ia * kHigh + (TWO ? rank * kTileA : 0));
+      const int b0 = (int)(ib * BN + (TWO ? rank * S::b_rows : 0));
       for (uint32_t k = k_first; k < k_last; ++k, ++it) {
         const uint32_t s = it % S::count;
         if (it >= S::count && !(ok = wait(&empty[s], (it / S::count - 1) & 1, &gave_up, p))) break;
         uint8_t* a = ring + s * S::bytes;
         uint8_t* b = a + S::a_bytes;
-        mbar_arrive_expect_tx(&full[s], S::bytes);
+        // a pair's first block counts the bytes of both
+        const uint32_t bar = TWO ? peer_smem(&full[s], 0) : 0;
+        if (!TWO || rank == 0) mbar_arrive_expect_tx(&full[s], TWO ? 2 * S::bytes : S::bytes);
+        auto load = [&](uint8_t* to, const CUtensorMap* map, int x, int y) {
+          if constexpr (TWO) tensor_load_pair(to, map, x, y, bar);
+          else tensor_load(to, map, x, y, &full[s]);
+        };
+        const int k0 = (int)(k * kTileK);
         if (p.a_k_major) {
-          tensor_load(a, &p.a, (int)(k * kTileK), (int)(ia * kTileA), &full[s]);
+          load(a, &p.a, k0, a0);
         } else {
 #pragma unroll
-          for (uint32_t j = 0; j < kTileA / 64; ++j)
-            tensor_load(a + j * 8192, &p.a, (int)(ia * kTileA + j * 64), (int)(k * kTileK),
-                        &full[s]);
+          for (uint32_t j = 0; j < kTileA / 64; ++j) load(a + j * 8192, &p.a, a0 + j * 64, k0);
         }
         if (p.b_k_major) {
-          tensor_load(b, &p.b, (int)(k * kTileK), (int)(ib * BN), &full[s]);
+          load(b, &p.b, k0, b0);
         } else {
 #pragma unroll
-          for (uint32_t j = 0; j < (BN + 63) / 64; ++j)
-            tensor_load(b + j * 8192, &p.b, (int)(ib * BN + j * 64), (int)(k * kTileK), &full[s]);
+          for (uint32_t j = 0; j < (S::b_rows + 63) / 64; ++j)
+            load(b + j * 8192, &p.b, b0 + j * 64, k0);
         }
       }
     }
-    if (!ok)  // what is still on its way
+    if (!ok && (!TWO || rank == 0))  // what is still on its way
       for (uint32_t j = it > S::count ? it - S::count : 0; j < it; ++j)
         mbar_wait_bounded(&full[j % S::count], (j / S::count) & 1, p.timeout_ns);
-  } else if (warp == 1 && lane == 0) {  // products
+  } else if (warp == 1 && lane == 0 && (!TWO || rank == 0)) {  // products
     uint32_t it = 0, turn = 0;
     bool ok = true;
     for (uint32_t tile = tile0; ok && tile < tiles; tile += step, ++turn) {
@@ -233,10 +258,10 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
         const uint32_t da = p.a_k_major ? 2 : 128, db = p.b_k_major ? 2 : 128;
 #pragma unroll
         for (uint32_t j = 0; j < kTileK / 16; ++j)
-          tensor_product(to, a + j * da, b + j * db, p.kind, k > k_first || j > 0);
-        products_arrive(&empty[s]);
+          tensor_product<TWO>(to, a + j * da, b + j * db, p.kind, k > k_first || j > 0);
+        products_arrive<TWO>(&empty[s]);
       }
-      if (ok) products_arrive(&done[half]);
+      if (ok) products_arrive<TWO>(&done[half]);
     }
   } else if (warp >= 2) {  // finishing
     const uint32_t quarter = warp % 4, side = (warp - 2) / 4;  // lanes of TMEM; half of the columns
@@ -245,10 +270,11 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
       uint32_t ia, ib;
       place(tile, ia, ib);
       const uint32_t half = turn & 1;
-      const uint32_t i = ia * kTileA + quarter * 32 + lane;  // on a's side
+      // on a's side
+      const uint32_t i = ia * kHigh + (TWO ? rank * kTileA : 0) + quarter * 32 + lane;
       const bool sound = __all_sync(~0u, wait(&done[half], (turn / 2) & 1, &gave_up, p));
       tmem_fence_after();
-      if (!sound && !SPLIT) break;
+      if (!sound && MODE != SPLIT) break;
 #pragma unroll 1
       for (uint32_t c = BN < 32 ? 0 : side * (BN / 2); c < (BN < 32 ? BN : (side + 1) * (BN / 2));
            c += C) {
@@ -257,14 +283,25 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
         if constexpr (C == 32) tmem_load32(sums + half * BN + (quarter << 21) + c, v);
         else tmem_load16(sums + half * BN + (quarter << 21) + c, v);
         const uint32_t j0 = ib * BN + c;
-        if constexpr (SPLIT) {
-          const bool any = k_last > k_first;
-          float* mine = reinterpret_cast<float*>(ring);
+        if constexpr (MODE == SPLIT) {
+          if (k_last <= k_first)
 #pragma unroll
-          for (uint32_t e = 0; e < C; ++e) {
-            const uint32_t at = p.swapped ? (c + e) * kTileA + quarter * 32 + lane
-                                          : (quarter * 32 + lane) * (BN + 1) + c + e;
-            mine[at] = any ? v[e] : 0.0f;
+            for (uint32_t e = 0; e < C; ++e) v[e] = 0.0f;
+          // to the block that the row is of: [block that sends][row of its own][column]
+          const uint32_t row = quarter * 32 + lane;
+          if (p.swapped) {
+            const uint32_t own = BN / parts;
+#pragma unroll
+            for (uint32_t e = 0; e < C; ++e)
+              st_peer(peer_smem(sent + (rank * own + (c + e) % own) * kTileA + row, (c + e) / own),
+                      v[e]);
+          } else {
+            const uint32_t own = kTileA / parts;
+            const uint32_t to =
+                peer_smem(sent + (rank * own + row % own) * (BN + 4) + c, row / own);
+#pragma unroll
+            for (uint32_t e = 0; e < C; e += 4)
+              st_peer(to + e * 4, make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]));
           }
         } else if (p.swapped) {
           if (i < p.rows)
@@ -277,78 +314,78 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
       }
       tmem_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&taken[half]);
+      if (lane == 0) {
+        if constexpr (TWO) mbar_arrive_peer(peer_smem(&taken[half], 0));
+        else mbar_arrive(&taken[half]);
+      }
     }
   }
   __syncwarp();
   tmem_fence_before();
   __syncthreads();
+  if constexpr (MODE != ONE) cluster_barrier();  // SPLIT: every block's sums are there
   tmem_fence_after();
   __syncwarp();
-  if (warp == 1) tmem_free(sums, S::columns);
-  if constexpr (SPLIT) {
-    cluster_barrier();  // every block's sums are there
+  if (warp == 1) tmem_free<TWO>(sums, S::columns);
+  if constexpr (MODE == SPLIT) {
     uint32_t ia, ib;
     place(tile0, ia, ib);
-    const uint32_t inner = p.swapped ? kTileA : BN, outer = p.swapped ? BN : kTileA;
-    const uint32_t pitch = p.swapped ? kTileA : BN + 1;
-    const float* mine = reinterpret_cast<const float*>(ring);
-    // every parts-th row of the result's is this block's
-    for (uint32_t at = threadIdx.x; at < outer / parts * inner; at += kThreads) {
-      const uint32_t o = at / inner * parts + rank, n = at % inner;
-      const uint32_t row = p.swapped ? ib * BN + o : ia * kTileA + o;
-      const uint32_t col = p.swapped ? ia * kTileA + n : ib * BN + n;
-      const uint32_t rows = p.swapped ? p.cols : p.rows, cols = p.swapped ? p.rows : p.cols;
+    const uint32_t inner = p.swapped ? kTileA : BN, own = (p.swapped ? BN : kTileA) / parts;
+    const uint32_t pitch = p.swapped ? kTileA : BN + 4;
+    const uint32_t rows = p.swapped ? p.cols : p.rows, cols = p.swapped ? p.rows : p.cols;
+    for (uint32_t at = threadIdx.x; at < own * inner / 4; at += kThreads) {
+      const uint32_t o = at / (inner / 4), n = at % (inner / 4) * 4;
+      const uint32_t row = (p.swapped ? ib * BN : ia * kTileA) + rank * own + o;
+      const uint32_t col = (p.swapped ? ia * kTileA : ib * BN) + n;
       if (row >= rows || col >= cols) continue;
-      float z = 0.0f;
-      for (uint32_t r = 0; r < parts; ++r) z += ld_peer(peer_smem(mine + o * pitch + n, r));
-      finish_one<T>(p.f, row, col, cols, z);
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (uint32_t r = 0; r < parts; ++r) {
+        const float4 z = *reinterpret_cast<const float4*>(sent + (r * own + o) * pitch + n);
+        v[0] += z.x;
+        v[1] += z.y;
+        v[2] += z.z;
+        v[3] += z.w;
+      }
+      finish_row<T, 4>(p.f, row, col, cols, wide && col + 4 <= cols, v);
     }
-    cluster_barrier();  // nobody reads this block's any more
   }
 }
 
-template <typename T, int BN>
+template <typename T, int BN, Mode MODE>
 int launch(plx_ctx* ctx, TensorProduct& t, const Product& p, const Operand& a, const Operand& b,
            uint32_t parts, bool wide) {
-  using S = Stages<BN>;
+  using S = Stages<BN, MODE>;
   constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
-  t.tiles_a = (t.rows + kTileA - 1) / kTileA;
+  constexpr uint32_t high = MODE == PAIR ? 2 * kTileA : kTileA;
+  t.tiles_a = (t.rows + high - 1) / high;
   t.tiles_b = (t.cols + BN - 1) / BN;
-  t.kind = product_kind(bf16, !a.k_major, !b.k_major, BN);
+  t.kind = product_kind(bf16, !a.k_major, !b.k_major, high, BN);
   auto map = [&](CUtensorMap* m, const Operand& o, uint32_t count, uint32_t tile) {
     return tensor_map(m, bf16 ? PLX_BF16 : PLX_F16, o.p, o.k_major ? t.depth : count,
                       o.k_major ? count : t.depth, o.ld, 64, o.k_major ? tile : kTileK, true);
   };
   if (int rc = map(&t.a, a, t.rows, kTileA)) return rc;
-  if (int rc = map(&t.b, b, t.cols, BN)) return rc;
+  if (int rc = map(&t.b, b, t.cols, S::b_rows)) return rc;
   const uint64_t tiles = (uint64_t)t.tiles_a * t.tiles_b;
   if (tiles >= (1ull << 28))
     return set_error(PLX_ERR_CAPACITY, "%u x %u results are too many for one call", p.rows, p.cols);
-  if (parts > 1) {
-    constexpr auto kernel = k_product_tensor<T, BN, true>;
-    constexpr uint32_t sums = (BN + 1) * kTileA * 4;
-    constexpr uint32_t smem = S::smem < sums + 1024 ? sums + 1024 : S::smem;
-    PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, smem));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * parts));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = ctx->stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = parts;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    PLX_TRY_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const TensorProduct)t, wide));
-  } else {
-    constexpr auto kernel = k_product_tensor<T, BN, false>;
-    PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, S::smem));
-    const unsigned grid = (unsigned)std::min<uint64_t>(tiles, ctx->num_sms);
-    kernel<<<grid, kThreads, S::smem, ctx->stream>>>(t, wide);
-    PLX_LAUNCH_CHECK("k_product_tensor");
-  }
+  constexpr auto kernel = k_product_tensor<T, BN, MODE>;
+  PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, S::smem));
+  cudaLaunchConfig_t cfg = {};
+  const uint32_t sms = (uint32_t)ctx->num_sms;
+  cfg.gridDim = dim3((unsigned)(MODE == SPLIT  ? tiles * parts
+                                : MODE == PAIR ? 2 * std::min<uint64_t>(tiles, sms / 2)
+                                               : std::min<uint64_t>(tiles, sms)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::smem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = MODE == SPLIT ? parts : 2;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = MODE == ONE ? 0 : 1;
+  PLX_TRY_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const TensorProduct)t, wide));
   return PLX_OK;
 }
 
@@ -373,9 +410,11 @@ int product_tensor(plx_ctx* ctx, int dtype, const Product& p) {
   const bool wide = p.f.ldy % 8 == 0 && aligned16(p.f.y) &&
                     (!p.f.residual || (p.f.ldr % 8 == 0 && aligned16(p.f.residual))) &&
                     (!p.f.pre || (p.cols % 4 == 0 && aligned16(p.f.pre)));
-  // What the tiles of a width take: rounds of blocks, each with its share of k.
+  // What the tiles of a width take: rounds of blocks, each with its share of k (in
+  // products of 64 values of k by one column; the rest measured).
   const uint32_t sms = (uint32_t)ctx->num_sms, ks = (p.depth + kTileK - 1) / kTileK;
   uint32_t bn = 0, parts = 1;
+  bool pair = false;
   double best = 0;
   for (uint32_t width : {256u, 128u, 64u, 32u, 16u}) {
     if (width < 64 && !b.k_major) break;
@@ -383,9 +422,9 @@ int product_tensor(plx_ctx* ctx, int dtype, const Product& p) {
     const uint64_t tiles =
         (uint64_t)((t.rows + kTileA - 1) / kTileA) * ((t.cols + width - 1) / width);
     for (uint32_t s = 1; s <= 8; s *= 2) {
-      if (s > 1 && (tiles * s > sms || s > ks)) break;
+      if (s > 1 && (tiles * s > sms || s > ks || width > 128)) break;
       const double rounds = (double)((tiles * s + sms - 1) / sms);
-      const double took = rounds * ((width + 64.0) * ((ks + s - 1) / s) + (s > 1 ? 800 : 400));
+      const double took = rounds * ((width + 96.0) * ((ks + s - 1) / s) + (s > 1 ? 1000 : 500));
       if (bn == 0 || took < best) {
         best = took;
         bn = width;
@@ -393,14 +432,22 @@ int product_tensor(plx_ctx* ctx, int dtype, const Product& p) {
       }
     }
   }
+  if (t.rows > kTileA && t.cols > 128) {
+    const uint64_t tiles =
+        (uint64_t)((t.rows + 2 * kTileA - 1) / (2 * kTileA)) * ((t.cols + 255) / 256);
+    const double rounds = (double)((tiles + sms / 2 - 1) / (sms / 2));
+    pair = rounds * (270.0 * ks + 500) < best;
+  }
   auto go = [&](auto v) -> int {
     using T = decltype(v);
+    if (pair) return launch<T, 256, PAIR>(ctx, t, p, a, b, 1, wide);
+    const bool split = parts > 1;
     switch (bn) {
-      case 256: return launch<T, 256>(ctx, t, p, a, b, parts, wide);
-      case 128: return launch<T, 128>(ctx, t, p, a, b, parts, wide);
-      case 64: return launch<T, 64>(ctx, t, p, a, b, parts, wide);
-      case 32: return launch<T, 32>(ctx, t, p, a, b, parts, wide);
-      default: return launch<T, 16>(ctx, t, p, a, b, parts, wide);
+      case 256: return launch<T, 256, ONE>(ctx, t, p, a, b, parts, wide);
+      case 128: return (split ? launch<T, 128, SPLIT> : launch<T, 128, ONE>)(ctx, t, p, a, b, parts, wide);
+      case 64: return (split ? launch<T, 64, SPLIT> : launch<T, 64, ONE>)(ctx, t, p, a, b, parts, wide);
+      case 32: return (split ? launch<T, 32, SPLIT> : launch<T, 32, ONE>)(ctx, t, p, a, b, parts, wide);
+      default: return (split ? launch<T, 16, SPLIT> : launch<T, 16, ONE>)(ctx, t, p, a, b, parts, wide);
     }
   };
   return dtype == PLX_BF16 ? go(__nv_bfloat16{}) : go(__half{});

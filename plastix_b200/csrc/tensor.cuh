@@ -26,18 +26,42 @@ __device__ __forceinline__ void tensor_load(void* dst_smem, const CUtensorMap* m
       : "memory");
 }
 
+// The same for a pair of blocks whose products are issued together: `bar` (an
+// address as peer_smem gives) may be the other block's.
+__device__ __forceinline__ void tensor_load_pair(void* dst_smem, const CUtensorMap* map, int x,
+                                                 int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst_smem)),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
 // ---- tensor memory -----------------------------------------------------------
 // Columns (a power of two from 32) for the block, their address to `to`; by one
-// whole warp, which gives them back as well.
+// whole warp, which gives them back as well. PAIR: by both blocks of a pair.
+template <bool PAIR>
 __device__ __forceinline__ void tmem_alloc(uint32_t* to, uint32_t columns) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                   smem_addr(to)),
-               "r"(columns)
-               : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_addr(to)),
+                 "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_addr(to)),
+                 "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
 }
+template <bool PAIR>
 __device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+  if constexpr (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
 }
 __device__ __forceinline__ void tmem_fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -90,27 +114,47 @@ __device__ __forceinline__ uint64_t operand_i_major(const void* at, uint32_t apa
   return (uint64_t)((smem_addr(at) & 0x3FFFF) >> 4) | (uint64_t)(apart >> 4) << 16 |
          (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-// What is multiplied: 128 x n values of 16 bits, sums in 32 bits. Both operands
-// are of one type.
-inline uint32_t product_kind(bool bf16, bool a_i_major, bool b_i_major, uint32_t n) {
+// What is multiplied: m (128, or 256 by a pair of blocks) x n values of 16 bits, sums
+// in 32 bits. Both operands are of one type.
+inline uint32_t product_kind(bool bf16, bool a_i_major, bool b_i_major, uint32_t m, uint32_t n) {
   return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_i_major ? 1u << 15 : 0u) |
-         (b_i_major ? 1u << 16 : 0u) | (n >> 3) << 17 | (128u >> 4) << 24;
+         (b_i_major ? 1u << 16 : 0u) | (n >> 3) << 17 | (m >> 4) << 24;
 }
-// Adds the products over 16 values of k to (or, first, puts them in) TMEM.
+// Adds the products over 16 values of k to (or, first, puts them in) TMEM. PAIR: each
+// block has half of a's rows, of b's and of the sums' rows; one of the two issues.
+template <bool PAIR>
 __device__ __forceinline__ void tensor_product(uint32_t at, uint64_t a, uint64_t b, uint32_t kind,
                                                bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(at),
-      "l"(a), "l"(b), "r"(kind), "r"((uint32_t)add)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(at),
+        "l"(a), "l"(b), "r"(kind), "r"((uint32_t)add)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(at),
+        "l"(a), "l"(b), "r"(kind), "r"((uint32_t)add)
+        : "memory");
 }
-// Arrives at the barrier once the products issued before are done.
+// Arrives at the barrier (PAIR: at both blocks') once the products issued before are
+// done.
+template <bool PAIR>
 __device__ __forceinline__ void products_arrive(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_addr(bar))
-               : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(smem_addr(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+            smem_addr(bar))
+        : "memory");
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
