@@ -128,7 +128,8 @@ int operand(plx_ctx* ctx, int dtype, const void* p, int64_t ld, uint64_t rows, u
   return PLX_OK;
 }
 
-int product(plx_ctx* ctx, int dtype, const Product& p) {
+int product(plx_ctx* ctx, int dtype, Product p) {
+  if (p.rows == 1) p.f.ldy = p.f.ldr = (int64_t)round_up(p.cols, 8);  // strides of one row
   return dtype == PLX_F32 ? product_f32(ctx, dtype, p) : product_tensor(ctx, dtype, p);
 }
 

@@ -33,14 +33,19 @@ struct Stages {
   static constexpr uint32_t bytes = a_bytes + b_bytes;
   // sums that the blocks of a cluster are sent, of a tile in all
   static constexpr uint32_t sums = MODE == SPLIT ? (BN + 4) * kTileA * 4 : 0;
-  static constexpr uint32_t most = (kSmem - 2048 - sums) / bytes;
+  // pieces of results (32 rows of 128 bytes) on their way out, of each warp
+  static constexpr uint32_t pieces = MODE == SPLIT || BN < 128 ? 0 : MODE == PAIR ? 2 : 1;
+  static constexpr uint32_t out = pieces * kFinishWarps * 4096;
+  static constexpr uint32_t most = (kSmem - 2048 - sums - out) / bytes;
   static constexpr uint32_t count = most < 12 ? most : 12;
-  static constexpr uint32_t smem = count * bytes + sums + 1024;  // to a multiple of 1,024
+  static constexpr uint32_t smem = count * bytes + out + sums + 1024;  // to a multiple of 1,024
   static constexpr uint32_t columns = 2 * BN < 32 ? 32 : 2 * BN;
 };
 
 struct TensorProduct {
   CUtensorMap a, b;  // a has the tile's 128
+  CUtensorMap y, residual, pre;  // where results go by tensor copies
+  bool copied;
   uint32_t rows, cols, depth;  // of the tiles' sides
   uint32_t tiles_a, tiles_b;
   uint32_t kind;
@@ -93,16 +98,37 @@ __device__ __forceinline__ void finish_one(const Finish& f, uint32_t row, uint32
   ((T*)f.y)[(int64_t)row * f.ldy + col] = from_f32<T>(v[0]);
 }
 
+// Adds the bias of C consecutive columns; `wide`: all there, in 16-byte pieces.
+template <typename T, int C>
+__device__ __forceinline__ void add_bias(const Finish& f, uint32_t col, uint32_t cols, bool wide,
+                                         float (&v)[C]) {
+  if (!f.bias) return;
+  if (!wide) {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (col + i < cols) v[i] += bias_at<T>(f, col + i);
+  } else if (f.param_dtype == PLX_F32) {
+    Pack<float, 4> q[C / 4];
+#pragma unroll
+    for (int i = 0; i < C / 4; ++i) q[i] = load_pack<float, 4>((const float*)f.bias + col + i * 4);
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] += q[i / 4].v[i % 4];
+  } else {
+    constexpr int N = C < 8 ? C : 8;
+    Pack<T, N> q[C / N];
+#pragma unroll
+    for (int i = 0; i < C / N; ++i) q[i] = load_pack<T, N>((const T*)f.bias + col + i * N);
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] += to_f32(q[i / N].v[i % N]);
+  }
+}
+
 // A thread's C consecutive columns of a row of the result; `wide`: all there, in
 // 16-byte pieces.
 template <typename T, int C>
 __device__ __forceinline__ void finish_row(const Finish& f, uint32_t row, uint32_t col,
                                            uint32_t cols, bool wide, float (&v)[C]) {
-  if (f.bias) {
-#pragma unroll
-    for (int i = 0; i < C; ++i)
-      if (wide || col + i < cols) v[i] += bias_at<T>(f, col + i);
-  }
+  add_bias<T, C>(f, col, cols, wide, v);
   if (f.pre) {
     float* to = f.pre + (uint64_t)row * cols + col;
     if (wide) {
@@ -152,7 +178,10 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
   constexpr uint32_t kHigh = TWO ? 2 * kTileA : kTileA;  // of a tile
   extern __shared__ __align__(128) uint8_t product_bytes[];
   uint8_t* ring = product_bytes + (1024 - (smem_addr(product_bytes) & 1023)) % 1024;
-  float* sent = reinterpret_cast<float*>(ring + S::count * S::bytes);
+  uint8_t* out = ring + S::count * S::bytes;
+  float* sent = reinterpret_cast<float*>(out + S::out);
+  constexpr int kPieces = S::pieces ? S::pieces : 1;
+  __shared__ uint64_t arrived[kFinishWarps][kPieces];  // the residual's piece is there
   __shared__ uint64_t full[S::count], empty[S::count], done[2], taken[2];
   __shared__ uint32_t tmem, gave_up;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -182,6 +211,8 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
       mbar_init(&done[h], 1);
       mbar_init(&taken[h], TWO ? 2 * kFinishWarps : kFinishWarps);
     }
+    for (int w = 0; w < kFinishWarps; ++w)
+      for (int i = 0; i < kPieces; ++i) mbar_init(&arrived[w][i], 1);
     mbar_init_fence();
     gave_up = 0;
   }
@@ -265,16 +296,109 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
     }
   } else if (warp >= 2) {  // finishing
     const uint32_t quarter = warp % 4, side = (warp - 2) / 4;  // lanes of TMEM; half of the columns
-    uint32_t turn = 0;
+    uint32_t turn = 0, arrivals = 0;  // the parities of `arrived`
     for (uint32_t tile = tile0; tile < tiles; tile += step, ++turn) {
       uint32_t ia, ib;
       place(tile, ia, ib);
       const uint32_t half = turn & 1;
       // on a's side
       const uint32_t i = ia * kHigh + (TWO ? rank * kTileA : 0) + quarter * 32 + lane;
+      // Pieces of 64 columns: the residual's are on their way before the sums are done.
+      constexpr uint32_t kChunks = S::pieces ? BN / 128 : 0;
+      const uint32_t row0 = i - lane, col0 = ib * BN + side * (BN / 2);
+      const bool copied = S::pieces && p.copied;
+      auto piece = [&](uint32_t c) { return out + ((warp - 2) * kPieces + c % kPieces) * 4096; };
+      auto there = [&](uint32_t c) { return row0 < p.rows && col0 + c * 64 < p.cols; };
+      auto fetch = [&](uint32_t c) {  // by one lane, which has stored what was there
+        if (!there(c)) return;
+        uint64_t* bar = &arrived[warp - 2][c % kPieces];
+        mbar_arrive_expect_tx(bar, 4096);
+        tensor_load(piece(c), &p.residual, (int)(col0 + c * 64), (int)row0, bar);
+      };
+      if (copied && p.f.residual && lane == 0) {
+        bulk_wait_read<0>();
+        for (uint32_t c = 0; c < kChunks && c < kPieces; ++c) fetch(c);
+      }
       const bool sound = __all_sync(~0u, wait(&done[half], (turn / 2) & 1, &gave_up, p));
       tmem_fence_after();
-      if (!sound && MODE != SPLIT) break;
+      if (!sound && MODE != SPLIT) {
+        if (copied && p.f.residual && lane == 0)  // what is still on its way
+          for (uint32_t c = 0; c < kChunks && c < kPieces; ++c)
+            if (there(c)) mbar_wait_bounded(&arrived[warp - 2][c], arrivals >> c & 1, p.timeout_ns);
+        break;
+      }
+      if (copied) {
+#pragma unroll 1
+        for (uint32_t c = 0; c < kChunks; ++c) {
+          if (!there(c)) continue;
+          uint8_t* at = piece(c);
+          if (p.f.residual) {
+            wait(&arrived[warp - 2][c % kPieces], arrivals >> (c % kPieces) & 1, &gave_up, p);
+            arrivals ^= 1u << (c % kPieces);
+          } else {
+            if (lane == 0) bulk_wait_read<0>();
+            __syncwarp();
+          }
+          // of this lane's row, the 16-byte chunk k of a piece
+          auto chunk = [&](uint8_t* of, uint32_t k) { return of + lane * 128 + ((k ^ (lane & 7)) << 4); };
+#pragma unroll 1
+          for (uint32_t h = 0; h < 2; ++h) {
+            float v[32];
+            tmem_load32(sums + half * BN + (quarter << 21) + side * (BN / 2) + c * 64 + h * 32, v);
+            const uint32_t j0 = col0 + c * 64 + h * 32;
+            const bool whole = j0 + 32 <= p.cols;
+            add_bias<T, 32>(p.f, j0, p.cols, whole, v);
+            if (p.f.pre) {
+              if (kPieces == 2 && !p.f.residual) {  // the other piece takes it out
+                uint8_t* z = piece(c + 1);
+                if (lane == 0) bulk_wait_read<0>();
+                __syncwarp();
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k)
+                  *reinterpret_cast<float4*>(chunk(z, k)) =
+                      make_float4(v[k * 4], v[k * 4 + 1], v[k * 4 + 2], v[k * 4 + 3]);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0 && j0 < p.cols) {
+                  tensor_store(&p.pre, (int)j0, (int)row0, z);
+                  bulk_commit();
+                }
+              } else if (i < p.rows) {
+                float* to = p.f.pre + (uint64_t)i * p.cols + j0;
+#pragma unroll
+                for (uint32_t k = 0; k < 32; k += 4)
+                  if (j0 + k < p.cols)  // a multiple of four
+                    *reinterpret_cast<float4*>(to + k) =
+                        make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+              }
+            }
+            activate(p.f.act, v);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+              auto* q = reinterpret_cast<Pack<T, 8>*>(chunk(at, h * 4 + k));
+              Pack<T, 8> o;
+              if (p.f.residual) {
+                o = *q;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k * 8 + e] += to_f32(o.v[e]);
+              }
+#pragma unroll
+              for (int e = 0; e < 8; e += 2) put_pair(o, e, pack2(v[k * 8 + e], v[k * 8 + e + 1]));
+              *q = o;
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tensor_store(&p.y, (int)(col0 + c * 64), (int)row0, at);
+            bulk_commit();
+            if (kPieces == 1 && p.f.residual && c + 1 < kChunks) {
+              bulk_wait_read<0>();
+              fetch(c + 1);
+            }
+          }
+        }
+      } else
 #pragma unroll 1
       for (uint32_t c = BN < 32 ? 0 : side * (BN / 2); c < (BN < 32 ? BN : (side + 1) * (BN / 2));
            c += C) {
@@ -319,6 +443,7 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
         else mbar_arrive(&taken[half]);
       }
     }
+    if (S::pieces && lane == 0) bulk_wait_all<0>();
   }
   __syncwarp();
   tmem_fence_before();
@@ -366,6 +491,16 @@ int launch(plx_ctx* ctx, TensorProduct& t, const Product& p, const Operand& a, c
   };
   if (int rc = map(&t.a, a, t.rows, kTileA)) return rc;
   if (int rc = map(&t.b, b, t.cols, S::b_rows)) return rc;
+  t.copied = S::pieces && wide;
+  if (t.copied) {
+    const int dtype = bf16 ? PLX_BF16 : PLX_F16;
+    if (int rc = tensor_map(&t.y, dtype, p.f.y, t.cols, t.rows, p.f.ldy, 64, 32, true)) return rc;
+    if (p.f.residual)
+      if (int rc = tensor_map(&t.residual, dtype, p.f.residual, t.cols, t.rows, p.f.ldr, 64, 32, true))
+        return rc;
+    if (p.f.pre)
+      if (int rc = tensor_map(&t.pre, PLX_F32, p.f.pre, t.cols, t.rows, t.cols, 32, 32, true)) return rc;
+  }
   const uint64_t tiles = (uint64_t)t.tiles_a * t.tiles_b;
   if (tiles >= (1ull << 28))
     return set_error(PLX_ERR_CAPACITY, "%u x %u results are too many for one call", p.rows, p.cols);
@@ -409,7 +544,7 @@ int product_tensor(plx_ctx* ctx, int dtype, const Product& p) {
   t.b_k_major = b.k_major;
   const bool wide = p.f.ldy % 8 == 0 && aligned16(p.f.y) &&
                     (!p.f.residual || (p.f.ldr % 8 == 0 && aligned16(p.f.residual))) &&
-                    (!p.f.pre || (p.cols % 4 == 0 && aligned16(p.f.pre)));
+                    (!p.f.pre || (p.cols % 4 == 0 && aligned16(p.f.pre))) && aligned16(p.f.bias);
   // What the tiles of a width take: rounds of blocks, each with its share of k (in
   // products of 64 values of k by one column; the rest measured).
   const uint32_t sms = (uint32_t)ctx->num_sms, ks = (p.depth + kTileK - 1) / kTileK;

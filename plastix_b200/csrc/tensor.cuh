@@ -37,6 +37,16 @@ __device__ __forceinline__ void tensor_load_pair(void* dst_smem, const CUtensorM
       : "memory");
 }
 
+// A box from shared memory to the array (what is outside stays as it is); bulk_commit
+// and bulk_wait_read or bulk_wait_all by the same thread.
+__device__ __forceinline__ void tensor_store(const CUtensorMap* map, int x, int y,
+                                             const void* src_smem) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   map),
+               "r"(x), "r"(y), "r"(smem_addr(src_smem))
+               : "memory");
+}
+
 // ---- tensor memory -----------------------------------------------------------
 // Columns (a power of two from 32) for the block, their address to `to`; by one
 // whole warp, which gives them back as well. PAIR: by both blocks of a pair.
