@@ -6,8 +6,9 @@
 // is made of the r that has not been rounded.
 //
 // Bound by memory: x, o and a gate of every value are read once, r and u written
-// once, so a row is held in the registers of the threads that share it (a warp up
-// to 512 values, a block above).
+// once. A block (or a warp, for rows of up to 512 values) stays and takes every
+// gridDim-th row, with the parameters of its threads' sixteen columns in registers
+// and the next rows on their way into shared memory.
 #include "block_norm.cuh"
 
 namespace plx {
@@ -16,42 +17,75 @@ namespace {
 // What is left of a mean in deviations that a mean four times their size was
 // taken from is taken away as well (the first mean is off by its sum's roundings).
 constexpr float kFar = 4.0f;
+template <typename T>
+constexpr int kStages = sizeof(T) == 4 ? 2 : 4;
 
-template <typename T, typename P, int V, int NV, int TPR>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR)
+template <typename T, int V, int NV, int TPR, bool BIAS, bool VALUES, int EACH>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, EACH)
 k_block_norm(const __grid_constant__ BlockNorm a) {
-  constexpr int ROWS = TPR == 32 ? 8 : 1, E = NV * V, STEP = TPR * V;
+  using C = Columns<T, V, NV, TPR>;
+  using R = BlockRing<T, V, NV, TPR, VALUES ? 3 : 2, kStages<T>>;
+  constexpr int ROWS = TPR == 32 ? 8 : 1, G = C::G, HV = C::HV, H = C::H, S = R::stages;
+  enum { O, X, GATE };
+  extern __shared__ uint4 ring_bytes[];
   __shared__ float red[2 * (TPR / 32)];
-  const uint32_t lane = threadIdx.x % TPR, c0 = lane * V;
-  const uint32_t r = blockIdx.x * ROWS + threadIdx.x / TPR;
-  if (ROWS > 1 && r >= a.rows) return;
-  const int left = (int)a.n - (int)c0;
-  Pack<T, V> qx[NV], qo[NV], qg[NV];
-  load_row<STEP>((const T*)a.o + (int64_t)r * a.ldo + c0, left, qo);
-  load_row<STEP>((const T*)a.x + (int64_t)r * a.ldx + c0, left, qx);
-  if (a.gate == PLX_BLOCK_GATE_VALUES)
-    load_row<STEP>((const T*)a.gate_values + (int64_t)r * a.ldg + c0, left, qg);
+  const uint32_t lane = threadIdx.x % TPR;
+  const C c(a.n, lane * V);
+  uint32_t r = blockIdx.x * ROWS + threadIdx.x / TPR;
+  const uint32_t step = gridDim.x * ROWS;
+  R ring;
+  ring.ring = reinterpret_cast<char*>(ring_bytes);
+  ring.from[O] = (const T*)a.o + (int64_t)r * a.ldo + c.c0;
+  ring.from[X] = (const T*)a.x + (int64_t)r * a.ldx + c.c0;
+  ring.step[O] = step * a.ldo;
+  ring.step[X] = step * a.ldx;
+  if constexpr (VALUES) {
+    ring.from[GATE] = (const T*)a.gate_values + (int64_t)r * a.ldg + c.c0;
+    ring.step[GATE] = step * a.ldg;
+  }
+  ring.clear(c);
+  const F2 none = pack2(0.0f, 0.0f);
+  F2 w1[H], w2[H], gate[VALUES ? 1 : H];
+  c.param(a.post_weight, a.param_f32, w1, 1.0f);
+  c.param(a.pre_weight, a.param_f32, w2, 1.0f);
+  if constexpr (!VALUES) {
+    c.param(a.gate == PLX_BLOCK_GATE_UNITS ? a.gate_values : nullptr, a.param_f32, gate, 1.0f);
+    if (a.gate == PLX_BLOCK_GATE_UNITS && a.sigmoid)
+#pragma unroll
+      for (int h = 0; h < H; ++h) gate[h] = pack2(sigmoid(gate[h].x).a, sigmoid(gate[h].y).a);
+  }
+  T* to_r = (T*)a.r + (int64_t)r * a.ldr + c.c0;
+  T* to_u = (T*)a.u + (int64_t)r * a.ldu + c.c0;
   int turn = 0;
-  // Takes the row's values to h = N(v).
-  auto normalise = [&](float (&v)[E], float& mean, float& rstd) {
+  // The row's values less their mean (where that is taken away), and rstd.
+  auto normal = [&](F2 (&v)[H], float& mean, float& rstd) {
     float s[1];
     mean = 0.0f;
     auto squares = [&] {
-      s[0] = 0.0f;
+      F2 t = none;
 #pragma unroll
-      for (int e = 0; e < E; ++e) s[0] = fmaf(v[e], v[e], s[0]);
+      for (int h = 0; h < H; ++h) t = fma2(v[h], v[h], t);
+      s[0] = t.x + t.y;
       row_sum<TPR>(s, red, turn);
       return rsqrtf(s[0] * a.inv_n + a.eps);
     };
     auto shift = [&] {
-      s[0] = 0.0f;
+      F2 t = none;
 #pragma unroll
-      for (int e = 0; e < E; ++e) s[0] += v[e];
+      for (int h = 0; h < H; ++h) t = add2(v[h], t);
+      s[0] = t.x + t.y;
       row_sum<TPR>(s, red, turn);
       const float m = s[0] * a.inv_n;
+      const F2 minus = pack2(-m, -m);
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (e / V * STEP < left) v[e] -= m;
+      for (int g = 0; g < G; ++g)
+        if (c.in(g))
+#pragma unroll
+          for (int e = 0; e < HV; ++e) {
+            F2& w = v[g * HV + e];
+            w = add2(w, minus);
+            if (V == 1 && !c.both(g)) w.y = 0.0f;
+          }
       mean += m;
     };
     if (a.layer) shift();
@@ -60,46 +94,85 @@ k_block_norm(const __grid_constant__ BlockNorm a) {
       shift();
       rstd = squares();
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] *= rstd;
   };
-  float v[E], m1 = 0.0f, s1 = 0.0f, m2, s2;
-  widen<NV, V>(qo, v);
-  if (a.post) {
-    normalise(v, m1, s1);
-    affine<STEP, P, NV, V>(v, (const P*)a.post_weight, (const P*)a.post_bias, c0, left);
-  }
+  uint32_t stage = 0;
+  if constexpr (R::used) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    if (j * STEP >= left) continue;
-    Pack<P, V> pg;
-    if (a.gate == PLX_BLOCK_GATE_UNITS)
-      pg = load_pack<P, V>((const P*)a.gate_values + c0 + j * STEP);
-    Pack<T, V> out;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float g = 1.0f;
-      if (a.gate != PLX_BLOCK_GATE_NONE) {
-        g = a.gate == PLX_BLOCK_GATE_UNITS ? to_f32(pg.v[e]) : to_f32(qg[j].v[e]);
-        if (a.sigmoid) g = sigmoid(g).a;
-      }
-      float& w = v[j * V + e];
-      w = fmaf(g, w, a.scale * to_f32(qx[j].v[e]));
-      out.v[e] = from_f32<T>(w);
+    for (int s = 0; s < S - 1; ++s) {
+      ring.fetch(c, r + (uint64_t)s * step < a.rows, s);
+      copy_commit();
     }
-    *reinterpret_cast<Pack<T, V>*>((T*)a.r + (int64_t)r * a.ldr + c0 + j * STEP) = out;
   }
-  normalise(v, m2, s2);
-  affine<STEP, P, NV, V>(v, (const P*)a.pre_weight, (const P*)a.pre_bias, c0, left);
+  for (; r < a.rows; r += step) {
+    if constexpr (R::used) {
+      copy_wait<S - 2>();
+      ring.fetch(c, r + (uint64_t)(S - 1) * step < a.rows, stage == 0 ? S - 1 : stage - 1);
+      copy_commit();
+    } else {
+      ring.fetch(c, true, 0);
+    }
+    F2 v[H];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    if (j * STEP >= left) continue;
-    Pack<T, V> out;
+    for (int g = 0; g < G; ++g) {
+      F2 o[HV];
+      ring.get(stage, O, g, o);
 #pragma unroll
-    for (int e = 0; e < V; ++e) out.v[e] = from_f32<T>(v[j * V + e]);
-    *reinterpret_cast<Pack<T, V>*>((T*)a.u + (int64_t)r * a.ldu + c0 + j * STEP) = out;
+      for (int e = 0; e < HV; ++e) v[g * HV + e] = o[e];
+    }
+    float m1 = 0.0f, s1 = 0.0f, m2, s2;
+    if (a.post) {
+      normal(v, m1, s1);
+      const F2 by = pack2(s1, s1);
+#pragma unroll
+      for (int h = 0; h < H; ++h) v[h] = mul2(mul2(v[h], by), w1[h]);
+      if (BIAS && a.post_bias) {
+        F2 b[H];
+        c.param(a.post_bias, a.param_f32, b, 0.0f);
+#pragma unroll
+        for (int h = 0; h < H; ++h) v[h] = add2(v[h], b[h]);
+      }
+    }
+    const F2 scale = pack2(a.scale, a.scale);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      F2 x[HV], gv[HV], out[HV];
+      ring.get(stage, X, g, x);
+      if constexpr (VALUES) {
+        ring.get(stage, GATE, g, gv);
+        if (a.sigmoid)
+#pragma unroll
+          for (int e = 0; e < HV; ++e) gv[e] = pack2(sigmoid(gv[e].x).a, sigmoid(gv[e].y).a);
+      }
+#pragma unroll
+      for (int e = 0; e < HV; ++e) {
+        F2& w = v[g * HV + e];
+        w = fma2(VALUES ? gv[e] : gate[VALUES ? 0 : g * HV + e], w, mul2(scale, x[e]));
+        out[e] = w;
+      }
+      if (c.in(g)) c.put(to_r, g, out);
+    }
+    normal(v, m2, s2);
+    const F2 by = pack2(s2, s2);
+#pragma unroll
+    for (int h = 0; h < H; ++h) v[h] = mul2(mul2(v[h], by), w2[h]);
+    if (BIAS && a.pre_bias) {
+      F2 b[H];
+      c.param(a.pre_bias, a.param_f32, b, 0.0f);
+#pragma unroll
+      for (int h = 0; h < H; ++h) v[h] = add2(v[h], b[h]);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      F2 out[HV];
+#pragma unroll
+      for (int e = 0; e < HV; ++e) out[e] = v[g * HV + e];
+      if (c.in(g)) c.put(to_u, g, out);
+    }
+    if (lane == 0 && a.stats_out) a.stats_out[r] = make_float4(m1, s1, m2, s2);
+    to_r += step * a.ldr;
+    to_u += step * a.ldu;
+    stage = stage == S - 1 ? 0 : stage + 1;
   }
-  if (lane == 0 && a.stats_out) a.stats_out[r] = make_float4(m1, s1, m2, s2);
 }
 
 // Rows too long for registers: values are made anew from what was read in each
@@ -223,33 +296,44 @@ extern "C" int plx_block_norm(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype
     constexpr int V = 16 / sizeof(T);
     auto go = [&](auto p) {
       using P = decltype(p);
-      const unsigned one = (unsigned)rows, eighth = (unsigned)((rows + 7) / 8);
-      auto launch = [&](auto kernel, unsigned grid, unsigned block) {
-        kernel<<<grid, block, 0, ctx->stream>>>(a);
+      int rc = PLX_OK;
+      // EACH blocks an SM.
+      auto launch = [&](auto v_c, auto nv_c, auto tpr_c, auto each_c) {
+        constexpr int VV = decltype(v_c)::value, NV = decltype(nv_c)::value;
+        constexpr int TPR = decltype(tpr_c)::value, EACH = decltype(each_c)::value;
+        constexpr unsigned per_block = TPR == 32 ? 8 : 1;
+        auto with = [&](auto bias_c, auto values_c) -> int {
+          constexpr bool VALUES = decltype(values_c)::value;
+          using R = BlockRing<T, VV, NV, TPR, VALUES ? 3 : 2, kStages<T>>;
+          constexpr auto kernel = k_block_norm<T, VV, NV, TPR, decltype(bias_c)::value, VALUES, EACH>;
+          if (R::bytes > 32 * 1024) PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, R::bytes));
+          const unsigned grid = (unsigned)std::min<uint64_t>((rows + per_block - 1) / per_block,
+                                                             (uint64_t)ctx->num_sms * EACH);
+          kernel<<<grid, R::threads, R::bytes, ctx->stream>>>(a);
+          return PLX_OK;
+        };
+        using Yes = std::true_type;
+        using No = std::false_type;
+        const bool values = a.gate == PLX_BLOCK_GATE_VALUES;
+        if (a.post_bias || a.pre_bias) rc = values ? with(Yes{}, Yes{}) : with(Yes{}, No{});
+        else rc = values ? with(No{}, Yes{}) : with(No{}, No{});
       };
       const uint32_t v = block_piece<T, P>(a, {x, o, r, u}, {a.ldx, a.ldo, a.ldr, a.ldu});
       // A row takes the first launch that holds it.
-      if (v == V) {
-        constexpr int NV = 16 / V;
-        if (n <= 512) launch(k_block_norm<T, P, V, NV, 32>, eighth, 256);
-        else if (n <= 2048) launch(k_block_norm<T, P, V, NV, 128>, one, 128);
-        else if (n <= 4096) launch(k_block_norm<T, P, V, NV, 256>, one, 256);
-        else if (n <= 8192) launch(k_block_norm<T, P, V, NV, 512>, one, 512);
-        else if (n <= 16384) launch(k_block_norm<T, P, V, NV, 1024>, one, 1024);
-        else launch(k_block_norm_long<T, P>, one, 1024);
-      } else if (sizeof(T) == 2 && v >= 2) {
-        if (n <= 512) launch(k_block_norm<T, P, 2, 8, 32>, eighth, 256);
-        else if (n <= 2048) launch(k_block_norm<T, P, 2, 8, 128>, one, 128);
-        else if (n <= 4096) launch(k_block_norm<T, P, 2, 8, 256>, one, 256);
-        else if (n <= 8192) launch(k_block_norm<T, P, 2, 8, 512>, one, 512);
-        else launch(k_block_norm_long<T, P>, one, 1024);
-      } else {
-        if (n <= 256) launch(k_block_norm<T, P, 1, 8, 32>, eighth, 256);
-        else if (n <= 2048) launch(k_block_norm<T, P, 1, 16, 128>, one, 128);
-        else if (n <= 4096) launch(k_block_norm<T, P, 1, 16, 256>, one, 256);
-        else if (n <= 8192) launch(k_block_norm<T, P, 1, 16, 512>, one, 512);
-        else launch(k_block_norm_long<T, P>, one, 1024);
-      }
+      using std::integral_constant;
+#define PLX_C(v) integral_constant<int, v>{}
+      auto ladder = [&](auto vv, auto nv) {
+        if (n <= 512) launch(vv, nv, PLX_C(32), PLX_C(2));
+        else if (n <= 2048) launch(vv, nv, PLX_C(128), PLX_C(4));
+        else if (n <= 4096) launch(vv, nv, PLX_C(256), PLX_C(2));
+        else if (n <= 8192) launch(vv, nv, PLX_C(512), PLX_C(1));
+        else k_block_norm_long<T, P><<<(unsigned)rows, 1024, 0, ctx->stream>>>(a);
+      };
+      if (v == V) ladder(PLX_C(V), PLX_C(16 / V));
+      else if (sizeof(T) == 2 && v >= 2) ladder(PLX_C(2), PLX_C(8));
+      else ladder(PLX_C(1), PLX_C(16));
+#undef PLX_C
+      if (rc != PLX_OK) return rc;
       PLX_LAUNCH_CHECK("k_block_norm");
       return PLX_OK;
     };

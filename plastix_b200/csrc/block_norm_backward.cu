@@ -31,150 +31,61 @@ struct SumsOut {
   void* out[kSums];
 };
 
-// Pairs of values of a parameter, of either type: V consecutive ones, or where V
-// is 1 the one at i and, if there is one in the row, the one at `next`.
-template <typename T, int V>
-__device__ __forceinline__ void param_pairs(const void* w, bool f32, uint32_t i, uint32_t next,
-                                            uint32_t n, F2 (&v)[V == 1 ? 1 : V / 2]) {
-  if constexpr (V == 1) {
-    const bool two = next < n;
-    v[0] = f32 ? pack2(((const float*)w)[i], two ? ((const float*)w)[next] : 0.0f)
-               : pack2(to_f32(((const T*)w)[i]), two ? to_f32(((const T*)w)[next]) : 0.0f);
-  } else if (f32) {
-    const Pack<float, V> q = load_pack<float, V>((const float*)w + i);
-#pragma unroll
-    for (int e = 0; e < V / 2; ++e) v[e] = pair_of(q, 2 * e);
-  } else {
-    const Pack<T, V> q = load_pack<T, V>((const T*)w + i);
-#pragma unroll
-    for (int e = 0; e < V / 2; ++e) v[e] = pair_of(q, 2 * e);
-  }
-}
+template <typename T>
+constexpr int kStages = sizeof(T) == 4 ? 2 : 4;
 
-// Rows under way at once, in shared memory; a thread reads what it copied itself.
-// Pieces of less than four bytes go to registers.
-template <typename T, int V, int NV, int TPR>
-struct BlockRing {
-  static constexpr int piece = V * sizeof(T);
-  static constexpr bool used = piece >= 4;
-  static constexpr int threads = TPR == 32 ? 256 : TPR;
-  static constexpr int array_bytes = NV * threads * piece;
-  static constexpr int stage_bytes = 5 * array_bytes;  // x, o, dr, du, gate
-  // 512 threads an SM (in one block or more): 160 KB of its shared memory
-  static constexpr int stages = sizeof(T) == 4 ? 2 : 4;
-  static constexpr int bytes = used ? stages * stage_bytes : 0;
-};
-
-template <typename T, int V, int NV, int TPR, int CL, bool BIAS, int EACH>
+template <typename T, int V, int NV, int TPR, int CL, bool BIAS, bool VALUES, int EACH>
 __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, EACH)
 k_block_norm_bwd(const __grid_constant__ BlockNorm a) {
-  using R = BlockRing<T, V, NV, TPR>;
-  constexpr int ROWS = TPR == 32 ? 8 : 1, E = NV * V, H = E / 2, STEP = TPR * V, S = R::stages;
-  // Pairs of a piece; where pieces are single values, of two of them (G groups).
-  constexpr int HV = V == 1 ? 1 : V / 2, G = V == 1 ? NV / 2 : NV, BLOCK = R::threads;
-  constexpr int GSTEP = V == 1 ? 2 * STEP : STEP;
-  static_assert(E == 8, "columns of a thread");
+  using C = Columns<T, V, NV, TPR>;
+  using R = BlockRing<T, V, NV, TPR, VALUES ? 5 : 4, kStages<T>>;
+  constexpr int ROWS = TPR == 32 ? 8 : 1, G = C::G, HV = C::HV, H = C::H, S = R::stages;
+  constexpr int BLOCK = R::threads;
+  static_assert(C::E == 8, "columns of a thread");
+  enum { X, O, DR, DU, GATE };
   extern __shared__ uint4 ring_bytes[];
-  char* ring = reinterpret_cast<char*>(ring_bytes);
   __shared__ float red[4 * (TPR / 32)];
   __shared__ float4 stats[S][BLOCK / 32];
   __shared__ float2 shared_sums[2][8];
   const uint32_t lane = threadIdx.x % TPR, warp = threadIdx.x / 32;
   const uint32_t part = CL > 1 ? cluster_rank() : 0, team = blockIdx.x / CL;
-  const uint32_t teams = gridDim.x / CL;
-  const uint32_t c0 = part * (TPR * E) + lane * V;
-  const int left = (int)a.n - (int)c0;
-  const bool units = a.gate == PLX_BLOCK_GATE_UNITS, values = a.gate == PLX_BLOCK_GATE_VALUES;
-  enum { X, O, DR, DU, GATE };
-  auto slot = [&](uint32_t stage, int array, int j) {
-    char* at = ring + stage * R::stage_bytes + array * R::array_bytes;
-    return reinterpret_cast<Pack<T, V>*>(at) + j * BLOCK + threadIdx.x;
-  };
-  Pack<T, V> held[R::used ? 1 : 5][NV];  // a row's values, where no ring has them
-  const T* from[5] = {(const T*)a.x, (const T*)a.o, (const T*)a.dr, (const T*)a.du,
-                      values ? (const T*)a.gate_values : nullptr};
-  const int64_t ld[5] = {a.ldx, a.ldo, a.lddr, a.lddu, a.ldg};
-  const uint32_t step = teams * ROWS;
+  const uint32_t step = gridDim.x / CL * ROWS;
+  const C c(a.n, part * (TPR * C::E) + lane * V);
   uint32_t r = team * ROWS + threadIdx.x / TPR;
-  auto fetch = [&](uint64_t row, uint32_t stage) {
-    if (row < a.rows) {
-      if constexpr (R::used) {
-#pragma unroll
-        for (int k = 0; k < 5; ++k)
-          if (from[k])
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-              if (j * STEP < left)
-                copy_async<R::piece>(slot(stage, k, j), from[k] + (int64_t)row * ld[k] + c0 + j * STEP);
-      }
-      if ((threadIdx.x & 31) == 0) copy_async<16>(&stats[stage][warp], a.stats + row);
-    }
+  R ring;
+  ring.ring = reinterpret_cast<char*>(ring_bytes);
+  auto array = [&](int k, const void* p, int64_t ld) {
+    ring.from[k] = p ? (const T*)p + (int64_t)r * ld + c.c0 : nullptr;
+    ring.step[k] = step * ld;
+  };
+  array(X, a.x, a.ldx);
+  array(O, a.o, a.ldo);
+  array(DR, a.dr, a.lddr);
+  array(DU, a.du, a.lddu);
+  if constexpr (VALUES) array(GATE, a.gate_values, a.ldg);
+  ring.clear(c);
+  const float4* from_stats = a.stats + r;
+  auto fetch = [&](bool there, uint32_t stage) {
+    if constexpr (R::used) ring.fetch(c, there, stage);
+    if (there && (threadIdx.x & 31) == 0) copy_async<16>(&stats[stage][warp], from_stats);
+    from_stats += step;
     copy_commit();
   };
-  // Columns past the row's end, and arrays that are not given, are 0.
-  Pack<T, V> zero;
+  const F2 none = pack2(0.0f, 0.0f);
+  F2 w1[H], w2[H], b1[BIAS ? H : 1], gate[VALUES ? 1 : H];
+  c.param(a.post_weight, a.param_f32, w1, 1.0f);
+  c.param(a.pre_weight, a.param_f32, w2, 1.0f);
+  if constexpr (BIAS) c.param(a.post_bias, a.param_f32, b1, 0.0f);
+  if constexpr (!VALUES) {
+    c.param(a.gate == PLX_BLOCK_GATE_UNITS ? a.gate_values : nullptr, a.param_f32, gate, 1.0f);
+    if (a.gate == PLX_BLOCK_GATE_UNITS && a.sigmoid)
 #pragma unroll
-  for (int e = 0; e < V; ++e) zero.v[e] = from_f32<T>(0.0f);
-  if constexpr (R::used) {
-    for (int s = 0; s < S; ++s)
-      for (int k = 0; k < 5; ++k)
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-          if (!from[k] || j * STEP >= left) *slot(s, k, j) = zero;
+      for (int h = 0; h < H; ++h) gate[h] = pack2(sigmoid(gate[h].x).a, sigmoid(gate[h].y).a);
   }
-  uint32_t stage = 0;
-  // Pairs of values of group j of an array of the row under way.
-  auto get = [&](int array, int j, F2 (&v)[HV]) {
-    auto piece = [&](int k) {
-      if constexpr (R::used) return *slot(stage, array, k);
-      else return held[array][k];
-    };
-    if constexpr (V == 1) {
-      v[0] = pack2(to_f32(piece(2 * j).v[0]), to_f32(piece(2 * j + 1).v[0]));
-    } else {
-      const Pack<T, V> q = piece(j);
-#pragma unroll
-      for (int e = 0; e < HV; ++e) v[e] = pair_of(q, 2 * e);
-    }
-  };
-  auto put = [&](void* array, int64_t lda, uint32_t row, int j, const F2 (&v)[HV]) {
-    T* to = (T*)array + (int64_t)row * lda + c0 + j * GSTEP;
-    if constexpr (V == 1) {
-      to[0] = from_f32<T>(v[0].x);
-      if (j * GSTEP + STEP < left) to[STEP] = from_f32<T>(v[0].y);
-    } else {
-      Pack<T, V> q;
-#pragma unroll
-      for (int e = 0; e < HV; ++e) put_pair(q, 2 * e, v[e]);
-      *reinterpret_cast<Pack<T, V>*>(to) = q;
-    }
-  };
-  auto param = [&](const void* w, int j, F2 (&v)[HV]) {
-    const uint32_t i = c0 + j * GSTEP;
-    param_pairs<T, V>(w, a.param_f32, i, i + STEP, a.n, v);
-  };
-  const F2 none = pack2(0.0f, 0.0f), ones = pack2(1.0f, 1.0f);
-  // A piece's gate and its derivative.
-  auto gate_of = [&](int j, F2 (&g)[HV], F2 (&slope)[HV]) {
-    if (units) param(a.gate_values, j, g);
-    else if (values) get(GATE, j, g);
-    else
-#pragma unroll
-      for (int e = 0; e < HV; ++e) g[e] = ones;
-#pragma unroll
-    for (int e = 0; e < HV; ++e) {
-      slope[e] = ones;
-      if (a.sigmoid) {
-        const Sigmoid s = sigmoid(g[e].x), t = sigmoid(g[e].y);
-        g[e] = pack2(s.a, t.a);
-        slope[e] = pack2(s.a * s.keep, t.a * t.keep);
-      }
-    }
-  };
   int turn = 0, turn2 = 0;
   // Two sums over the row.
-  auto sums_of = [&](F2 c) {
-    F2 s = row_sum2<TPR>(c, red, turn);
+  auto sums_of = [&](F2 v) {
+    F2 s = row_sum2<TPR>(v, red, turn);
     if constexpr (CL > 1) {
       if (threadIdx.x < CL) st_peer(peer_smem(&shared_sums[turn2][part], threadIdx.x), s);
       cluster_barrier();
@@ -185,156 +96,156 @@ k_block_norm_bwd(const __grid_constant__ BlockNorm a) {
     }
     return s;
   };
-  constexpr int HT = G * HV;  // pairs of a thread
-  F2 w2sum[HT], w1sum[HT], gsum[HT], b2sum[BIAS ? HT : 1], b1sum[BIAS ? HT : 1];
+  F2 w2sum[H], w1sum[H], gsum[VALUES ? 1 : H], b2sum[BIAS ? H : 1], b1sum[BIAS ? H : 1];
 #pragma unroll
-  for (int h = 0; h < HT; ++h) {
-    w2sum[h] = w1sum[h] = gsum[h] = none;
-    if (BIAS) b2sum[h] = b1sum[h] = none;
+  for (int h = 0; h < H; ++h) {
+    w2sum[h] = w1sum[h] = none;
+    if constexpr (!VALUES) gsum[h] = none;
+    if constexpr (BIAS) b2sum[h] = b1sum[h] = none;
   }
+  T* to_x = (T*)a.dx + (int64_t)r * a.lddx + c.c0;
+  T* to_o = (T*)a.d_o + (int64_t)r * a.lddo + c.c0;
+  T* to_g = VALUES && a.dgate ? (T*)a.dgate + (int64_t)r * a.lddg + c.c0 : nullptr;
+  const F2 scale = pack2(a.scale, a.scale);
+  uint32_t stage = 0;
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s) fetch(r + (uint64_t)s * step, s);
+  for (int s = 0; s < S - 1; ++s) fetch(r + (uint64_t)s * step < a.rows, s);
   for (; r < a.rows; r += step) {
     copy_wait<S - 2>();
     __syncwarp();
-    fetch(r + (uint64_t)(S - 1) * step, stage == 0 ? S - 1 : stage - 1);
-    if constexpr (!R::used) {
-#pragma unroll
-      for (int k = 0; k < 5; ++k)
-        if (from[k]) load_row<STEP>(from[k] + (int64_t)r * ld[k] + c0, left, held[k]);
-        else
-#pragma unroll
-          for (int j = 0; j < NV; ++j) held[k][j] = zero;
-    }
-    const float4 st = stats[stage][warp];
+    fetch(r + (uint64_t)(S - 1) * step < a.rows, stage == 0 ? S - 1 : stage - 1);
+    if constexpr (!R::used) ring.fetch(c, true, 0);
+    float4 st = stats[stage][warp];
+    if (!a.post) st.x = 0.0f, st.y = 1.0f;  // h1 is o
     const F2 m1 = pack2(-st.x, -st.x), s1 = pack2(st.y, st.y);
     const F2 m2 = pack2(-st.z, -st.z), s2 = pack2(st.w, st.w);
-    const F2 scale = pack2(a.scale, a.scale);
-    F2 h1[HT], h2[HT], d[HT], c0s = none, c1s = none;
+    F2 h1[H], h2[H], d[H], c0 = none, c1 = none;
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-      if (j * GSTEP >= left) {
+    for (int g = 0; g < G; ++g) {
+      F2 x[HV], o[HV], du[HV], gv[HV];
+      ring.get(stage, X, g, x);
+      ring.get(stage, O, g, o);
+      ring.get(stage, DU, g, du);
+      if constexpr (VALUES) {
+        ring.get(stage, GATE, g, gv);
+        if (a.sigmoid)
 #pragma unroll
-        for (int e = 0; e < HV; ++e) h1[j * HV + e] = h2[j * HV + e] = d[j * HV + e] = none;
-        continue;
+          for (int e = 0; e < HV; ++e) gv[e] = pack2(sigmoid(gv[e].x).a, sigmoid(gv[e].y).a);
       }
-      F2 x[HV], p[HV], g[HV], slope[HV], w[HV];
-      get(X, j, x);
-      get(O, j, p);
-      if (a.post) {
-#pragma unroll
-        for (int e = 0; e < HV; ++e) p[e] = mul2(add2(p[e], m1), s1);
-      }
-#pragma unroll
-      for (int e = 0; e < HV; ++e) h1[j * HV + e] = p[e];
-      if (a.post_weight) {
-        param(a.post_weight, j, w);
-#pragma unroll
-        for (int e = 0; e < HV; ++e) p[e] = mul2(p[e], w[e]);
-      }
-      if (BIAS && a.post_bias) {
-        param(a.post_bias, j, w);
-#pragma unroll
-        for (int e = 0; e < HV; ++e) p[e] = add2(p[e], w[e]);
-      }
-      gate_of(j, g, slope);
-      F2 du[HV];
-      get(DU, j, du);
-      if (a.pre_weight) param(a.pre_weight, j, w);
 #pragma unroll
       for (int e = 0; e < HV; ++e) {
-        const int h = j * HV + e;
-        const F2 rv = fma2(g[e], p[e], mul2(scale, x[e]));
+        const int h = g * HV + e;
+        h1[h] = mul2(add2(o[e], m1), s1);
+        F2 p = mul2(h1[h], w1[h]);
+        if constexpr (BIAS) p = add2(p, b1[h]);
+        const F2 rv = fma2(VALUES ? gv[e] : gate[VALUES ? 0 : h], p, mul2(scale, x[e]));
         h2[h] = mul2(add2(rv, m2), s2);
         w2sum[h] = fma2(du[e], h2[h], w2sum[h]);
-        if (BIAS) b2sum[h] = add2(b2sum[h], du[e]);
-        d[h] = a.pre_weight ? mul2(du[e], w[e]) : du[e];
-        c0s = add2(c0s, d[h]);
-        c1s = fma2(d[h], h2[h], c1s);
+        if constexpr (BIAS) b2sum[h] = add2(b2sum[h], du[e]);
+        d[h] = mul2(du[e], w2[h]);
+        c0 = add2(c0, d[h]);
+        c1 = fma2(d[h], h2[h], c1);
       }
     }
     if (a.du) {
-      const F2 c = sums_of(pack2(c0s.x + c0s.y, c1s.x + c1s.y));
+      const F2 c = sums_of(pack2(c0.x + c0.y, c1.x + c1.y));
       const float e0 = a.layer ? -c.x * a.inv_n : 0.0f, e1 = -c.y * a.inv_n;
       const F2 e02 = pack2(e0, e0), e12 = pack2(e1, e1);
 #pragma unroll
-      for (int h = 0; h < HT; ++h) d[h] = mul2(s2, fma2(h2[h], e12, add2(d[h], e02)));
+      for (int h = 0; h < H; ++h) d[h] = mul2(s2, fma2(h2[h], e12, add2(d[h], e02)));
     }
-    c0s = c1s = none;
+    c0 = c1 = none;
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-      if (j * GSTEP >= left) {
+    for (int g = 0; g < G; ++g) {
+      F2 dr[HV], gv[HV], out[HV], slope[HV];
+      ring.get(stage, DR, g, dr);
+      if constexpr (VALUES) {
+        ring.get(stage, GATE, g, gv);
 #pragma unroll
-        for (int e = 0; e < HV; ++e) d[j * HV + e] = none;
-        continue;
+        for (int e = 0; e < HV; ++e) slope[e] = pack2(1.0f, 1.0f);
+        if (a.sigmoid)
+#pragma unroll
+          for (int e = 0; e < HV; ++e) {
+            const Sigmoid s = sigmoid(gv[e].x), t = sigmoid(gv[e].y);
+            gv[e] = pack2(s.a, t.a);
+            slope[e] = pack2(s.a * s.keep, t.a * t.keep);
+          }
       }
-      F2 dr[HV], p[HV], g[HV], slope[HV], w[HV], out[HV];
-      get(DR, j, dr);
-      gate_of(j, g, slope);
-      if (a.post_weight) param(a.post_weight, j, w);
+      const bool in = c.in(g);
 #pragma unroll
       for (int e = 0; e < HV; ++e) {
-        const int h = j * HV + e;
+        const int h = g * HV + e;
         d[h] = add2(d[h], dr[e]);
-        if (V == 1 && j * GSTEP + STEP >= left) d[h].y = 0.0f;
-        p[e] = a.post_weight ? mul2(h1[h], w[e]) : h1[h];
+        if (!in) d[h] = none;  // columns past the row's end have no part in what follows
+        if (V == 1 && !c.both(g)) d[h].y = 0.0f;
         out[e] = mul2(scale, d[h]);
       }
-      put(a.dx, a.lddx, r, j, out);
-      if (BIAS && a.post_bias) {
-        F2 b[HV];
-        param(a.post_bias, j, b);
-#pragma unroll
-        for (int e = 0; e < HV; ++e) p[e] = add2(p[e], b[e]);
-      }
+      if (in) c.put(to_x, g, out);
 #pragma unroll
       for (int e = 0; e < HV; ++e) {
-        const int h = j * HV + e;
-        out[e] = mul2(mul2(d[h], p[e]), slope[e]);
-        gsum[h] = add2(gsum[h], out[e]);
-        F2 dp = mul2(d[h], g[e]);
+        const int h = g * HV + e;
+        F2 p = mul2(h1[h], w1[h]);
+        if constexpr (BIAS) p = add2(p, b1[h]);
+        if constexpr (VALUES) out[e] = mul2(mul2(d[h], p), slope[e]);
+        else gsum[h] = fma2(d[h], p, gsum[h]);
+        const F2 dp = mul2(d[h], VALUES ? gv[e] : gate[VALUES ? 0 : h]);
         w1sum[h] = fma2(dp, h1[h], w1sum[h]);
-        if (BIAS) b1sum[h] = add2(b1sum[h], dp);
-        if (a.post_weight) dp = mul2(dp, w[e]);
-        d[h] = dp;
-        c0s = add2(c0s, dp);
-        c1s = fma2(dp, h1[h], c1s);
+        if constexpr (BIAS) b1sum[h] = add2(b1sum[h], dp);
+        d[h] = mul2(dp, w1[h]);
+        c0 = add2(c0, d[h]);
+        c1 = fma2(d[h], h1[h], c1);
       }
-      if (a.dgate) put(a.dgate, a.lddg, r, j, out);
+      if constexpr (VALUES) {
+        if (in && to_g) c.put(to_g, g, out);
+      }
     }
     if (a.post) {
-      const F2 c = sums_of(pack2(c0s.x + c0s.y, c1s.x + c1s.y));
+      const F2 c = sums_of(pack2(c0.x + c0.y, c1.x + c1.y));
       const float e0 = a.layer ? -c.x * a.inv_n : 0.0f, e1 = -c.y * a.inv_n;
       const F2 e02 = pack2(e0, e0), e12 = pack2(e1, e1);
 #pragma unroll
-      for (int h = 0; h < HT; ++h) d[h] = mul2(s1, fma2(h1[h], e12, add2(d[h], e02)));
+      for (int h = 0; h < H; ++h) d[h] = mul2(s1, fma2(h1[h], e12, add2(d[h], e02)));
     }
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-      if (j * GSTEP >= left) continue;
+    for (int g = 0; g < G; ++g) {
       F2 out[HV];
 #pragma unroll
-      for (int e = 0; e < HV; ++e) out[e] = d[j * HV + e];
-      put(a.d_o, a.lddo, r, j, out);
+      for (int e = 0; e < HV; ++e) out[e] = d[g * HV + e];
+      if (c.in(g)) c.put(to_o, g, out);
     }
+    to_x += step * a.lddx;
+    to_o += step * a.lddo;
+    if (to_g) to_g += step * a.lddg;
     stage = stage == S - 1 ? 0 : stage + 1;
   }
   if constexpr (CL > 1) cluster_barrier();  // nobody writes to a block that has gone
   if (!a.partial) return;
+  if constexpr (!VALUES) {  // the derivative of the gate, once
+    if (a.gate == PLX_BLOCK_GATE_UNITS && a.sigmoid) {
+      F2 raw[H];
+      c.param(a.gate_values, a.param_f32, raw, 0.0f);
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const Sigmoid s = sigmoid(raw[h].x), t = sigmoid(raw[h].y);
+        gsum[h] = mul2(gsum[h], pack2(s.a * s.keep, t.a * t.keep));
+      }
+    }
+  }
   float* out = a.partial + (uint64_t)team * kSums * a.n;
+  constexpr int K = BIAS ? 5 : 3, STEP = C::STEP;
   auto column = [&](int k, int e) {  // of value e of the thread
     const int h = e / 2;
-    F2 v = k == 0 ? w2sum[h] : k == 1 ? w1sum[h] : gsum[h];
-    if (k > 2) v = BIAS ? (k == 3 ? b2sum[h] : b1sum[h]) : none;
+    F2 v = k == 0 ? w2sum[h] : k == 1 ? w1sum[h] : VALUES ? none : gsum[VALUES ? 0 : h];
+    if (k > 2) v = BIAS ? (k == 3 ? b2sum[BIAS ? h : 0] : b1sum[BIAS ? h : 0]) : none;
     return e % 2 ? v.y : v.x;
   };
   if constexpr (ROWS == 1) {
 #pragma unroll
-    for (int k = 0; k < (BIAS ? 5 : 3); ++k)
+    for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (j * STEP >= left) continue;
-        float* to = out + (uint64_t)k * a.n + c0 + j * STEP;
+        if (j * STEP >= c.left) continue;
+        float* to = out + (uint64_t)k * a.n + c.c0 + j * STEP;
         if constexpr (V >= 4) {  // n and the columns are multiples of four
 #pragma unroll
           for (int e = 0; e < V; e += 4)
@@ -347,9 +258,9 @@ k_block_norm_bwd(const __grid_constant__ BlockNorm a) {
         }
       }
   } else {  // the eight warps' sums, added in their order
-    __shared__ float joined[8][32 * E];
+    __shared__ float joined[8][32 * C::E];
 #pragma unroll
-    for (int k = 0; k < (BIAS ? 5 : 3); ++k) {
+    for (int k = 0; k < K; ++k) {
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < NV; ++j)
@@ -559,9 +470,11 @@ extern "C" int plx_block_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
         constexpr int VV = decltype(v_c)::value, NV = decltype(nv_c)::value;
         constexpr int TPR = decltype(tpr_c)::value, CL = decltype(cl_c)::value;
         constexpr int EACH = decltype(each_c)::value;
-        using R = BlockRing<T, VV, NV, TPR>;
-        auto with = [&](auto bias_c) -> int {
-          constexpr auto kernel = k_block_norm_bwd<T, VV, NV, TPR, CL, decltype(bias_c)::value, EACH>;
+        auto with = [&](auto bias_c, auto values_c) -> int {
+          constexpr bool VALUES = decltype(values_c)::value;
+          using R = BlockRing<T, VV, NV, TPR, VALUES ? 5 : 4, kStages<T>>;
+          constexpr auto kernel =
+              k_block_norm_bwd<T, VV, NV, TPR, CL, decltype(bias_c)::value, VALUES, EACH>;
           groups = groups_of(rows, TPR == 32 ? 8 : 1, kSms * EACH / CL);
           if (groups == 0) return PLX_OK;
           if (R::bytes > 32 * 1024) PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, R::bytes));
@@ -579,9 +492,14 @@ extern "C" int plx_block_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
           PLX_TRY_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const BlockNorm)a));
           return PLX_OK;
         };
+        using Yes = std::true_type;
+        using No = std::false_type;
+        const bool values = a.gate == PLX_BLOCK_GATE_VALUES;
         // Sums of biases where they are asked for (or biases to be applied).
-        rc = outs.out[3] || outs.out[4] || a.post_bias ? with(std::true_type{})
-                                                       : with(std::false_type{});
+        if (outs.out[3] || outs.out[4] || a.post_bias)
+          rc = values ? with(Yes{}, Yes{}) : with(Yes{}, No{});
+        else
+          rc = values ? with(No{}, Yes{}) : with(No{}, No{});
       };
       auto loops = [&] {
         if (!rows) return;
