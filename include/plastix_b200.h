@@ -704,7 +704,8 @@ int plx_distill(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* 
 
 /* Scratch of plx_dense, or (backward not 0) of plx_dense_backward; aligned: the
  * rows that a call multiplies (x, weight, dy) all start at, and have strides of,
- * multiples of 16 bytes (16-bit rows are copied where they do not). */
+ * multiples of 16 bytes (16-bit rows are copied where they do not, 32-bit ones are
+ * cut into parts unless there are at most eight of them). */
 size_t plx_dense_scratch_bytes(uint64_t rows, uint32_t n, uint32_t m, int dtype, int backward,
                                int aligned);
 

@@ -167,8 +167,8 @@ def dense(ctx: Context, x: torch.Tensor, weight: torch.Tensor,
         if residual is not None:
             _check_result(out, ldy, residual, ldr, "out")
         _check_apart(out, ldy, "out", (x, ldx, "x"), (weight, ldw, "weight"))
-    # aligned rows need no scratch
-    size = 0 if _aligned((x, ldx, rows), (weight, ldw, m)) else \
+    # aligned rows of 16-bit values need no scratch
+    size = 0 if dtype != _abi.F32 and _aligned((x, ldx, rows), (weight, ldw, m)) else \
         _abi.lib().plx_dense_scratch_bytes(rows, n, m, dtype, 0, 0)
     with _scope(ctx, x, weight, bias, residual, out):
         if out is None:

@@ -1,11 +1,15 @@
 // A fully connected layer on rows, and its gradients.
 //   z = x W^T + b;  y = act(z) + residual
 //   dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = sum over rows of dz
-// Three products over one kernel each (their operands differ in which of their
-// dimensions is contiguous), and one pass that makes dz and the sums of its
+// Products on the tensor cores (product_tensor.cu; the three differ in which of their
+// operands' dimensions is contiguous), and one pass that makes dz and the sums of its
 // columns. z is kept in 32 bits: its rounding would go into every gradient. dz is
-// rounded to the rows' type, which the products take; that is as much as one
+// rounded to 16-bit rows' type, which the products take; that is as much as one
 // rounding of the gradients themselves.
+// 32-bit values are cut into three bfloat16 values whose sum they are, toward zero, so
+// that all have one sign; of the nine products of parts six are made, the others are
+// below 2^-24 of the value's. A part that would be 0 is the first one times 2^-30 or
+// 2^-40, so that an infinity beside it stays one.
 #include "dense.cuh"
 
 namespace plx {
@@ -13,12 +17,42 @@ namespace {
 
 constexpr uint32_t kGroups = 128;  // runs of rows whose column sums are joined
 
+// The three parts of a 32-bit value.
+__device__ __forceinline__ void cut(float v, __nv_bfloat16 (&part)[3]) {
+  auto top = [](float f) { return __uint_as_float(__float_as_uint(f) & 0xffff0000u); };
+  float h = top(v), m, l;
+  if (fabsf(v) < INFINITY) {
+    const float rest = __fsub_rn(v, h);
+    m = top(rest);
+    l = __fsub_rn(rest, m);
+    if (m == 0.0f) m = h * 0x1p-30f;
+    if (l == 0.0f) l = h * 0x1p-40f;
+  } else {
+    h = v != v ? v : h;
+    m = l = copysignf(1.0f, v);
+  }
+  const float p[3] = {h, m, l};
+#pragma unroll
+  for (int k = 0; k < 3; ++k) part[k] = __float2bfloat16_rn(p[k]);
+}
+// Two neighbouring values' parts, to three planes.
+__device__ __forceinline__ void put_parts(__nv_bfloat16* to, int64_t plane, float a, float b) {
+  __nv_bfloat16 x[3], y[3];
+  cut(a, x);
+  cut(b, y);
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+    *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<char*>(to) + k * plane) =
+        __halves2bfloat162(x[k], y[k]);
+}
+
 // dz of one of gridDim.y runs of rows and the sums of its columns: a lane V
 // columns, a warp every eighth row.
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(256)
 k_dense_dz(uint32_t rows, uint32_t m, uint32_t run, const T* dy, int64_t lddy,
-           const float* __restrict__ pre, T* dz, int64_t lddz, float* __restrict__ partial) {
+           const float* __restrict__ pre, void* dz, int64_t lddz, int64_t plane,
+           float* __restrict__ partial) {
   __shared__ float joined[8][32 * V];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t c = (blockIdx.x * 32 + lane) * V;
@@ -32,14 +66,28 @@ k_dense_dz(uint32_t rows, uint32_t m, uint32_t run, const T* dy, int64_t lddy,
       Pack<float, V> z;
       if (ACT != PLX_ACT_IDENTITY) z = load_pack<float, V>(pre + (uint64_t)r * m + c);
       Pack<T, V> out;
+      float d[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        float d = to_f32(g.v[e]);
-        if (ACT != PLX_ACT_IDENTITY) d *= act_slope<ACT>(z.v[e]);
-        sum[e] += d;
-        out.v[e] = from_f32<T>(d);
+        d[e] = to_f32(g.v[e]);
+        if (ACT != PLX_ACT_IDENTITY) d[e] *= act_slope<ACT>(z.v[e]);
+        sum[e] += d[e];
+        out.v[e] = from_f32<T>(d[e]);
       }
-      if (dz) *reinterpret_cast<Pack<T, V>*>(dz + r * lddz + c) = out;
+      if (!dz) continue;
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<Pack<T, V>*>((T*)dz + r * lddz + c) = out;
+      } else if constexpr (V > 1) {
+#pragma unroll
+        for (int e = 0; e < V; e += 2)
+          put_parts((__nv_bfloat16*)dz + r * lddz + c + e, plane, d[e], d[e + 1]);
+      } else {
+        __nv_bfloat16 part[3];
+        cut(d[0], part);
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          *((__nv_bfloat16*)((char*)dz + k * plane) + r * lddz + c) = part[k];
+      }
     }
   if (!partial) return;
 #pragma unroll
@@ -103,34 +151,129 @@ k_dense_pack(uint32_t rows, uint32_t n, const uint16_t* __restrict__ from, int64
   }
 }
 
-bool packed(const void* p, int64_t ld, uint64_t rows, int dtype) {
-  return dtype == PLX_F32 || (aligned16(p) && (rows <= 1 || ld % 8 == 0));
+// 32-bit rows as three planes.
+__global__ void __launch_bounds__(256)
+k_dense_cut(uint32_t rows, uint32_t n, const float* __restrict__ from, int64_t ld,
+            __nv_bfloat16* __restrict__ to, int64_t ldto, int64_t plane) {
+  const uint32_t c = (blockIdx.x * 32 + (threadIdx.x & 31)) * 2;
+  if (c >= n) return;
+  for (uint32_t r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
+    const float* at = from + r * ld + c;
+    put_parts(to + r * ldto + c, plane, at[0], c + 1 < n ? at[1] : 0.0f);
+  }
 }
-// Bytes of a packed copy, whose rows are round_up(n, 8) apart.
-uint64_t pack_bytes(uint64_t rows, uint32_t n) { return round_up(rows * round_up(n, 8) * 2, 256); }
+
+// Few 32-bit rows: R of them against U units a warp, whose lanes share k and add in
+// a fixed order. Reading the weights once bounds it; cutting them would read and write
+// four times as much.
+template <typename P, int R, int U, int V>
+__global__ void __launch_bounds__(256)
+k_dense_few(uint32_t rows, uint32_t n, uint32_t m, const float* __restrict__ x, int64_t ldx,
+            const float* __restrict__ w, int64_t ldw, const __grid_constant__ Finish f) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t u0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * U;
+  if (u0 >= m) return;
+  float acc[R][U];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc[r][u] = 0.0f;
+  const float* wu[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) wu[u] = w + (int64_t)min(u0 + u, m - 1) * ldw;
+#pragma unroll 2
+  for (uint32_t k = lane * V; k < n; k += 32 * V) {
+    Pack<float, V> wv[U], xv[R];
+#pragma unroll
+    for (int u = 0; u < U; ++u) wv[u] = load_pack<float, V>(wu[u] + k);
+#pragma unroll
+    for (int r = 0; r < R; ++r) xv[r] = load_pack<float, V>(x + (r < rows ? r : 0) * ldx + k);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[r][u] = fmaf(xv[r].v[e], wv[u].v[e], acc[r][u]);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float z = warp_sum(acc[r][u]);
+      if (lane || (uint32_t)r >= rows || u0 + u >= m) continue;
+      const uint32_t col = u0 + u;
+      if (f.bias) z += to_f32(((const P*)f.bias)[col]);
+      if (f.pre) f.pre[(uint64_t)r * m + col] = z;
+      float y = z;
+      switch (f.act) {
+        case PLX_ACT_SIGMOID: y = act_value<PLX_ACT_SIGMOID>(z); break;
+        case PLX_ACT_TANH: y = act_value<PLX_ACT_TANH>(z); break;
+        case PLX_ACT_RELU: y = act_value<PLX_ACT_RELU>(z); break;
+        case PLX_ACT_SILU: y = act_value<PLX_ACT_SILU>(z); break;
+        case PLX_ACT_GELU: y = act_value<PLX_ACT_GELU>(z); break;
+        default: break;
+      }
+      if (f.residual) y += ((const float*)f.residual)[r * f.ldr + col];
+      ((float*)f.y)[r * f.ldy + col] = y;
+    }
+}
+constexpr uint32_t kFew = 8;
+
+int few_rows(plx_ctx* ctx, uint32_t rows, uint32_t n, uint32_t m, const float* x, int64_t ldx,
+             const float* w, int64_t ldw, const Finish& f) {
+  const bool wide = n % 4 == 0 && (rows == 1 || ldx % 4 == 0) && (m == 1 || ldw % 4 == 0) &&
+                    aligned16(x) && aligned16(w);
+  auto go = [&](auto r, auto u, auto v) {
+    constexpr int R = decltype(r)::value, U = decltype(u)::value, V = decltype(v)::value;
+    k_dense_few<float, R, U, V><<<(m + 8 * U - 1) / (8 * U), 256, 0, ctx->stream>>>(
+        rows, n, m, x, rows > 1 ? ldx : 0, w, ldw, f);
+    PLX_LAUNCH_CHECK("k_dense_few");
+    return PLX_OK;
+  };
+  using std::integral_constant;
+  auto width = [&](auto r, auto u) {
+    return wide ? go(r, u, integral_constant<int, 4>{}) : go(r, u, integral_constant<int, 1>{});
+  };
+  if (rows == 1) return width(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+  if (rows <= 4) return width(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+  return width(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+}
+
+// 16-bit rows that the tensor copies take as they are.
+bool packed(const void* p, int64_t ld, uint64_t rows, int dtype) {
+  return dtype != PLX_F32 && aligned16(p) && (rows <= 1 || ld % 8 == 0);
+}
+// Bytes of what they are copied or cut to; rows are round_up(n, 8) apart.
+uint64_t plane_bytes(uint64_t rows, uint32_t n) { return round_up(rows * round_up(n, 8) * 2, 256); }
+uint64_t pack_bytes(uint64_t rows, uint32_t n, int dtype) {
+  return plane_bytes(rows, n) * (dtype == PLX_F32 ? 3 : 1);
+}
 
 // Makes rows of values an operand; `at` is where a copy goes, and is moved past it.
 int operand(plx_ctx* ctx, int dtype, const void* p, int64_t ld, uint64_t rows, uint32_t n,
             bool k_major, char** at, Operand* out) {
-  *out = {p, ld, k_major};
-  if (dtype == PLX_F32) return PLX_OK;
+  if (rows <= 1) ld = 0;
   if (packed(p, ld, rows, dtype)) {
-    if (rows <= 1) out->ld = (int64_t)round_up(n, 8);
+    *out = {p, rows <= 1 ? (int64_t)round_up(n, 8) : ld, 0, k_major};
     return PLX_OK;
   }
-  out->p = *at;
-  out->ld = (int64_t)round_up(n, 8);
-  const dim3 grid((n + 255) / 256, (unsigned)std::min<uint64_t>((rows + 7) / 8, 4096));
-  k_dense_pack<<<grid, 256, 0, ctx->stream>>>((uint32_t)rows, n, (const uint16_t*)p, ld,
-                                              (uint16_t*)*at, out->ld);
+  *out = {*at, (int64_t)round_up(n, 8), (int64_t)plane_bytes(rows, n), k_major};
+  const uint32_t each = dtype == PLX_F32 ? 64 : 256;  // columns of a block
+  const dim3 grid((n + each - 1) / each, (unsigned)std::min<uint64_t>((rows + 7) / 8, 4096));
+  if (dtype == PLX_F32)
+    k_dense_cut<<<grid, 256, 0, ctx->stream>>>((uint32_t)rows, n, (const float*)p, ld,
+                                               (__nv_bfloat16*)*at, out->ld, out->plane);
+  else
+    k_dense_pack<<<grid, 256, 0, ctx->stream>>>((uint32_t)rows, n, (const uint16_t*)p, ld,
+                                                (uint16_t*)*at, out->ld);
   PLX_LAUNCH_CHECK("k_dense_pack");
-  *at += pack_bytes(rows, n);
+  *at += pack_bytes(rows, n, dtype);
   return PLX_OK;
 }
 
 int product(plx_ctx* ctx, int dtype, Product p) {
   if (p.rows == 1) p.f.ldy = p.f.ldr = (int64_t)round_up(p.cols, 8);  // strides of one row
-  return dtype == PLX_F32 ? product_f32(ctx, dtype, p) : product_tensor(ctx, dtype, p);
+  return product_tensor(ctx, dtype, p);
 }
 
 // dz and the column sums' groups, at the head of a backward call's scratch.
@@ -138,7 +281,7 @@ struct BackwardScratch {
   uint64_t lddz, dz_bytes, sums_bytes;
   BackwardScratch(uint64_t rows, uint32_t m, int dtype) {
     lddz = round_up(m, 8);
-    dz_bytes = round_up(rows * lddz * dtype_bytes(dtype), 256);
+    dz_bytes = pack_bytes(rows, m, dtype);
     sums_bytes = round_up((uint64_t)kGroups * m * 4, 256);
   }
 };
@@ -156,8 +299,10 @@ extern "C" size_t plx_dense_scratch_bytes(uint64_t rows, uint32_t n, uint32_t m,
     const BackwardScratch s(rows, m, dtype);
     bytes = s.dz_bytes + s.sums_bytes;
   }
-  if (!aligned && dtype != PLX_F32)
-    bytes += pack_bytes(rows, n) + pack_bytes(m, n) + (backward ? pack_bytes(rows, m) : 0);
+  if (dtype == PLX_F32 && !backward && rows <= kFew) return 0;
+  if (!aligned || dtype == PLX_F32)
+    bytes += pack_bytes(rows, n, dtype) + pack_bytes(m, n, dtype) +
+             (backward && dtype != PLX_F32 ? pack_bytes(rows, m, dtype) : 0);
   return bytes;
 }
 
@@ -185,6 +330,9 @@ extern "C" int plx_dense(plx_ctx* ctx, uint64_t rows, uint32_t n, uint32_t m, in
   if (int rc = check_aligned(4, {pre})) return rc;
   DeviceGuard guard(ctx->device);
   PLX_TRY_CUDA(guard.err);
+  const Finish f = {param_dtype, act, bias, residual, ldr, y, ldy, pre};
+  if (dtype == PLX_F32 && rows <= kFew)
+    return few_rows(ctx, (uint32_t)rows, n, m, (const float*)x, ldx, (const float*)weight, ldw, f);
   Product p = {};
   p.rows = (uint32_t)rows;
   p.cols = m;
@@ -192,7 +340,7 @@ extern "C" int plx_dense(plx_ctx* ctx, uint64_t rows, uint32_t n, uint32_t m, in
   char* at = (char*)scratch;
   if (int rc = operand(ctx, dtype, x, ldx, rows, n, true, &at, &p.a)) return rc;
   if (int rc = operand(ctx, dtype, weight, ldw, m, n, true, &at, &p.b)) return rc;
-  p.f = {param_dtype, act, bias, residual, ldr, y, ldy, pre};
+  p.f = f;
   return product(ctx, dtype, p);
 }
 
@@ -242,7 +390,8 @@ extern "C" int plx_dense_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, uint3
           constexpr int V = decltype(v_c)::value;
           k_dense_dz<T, V, ACT><<<dim3((m + 32 * V - 1) / (32 * V), groups), 256, 0, ctx->stream>>>(
               (uint32_t)rows, m, run, (const T*)dy, rows > 1 ? lddy : 0, pre,
-              own ? (T*)dz : nullptr, (int64_t)s.lddz, dbias ? partial : nullptr);
+              own ? dz : nullptr, (int64_t)s.lddz, (int64_t)plane_bytes(rows, m),
+              dbias ? partial : nullptr);
         };
         const bool wide = m % W == 0 && (rows == 1 || lddy % W == 0) && aligned16(dy) &&
                           (ACT == PLX_ACT_IDENTITY || aligned16(pre));
@@ -264,9 +413,12 @@ extern "C" int plx_dense_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, uint3
     if (int rc = param_dtype == PLX_F32 ? join(float{}) : with_dtype(dtype, join)) return rc;
   }
   char* at = (char*)scratch + s.dz_bytes + s.sums_bytes;
-  Operand d = {dz, (int64_t)s.lddz, true};
-  if (!own && rows && (dx || dweight))
-    if (int rc = operand(ctx, dtype, dy, lddy, rows, m, true, &at, &d)) return rc;
+  Operand d = {dz, (int64_t)s.lddz, (int64_t)plane_bytes(rows, m), true};
+  if (!own && rows && (dx || dweight)) {
+    char* to = dtype == PLX_F32 ? (char*)dz : at;  // parts take dz's place
+    if (int rc = operand(ctx, dtype, dy, lddy, rows, m, true, &to, &d)) return rc;
+    if (dtype != PLX_F32) at = to;
+  }
   if (dx && rows) {
     Product p = {};
     p.rows = (uint32_t)rows;

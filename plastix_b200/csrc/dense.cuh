@@ -99,10 +99,11 @@ int with_act(int act, F f) {
 }
 
 // One operand of a product over k: value (i, k) is p[i * ld + k] (k_major) or
-// p[k * ld + i].
+// p[k * ld + i]. 32-bit values come as three planes of bfloat16 whose sum they are,
+// `plane` bytes apart.
 struct Operand {
   const void* p;
-  int64_t ld;
+  int64_t ld, plane;
   bool k_major;
 };
 
@@ -124,8 +125,8 @@ struct Product {
   Finish f;
 };
 
-int product_f32(plx_ctx* ctx, int dtype, const Product& p);
-// 16-bit types; operands start at, and have strides of, multiples of 16 bytes.
+// Operands start at, and have strides of, multiples of 16 bytes; residual and result
+// are of type dtype.
 int product_tensor(plx_ctx* ctx, int dtype, const Product& p);
 
 }  // namespace plx

@@ -1,4 +1,7 @@
-// Products of 16-bit rows and weights on the tensor cores.
+// Products of rows and weights on the tensor cores. 32-bit values come as three
+// planes of 16 bits each (dense.cu), and the six products of planes that matter are
+// added one after the other, the small ones first: as exact as multiply-adds in 32
+// bits.
 //
 // Bound by the products (large calls) or by reading the weights (few rows). A
 // block makes tiles of 128 x BN sums: one thread has tensor copies fill a ring of
@@ -43,9 +46,9 @@ struct Stages {
 };
 
 struct TensorProduct {
-  CUtensorMap a, b;  // a has the tile's 128
+  CUtensorMap a[3], b[3];  // a has the tile's 128; planes of 32-bit values
+  uint32_t segments;       // products of planes: 1 or 6
   CUtensorMap y, residual, pre;  // where results go by tensor copies
-  bool copied;
   uint32_t rows, cols, depth;  // of the tiles' sides
   uint32_t tiles_a, tiles_b;
   uint32_t kind;
@@ -54,6 +57,9 @@ struct TensorProduct {
   int32_t* status;
   uint64_t timeout_ns;
 };
+
+// The planes of each product, the largest last (one product: the last).
+__device__ __constant__ const uint8_t kPlaneA[6] = {1, 0, 2, 0, 1, 0}, kPlaneB[6] = {1, 2, 0, 1, 0, 0};
 
 // Waits, with a limit, unless another thread of the block has given up.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* gave_up,
@@ -65,11 +71,12 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile ui
   return false;
 }
 
-template <int C>
+template <typename T, int C>
 __device__ __forceinline__ void activate(int act, float (&v)[C]) {
   auto all = [&](auto a) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] = act_value16<decltype(a)::value>(v[i]);
+    for (int i = 0; i < C; ++i)
+      v[i] = sizeof(T) == 2 ? act_value16<decltype(a)::value>(v[i]) : act_value<decltype(a)::value>(v[i]);
   };
   using std::integral_constant;
   switch (act) {
@@ -93,7 +100,7 @@ __device__ __forceinline__ void finish_one(const Finish& f, uint32_t row, uint32
                                            uint32_t cols, float z) {
   float v[1] = {f.bias ? z + bias_at<T>(f, col) : z};
   if (f.pre) f.pre[(uint64_t)row * cols + col] = v[0];
-  activate(f.act, v);
+  activate<T>(f.act, v);
   if (f.residual) v[0] += to_f32(((const T*)f.residual)[(int64_t)row * f.ldr + col]);
   ((T*)f.y)[(int64_t)row * f.ldy + col] = from_f32<T>(v[0]);
 }
@@ -141,7 +148,7 @@ __device__ __forceinline__ void finish_row(const Finish& f, uint32_t row, uint32
         if (col + i < cols) to[i] = v[i];
     }
   }
-  activate(f.act, v);
+  activate<T>(f.act, v);
   T* to = (T*)f.y + (int64_t)row * f.ldy + col;
   const T* res = (const T*)f.residual + (int64_t)row * f.ldr + col;
   if (wide) {
@@ -185,7 +192,7 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
   __shared__ uint64_t full[S::count], empty[S::count], done[2], taken[2];
   __shared__ uint32_t tmem, gave_up;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t blocks = (p.depth + kTileK - 1) / kTileK;
+  const uint32_t one = (p.depth + kTileK - 1) / kTileK, blocks = one * p.segments;
   uint32_t k_first = 0, k_last = blocks, rank = 0, parts = 1;
   uint32_t tile0 = blockIdx.x, step = gridDim.x;
   const uint32_t tiles = p.tiles_a * p.tiles_b;
@@ -251,19 +258,22 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
           if constexpr (TWO) tensor_load_pair(to, map, x, y, bar);
           else tensor_load(to, map, x, y, &full[s]);
         };
-        const int k0 = (int)(k * kTileK);
+        const uint32_t segment = k / one;
+        const int k0 = (int)((k - segment * one) * kTileK);
+        const CUtensorMap* map_a = &p.a[kPlaneA[segment + 6 - p.segments]];
+        const CUtensorMap* map_b = &p.b[kPlaneB[segment + 6 - p.segments]];
         if (p.a_k_major) {
-          load(a, &p.a, k0, a0);
+          load(a, map_a, k0, a0);
         } else {
 #pragma unroll
-          for (uint32_t j = 0; j < kTileA / 64; ++j) load(a + j * 8192, &p.a, a0 + j * 64, k0);
+          for (uint32_t j = 0; j < kTileA / 64; ++j) load(a + j * 8192, map_a, a0 + j * 64, k0);
         }
         if (p.b_k_major) {
-          load(b, &p.b, k0, b0);
+          load(b, map_b, k0, b0);
         } else {
 #pragma unroll
           for (uint32_t j = 0; j < (S::b_rows + 63) / 64; ++j)
-            load(b + j * 8192, &p.b, b0 + j * 64, k0);
+            load(b + j * 8192, map_b, b0 + j * 64, k0);
         }
       }
     }
@@ -303,102 +313,132 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
       const uint32_t half = turn & 1;
       // on a's side
       const uint32_t i = ia * kHigh + (TWO ? rank * kTileA : 0) + quarter * 32 + lane;
-      // Pieces of 64 columns: the residual's are on their way before the sums are done.
-      constexpr uint32_t kChunks = S::pieces ? BN / 128 : 0;
+      // Pieces of 32 rows of 128 bytes go out through shared memory, by tensor copies or
+      // (rows that are no multiples of 16 bytes) row by row. The residual's are on
+      // their way in before the sums are done.
+      constexpr uint32_t kWide = 128 / sizeof(T), kChunks = S::pieces ? BN / 2 / kWide : 0;
+      constexpr uint32_t kHalves = kWide / 32;
       const uint32_t row0 = i - lane, col0 = ib * BN + side * (BN / 2);
-      const bool copied = S::pieces && p.copied;
+      constexpr bool staged = S::pieces > 0;
       auto piece = [&](uint32_t c) { return out + ((warp - 2) * kPieces + c % kPieces) * 4096; };
-      auto there = [&](uint32_t c) { return row0 < p.rows && col0 + c * 64 < p.cols; };
+      auto there = [&](uint32_t c) { return row0 < p.rows && col0 + c * kWide < p.cols; };
       auto fetch = [&](uint32_t c) {  // by one lane, which has stored what was there
         if (!there(c)) return;
         uint64_t* bar = &arrived[warp - 2][c % kPieces];
         mbar_arrive_expect_tx(bar, 4096);
-        tensor_load(piece(c), &p.residual, (int)(col0 + c * 64), (int)row0, bar);
+        tensor_load(piece(c), &p.residual, (int)(col0 + c * kWide), (int)row0, bar);
       };
-      if (copied && p.f.residual && lane == 0) {
+      const bool fetched = staged && wide && p.f.residual;
+      if (fetched && lane == 0) {
         bulk_wait_read<0>();
         for (uint32_t c = 0; c < kChunks && c < kPieces; ++c) fetch(c);
       }
       const bool sound = __all_sync(~0u, wait(&done[half], (turn / 2) & 1, &gave_up, p));
       tmem_fence_after();
       if (!sound && MODE != SPLIT) {
-        if (copied && p.f.residual && lane == 0)  // what is still on its way
+        if (fetched && lane == 0)  // what is still on its way
           for (uint32_t c = 0; c < kChunks && c < kPieces; ++c)
             if (there(c)) mbar_wait_bounded(&arrived[warp - 2][c], arrivals >> c & 1, p.timeout_ns);
         break;
       }
-      if (copied) {
+      if constexpr (staged) {
+        // of this lane's row, the 16-byte chunk k of a piece; and value `col` of a row
+        auto chunk = [&](uint8_t* of, uint32_t k) { return of + lane * 128 + ((k ^ (lane & 7)) << 4); };
+        auto value = [&](auto* of, uint32_t row, uint32_t col) {
+          using Q = std::remove_pointer_t<decltype(of)>;
+          const uint32_t byte = col * sizeof(Q);
+          return reinterpret_cast<Q*>(reinterpret_cast<uint8_t*>(of) + row * 128 +
+                                      (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15));
+        };
+        // Sends a piece out: columns from j0 of rows from row0 of an array.
+        auto send = [&](const CUtensorMap* map, auto* array, int64_t ld, uint32_t j0, uint8_t* of) {
+          using Q = std::remove_pointer_t<decltype(array)>;
+          if (wide) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tensor_store(map, (int)j0, (int)row0, of);
+              bulk_commit();
+            }
+          } else {
+            __syncwarp();
+            const uint32_t rows = min(32u, p.rows - row0);
+            for (uint32_t r = 0; r < rows; ++r)
+              for (uint32_t col = lane; col < 128 / sizeof(Q); col += 32)
+                if (j0 + col < p.cols)
+                  array[(int64_t)(row0 + r) * ld + j0 + col] = *value(reinterpret_cast<Q*>(of), r, col);
+            __syncwarp();
+          }
+        };
 #pragma unroll 1
         for (uint32_t c = 0; c < kChunks; ++c) {
           if (!there(c)) continue;
           uint8_t* at = piece(c);
-          if (p.f.residual) {
+          const uint32_t j1 = col0 + c * kWide;
+          if (fetched) {
             wait(&arrived[warp - 2][c % kPieces], arrivals >> (c % kPieces) & 1, &gave_up, p);
             arrivals ^= 1u << (c % kPieces);
-          } else {
+          } else if (p.f.residual) {
+            const T* res = (const T*)p.f.residual;
+            const uint32_t rows = min(32u, p.rows - row0);
+            for (uint32_t r = 0; r < rows; ++r)
+              for (uint32_t col = lane; col < kWide; col += 32)
+                if (j1 + col < p.cols)
+                  *value(reinterpret_cast<T*>(at), r, col) = res[(int64_t)(row0 + r) * p.f.ldr + j1 + col];
+            __syncwarp();
+          } else if (wide) {
             if (lane == 0) bulk_wait_read<0>();
             __syncwarp();
           }
-          // of this lane's row, the 16-byte chunk k of a piece
-          auto chunk = [&](uint8_t* of, uint32_t k) { return of + lane * 128 + ((k ^ (lane & 7)) << 4); };
 #pragma unroll 1
-          for (uint32_t h = 0; h < 2; ++h) {
+          for (uint32_t h = 0; h < kHalves; ++h) {
             float v[32];
-            tmem_load32(sums + half * BN + (quarter << 21) + side * (BN / 2) + c * 64 + h * 32, v);
-            const uint32_t j0 = col0 + c * 64 + h * 32;
-            const bool whole = j0 + 32 <= p.cols;
-            add_bias<T, 32>(p.f, j0, p.cols, whole, v);
+            tmem_load32(sums + half * BN + (quarter << 21) + side * (BN / 2) + c * kWide + h * 32, v);
+            const uint32_t j0 = j1 + h * 32;
+            add_bias<T, 32>(p.f, j0, p.cols, wide && j0 + 32 <= p.cols, v);
             if (p.f.pre) {
               if (kPieces == 2 && !p.f.residual) {  // the other piece takes it out
                 uint8_t* z = piece(c + 1);
-                if (lane == 0) bulk_wait_read<0>();
-                __syncwarp();
+                if (wide) {
+                  if (lane == 0) bulk_wait_read<0>();
+                  __syncwarp();
+                }
 #pragma unroll
                 for (uint32_t k = 0; k < 8; ++k)
                   *reinterpret_cast<float4*>(chunk(z, k)) =
                       make_float4(v[k * 4], v[k * 4 + 1], v[k * 4 + 2], v[k * 4 + 3]);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0 && j0 < p.cols) {
-                  tensor_store(&p.pre, (int)j0, (int)row0, z);
-                  bulk_commit();
-                }
+                if (j0 < p.cols) send(&p.pre, p.f.pre, (int64_t)p.cols, j0, z);
               } else if (i < p.rows) {
                 float* to = p.f.pre + (uint64_t)i * p.cols + j0;
 #pragma unroll
-                for (uint32_t k = 0; k < 32; k += 4)
-                  if (j0 + k < p.cols)  // a multiple of four
-                    *reinterpret_cast<float4*>(to + k) =
-                        make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                for (uint32_t k = 0; k < 32; ++k)
+                  if (j0 + k < p.cols) to[k] = v[k];
               }
             }
-            activate(p.f.act, v);
+            activate<T>(p.f.act, v);
+            constexpr uint32_t N = 16 / sizeof(T);
 #pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) {
-              auto* q = reinterpret_cast<Pack<T, 8>*>(chunk(at, h * 4 + k));
-              Pack<T, 8> o;
+            for (uint32_t k = 0; k < 32 / N; ++k) {
+              auto* q = reinterpret_cast<Pack<T, N>*>(chunk(at, h * 4 + k));
+              Pack<T, N> o;
               if (p.f.residual) {
                 o = *q;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[k * 8 + e] += to_f32(o.v[e]);
+                for (int e = 0; e < N; ++e) v[k * N + e] += to_f32(o.v[e]);
               }
 #pragma unroll
-              for (int e = 0; e < 8; e += 2) put_pair(o, e, pack2(v[k * 8 + e], v[k * 8 + e + 1]));
+              for (int e = 0; e < N; e += 2) put_pair(o, e, pack2(v[k * N + e], v[k * N + e + 1]));
               *q = o;
             }
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tensor_store(&p.y, (int)(col0 + c * 64), (int)row0, at);
-            bulk_commit();
-            if (kPieces == 1 && p.f.residual && c + 1 < kChunks) {
-              bulk_wait_read<0>();
-              fetch(c + 1);
-            }
+          send(&p.y, (T*)p.f.y, p.f.ldy, j1, at);
+          if (fetched && lane == 0 && c + kPieces < kChunks) {
+            bulk_wait_read<0>();
+            fetch(c + kPieces);
           }
         }
-      } else
+      }
+      if constexpr (!staged)
 #pragma unroll 1
       for (uint32_t c = BN < 32 ? 0 : side * (BN / 2); c < (BN < 32 ? BN : (side + 1) * (BN / 2));
            c += C) {
@@ -480,26 +520,31 @@ template <typename T, int BN, Mode MODE>
 int launch(plx_ctx* ctx, TensorProduct& t, const Product& p, const Operand& a, const Operand& b,
            uint32_t parts, bool wide) {
   using S = Stages<BN, MODE>;
-  constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
+  constexpr bool bf16 = !std::is_same_v<T, __half>;  // what is multiplied
   constexpr uint32_t high = MODE == PAIR ? 2 * kTileA : kTileA;
   t.tiles_a = (t.rows + high - 1) / high;
   t.tiles_b = (t.cols + BN - 1) / BN;
   t.kind = product_kind(bf16, !a.k_major, !b.k_major, high, BN);
-  auto map = [&](CUtensorMap* m, const Operand& o, uint32_t count, uint32_t tile) {
-    return tensor_map(m, bf16 ? PLX_BF16 : PLX_F16, o.p, o.k_major ? t.depth : count,
-                      o.k_major ? count : t.depth, o.ld, 64, o.k_major ? tile : kTileK, true);
-  };
-  if (int rc = map(&t.a, a, t.rows, kTileA)) return rc;
-  if (int rc = map(&t.b, b, t.cols, S::b_rows)) return rc;
-  t.copied = S::pieces && wide;
-  if (t.copied) {
-    const int dtype = bf16 ? PLX_BF16 : PLX_F16;
-    if (int rc = tensor_map(&t.y, dtype, p.f.y, t.cols, t.rows, p.f.ldy, 64, 32, true)) return rc;
-    if (p.f.residual)
-      if (int rc = tensor_map(&t.residual, dtype, p.f.residual, t.cols, t.rows, p.f.ldr, 64, 32, true))
+  auto maps = [&](CUtensorMap (&m)[3], const Operand& o, uint32_t count, uint32_t tile) {
+    for (int plane = 0; plane < (sizeof(T) == 4 ? 3 : 1); ++plane)
+      if (int rc = tensor_map(&m[plane], bf16 ? PLX_BF16 : PLX_F16,
+                              (const char*)o.p + plane * o.plane, o.k_major ? t.depth : count,
+                              o.k_major ? count : t.depth, o.ld, 64, o.k_major ? tile : kTileK, true))
         return rc;
+    return PLX_OK;
+  };
+  if (int rc = maps(t.a, a, t.rows, kTileA)) return rc;
+  if (int rc = maps(t.b, b, t.cols, S::b_rows)) return rc;
+  if (S::pieces && wide) {
+    const int dtype = sizeof(T) == 4 ? PLX_F32 : bf16 ? PLX_BF16 : PLX_F16;
+    auto map = [&](CUtensorMap* m, int of, const void* q, int64_t ld) {
+      return tensor_map(m, of, q, t.cols, t.rows, ld, of == PLX_F32 ? 32 : 64, 32, true);
+    };
+    if (int rc = map(&t.y, dtype, p.f.y, p.f.ldy)) return rc;
+    if (p.f.residual)
+      if (int rc = map(&t.residual, dtype, p.f.residual, p.f.ldr)) return rc;
     if (p.f.pre)
-      if (int rc = tensor_map(&t.pre, PLX_F32, p.f.pre, t.cols, t.rows, t.cols, 32, 32, true)) return rc;
+      if (int rc = map(&t.pre, PLX_F32, p.f.pre, t.cols)) return rc;
   }
   const uint64_t tiles = (uint64_t)t.tiles_a * t.tiles_b;
   if (tiles >= (1ull << 28))
@@ -542,12 +587,14 @@ int product_tensor(plx_ctx* ctx, int dtype, const Product& p) {
   }
   t.a_k_major = a.k_major;
   t.b_k_major = b.k_major;
-  const bool wide = p.f.ldy % 8 == 0 && aligned16(p.f.y) &&
-                    (!p.f.residual || (p.f.ldr % 8 == 0 && aligned16(p.f.residual))) &&
+  const int per = 16 / (int)dtype_bytes(dtype);
+  t.segments = dtype == PLX_F32 ? 6 : 1;
+  const bool wide = p.f.ldy % per == 0 && aligned16(p.f.y) &&
+                    (!p.f.residual || (p.f.ldr % per == 0 && aligned16(p.f.residual))) &&
                     (!p.f.pre || (p.cols % 4 == 0 && aligned16(p.f.pre))) && aligned16(p.f.bias);
   // What the tiles of a width take: rounds of blocks, each with its share of k (in
   // products of 64 values of k by one column; the rest measured).
-  const uint32_t sms = (uint32_t)ctx->num_sms, ks = (p.depth + kTileK - 1) / kTileK;
+  const uint32_t sms = (uint32_t)ctx->num_sms, ks = (p.depth + kTileK - 1) / kTileK * t.segments;
   uint32_t bn = 0, parts = 1;
   bool pair = false;
   double best = 0;
@@ -585,7 +632,7 @@ int product_tensor(plx_ctx* ctx, int dtype, const Product& p) {
       default: return (split ? launch<T, 16, SPLIT> : launch<T, 16, ONE>)(ctx, t, p, a, b, parts, wide);
     }
   };
-  return dtype == PLX_BF16 ? go(__nv_bfloat16{}) : go(__half{});
+  return with_dtype(dtype, go);
 }
 
 }  // namespace plx
