@@ -151,15 +151,23 @@ k_dense_pack(uint32_t rows, uint32_t n, const uint16_t* __restrict__ from, int64
   }
 }
 
-// 32-bit rows as three planes.
+// 32-bit rows as three planes; of two arrays at once.
+struct CutRows {
+  const float* from;
+  int64_t ld;
+  uint32_t rows, n;
+  __nv_bfloat16* to;
+  int64_t ldto, plane;
+};
 __global__ void __launch_bounds__(256)
-k_dense_cut(uint32_t rows, uint32_t n, const float* __restrict__ from, int64_t ld,
-            __nv_bfloat16* __restrict__ to, int64_t ldto, int64_t plane) {
+k_dense_cut(const __grid_constant__ CutRows first, const __grid_constant__ CutRows second) {
+  const CutRows& q = blockIdx.z ? second : first;
   const uint32_t c = (blockIdx.x * 32 + (threadIdx.x & 31)) * 2;
-  if (c >= n) return;
-  for (uint32_t r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
-    const float* at = from + r * ld + c;
-    put_parts(to + r * ldto + c, plane, at[0], c + 1 < n ? at[1] : 0.0f);
+  if (c >= q.n) return;
+#pragma unroll 2
+  for (uint32_t r = blockIdx.y * 8 + (threadIdx.x >> 5); r < q.rows; r += gridDim.y * 8) {
+    const float* at = q.from + r * q.ld + c;
+    put_parts(q.to + r * q.ldto + c, q.plane, at[0], c + 1 < q.n ? at[1] : 0.0f);
   }
 }
 
@@ -250,24 +258,38 @@ uint64_t pack_bytes(uint64_t rows, uint32_t n, int dtype) {
 }
 
 // Makes rows of values an operand; `at` is where a copy goes, and is moved past it.
+// Rows to be cut are noted in `cuts`, for cut_rows.
+struct Cuts {
+  CutRows of[2];
+  int count = 0;
+};
 int operand(plx_ctx* ctx, int dtype, const void* p, int64_t ld, uint64_t rows, uint32_t n,
-            bool k_major, char** at, Operand* out) {
+            bool k_major, char** at, Operand* out, Cuts* cuts) {
   if (rows <= 1) ld = 0;
   if (packed(p, ld, rows, dtype)) {
     *out = {p, rows <= 1 ? (int64_t)round_up(n, 8) : ld, 0, k_major};
     return PLX_OK;
   }
   *out = {*at, (int64_t)round_up(n, 8), (int64_t)plane_bytes(rows, n), k_major};
-  const uint32_t each = dtype == PLX_F32 ? 64 : 256;  // columns of a block
-  const dim3 grid((n + each - 1) / each, (unsigned)std::min<uint64_t>((rows + 7) / 8, 4096));
-  if (dtype == PLX_F32)
-    k_dense_cut<<<grid, 256, 0, ctx->stream>>>((uint32_t)rows, n, (const float*)p, ld,
-                                               (__nv_bfloat16*)*at, out->ld, out->plane);
-  else
+  if (dtype == PLX_F32) {
+    cuts->of[cuts->count++] = {(const float*)p, ld, (uint32_t)rows, n, (__nv_bfloat16*)*at,
+                               out->ld, out->plane};
+  } else {
+    const dim3 grid((n + 255) / 256, (unsigned)std::min<uint64_t>((rows + 7) / 8, 4096));
     k_dense_pack<<<grid, 256, 0, ctx->stream>>>((uint32_t)rows, n, (const uint16_t*)p, ld,
                                                 (uint16_t*)*at, out->ld);
-  PLX_LAUNCH_CHECK("k_dense_pack");
+    PLX_LAUNCH_CHECK("k_dense_pack");
+  }
   *at += pack_bytes(rows, n, dtype);
+  return PLX_OK;
+}
+int cut_rows(plx_ctx* ctx, const Cuts& cuts) {
+  if (!cuts.count) return PLX_OK;
+  const CutRows &a = cuts.of[0], &b = cuts.of[cuts.count - 1];
+  const uint32_t n = std::max(a.n, b.n), rows = std::max(a.rows, b.rows);
+  const dim3 grid((n + 63) / 64, std::min<uint32_t>((rows + 15) / 16, 2048), cuts.count);
+  k_dense_cut<<<grid, 256, 0, ctx->stream>>>(a, b);
+  PLX_LAUNCH_CHECK("k_dense_cut");
   return PLX_OK;
 }
 
@@ -338,8 +360,10 @@ extern "C" int plx_dense(plx_ctx* ctx, uint64_t rows, uint32_t n, uint32_t m, in
   p.cols = m;
   p.depth = n;
   char* at = (char*)scratch;
-  if (int rc = operand(ctx, dtype, x, ldx, rows, n, true, &at, &p.a)) return rc;
-  if (int rc = operand(ctx, dtype, weight, ldw, m, n, true, &at, &p.b)) return rc;
+  Cuts cuts;
+  if (int rc = operand(ctx, dtype, x, ldx, rows, n, true, &at, &p.a, &cuts)) return rc;
+  if (int rc = operand(ctx, dtype, weight, ldw, m, n, true, &at, &p.b, &cuts)) return rc;
+  if (int rc = cut_rows(ctx, cuts)) return rc;
   p.f = f;
   return product(ctx, dtype, p);
 }
@@ -416,16 +440,25 @@ extern "C" int plx_dense_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, uint3
   Operand d = {dz, (int64_t)s.lddz, (int64_t)plane_bytes(rows, m), true};
   if (!own && rows && (dx || dweight)) {
     char* to = dtype == PLX_F32 ? (char*)dz : at;  // parts take dz's place
-    if (int rc = operand(ctx, dtype, dy, lddy, rows, m, true, &to, &d)) return rc;
+    Cuts cuts;
+    if (int rc = operand(ctx, dtype, dy, lddy, rows, m, true, &to, &d, &cuts)) return rc;
+    if (int rc = cut_rows(ctx, cuts)) return rc;
     if (dtype != PLX_F32) at = to;
   }
+  Cuts cuts;
+  Operand w = {}, xs = {};
+  if (dx && rows)
+    if (int rc = operand(ctx, dtype, weight, ldw, m, n, false, &at, &w, &cuts)) return rc;
+  if (dweight && rows)
+    if (int rc = operand(ctx, dtype, x, ldx, rows, n, false, &at, &xs, &cuts)) return rc;
+  if (int rc = cut_rows(ctx, cuts)) return rc;
+  Product p = {};
   if (dx && rows) {
-    Product p = {};
     p.rows = (uint32_t)rows;
     p.cols = n;
     p.depth = m;
     p.a = d;
-    if (int rc = operand(ctx, dtype, weight, ldw, m, n, false, &at, &p.b)) return rc;
+    p.b = w;
     p.f = {dtype, PLX_ACT_IDENTITY, nullptr, nullptr, 0, dx, lddx, nullptr};
     if (int rc = product(ctx, dtype, p)) return rc;
   }
@@ -433,13 +466,12 @@ extern "C" int plx_dense_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, uint3
     PLX_TRY_CUDA(cudaMemset2DAsync(dweight, (size_t)(m > 1 ? lddw : n) * dtype_bytes(dtype), 0,
                                    (size_t)n * dtype_bytes(dtype), m, ctx->stream));
   } else if (dweight) {
-    Product p = {};
     p.rows = m;
     p.cols = n;
     p.depth = (uint32_t)rows;
     d.k_major = false;
     p.a = d;
-    if (int rc = operand(ctx, dtype, x, ldx, rows, n, false, &at, &p.b)) return rc;
+    p.b = xs;
     p.f = {dtype, PLX_ACT_IDENTITY, nullptr, nullptr, 0, dweight, lddw, nullptr};
     if (int rc = product(ctx, dtype, p)) return rc;
   }

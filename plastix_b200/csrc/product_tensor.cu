@@ -1,6 +1,6 @@
 // Products of rows and weights on the tensor cores. 32-bit values come as three
-// planes of 16 bits each (dense.cu), and the six products of planes that matter are
-// added one after the other, the small ones first: as exact as multiply-adds in 32
+// planes of 16 bits each (dense.cu); a stage has all three of both operands, and the
+// six products of planes that matter are made of it: as exact as multiply-adds in 32
 // bits.
 //
 // Bound by the products (large calls) or by reading the weights (few rows). A
@@ -16,6 +16,8 @@
 // of the tile that are its own, in the order of the blocks.
 // Few rows (at most 64) are the tile's second side, so that the first one's 128
 // are units of the layer.
+#include <algorithm>
+
 #include "cluster.cuh"
 #include "dense.cuh"
 #include "tensor.cuh"
@@ -29,25 +31,27 @@ constexpr uint32_t kSmem = 232448;  // a block can have
 
 enum Mode { ONE, SPLIT, PAIR };
 
-template <int BN, Mode MODE>
+template <typename T, int BN, Mode MODE>
 struct Stages {
+  static constexpr uint32_t planes = sizeof(T) == 4 ? 3 : 1;
   static constexpr uint32_t b_rows = MODE == PAIR ? BN / 2 : BN;  // a block's
   static constexpr uint32_t a_bytes = kTileA * kTileK * 2, b_bytes = b_rows * kTileK * 2;
-  static constexpr uint32_t bytes = a_bytes + b_bytes;
+  static constexpr uint32_t bytes = planes * (a_bytes + b_bytes);
   // sums that the blocks of a cluster are sent, of a tile in all
   static constexpr uint32_t sums = MODE == SPLIT ? (BN + 4) * kTileA * 4 : 0;
   // pieces of results (32 rows of 128 bytes) on their way out, of each warp
-  static constexpr uint32_t pieces = MODE == SPLIT || BN < 128 ? 0 : MODE == PAIR ? 2 : 1;
+  static constexpr uint32_t pieces = MODE == SPLIT || BN < 128 ? 0 : MODE == PAIR || sizeof(T) == 2 ? 2 : 1;
+
   static constexpr uint32_t out = pieces * kFinishWarps * 4096;
   static constexpr uint32_t most = (kSmem - 2048 - sums - out) / bytes;
   static constexpr uint32_t count = most < 12 ? most : 12;
+  static_assert(count >= 2, "copies beside products");
   static constexpr uint32_t smem = count * bytes + out + sums + 1024;  // to a multiple of 1,024
   static constexpr uint32_t columns = 2 * BN < 32 ? 32 : 2 * BN;
 };
 
 struct TensorProduct {
   CUtensorMap a[3], b[3];  // a has the tile's 128; planes of 32-bit values
-  uint32_t segments;       // products of planes: 1 or 6
   CUtensorMap y, residual, pre;  // where results go by tensor copies
   uint32_t rows, cols, depth;  // of the tiles' sides
   uint32_t tiles_a, tiles_b;
@@ -57,9 +61,6 @@ struct TensorProduct {
   int32_t* status;
   uint64_t timeout_ns;
 };
-
-// The planes of each product, the largest last (one product: the last).
-__device__ __constant__ const uint8_t kPlaneA[6] = {1, 0, 2, 0, 1, 0}, kPlaneB[6] = {1, 2, 0, 1, 0, 0};
 
 // Waits, with a limit, unless another thread of the block has given up.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* gave_up,
@@ -178,7 +179,7 @@ __device__ __forceinline__ void finish_row(const Finish& f, uint32_t row, uint32
 template <typename T, int BN, Mode MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
-  using S = Stages<BN, MODE>;
+  using S = Stages<T, BN, MODE>;
   constexpr bool TWO = MODE == PAIR;
   constexpr uint32_t C = BN <= 32 ? 16 : 32;  // columns at a time, at most half of a tile's
   static_assert(BN == 16 || BN % (2 * C) == 0, "halves of a tile");
@@ -192,7 +193,7 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
   __shared__ uint64_t full[S::count], empty[S::count], done[2], taken[2];
   __shared__ uint32_t tmem, gave_up;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t one = (p.depth + kTileK - 1) / kTileK, blocks = one * p.segments;
+  const uint32_t blocks = (p.depth + kTileK - 1) / kTileK;
   uint32_t k_first = 0, k_last = blocks, rank = 0, parts = 1;
   uint32_t tile0 = blockIdx.x, step = gridDim.x;
   const uint32_t tiles = p.tiles_a * p.tiles_b;
@@ -209,6 +210,45 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
     tile0 = blockIdx.x / 2;
     step = gridDim.x / 2;
   }
+  // Tiles in groups of eight along a's side, so that what is under way at one
+  // time shares both operands.
+  auto place = [&](uint32_t tile, uint32_t& ia, uint32_t& ib) {
+    const uint32_t group = 8 * p.tiles_b, first = tile / group * 8;
+    const uint32_t size = min(p.tiles_a - first, 8u), in = tile % group;
+    ia = first + in % size;
+    ib = in / size;
+  };
+  // Starts the copies of a stage.
+  auto load_stage = [&](uint32_t s, uint32_t ia, uint32_t ib, uint32_t k) {
+    const int a0 = (int)(ia * kHigh + (TWO ? rank * kTileA : 0));
+    const int b0 = (int)(ib * BN + (TWO ? rank * S::b_rows : 0)), k0 = (int)(k * kTileK);
+    // a pair's first block counts the bytes of both
+    const uint32_t bar = TWO ? peer_smem(&full[s], 0) : 0;
+    if (!TWO || rank == 0) mbar_arrive_expect_tx(&full[s], TWO ? 2 * S::bytes : S::bytes);
+    auto load = [&](uint8_t* to, const CUtensorMap* map, int x, int y) {
+      if constexpr (TWO) tensor_load_pair(to, map, x, y, bar);
+      else tensor_load(to, map, x, y, &full[s]);
+    };
+#pragma unroll
+    for (uint32_t q = 0; q < S::planes; ++q) {
+      uint8_t* a = ring + s * S::bytes + q * S::a_bytes;
+      uint8_t* b = ring + s * S::bytes + S::planes * S::a_bytes + q * S::b_bytes;
+      if (p.a_k_major) {
+        load(a, &p.a[q], k0, a0);
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < kTileA / 64; ++j) load(a + j * 8192, &p.a[q], a0 + j * 64, k0);
+      }
+      if (p.b_k_major) {
+        load(b, &p.b[q], k0, b0);
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < (S::b_rows + 63) / 64; ++j)
+          load(b + j * 8192, &p.b[q], b0 + j * 64, k0);
+      }
+    }
+  };
+  uint32_t early = 0;  // stages of the first tile that are under way before all else is ready
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < S::count; ++s) {
       mbar_init(&full[s], 1);
@@ -222,21 +262,21 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
       for (int i = 0; i < kPieces; ++i) mbar_init(&arrived[w][i], 1);
     mbar_init_fence();
     gave_up = 0;
+    if constexpr (!TWO) {  // (a pair's barriers are not this block's alone)
+      uint32_t ia, ib;
+      place(tile0, ia, ib);
+      for (; early < S::count && k_first + early < k_last; ++early)
+        load_stage(early, ia, ib, k_first + early);
+    }
   }
   if (warp == 1) tmem_alloc<TWO>(&tmem, S::columns);
   tmem_fence_before();
   __syncthreads();
-  if constexpr (MODE != ONE) cluster_barrier();  // the others' barriers are there
+  // the others' barriers and memory are there (SPLIT: by the time that sums are sent)
+  if constexpr (TWO) cluster_barrier();
+  if constexpr (MODE == SPLIT) cluster_arrive();
   tmem_fence_after();
   const uint32_t sums = *(volatile uint32_t*)&tmem;
-  // Tiles in groups of eight along a's side, so that what is under way at one
-  // time shares both operands.
-  auto place = [&](uint32_t tile, uint32_t& ia, uint32_t& ib) {
-    const uint32_t group = 8 * p.tiles_b, first = tile / group * 8;
-    const uint32_t size = min(p.tiles_a - first, 8u), in = tile % group;
-    ia = first + in % size;
-    ib = in / size;
-  };
 
   if (warp == 0 && lane == 0) {  // copies
     uint32_t it = 0;
@@ -244,37 +284,11 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
     for (uint32_t tile = tile0; ok && tile < tiles; tile += step) {
       uint32_t ia, ib;
       place(tile, ia, ib);
-      const int a0 = (int)(ia * kHigh + (TWO ? rank * kTileA : 0));
-      const int b0 = (int)(ib * BN + (TWO ? rank * S::b_rows : 0));
       for (uint32_t k = k_first; k < k_last; ++k, ++it) {
+        if (it < early) continue;
         const uint32_t s = it % S::count;
         if (it >= S::count && !(ok = wait(&empty[s], (it / S::count - 1) & 1, &gave_up, p))) break;
-        uint8_t* a = ring + s * S::bytes;
-        uint8_t* b = a + S::a_bytes;
-        // a pair's first block counts the bytes of both
-        const uint32_t bar = TWO ? peer_smem(&full[s], 0) : 0;
-        if (!TWO || rank == 0) mbar_arrive_expect_tx(&full[s], TWO ? 2 * S::bytes : S::bytes);
-        auto load = [&](uint8_t* to, const CUtensorMap* map, int x, int y) {
-          if constexpr (TWO) tensor_load_pair(to, map, x, y, bar);
-          else tensor_load(to, map, x, y, &full[s]);
-        };
-        const uint32_t segment = k / one;
-        const int k0 = (int)((k - segment * one) * kTileK);
-        const CUtensorMap* map_a = &p.a[kPlaneA[segment + 6 - p.segments]];
-        const CUtensorMap* map_b = &p.b[kPlaneB[segment + 6 - p.segments]];
-        if (p.a_k_major) {
-          load(a, map_a, k0, a0);
-        } else {
-#pragma unroll
-          for (uint32_t j = 0; j < kTileA / 64; ++j) load(a + j * 8192, map_a, a0 + j * 64, k0);
-        }
-        if (p.b_k_major) {
-          load(b, map_b, k0, b0);
-        } else {
-#pragma unroll
-          for (uint32_t j = 0; j < (S::b_rows + 63) / 64; ++j)
-            load(b + j * 8192, map_b, b0 + j * 64, k0);
-        }
+        load_stage(s, ia, ib, k);
       }
     }
     if (!ok && (!TWO || rank == 0))  // what is still on its way
@@ -292,14 +306,22 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
         if (!(ok = wait(&full[s], (it / S::count) & 1, &gave_up, p))) break;
         tmem_fence_after();
         const uint8_t* at = ring + s * S::bytes;
-        const uint64_t a = p.a_k_major ? operand_k_major(at) : operand_i_major(at, 8192);
-        const uint64_t b = p.b_k_major ? operand_k_major(at + S::a_bytes)
-                                       : operand_i_major(at + S::a_bytes, 8192);
         // 16 values of k further on: 32 bytes of a row, or sixteen rows
         const uint32_t da = p.a_k_major ? 2 : 128, db = p.b_k_major ? 2 : 128;
+        // of the planes, the smallest products first
+        constexpr uint32_t kProducts = S::planes == 3 ? 6 : 1;
+        constexpr uint8_t plane_a[6] = {1, 0, 2, 0, 1, 0}, plane_b[6] = {1, 2, 0, 1, 0, 0};
 #pragma unroll
-        for (uint32_t j = 0; j < kTileK / 16; ++j)
-          tensor_product<TWO>(to, a + j * da, b + j * db, p.kind, k > k_first || j > 0);
+        for (uint32_t q = 6 - kProducts; q < 6; ++q) {
+          const uint8_t* at_a = at + plane_a[q] * S::a_bytes;
+          const uint8_t* at_b = at + S::planes * S::a_bytes + plane_b[q] * S::b_bytes;
+          const uint64_t a = p.a_k_major ? operand_k_major(at_a) : operand_i_major(at_a, 8192);
+          const uint64_t b = p.b_k_major ? operand_k_major(at_b) : operand_i_major(at_b, 8192);
+#pragma unroll
+          for (uint32_t j = 0; j < kTileK / 16; ++j)
+            tensor_product<TWO>(to, a + j * da, b + j * db, p.kind,
+                                k > k_first || q > 6 - kProducts || j > 0);
+        }
         products_arrive<TWO>(&empty[s]);
       }
       if (ok) products_arrive<TWO>(&done[half]);
@@ -335,6 +357,7 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
       }
       const bool sound = __all_sync(~0u, wait(&done[half], (turn / 2) & 1, &gave_up, p));
       tmem_fence_after();
+      if constexpr (MODE == SPLIT) cluster_wait();
       if (!sound && MODE != SPLIT) {
         if (fetched && lane == 0)  // what is still on its way
           for (uint32_t c = 0; c < kChunks && c < kPieces; ++c)
@@ -363,10 +386,14 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
           } else {
             __syncwarp();
             const uint32_t rows = min(32u, p.rows - row0);
-            for (uint32_t r = 0; r < rows; ++r)
-              for (uint32_t col = lane; col < 128 / sizeof(Q); col += 32)
-                if (j0 + col < p.cols)
-                  array[(int64_t)(row0 + r) * ld + j0 + col] = *value(reinterpret_cast<Q*>(of), r, col);
+#pragma unroll
+            for (uint32_t col = lane; col < 128 / sizeof(Q); col += 32) {
+              if (j0 + col >= p.cols) continue;
+              Q* to = array + (int64_t)row0 * ld + j0 + col;
+#pragma unroll 8
+              for (uint32_t r = 0; r < rows; ++r, to += ld)
+                *to = *value(reinterpret_cast<Q*>(of), r, col);
+            }
             __syncwarp();
           }
         };
@@ -381,10 +408,14 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
           } else if (p.f.residual) {
             const T* res = (const T*)p.f.residual;
             const uint32_t rows = min(32u, p.rows - row0);
-            for (uint32_t r = 0; r < rows; ++r)
-              for (uint32_t col = lane; col < kWide; col += 32)
-                if (j1 + col < p.cols)
-                  *value(reinterpret_cast<T*>(at), r, col) = res[(int64_t)(row0 + r) * p.f.ldr + j1 + col];
+#pragma unroll
+            for (uint32_t col = lane; col < kWide; col += 32) {
+              if (j1 + col >= p.cols) continue;
+              const T* from = res + (int64_t)row0 * p.f.ldr + j1 + col;
+#pragma unroll 8
+              for (uint32_t r = 0; r < rows; ++r, from += p.f.ldr)
+                *value(reinterpret_cast<T*>(at), r, col) = *from;
+            }
             __syncwarp();
           } else if (wide) {
             if (lane == 0) bulk_wait_read<0>();
@@ -397,7 +428,9 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
             const uint32_t j0 = j1 + h * 32;
             add_bias<T, 32>(p.f, j0, p.cols, wide && j0 + 32 <= p.cols, v);
             if (p.f.pre) {
-              if (kPieces == 2 && !p.f.residual) {  // the other piece takes it out
+              // the other piece takes it out, or the same one before the result (of as
+              // many columns)
+              if (!p.f.residual && (kPieces == 2 || sizeof(T) == 4)) {
                 uint8_t* z = piece(c + 1);
                 if (wide) {
                   if (lane == 0) bulk_wait_read<0>();
@@ -408,11 +441,22 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
                   *reinterpret_cast<float4*>(chunk(z, k)) =
                       make_float4(v[k * 4], v[k * 4 + 1], v[k * 4 + 2], v[k * 4 + 3]);
                 if (j0 < p.cols) send(&p.pre, p.f.pre, (int64_t)p.cols, j0, z);
+                if (kPieces == 1 && wide) {
+                  if (lane == 0) bulk_wait_read<0>();
+                  __syncwarp();
+                }
               } else if (i < p.rows) {
                 float* to = p.f.pre + (uint64_t)i * p.cols + j0;
+                if (wide && j0 + 32 <= p.cols) {
 #pragma unroll
-                for (uint32_t k = 0; k < 32; ++k)
-                  if (j0 + k < p.cols) to[k] = v[k];
+                  for (uint32_t k = 0; k < 32; k += 4)
+                    *reinterpret_cast<float4*>(to + k) =
+                        make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                } else {
+#pragma unroll
+                  for (uint32_t k = 0; k < 32; ++k)
+                    if (j0 + k < p.cols) to[k] = v[k];
+                }
               }
             }
             activate<T>(p.f.act, v);
@@ -486,6 +530,7 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
     if (S::pieces && lane == 0) bulk_wait_all<0>();
   }
   __syncwarp();
+  if (MODE == SPLIT && warp < 2) cluster_wait();
   tmem_fence_before();
   __syncthreads();
   if constexpr (MODE != ONE) cluster_barrier();  // SPLIT: every block's sums are there
@@ -519,14 +564,14 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
 template <typename T, int BN, Mode MODE>
 int launch(plx_ctx* ctx, TensorProduct& t, const Product& p, const Operand& a, const Operand& b,
            uint32_t parts, bool wide) {
-  using S = Stages<BN, MODE>;
+  using S = Stages<T, BN, MODE>;
   constexpr bool bf16 = !std::is_same_v<T, __half>;  // what is multiplied
   constexpr uint32_t high = MODE == PAIR ? 2 * kTileA : kTileA;
   t.tiles_a = (t.rows + high - 1) / high;
   t.tiles_b = (t.cols + BN - 1) / BN;
   t.kind = product_kind(bf16, !a.k_major, !b.k_major, high, BN);
   auto maps = [&](CUtensorMap (&m)[3], const Operand& o, uint32_t count, uint32_t tile) {
-    for (int plane = 0; plane < (sizeof(T) == 4 ? 3 : 1); ++plane)
+    for (int plane = 0; plane < (int)S::planes; ++plane)
       if (int rc = tensor_map(&m[plane], bf16 ? PLX_BF16 : PLX_F16,
                               (const char*)o.p + plane * o.plane, o.k_major ? t.depth : count,
                               o.k_major ? count : t.depth, o.ld, 64, o.k_major ? tile : kTileK, true))
@@ -588,25 +633,34 @@ int product_tensor(plx_ctx* ctx, int dtype, const Product& p) {
   t.a_k_major = a.k_major;
   t.b_k_major = b.k_major;
   const int per = 16 / (int)dtype_bytes(dtype);
-  t.segments = dtype == PLX_F32 ? 6 : 1;
   const bool wide = p.f.ldy % per == 0 && aligned16(p.f.y) &&
                     (!p.f.residual || (p.f.ldr % per == 0 && aligned16(p.f.residual))) &&
                     (!p.f.pre || (p.cols % 4 == 0 && aligned16(p.f.pre))) && aligned16(p.f.bias);
-  // What the tiles of a width take: rounds of blocks, each with its share of k (in
-  // products of 64 values of k by one column; the rest measured).
-  const uint32_t sms = (uint32_t)ctx->num_sms, ks = (p.depth + kTileK - 1) / kTileK * t.segments;
+  // What the tiles of a width take: rounds of blocks, each with its share of k (a unit is
+  // the products of 64 values of k by one column). A block waits for its products or
+  // for its operands, of 128 + width rows; starting and finishing a tile takes 500
+  // units, sending and joining a shared one's sums another 500.
+  const bool f32 = dtype == PLX_F32;
+  const uint32_t sms = (uint32_t)ctx->num_sms, ks = (p.depth + kTileK - 1) / kTileK;
+  // by products; by their operands out of shared memory; by copies into it
+  auto step_of = [&](uint32_t width, uint32_t b_rows) {
+    const double read = 128 + b_rows;
+    return std::max({(f32 ? 6.3 : 1.05) * width, (f32 ? 3.45 : 0.575) * read, (f32 ? 2.7 : 0.9) * read});
+  };
   uint32_t bn = 0, parts = 1;
   bool pair = false;
   double best = 0;
   for (uint32_t width : {256u, 128u, 64u, 32u, 16u}) {
     if (width < 64 && !b.k_major) break;
+    if (width > 128 && f32) continue;
     if (width > (b.k_major ? 16u : 64u) && width / 2 >= t.cols) continue;
     const uint64_t tiles =
         (uint64_t)((t.rows + kTileA - 1) / kTileA) * ((t.cols + width - 1) / width);
     for (uint32_t s = 1; s <= 8; s *= 2) {
-      if (s > 1 && (tiles * s > sms || s > ks || width > 128)) break;
+      if (s > 1 && (tiles * s > sms || s > ks || width > (f32 ? 64 : 128))) break;
       const double rounds = (double)((tiles * s + sms - 1) / sms);
-      const double took = rounds * ((width + 96.0) * ((ks + s - 1) / s) + (s > 1 ? 1000 : 500));
+      const double took =
+          rounds * (step_of(width, width) * ((ks + s - 1) / s) + (s > 1 ? 1000 : 500));
       if (bn == 0 || took < best) {
         best = took;
         bn = width;
@@ -614,19 +668,24 @@ int product_tensor(plx_ctx* ctx, int dtype, const Product& p) {
       }
     }
   }
-  if (t.rows > kTileA && t.cols > 128) {
+  if (t.rows > kTileA && t.cols > 64) {
+    const uint32_t width = f32 ? 128 : 256;
     const uint64_t tiles =
-        (uint64_t)((t.rows + 2 * kTileA - 1) / (2 * kTileA)) * ((t.cols + 255) / 256);
+        (uint64_t)((t.rows + 2 * kTileA - 1) / (2 * kTileA)) * ((t.cols + width - 1) / width);
     const double rounds = (double)((tiles + sms / 2 - 1) / (sms / 2));
-    pair = rounds * (270.0 * ks + 500) < best;
+    pair = rounds * (step_of(width, width / 2) * ks + 500) < best;
   }
   auto go = [&](auto v) -> int {
     using T = decltype(v);
-    if (pair) return launch<T, 256, PAIR>(ctx, t, p, a, b, 1, wide);
+    constexpr int WIDEST = sizeof(T) == 4 ? 128 : 256;  // stages of 32-bit values are long
     const bool split = parts > 1;
+    if (pair) return launch<T, WIDEST, PAIR>(ctx, t, p, a, b, 1, wide);
     switch (bn) {
-      case 256: return launch<T, 256, ONE>(ctx, t, p, a, b, parts, wide);
-      case 128: return (split ? launch<T, 128, SPLIT> : launch<T, 128, ONE>)(ctx, t, p, a, b, parts, wide);
+      case 256: return launch<T, WIDEST, ONE>(ctx, t, p, a, b, parts, wide);
+      case 128:
+        if constexpr (sizeof(T) == 2)
+          if (split) return launch<T, 128, SPLIT>(ctx, t, p, a, b, parts, wide);
+        return launch<T, 128, ONE>(ctx, t, p, a, b, parts, wide);
       case 64: return (split ? launch<T, 64, SPLIT> : launch<T, 64, ONE>)(ctx, t, p, a, b, parts, wide);
       case 32: return (split ? launch<T, 32, SPLIT> : launch<T, 32, ONE>)(ctx, t, p, a, b, parts, wide);
       default: return (split ? launch<T, 16, SPLIT> : launch<T, 16, ONE>)(ctx, t, p, a, b, parts, wide);
