@@ -787,8 +787,8 @@ int plx_block_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, 
 
 /* Scratch of plx_recurrence and plx_recurrence_backward; ragged: offsets are
  * given. */
-size_t plx_recurrence_scratch_bytes(uint32_t n_streams, uint64_t rows, uint32_t n, int ragged,
-                                    int backward);
+size_t plx_recurrence_scratch_bytes(uint32_t n_streams, uint64_t rows, uint32_t n, int dtype,
+                                    int ragged, int mix, int backward);
 
 /* Gated linear recurrence over the steps of streams (the trace e' = d e + x of
  * HebbianTraceUpdate, of every unit, with a decay of every step):

@@ -236,8 +236,8 @@ _SIGNATURES = {
                                         c_void_p, POINTER(BlockNormParams), c_void_p, c_int64,
                                         c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
                                         c_void_p, c_void_p, c_void_p, ctypes.c_size_t]),
-    "plx_recurrence_scratch_bytes": (ctypes.c_size_t, [c_uint32, c_uint64, c_uint32, c_int,
-                                                      c_int]),
+    "plx_recurrence_scratch_bytes": (ctypes.c_size_t, [c_uint32, c_uint64, c_uint32, c_int, c_int,
+                                                      c_int, c_int]),
     "plx_recurrence": (c_int, [c_void_p, c_uint32, c_uint64, c_uint32, c_int, c_void_p, c_void_p,
                                c_int64, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p,
                                c_int64, c_void_p, c_void_p, ctypes.c_size_t]),

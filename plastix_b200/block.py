@@ -375,8 +375,8 @@ def recurrence(ctx: Context, x: torch.Tensor, gate: torch.Tensor,
             h = _new(x)
         if final is None:
             final = x.new_empty((streams, n), dtype=torch.float32)
-        size = _abi.lib().plx_recurrence_scratch_bytes(streams, rows, n, offsets is not None,
-                                                       0)
+        size = _abi.lib().plx_recurrence_scratch_bytes(streams, rows, n, dtype,
+                                                       offsets is not None, int(mix), 0)
         scratch = x.new_empty(size, dtype=torch.uint8) if size else None
         _abi.call("plx_recurrence", ctx.handle, streams, rows, n, dtype, offsets_p, x.data_ptr(),
                   ldx, gate.data_ptr(), ldg, gate_kind, int(mix), state_p, h.data_ptr(), ldh,
@@ -406,8 +406,8 @@ def recurrence_backward(ctx: Context, dh: torch.Tensor, gate: torch.Tensor, h: t
     with _scope(ctx, dh, gate, h, x, state, dfinal, offsets):
         dx, dgate = _new(gate), _new(gate)
         dstate = None if state is None else torch.empty_like(state)
-        size = _abi.lib().plx_recurrence_scratch_bytes(streams, rows, n, offsets is not None,
-                                                       1)
+        size = _abi.lib().plx_recurrence_scratch_bytes(streams, rows, n, dtype,
+                                                       offsets is not None, int(mix), 1)
         scratch = gate.new_empty(size, dtype=torch.uint8) if size else None
         _abi.call("plx_recurrence_backward", ctx.handle, streams, rows, n, dtype, offsets_p,
                   dh.data_ptr(), lddh, _address(x), ldx, gate.data_ptr(), ldg, gate_kind,

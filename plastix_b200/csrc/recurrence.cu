@@ -173,20 +173,53 @@ struct Step {
   __device__ __forceinline__ W dx(W g) const { return MIX ? mulw(g, keep) : g; }
 };
 
-template <int V>
-__device__ __forceinline__ Units<V> load_units(const float* p, bool in) {
-  if constexpr (V == 2) return in ? pack2(p[0], p[1]) : pack2(0.0f, 0.0f);
-  else return in ? p[0] : 0.0f;
-}
-template <int V>
-__device__ __forceinline__ void store_units(float* p, Units<V> v) {
-  if constexpr (V == 2) {
-    p[0] = v.x;
-    p[1] = v.y;
-  } else {
-    p[0] = v;
+// A lane's units of an array: V of them, GAP apart; those there are.
+template <int V, int GAP>
+struct Lane {
+  uint32_t unit;
+  bool in[V];
+  __device__ __forceinline__ Lane(uint32_t tile, uint32_t n)
+      : unit(tile * 32 * V + (threadIdx.x & 31) * (GAP == 1 ? V : 1)) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) in[e] = unit + e * GAP < n;  // GAP 1: V divides n
   }
-}
+  __device__ __forceinline__ Units<V> load(const float* p) const {
+    if constexpr (V == 2) return pack2(in[0] ? p[0] : 0.0f, in[1] ? p[GAP] : 0.0f);
+    else return in[0] ? p[0] : 0.0f;
+  }
+  __device__ __forceinline__ void store(float* p, Units<V> v) const {
+    if constexpr (V == 2) {
+      if (in[0]) p[0] = v.x;
+      if (in[1]) p[GAP] = v.y;
+    } else {
+      if (in[0]) p[0] = v;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ Pack<T, V> load_rows(const T* p) const {
+    Pack<T, V> q;
+#pragma unroll
+    for (int e = 0; e < V; ++e) q.v[e] = from_f32<T>(0.0f);
+    if constexpr (GAP == 1) {
+      if (in[0]) q = load_pack<T, V>(p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (in[e]) q.v[e] = p[e * GAP];
+    }
+    return q;
+  }
+  template <typename T>
+  __device__ __forceinline__ void store_rows(T* p, Pack<T, V> q) const {
+    if constexpr (GAP == 1) {
+      if (in[0]) *reinterpret_cast<Pack<T, V>*>(p) = q;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (in[e]) p[e * GAP] = q.v[e];
+    }
+  }
+};
 
 // Short streams, whole ones in a tile.
 template <typename T, int V, bool SIGMOID, bool MIX, bool BACK>
@@ -204,10 +237,10 @@ k_recurrence_tile(const __grid_constant__ Args p) {
   const W zero = all<W>(0.0f);
   const uint64_t row0 = (uint64_t)(blockIdx.x / p.tiles) * p.tile_rows;
   const uint64_t row1 = min(row0 + p.tile_rows, p.rows);
-  const uint32_t unit = (blockIdx.x % p.tiles * 32 + lane) * V;
-  const bool in = unit < p.n;  // V divides n
+  const Lane<V, 1> mine(blockIdx.x % p.tiles, p.n);
+  const uint32_t unit = mine.unit;
   // This warp's run, in the order that it is walked.
-  const uint32_t run = BACK ? kWarps - 1 - warp : warp;
+  const uint32_t run = BACK ? blockDim.x / 32 - 1 - warp : warp;
   const uint64_t at = row0 + run * kRun;
   const int len = at < row1 ? (int)min((uint64_t)kRun, row1 - at) : 0;
 
@@ -220,7 +253,7 @@ k_recurrence_tile(const __grid_constant__ Args p) {
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
       q[i] = nothing;
-      if (in && i < len) q[i] = load_pack<T, V>(from + i * ld);
+      if (i < len) q[i] = mine.load_rows(from + i * ld);
     }
   };
   load(qg, p.gate, p.ldg);
@@ -236,14 +269,21 @@ k_recurrence_tile(const __grid_constant__ Args p) {
   const uint32_t last = __ballot_sync(~0u, (int)lane < len && place + 1 == p.steps);
   auto state_at = [&](const float* states, int i) {
     const uint32_t s = __shfl_sync(~0u, stream, i);
-    return states ? load_units<V>(states + (uint64_t)s * p.n + unit, in) : zero;
+    return states ? mine.load(states + (uint64_t)s * p.n + unit) : zero;
   };
+  // what streams are given where their walk begins
+  W given[kRun];
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) {
+    given[i] = zero;
+    if ((BACK ? last : first) >> i & 1) given[i] = state_at(BACK ? p.dfinal : p.state, i);
+  }
   if constexpr (BACK) {
     const T* from = (const T*)p.h + ((int64_t)at - 1) * p.ldh + unit;
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
       q2[i] = nothing;
-      if (in && i < len && !(first >> i & 1)) q2[i] = load_pack<T, V>(from + i * p.ldh);
+      if (i < len && !(first >> i & 1)) q2[i] = mine.load_rows(from + i * p.ldh);
     }
   }
 
@@ -261,7 +301,7 @@ k_recurrence_tile(const __grid_constant__ Args p) {
       if (first >> i & 1) before = state_at(p.state, i);
       st.backward(qg[i], q1[i], before, q3[MIX ? i : 0]);
       if (stop >> i & 1) {  // the same for the whole warp
-        H = state_at(p.dfinal, i);
+        H = given[i];
         A = zero;
       }
       H = mulw(st.a, addw(wide<T, V>(st.dh), H));
@@ -269,7 +309,7 @@ k_recurrence_tile(const __grid_constant__ Args p) {
     } else {
       st.forward(qg[i], q1[i]);
       if (stop >> i & 1) {
-        st.b = fmaw(st.a, state_at(p.state, i), st.b);
+        st.b = fmaw(st.a, given[i], st.b);
         H = st.b;
         A = zero;
       } else {
@@ -298,36 +338,30 @@ k_recurrence_tile(const __grid_constant__ Args p) {
       if (stop >> i & 1) carry = state_at(p.dfinal, i);
       const W g = addw(wide<T, V>(st.dh), carry);
       carry = mulw(st.a, g);
-      if (in) {
-        *reinterpret_cast<P*>((T*)p.out + row * p.ldo + unit) = narrow<T, V>(st.dx(g));
-        *reinterpret_cast<P*>((T*)p.out2 + row * p.ldo2 + unit) = narrow<T, V>(mulw(g, st.slope));
-      }
+      mine.store_rows((T*)p.out + row * p.ldo + unit, narrow<T, V>(st.dx(g)));
+      mine.store_rows((T*)p.out2 + row * p.ldo2 + unit, narrow<T, V>(mulw(g, st.slope)));
     } else {
       carry = stop >> i & 1 ? st.b : fmaw(st.a, carry, st.b);
-      if (in) *reinterpret_cast<P*>((T*)p.out + row * p.ldo + unit) = narrow<T, V>(carry);
+      mine.store_rows((T*)p.out + row * p.ldo + unit, narrow<T, V>(carry));
     }
     if (p.state_out && ((BACK ? first : last) >> i & 1)) {
       const uint32_t s = __shfl_sync(~0u, stream, i);
-      if (in) store_units<V>(p.state_out + (uint64_t)s * p.n + unit, carry);
+      mine.store(p.state_out + (uint64_t)s * p.n + unit, carry);
     }
   }
 }
 
-// Stages of a walk under way: a run of every array that it reads, a lane's own
-// values (no other lane reads them, so that no barrier is needed). Values of less
-// than four bytes are read when their turn comes.
-constexpr int kWalkWarps = 8;
+// Stages of a walk under way: tiles of every array that it reads.
+constexpr int kWalkWarps = 8, kWalkUnits = 64;
 constexpr uint32_t kWalkSteps = kWalkWarps * kRun;  // of a tile
-template <typename T, int V, int ARRAYS>
+template <typename T, int ARRAYS, bool TENSOR>
 struct WalkRing {
-  static constexpr int piece = V * sizeof(T);
-  static constexpr bool used = piece >= 4;
-  static constexpr int row = 32 * piece;
+  static constexpr int row = kWalkUnits * sizeof(T);
   static constexpr int run = kRun * row;
   static constexpr int array = kWalkWarps * run;
   static constexpr int stage = ARRAYS * array;
   static constexpr int stages = stage <= 16 * 1024 ? 4 : stage <= 32 * 1024 ? 3 : 2;
-  static constexpr int bytes = used ? stages * stage : 0;
+  static constexpr int bytes = TENSOR ? stages * stage : 0;
 };
 
 struct Maps {
@@ -336,15 +370,17 @@ struct Maps {
 
 // A part of a long stream (or of ragged ones behind each other), tile after tile.
 // LEAVE: the part's pair, else its results. TENSOR: one thread has a tile's arrays
-// copied by tensor copies (rows whose start and stride are multiples of 16 bytes),
-// else every lane has its own values copied, in three times the instructions.
-template <typename T, int V, bool SIGMOID, bool MIX, bool BACK, bool LEAVE, bool TENSOR>
+// copied by tensor copies (rows whose start and stride are multiples of 16 bytes) and
+// a lane has two units side by side; else every lane reads its own, of two units 32
+// apart (through shared memory by four-byte copies took a quarter longer).
+template <typename T, bool SIGMOID, bool MIX, bool BACK, bool LEAVE, bool TENSOR>
 __global__ void __launch_bounds__(kWalkWarps * 32, BACK && !LEAVE ? 2 : 3)
 k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps maps) {
+  constexpr int V = 2, GAP = TENSOR ? 1 : 32;
   using W = Units<V>;
   using P = Pack<T, V>;
   constexpr int ARRAYS = LEAVE || !BACK ? 2 : MIX ? 4 : 3;
-  using R = WalkRing<T, V, ARRAYS>;
+  using R = WalkRing<T, ARRAYS, TENSOR>;
   constexpr int S = R::stages;
   struct alignas(8 * V) Pair {
     W a, h;
@@ -370,8 +406,8 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
   }
   const uint32_t across = blockIdx.x % p.tiles, rest = blockIdx.x / p.tiles;
   const uint32_t group = rest / p.parts, part = rest % p.parts;
-  const uint32_t unit = (across * 32 + lane) * V;
-  const bool in = unit < p.n;  // V divides n
+  const Lane<V, GAP> own(across, p.n);
+  const uint32_t unit = own.unit;
   const int64_t g0 = (int64_t)group * p.group_rows, g1 = min(g0 + p.group_rows, (int64_t)p.rows);
   const int64_t row0 = min(g0 + (int64_t)part * p.part_rows, g1);
   const int64_t row1 = min(row0 + p.part_rows, g1);
@@ -390,12 +426,8 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
                       (const T*)p.x};
   const int64_t ld[4] = {p.ldg, BACK ? p.lddh : p.ldx, p.ldh, p.ldx};
   // of this warp's run in a tile in the ring, this lane's values
-  const char* ring = reinterpret_cast<const char*>(walk_bytes) + lane * R::piece +
+  const char* ring = reinterpret_cast<const char*>(walk_bytes) + lane * V * sizeof(T) +
                      (BACK ? kWalkWarps - 1 - warp : warp) * R::run;
-  const T* next[ARRAYS];  // where the run fetched next begins
-#pragma unroll
-  for (int k = 0; k < ARRAYS; ++k) next[k] = from[k] + (at - (k == 2 ? 1 : 0)) * ld[k] + unit;
-  int64_t next_at = at;
   int fetched = 0;
   auto fetch = [&](uint32_t stage) {
     if constexpr (TENSOR) {  // by one thread
@@ -408,30 +440,6 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
                       (int)(across * 32 * V), y - (k == 2 ? 1 : 0), &full[stage]);
       }
       ++fetched;
-    } else if constexpr (R::used) {
-      if (in && fetched < tiles) {
-        const int left = (int)min((int64_t)kRun, row1 - next_at);
-        char* to = const_cast<char*>(ring) + stage * R::stage;
-        auto copy = [&](auto whole) {
-#pragma unroll
-          for (int k = 0; k < ARRAYS; ++k) {
-            const T* q = next[k];
-#pragma unroll
-            for (int i = 0; i < kRun; ++i) {
-              // h before the first row of all is no row's
-              if (decltype(whole)::value || (i < left && !(k == 2 && i == 0 && next_at == 0)))
-                copy_async<R::piece>(to + k * R::array + i * R::row, q);
-              q += ld[k];
-            }
-            next[k] += tile_dir * (int)kWalkSteps * ld[k];
-          }
-        };
-        if (left == kRun && next_at > 0) copy(std::true_type{});
-        else copy(std::false_type{});
-      }
-      next_at += tile_dir * (int)kWalkSteps;
-      ++fetched;
-      copy_commit();
     }
   };
   if constexpr (TENSOR) {
@@ -442,9 +450,6 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
       for (int s = 0; s < S; ++s) fetch(s);
     }
     __syncthreads();
-  } else {
-#pragma unroll
-    for (int s = 0; s < S - 1; ++s) fetch(s);
   }
 
   W A = all<W>(1.0f), given = zero;  // forwards h; backwards what a step hands to the one before
@@ -476,12 +481,10 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
   for (int tile = 0; tile < tiles; ++tile, at += tile_dir * (int)kWalkSteps, half ^= 1) {
     const int len = (int)max((int64_t)0, min((int64_t)kRun, row1 - at));
     P q[4][kRun];
-    if constexpr (R::used) {
-      if constexpr (!TENSOR) {
-        copy_wait<S - 2>();
-      } else if (!mbar_try_wait(&full[stage], parity) &&
-                 (*(volatile uint32_t*)&gave_up ||
-                  !mbar_wait_bounded(&full[stage], parity, p.timeout_ns))) {
+    if constexpr (TENSOR) {
+      if (!mbar_try_wait(&full[stage], parity) &&
+          (*(volatile uint32_t*)&gave_up ||
+           !mbar_wait_bounded(&full[stage], parity, p.timeout_ns))) {
         *(volatile uint32_t*)&gave_up = 1;
         record_status(p.status, kStatusTimeout);
       }
@@ -491,7 +494,6 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
 #pragma unroll
         for (int i = 0; i < kRun; ++i)
           q[k][i] = *reinterpret_cast<const P*>(to + k * R::array + i * R::row);
-      if constexpr (!TENSOR) fetch(stage == 0 ? S - 1 : stage - 1);
     } else {
 #pragma unroll
       for (int k = 0; k < ARRAYS; ++k)
@@ -499,7 +501,7 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
         for (int i = 0; i < kRun; ++i) {
           q[k][i] = nothing;
           const int64_t r = at + i - (k == 2 ? 1 : 0);
-          if (in && i < len && r >= 0) q[k][i] = load_pack<T, V>(from[k] + r * ld[k] + unit);
+          if (i < len && r >= 0) q[k][i] = own.load_rows(from[k] + r * ld[k] + unit);
         }
     }
     uint32_t valid = 0xff, first = 0, last = 0;
@@ -516,7 +518,7 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
     const uint32_t stop = BACK ? last : first;  // rows at which what was before does not count
     auto state_at = [&](const float* states, int i) {
       const uint32_t s = __shfl_sync(~0u, mine.stream, i);
-      return states ? load_units<V>(states + (uint64_t)s * p.n + unit, in) : zero;
+      return states ? own.load(states + (uint64_t)s * p.n + unit) : zero;
     };
 
     // ---- the run's pair
@@ -607,15 +609,15 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
         if constexpr (BACK) {
           const W g = addw(wide<T, V>(st[i].dh), carry);
           carry = mulw(st[i].a, g);
-          *reinterpret_cast<P*>(o1) = narrow<T, V>(st[i].dx(g));
-          *reinterpret_cast<P*>(o2) = narrow<T, V>(mulw(g, st[i].slope));
+          own.store_rows(o1, narrow<T, V>(st[i].dx(g)));
+          own.store_rows(o2, narrow<T, V>(mulw(g, st[i].slope)));
         } else {
           carry = fmaw(st[i].a, carry, st[i].b);
-          *reinterpret_cast<P*>(o1) = narrow<T, V>(carry);
+          own.store_rows(o1, narrow<T, V>(carry));
         }
       };
       if (len == kRun && valid == 0xff && !first && !last) {
-        if (in)
+        if (own.in[0])
 #pragma unroll
           for (int k = 0; k < kRun; ++k) {
             results(BACK ? kRun - 1 - k : k);
@@ -628,10 +630,10 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
           const int i = BACK ? kRun - 1 - k : k;
           if (i < len) {
             if (stop >> i & 1) carry = state_at(BACK ? p.dfinal : p.state, i);
-            if (in && (valid >> i & 1)) results(i);
+            if (valid >> i & 1) results(i);
             if (p.state_out && ((BACK ? first : last) >> i & 1)) {
               const uint32_t s = __shfl_sync(~0u, mine.stream, i);
-              if (in) store_units<V>(p.state_out + (uint64_t)s * p.n + unit, carry);
+              own.store(p.state_out + (uint64_t)s * p.n + unit, carry);
             }
           }
           o1 += dir * p.ldo;
@@ -663,38 +665,45 @@ k_copy_state(uint64_t count, const float* from, float* to) {
 // How a call is cut, and what it needs of scratch.
 struct Plan {
   bool short_streams, states_apart;
-  int units;  // a lane's
   uint32_t tiles, tile_rows, groups, group_rows, parts, part_rows;
   uint64_t pair_bytes, shut_bytes;
 };
 
 // Streams of at most this many steps go in tiles.
 constexpr uint32_t kShort = 64;
-// Blocks that keep all SMs busy.
-constexpr uint32_t kWalks = 148 * 3;
+// Blocks of a walk for results that all SMs hold at a time (as many parts as that, so
+// that none waits for a second round).
+uint32_t walks_at_once(int dtype, bool mix, bool back, bool tensor) {
+  if (!tensor) return 148u * (back ? 2 : 3);
+  return 148u * (dtype == PLX_F32 && back && mix ? 1 : back || dtype == PLX_F32 ? 2 : 3);
+}
 
-Plan plan_of(uint32_t streams, uint64_t rows, uint32_t n, bool ragged, int units, bool back) {
+Plan plan_of(uint32_t streams, uint64_t rows, uint32_t n, int dtype, bool ragged, bool mix,
+             int units, bool back, bool tensor) {
   Plan c = {};
-  c.units = units;
   const uint32_t steps = ragged ? (uint32_t)rows : (uint32_t)(rows / streams);
-  c.tiles = (n + 32 * units - 1) / (32 * units);
   c.short_streams = !ragged && steps <= kShort;
   if (c.short_streams) {
-    c.tile_rows = tile_steps(back) / steps * steps;
+    c.tiles = (n + 32 * units - 1) / (32 * units);
+    // whole streams, as many as a block takes or as leave two blocks an SM
+    const uint64_t spread = rows * c.tiles / (2 * 148);
+    c.tile_rows = (uint32_t)std::min<uint64_t>(tile_steps(back), std::max<uint64_t>(spread, kRun));
+    c.tile_rows = std::max(c.tile_rows / steps, 1u) * steps;
     c.states_apart = back;
     return c;
   }
+  c.tiles = (n + kWalkUnits - 1) / kWalkUnits;
   c.group_rows = steps;
   c.groups = ragged ? 1 : streams;
+  const uint32_t most = walks_at_once(dtype, mix, back, tensor);
   const uint64_t walks = (uint64_t)c.groups * c.tiles;
-  c.parts = walks >= kWalks / 2 ? 1 : (uint32_t)((kWalks + walks - 1) / walks);
-  c.parts = std::max(1u, std::min(c.parts, steps / kShort));
+  c.parts = walks >= most / 2 ? 1 : std::max(1u, std::min((uint32_t)(most / walks), steps / kShort));
   c.part_rows = (steps + c.parts - 1) / c.parts;
   c.part_rows = (c.part_rows + kWalkSteps - 1) / kWalkSteps * kWalkSteps;
   c.parts = (steps + c.part_rows - 1) / c.part_rows;
   c.states_apart = c.parts > 1;
   if (c.parts > 1) {
-    c.pair_bytes = (uint64_t)c.groups * c.parts * c.tiles * 32 * units * 8;
+    c.pair_bytes = (uint64_t)c.groups * c.parts * c.tiles * kWalkUnits * 8;
     c.shut_bytes = ((uint64_t)c.groups * c.parts * 4 + 255) / 256 * 256;
   }
   return c;
@@ -705,7 +714,7 @@ uint64_t state_bytes(uint32_t streams, uint32_t n) {
 }
 
 int check_recurrence(const plx_ctx* ctx, uint32_t streams, uint64_t rows, uint32_t n, int dtype,
-                     const int32_t* offsets, int gate_kind, bool back, const void* scratch,
+                     const int32_t* offsets, int gate_kind, int mix, bool back, const void* scratch,
                      size_t scratch_bytes) {
   PLX_CHECK_ARG(ctx, "ctx is required");
   PLX_CHECK_ARG(valid_dtype(dtype), "dtype %d is none of PLX_F32, PLX_BF16, PLX_F16", dtype);
@@ -720,7 +729,7 @@ int check_recurrence(const plx_ctx* ctx, uint32_t streams, uint64_t rows, uint32
   PLX_CHECK_ARG(offsets || streams == 0 || rows % streams == 0,
                 "%llu rows are not the same number of steps for each of %u streams",
                 (unsigned long long)rows, streams);
-  const size_t need = plx_recurrence_scratch_bytes(streams, rows, n, offsets != nullptr, back);
+  const size_t need = plx_recurrence_scratch_bytes(streams, rows, n, dtype, offsets != nullptr, mix, back);
   PLX_CHECK_ARG(need == 0 || (scratch && scratch_bytes >= need),
                 "%zu bytes of scratch are needed, got %zu", need,
                 scratch ? scratch_bytes : (size_t)0);
@@ -758,7 +767,12 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
     auto go = [&](auto v_c, auto sigmoid_c, auto mix_c) -> int {
       constexpr int V = decltype(v_c)::value;
       constexpr bool SIGMOID = decltype(sigmoid_c)::value, MIX = decltype(mix_c)::value;
-      const Plan c = plan_of(a.streams, a.rows, a.n, a.offsets != nullptr, V, BACK);
+      // units side by side and 16-byte rows: whole tiles of long streams at a time
+      bool tensor = V == 2;
+      for (int64_t ld : {a.ldx, a.ldg, a.ldh, a.lddh}) tensor &= ld * sizeof(T) % 16 == 0;
+      for (const void* q : {a.x, a.gate, a.h, a.dh}) tensor &= aligned16(q);
+      const Plan c =
+          plan_of(a.streams, a.rows, a.n, dtype, a.offsets != nullptr, MIX, V, BACK, tensor);
       a.tiles = c.tiles;
       a.tile_rows = c.tile_rows;
       a.groups = c.groups;
@@ -781,7 +795,7 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
       }
       if (c.short_streams) {
         k_recurrence_tile<T, V, SIGMOID, MIX, BACK>
-            <<<(unsigned)blocks, warps_of(BACK) * 32, 0, ctx->stream>>>(a);
+            <<<(unsigned)blocks, (c.tile_rows + kRun - 1) / kRun * 32, 0, ctx->stream>>>(a);
         PLX_LAUNCH_CHECK("k_recurrence_tile");
         return PLX_OK;
       }
@@ -797,31 +811,25 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
           const void* of[4] = {a.gate, BACK ? a.dh : a.x, a.h, a.x};
           const int64_t ld[4] = {a.ldg, BACK ? a.lddh : a.ldx, a.ldh, a.ldx};
           for (int k = 0; k < ARRAYS; ++k)
-            if (int rc = tensor_map(&maps.of[k], dtype, of[k], a.n, a.rows, ld[k], 32 * V,
+            if (int rc = tensor_map(&maps.of[k], dtype, of[k], a.n, a.rows, ld[k], kWalkUnits,
                                     kWalkSteps, false))
               return rc;
         }
         if (c.parts > 1) {
-          constexpr auto leave = k_recurrence_walk<T, V, SIGMOID, MIX, BACK, true, TENSOR>;
-          using R = WalkRing<T, V, 2>;
+          constexpr auto leave = k_recurrence_walk<T, SIGMOID, MIX, BACK, true, TENSOR>;
+          using R = WalkRing<T, 2, TENSOR>;
           PLX_TRY_CUDA(allow_shared<leave>(ctx->device, R::bytes));
           leave<<<(unsigned)blocks, kWalkWarps * 32, R::bytes, ctx->stream>>>(a, maps);
           PLX_LAUNCH_CHECK("k_recurrence_walk");
         }
-        constexpr auto kernel = k_recurrence_walk<T, V, SIGMOID, MIX, BACK, false, TENSOR>;
-        using R = WalkRing<T, V, ARRAYS>;
+        constexpr auto kernel = k_recurrence_walk<T, SIGMOID, MIX, BACK, false, TENSOR>;
+        using R = WalkRing<T, ARRAYS, TENSOR>;
         PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, R::bytes));
         kernel<<<(unsigned)blocks, kWalkWarps * 32, R::bytes, ctx->stream>>>(a, maps);
         PLX_LAUNCH_CHECK("k_recurrence_walk");
         return PLX_OK;
       };
-      if constexpr (V == 2) {
-        bool tensor = true;
-        for (int64_t ld : {a.ldx, a.ldg, a.ldh, a.lddh}) tensor &= ld * sizeof(T) % 16 == 0;
-        for (const void* q : {a.x, a.gate, a.h, a.dh}) tensor &= aligned16(q);
-        if (tensor) return walk(std::true_type{});
-      }
-      return walk(std::false_type{});
+      return tensor ? walk(std::true_type{}) : walk(std::false_type{});
     };
     using std::integral_constant;
     auto kinds = [&](auto v) {
@@ -843,11 +851,13 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
 using namespace plx;
 
 extern "C" size_t plx_recurrence_scratch_bytes(uint32_t n_streams, uint64_t rows, uint32_t n,
-                                               int ragged, int backward) {
-  if (n_streams == 0 || rows == 0 || n == 0 || rows >= (1ull << 31)) return 0;
+                                               int dtype, int ragged, int mix, int backward) {
+  if (n_streams == 0 || rows == 0 || n == 0 || rows >= (1ull << 31) || !valid_dtype(dtype))
+    return 0;
   uint64_t most = 0;  // whatever the arrays' alignment
-  for (int units : {1, 2}) {
-    const Plan c = plan_of(n_streams, rows, n, ragged != 0, units, backward != 0);
+  for (bool tensor : {false, true}) {
+    const Plan c =
+        plan_of(n_streams, rows, n, dtype, ragged != 0, mix != 0, 1, backward != 0, tensor);
     most = std::max(most, (c.states_apart ? state_bytes(n_streams, n) : 0) + c.pair_bytes +
                               c.shut_bytes);
   }
@@ -859,7 +869,7 @@ extern "C" int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, u
                               const void* gate, int64_t ldg, int gate_kind, int mix,
                               const float* state, void* h, int64_t ldh, float* final_state,
                               void* scratch, size_t scratch_bytes) {
-  if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, false, scratch,
+  if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, mix, false, scratch,
                                 scratch_bytes))
     return rc;
   if (rows) PLX_CHECK_ARG(x && gate && h, "x, gate and h are required");
@@ -890,7 +900,7 @@ extern "C" int plx_recurrence_backward(plx_ctx* ctx, uint32_t n_streams, uint64_
                                        int64_t ldh, const float* state, const float* dfinal,
                                        void* dx, int64_t lddx, void* dgate, int64_t lddg,
                                        float* dstate, void* scratch, size_t scratch_bytes) {
-  if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, true, scratch,
+  if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, mix, true, scratch,
                                 scratch_bytes))
     return rc;
   if (rows) {
