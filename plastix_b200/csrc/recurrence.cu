@@ -102,14 +102,16 @@ __device__ __forceinline__ Pack<T, V> at_least_minus_87(Pack<T, V> q) {
 
 // a and 1 - a of a gate, neither by a difference that cancels: with e = exp(-gate),
 // 1 / (1 + e) and e / (1 + e). Gates below -87 count as -87 (which leaves e^-87 of
-// h). The quotient is off by 2^-23 at most.
+// h). The quotient gets one Newton step: what a is off by, a long memory raises to its
+// length.
 template <bool SIGMOID, typename T, int V>
 __device__ __forceinline__ void gate_value(Pack<T, V> gate, Units<V>& a, Units<V>& keep) {
   using W = Units<V>;
   if constexpr (SIGMOID) {
     const W g = wide<T, V>(at_least_minus_87(gate));
     const W e = each(mulw(g, all<W>(-kLog2e)), exp2_approx);
-    a = each(addw(e, all<W>(1.0f)), rcp_approx);
+    const W d = addw(e, all<W>(1.0f)), r = each(d, rcp_approx);
+    a = fmaw(r, fmaw(each(d, [](float t) { return -t; }), r, all<W>(1.0f)), r);
     keep = mulw(e, a);
   } else {
     a = wide<T, V>(gate);
