@@ -671,8 +671,6 @@ struct Plan {
   uint64_t pair_bytes, shut_bytes;
 };
 
-// Streams of at most this many steps go in tiles.
-constexpr uint32_t kShort = 64;
 // Blocks of a walk for results that all SMs hold at a time (as many parts as that, so
 // that none waits for a second round).
 uint32_t walks_at_once(int dtype, bool mix, bool back, bool tensor) {
@@ -680,11 +678,26 @@ uint32_t walks_at_once(int dtype, bool mix, bool back, bool tensor) {
   return 148u * (dtype == PLX_F32 && back && mix ? 1 : back || dtype == PLX_F32 ? 2 : 3);
 }
 
+// Short streams go in tiles, 16-bit ones that tensor copies take only where they are few.
+// Measured, in tiles and in walks, forwards and backwards: 1,024 streams of 16 steps of
+// 4,096 units bf16 203 and 468 us, 167 and 214; 4,096 of 4 steps of 2,048 units 107 and
+// 240, 129 and 144; 256 of 64 steps of 1,000 units f32 46 and 88, 82 and 96; of 96 steps
+// (in two tiles of a walk) 70 and 129, 75 and 112; 256 of 80 steps of 501 units bf16
+// without tensor copies 44 and 82, 42 and 75. A step of 256 streams of 2,048 units takes
+// 5 us in tiles.
 Plan plan_of(uint32_t streams, uint64_t rows, uint32_t n, int dtype, bool ragged, bool mix,
              int units, bool back, bool tensor) {
   Plan c = {};
   const uint32_t steps = ragged ? (uint32_t)rows : (uint32_t)(rows / streams);
-  c.short_streams = !ragged && steps <= kShort;
+  const uint32_t most = walks_at_once(dtype, mix, back, tensor);
+  c.tiles = (n + kWalkUnits - 1) / kWalkUnits;
+  const uint64_t share = rows * c.tiles / most;  // rows of a block, in one round of them
+  // Streams of up to 512 steps: as many whole ones a walk as make a round of blocks.
+  const bool half = tensor && dtype != PLX_F32;
+  const uint32_t brief = half ? 32 : tile_steps(true);
+  const bool several = !ragged && tensor && (half || steps > brief) && steps <= 512 &&
+                       share >= kWalkSteps;
+  c.short_streams = !ragged && !several && steps <= brief;
   if (c.short_streams) {
     c.tiles = (n + 32 * units - 1) / (32 * units);
     // whole streams, as many as a block takes or as leave two blocks an SM
@@ -694,16 +707,23 @@ Plan plan_of(uint32_t streams, uint64_t rows, uint32_t n, int dtype, bool ragged
     c.states_apart = back;
     return c;
   }
-  c.tiles = (n + kWalkUnits - 1) / kWalkUnits;
-  c.group_rows = steps;
-  c.groups = ragged ? 1 : streams;
-  const uint32_t most = walks_at_once(dtype, mix, back, tensor);
-  const uint64_t walks = (uint64_t)c.groups * c.tiles;
-  c.parts = walks >= most / 2 ? 1 : std::max(1u, std::min((uint32_t)(most / walks), steps / kShort));
-  c.part_rows = (steps + c.parts - 1) / c.parts;
-  c.part_rows = (c.part_rows + kWalkSteps - 1) / kWalkSteps * kWalkSteps;
-  c.parts = (steps + c.part_rows - 1) / c.part_rows;
-  c.states_apart = c.parts > 1;
+  c.parts = 1;
+  c.group_rows = c.part_rows = steps;
+  if (several) {
+    c.group_rows = c.part_rows =
+        std::max((uint32_t)std::min<uint64_t>(share, 1024) / steps, 1u) * steps;
+    c.groups = (uint32_t)((rows + c.group_rows - 1) / c.group_rows);
+  } else {
+    c.groups = ragged ? 1 : streams;
+    const uint64_t walks = (uint64_t)c.groups * c.tiles;
+    if (walks < most / 2)
+      c.parts = std::max(1u, std::min((uint32_t)(most / walks), steps / kWalkSteps));
+    c.part_rows = (steps + c.parts - 1) / c.parts;
+    c.part_rows = (c.part_rows + kWalkSteps - 1) / kWalkSteps * kWalkSteps;
+    c.parts = (steps + c.part_rows - 1) / c.part_rows;
+  }
+  // a stream may begin and end in one tile, or in two parts
+  c.states_apart = ragged || several || c.parts > 1 || steps <= kWalkSteps;
   if (c.parts > 1) {
     c.pair_bytes = (uint64_t)c.groups * c.parts * c.tiles * kWalkUnits * 8;
     c.shut_bytes = ((uint64_t)c.groups * c.parts * 4 + 255) / 256 * 256;

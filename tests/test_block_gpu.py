@@ -71,6 +71,14 @@ DENSE = [  # rows, n, m, dtype, apply, residual, extra row stride, shift, param
     (2, 4099, 1030, "bf16", "silu", False, 0, 0, "f32"),
     (16, 4096, 1024, "f32", "silu", True, 0, 0, "f32"),
     (1500, 40, 1000, "f32", "sigmoid", False, 0, 0, "f32"),
+    (3000, 130, 2056, "bf16", "silu", True, 0, 0, "f32"),  # large tiles, the last ones cut on both sides
+    (2700, 72, 1999, "f16", "gelu", True, 0, 0, "same"),
+    (2600, 200, 1400, "f32", "gelu", True, 0, 0, "f32"),
+    (2500, 70, 1401, "f32", "tanh", True, 3, 1, "f32"),
+    (40, 3000, 2000, "bf16", "tanh", True, 0, 0, "f32"),  # few rows, sums shared by blocks
+    (3, 1000, 300, "f32", "gelu", True, 1, 1, "f32"),
+    (7, 515, 130, "f32", "relu", False, 1, 0, "f32"),
+    (65, 1000, 33, "f16", "silu", True, 0, 0, "f32"),
 ]
 
 
@@ -121,6 +129,51 @@ def test_dense_backward(ctx, rows, n, m, dtype, apply, residual, more, shift, pa
     within(f64(db), wb, stored(wb, tb, dtype if param == "same" else "f32"), "dbias")
     for a, c in zip((dx, dw, db), again):
         assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("rows, m, dtype", [(700, 1100, "bf16"), (2600, 1400, "f32"), (5, 1100, "bf16"), (100, 72, "f16")])
+def test_dense_in_place_of_its_residual(ctx, rows, m, dtype):
+    """out is the residual, a part of wider rows whose other values stay."""
+    (x, _), (w, _), (b, _), (res, _), _ = dense_inputs(rows, 200, m, dtype, 8, 8, "f32", 3)
+    want = block.dense(ctx, x, w, b, apply="silu", residual=res)
+    wide = torch.full((rows, m + 16), 3.0, dtype=TYPES[dtype], device="cuda")
+    part = wide[:, 8:8 + m]
+    part.copy_(res)
+    y = block.dense(ctx, x, w, b, apply="silu", residual=part, out=part)
+    ctx.sync()
+    assert y is part and torch.equal(part, want)
+    assert (wide[:, :8] == 3.0).all() and (wide[:, 8 + m:] == 3.0).all()
+
+
+def test_dense_leaves_what_lies_between_rows(ctx):
+    """Results into a part of wider rows at every alignment: nothing beside them is written."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    for dtype in ("f32", "bf16"):
+        for rows, m in ((300, 500), (1500, 640), (9, 130)):
+            x = torch.randn(rows, 64, device="cuda", generator=g).to(TYPES[dtype])
+            w = torch.randn(m, 64, device="cuda", generator=g).to(TYPES[dtype])
+            want = block.dense(ctx, x, w)
+            for shift in (0, 1, 8):
+                wide = torch.full((rows + 2, m + 24), 5.0, dtype=TYPES[dtype], device="cuda")
+                y = block.dense(ctx, x, w, out=wide[1:-1, shift:shift + m])
+                ctx.sync()
+                assert torch.equal(y, want)
+                assert (wide[0] == 5.0).all() and (wide[-1] == 5.0).all()
+                assert (wide[:, :shift] == 5.0).all() and (wide[:, shift + m:] == 5.0).all()
+
+
+@pytest.mark.parametrize("apply", ["sigmoid", "tanh", "silu", "gelu"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_activations_over_their_range(ctx, dtype, apply):
+    """One weight of 1: z is x, from tails to tails, zero and the smallest values among it."""
+    z = np.concatenate([np.linspace(-13, 13, 4001), np.logspace(-8, 0, 300), -np.logspace(-8, 0, 300), [0.0]])
+    x, xv, _ = made(z[:, None], dtype)
+    y = block.dense(ctx, x, torch.ones(1, 1, device="cuda", dtype=TYPES[dtype]), apply=apply)
+    ctx.sync()
+    want = F.act(xv, apply)[0]
+    # of 16 bits: GELU's fitted factor is off by 1e-4 at most (|z| > 10), the others by a few steps
+    rel = act_error(xv, want) + (1e-4 * np.abs(want) if dtype != "f32" and apply == "gelu" else 0)
+    within(f64(y), want, stored(want, rel, dtype), "y")
 
 
 def test_dense_parts_and_empty(ctx):
@@ -254,6 +307,22 @@ def test_block_norm(ctx, case):
     within(f64(stats), wstats, (n / 16 + 500) * U * spread * srel, "stats")
 
 
+@pytest.mark.parametrize("n", [96, 1000, 4096, 9000])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_block_norm_of_rows_far_from_zero(ctx, n, dtype):
+    """Rows around a large value, whose deviations the first mean's roundings would drown."""
+    g = rng(n, 7)
+    x, xv, _ = made(g.normal(size=(5, n)) + 300.0, dtype)
+    o, ov, _ = made(g.normal(size=(5, n)) - 900.0, dtype)
+    r, u, _ = block.block_norm(ctx, x, o, kind="layer", stats=True)
+    ctx.sync()
+    how = dict(kind="layer", post=True, scale=1.0, gate_apply="identity", post_weight=None, post_bias=None,
+               pre_weight=None, pre_bias=None)
+    wr, rerr, wu, uerr, _ = block_forward(xv, ov, None, how, float(np.float32(1e-5)))
+    within(f64(r), wr, stored(wr, rerr, dtype), "r")
+    within(f64(u), wu, stored(wu, uerr, dtype), "u")
+
+
 def test_block_norm_in_place(ctx):
     g = torch.Generator(device="cuda").manual_seed(5)
     x = torch.randn(30, 515, device="cuda", generator=g)
@@ -369,6 +438,13 @@ STREAMS = [  # streams, steps, n, dtype, kind, mix, extra row stride, shift
     (1, 6000, 34, "f32", "sigmoid", False, 0, 0),
     (4, 2500, 20, "bf16", "decay", True, 0, 0),
     (9, 65, 257, "bf16", "sigmoid", True, 0, 0),
+    (1, 5000, 72, "bf16", "sigmoid", True, 0, 0),  # whole tiles at a time, in parts
+    (2, 700, 192, "f32", "decay", True, 0, 0),
+    (3, 1500, 64, "f16", "decay", False, 8, 8),
+    (1200, 30, 264, "bf16", "sigmoid", True, 0, 0),  # several streams a walk
+    (700, 100, 128, "f32", "sigmoid", False, 0, 0),
+    (1, 64, 16, "bf16", "sigmoid", True, 0, 0),
+    (2, 33, 64, "bf16", "sigmoid", True, 0, 0),
 ]
 
 
@@ -486,6 +562,7 @@ RAGGED = [  # offsets, rows, n, dtype, kind, mix
     (list(range(0, 201)), 200, 40, "f32", "sigmoid", True),
     ([0, 128, 256, 257, 4000], 4000, 33, "f16", "decay", True),
     ([7, 2400], 2500, 64, "f32", "sigmoid", False),
+    ([0, 3, 3, 70, 1000, 1064, 1065, 3000], 3001, 72, "bf16", "sigmoid", True),
 ]
 
 
@@ -532,13 +609,13 @@ def test_streams_keep_to_themselves(ctx):
         assert torch.equal(dstate[s], dstate2[s])
 
 
-@pytest.mark.parametrize("steps", [1, 5, 700])
-def test_recurrence_in_place_and_in_parts(ctx, steps):
-    """A step in place; and a stream cut in two has the values of the whole."""
+@pytest.mark.parametrize("streams, steps, dtype", [(6, 1, "f32"), (6, 5, "f32"), (6, 700, "f32"), (6, 700, "bf16"),
+                                                   (5000, 40, "bf16"), (6, 60, "bf16"), (6, 1, "f16")])
+def test_recurrence_in_place(ctx, streams, steps, dtype):
     g = torch.Generator(device="cuda").manual_seed(4)
-    x = torch.randn(6, steps, 48, device="cuda", generator=g)
-    gate = torch.randn(6, steps, 48, device="cuda", generator=g)
-    state = torch.randn(6, 48, device="cuda", generator=g)
+    x = torch.randn(streams, steps, 48, device="cuda", generator=g).to(TYPES[dtype])
+    gate = torch.randn(streams, steps, 48, device="cuda", generator=g).to(TYPES[dtype])
+    state = torch.randn(streams, 48, device="cuda", generator=g)
     h, final = block.recurrence(ctx, x, gate, state)
     for where in ("x", "gate"):
         t = {"x": x.clone(), "gate": gate.clone()}
@@ -546,8 +623,48 @@ def test_recurrence_in_place_and_in_parts(ctx, steps):
         h2, f2 = block.recurrence(ctx, t["x"], t["gate"], st, out=t[where], final_out=st)
         assert h2 is t[where] and f2 is st and torch.equal(h2, h) and torch.equal(st, final)
     empty, same = block.recurrence(ctx, x[:, :0], gate[:, :0], state)
-    assert empty.shape == (6, 0, 48) and torch.equal(same, state)
+    assert empty.shape == (streams, 0, 48) and torch.equal(same, state)
     ctx.sync()
+
+
+def test_a_stream_in_two_calls_has_the_values_of_one(ctx):
+    """The state that a call leaves is what the next one goes on from: to the last bit where the cut is
+    between tiles that are walked in the same order."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.randn(1, 128, 64, device="cuda", generator=g)
+    gate = torch.randn(1, 128, 64, device="cuda", generator=g) + 2
+    h, final = block.recurrence(ctx, x, gate)
+    one, state = block.recurrence(ctx, x[:, :64], gate[:, :64])
+    two, last = block.recurrence(ctx, x[:, 64:], gate[:, 64:], state)
+    ctx.sync()
+    both = torch.cat([one, two], 1)
+    # values of order one through a hundred roundings of half a step at most
+    assert (both - h).abs().max() < 100 * U * 4 and (last - final).abs().max() < 100 * U * 4
+
+
+@pytest.mark.parametrize("rows, cuts", [(None, None), (3000, [0, 10, 10, 1500, 3000])])
+def test_recurrence_backward_in_place_in_c(ctx, rows, cuts):
+    """dx over dh, dgate over gate and dstate over dfinal, as the C interface allows."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    for streams, steps, n in ((40, 6, 24), (3, 900, 64), (2, 333, 31)):
+        if cuts:
+            streams, total, offsets = len(cuts) - 1, rows, torch.tensor(cuts, dtype=torch.int32, device="cuda")
+        else:
+            total, offsets = streams * steps, None
+        shape = (total, n) if cuts else (streams, steps, n)
+        x, gate, dh = (torch.randn(shape, device="cuda", generator=g) for _ in range(3))
+        state, dfinal = (torch.randn(streams, n, device="cuda", generator=g) for _ in range(2))
+        h, _ = block.recurrence(ctx, x, gate, state, mix=True, offsets=offsets)
+        want = block.recurrence_backward(ctx, dh, gate, h, state, x=x, dfinal=dfinal, mix=True, offsets=offsets)
+        size = _abi.lib().plx_recurrence_scratch_bytes(streams, total, n, 0, int(offsets is not None), 1, 1)
+        scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
+        at = None if offsets is None else offsets.data_ptr()
+        _abi.call("plx_recurrence_backward", ctx.handle, streams, total, n, 0, at, dh.data_ptr(), n, x.data_ptr(), n,
+                  gate.data_ptr(), n, 1, 1, h.data_ptr(), n, state.data_ptr(), dfinal.data_ptr(), dh.data_ptr(), n,
+                  gate.data_ptr(), n, dfinal.data_ptr(), scratch.data_ptr(), size)
+        ctx.sync()
+        for a, b in zip((dh, gate, dfinal), want):
+            assert torch.equal(a, b)
 
 
 def test_bad_offsets_are_reported(ctx):
