@@ -30,19 +30,6 @@ int check_block_norm(const plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype,
                      const plx_block_norm_params* p);
 BlockNorm block_norm_of(uint64_t rows, uint32_t n, const plx_block_norm_params* p);
 
-// sigmoid(g) and 1 - sigmoid(g), neither by a difference that cancels.
-struct Sigmoid {
-  float a, keep;
-};
-__device__ __forceinline__ Sigmoid sigmoid(float g) {
-  const float e = exp2_approx(-fabsf(g) * kLog2e), d = 1.0f + e;
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-  r = fmaf(r, fmaf(-d, r, 1.0f), r);
-  const float er = e * r;
-  return g < 0.0f ? Sigmoid{er, r} : Sigmoid{r, er};
-}
-
 // Pieces of a row, STEP values apart; 0 past its end.
 template <int STEP, int NV, int V, typename T>
 __device__ __forceinline__ void load_row(const T* from, int left, Pack<T, V> (&q)[NV]) {

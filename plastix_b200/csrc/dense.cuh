@@ -5,25 +5,12 @@
 
 namespace plx {
 
-// sigmoid(g) and 1 - sigmoid(g), neither by a difference that cancels.
-struct Squash {
-  float a, keep;
-};
-__device__ __forceinline__ Squash squash(float g) {
-  const float e = exp2_approx(-fabsf(g) * kLog2e), d = 1.0f + e;
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-  r = fmaf(r, fmaf(-d, r, 1.0f), r);
-  const float er = e * r;
-  return g < 0.0f ? Squash{er, r} : Squash{r, er};
-}
-
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
-  if constexpr (ACT == PLX_ACT_SIGMOID) return squash(z).a;
+  if constexpr (ACT == PLX_ACT_SIGMOID) return sigmoid(z).a;
   else if constexpr (ACT == PLX_ACT_TANH) return tanhf(z);
   else if constexpr (ACT == PLX_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
-  else if constexpr (ACT == PLX_ACT_SILU) return z * squash(z).a;
+  else if constexpr (ACT == PLX_ACT_SILU) return z * sigmoid(z).a;
   else if constexpr (ACT == PLX_ACT_GELU)
     return z * (0.5f * erfcf(z * -0.70710678118654752f));
   else return z;
@@ -33,24 +20,19 @@ __device__ __forceinline__ float act_value(float z) {
 // 1e-23).
 template <int ACT>
 __device__ __forceinline__ float act_value16(float z) {
-  auto quotient = [](float d) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-    return r;
-  };
   if constexpr (ACT == PLX_ACT_SIGMOID) {
-    return quotient(1.0f + exp2_approx(z * -kLog2e));
+    return rcp_approx(1.0f + exp2_approx(z * -kLog2e));
   } else if constexpr (ACT == PLX_ACT_SILU) {
-    return z * quotient(1.0f + exp2_approx(z * -kLog2e));
+    return z * rcp_approx(1.0f + exp2_approx(z * -kLog2e));
   } else if constexpr (ACT == PLX_ACT_TANH) {
     // (1 - e) / (1 + e), e = exp(-2 |z|); near 0, where that cancels, z - z^3 / 3
     const float a = fabsf(z), e = exp2_approx(a * (-2.0f * kLog2e));
-    const float far = copysignf((1.0f - e) * quotient(1.0f + e), z);
+    const float far = copysignf((1.0f - e) * rcp_approx(1.0f + e), z);
     return a < 0.02f ? fmaf(z * z * z, -1.0f / 3.0f, z) : far;
   } else if constexpr (ACT == PLX_ACT_GELU) {
     // Phi(-|z|) = exp(-z^2 / 2) times a polynomial in t = 1 / (1 + 0.3 |z|) without a
     // constant, fitted for the least relative error over |z| <= 10
-    const float t = quotient(fmaf(fabsf(z), 0.3f, 1.0f));
+    const float t = rcp_approx(fmaf(fabsf(z), 0.3f, 1.0f));
     float q = -0.08074618130922318f;
     q = fmaf(q, t, 0.22719280421733856f);
     q = fmaf(q, t, -0.029975734651088715f);
@@ -66,7 +48,7 @@ __device__ __forceinline__ float act_value16(float z) {
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
   if constexpr (ACT == PLX_ACT_SIGMOID) {
-    const Squash s = squash(z);
+    const Sigmoid s = sigmoid(z);
     return s.a * s.keep;
   } else if constexpr (ACT == PLX_ACT_TANH) {
     const float t = tanhf(z);
@@ -74,7 +56,7 @@ __device__ __forceinline__ float act_slope(float z) {
   } else if constexpr (ACT == PLX_ACT_RELU) {
     return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
   } else if constexpr (ACT == PLX_ACT_SILU) {
-    const Squash s = squash(z);
+    const Sigmoid s = sigmoid(z);
     return s.a * fmaf(z, s.keep, 1.0f);
   } else if constexpr (ACT == PLX_ACT_GELU) {
     const float pdf = 0.39894228040143268f * exp2_approx(-0.5f * kLog2e * z * z);

@@ -371,6 +371,7 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
       constexpr uint32_t kHalves = kWide / 32;
       const uint32_t row0 = i - lane, col0 = ib * BN + side * (BN / 2);
       constexpr bool staged = S::pieces > 0;
+      constexpr uint32_t kFirst = kChunks < kPieces ? kChunks : kPieces;  // under way at once
       auto piece = [&](uint32_t c) { return out + ((warp - 2) * kPieces + c % kPieces) * 4096; };
       auto there = [&](uint32_t c) { return row0 < p.rows && col0 + c * kWide < p.cols; };
       auto fetch = [&](uint32_t c) {  // by one lane, which has stored what was there
@@ -380,9 +381,11 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
         tensor_load(piece(c), &p.residual, (int)(col0 + c * kWide), (int)row0, bar);
       };
       const bool fetched = staged && wide && p.f.residual;
-      if (fetched && lane == 0) {
-        bulk_wait_read<0>();
-        for (uint32_t c = 0; c < kChunks && c < kPieces; ++c) fetch(c);
+      if constexpr (staged) {
+        if (fetched && lane == 0) {
+          bulk_wait_read<0>();
+          for (uint32_t c = 0; c < kFirst; ++c) fetch(c);
+        }
       }
       const uint32_t column = sums + (quarter << 21) + (BN < 32 ? 0 : side * (BN / 2));
       bool sound = true;
@@ -421,9 +424,11 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
       constexpr int kUnroll = S::by_stage ? 8 : 1;  // registers have no addresses
       if constexpr (MODE == SPLIT) cluster_wait();
       if (!sound && MODE != SPLIT) {
-        if (fetched && lane == 0)  // what is still on its way
-          for (uint32_t c = 0; c < kChunks && c < kPieces; ++c)
-            if (there(c)) mbar_wait_bounded(&arrived[warp - 2][c], arrivals >> c & 1, p.timeout_ns);
+        if constexpr (staged)
+          if (fetched && lane == 0)  // what is still on its way
+            for (uint32_t c = 0; c < kFirst; ++c)
+              if (there(c))
+                mbar_wait_bounded(&arrived[warp - 2][c], arrivals >> c & 1, p.timeout_ns);
         break;
       }
       if constexpr (staged) {

@@ -79,11 +79,6 @@ __device__ __forceinline__ Pack<T, V> narrow(Units<V> v) {
   return q;
 }
 
-__device__ __forceinline__ float rcp_approx(float d) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-  return r;
-}
 // The larger of each value and -87 (NaN stays NaN): e^87 is a 32-bit number.
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> at_least_minus_87(Pack<T, V> q) {

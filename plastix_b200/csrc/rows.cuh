@@ -126,6 +126,24 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return r;
 }
 constexpr float kLog2e = 1.4426950408889634f;
+// 1 / x by the special-function unit (off by 2^-23 at most).
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// sigmoid(g) and 1 - sigmoid(g), neither by a difference that cancels.
+struct Sigmoid {
+  float a, keep;
+};
+__device__ __forceinline__ Sigmoid sigmoid(float g) {
+  const float e = exp2_approx(-fabsf(g) * kLog2e), d = 1.0f + e;
+  float r = rcp_approx(d);
+  r = fmaf(r, fmaf(-d, r, 1.0f), r);
+  const float er = e * r;
+  return g < 0.0f ? Sigmoid{er, r} : Sigmoid{r, er};
+}
 
 }  // namespace plx
 

@@ -30,7 +30,7 @@ int encoder(Encode* out) {
 
 int tensor_map(CUtensorMap* map, int dtype, const void* p, uint64_t inner, uint64_t outer,
                int64_t ld, uint32_t box_inner, uint32_t box_outer, bool swizzle) {
-  Encode encode;
+  Encode encode = nullptr;
   if (int rc = encoder(&encode)) return rc;
   const cuuint64_t dims[2] = {inner, outer};
   const cuuint64_t strides[1] = {(cuuint64_t)ld * dtype_bytes(dtype)};
