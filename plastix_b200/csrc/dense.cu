@@ -9,7 +9,8 @@
 // 32-bit values are cut into three bfloat16 values whose sum they are, toward zero, so
 // that all have one sign; of the nine products of parts six are made, the others are
 // below 2^-24 of the value's. A part that would be 0 is the first one times 2^-30 or
-// 2^-40, so that an infinity beside it stays one.
+// 2^-40, so that an infinity beside it stays one (values below 2^-100 have no room for
+// all parts).
 #include "dense.cuh"
 
 namespace plx {

@@ -4,17 +4,22 @@
 // Units are independent; steps are folded as pairs (A, H): a run of steps takes
 // what it is given, h, to A h + H, and two runs join to (A1 A2, A2 H1 + H2).
 //
-// Bound by memory. Long streams are walked by a block each (32 or 64 units),
-// tile after tile of 64 steps, the next tiles on their way into shared memory: a
-// warp has a run of eight steps, whose pairs are joined behind one barrier a tile. Where that leaves
+// Bound by memory. Long streams are walked by a block each (64 units), tile after
+// tile of 64 steps, the next tiles on their way into shared memory: a warp has a run
+// of eight steps, whose pairs are joined behind one barrier a tile. Where that leaves
 // SMs idle (few streams of few units) or streams have lengths that only the device
 // knows, rows are cut into parts: a first kernel leaves every part's pair, the
 // second folds those before its own and walks again with results. Reading twice
 // costs less than parts that wait for one another: tiles that look back over the
-// ones before them took 205 us for 65,536 steps of 512 units.
-// Short streams are taken in tiles, several to a block: a warp has the steps of
-// one run, runs are joined through shared memory, values stay in registers.
+// ones before them took 205 us for 65,536 steps of 512 units. Short streams are taken
+// in tiles that hold them whole: values stay in registers between the two walks.
 // Everything is folded in an order that the arguments set.
+// Measured: 8 streams of 2,048 steps of 4,096 units bf16, sigmoid gates, mixed,
+// forwards and backwards 225 us, 5.4 TB/s (205 without the Newton step in a, whose
+// error a long memory shows; 477 with a lane's own copies in place of tensor copies);
+// 65,536 steps of 512 units 72 us, 2.8 TB/s of what has to be read (4.7 of what is);
+// 37 ragged streams of 20,017 steps of 501 units f32 (no multiple of 16 bytes), both
+// ways, 124 us, 2.6 TB/s (3.5 of what is read).
 #include <type_traits>
 
 #include "norm.cuh"
