@@ -24,7 +24,8 @@
 // stored from registers, 16 bytes a lane, and biases read one by one took 24 us a tile
 // to finish, now 11, beside 29 of products. What is left is the tiles' operands out of
 // L2: 454 ns for 64 values of k where the tensor cores need 280 at full clock. 1,501 x
-// 1,001 x 777 f32 34 us (library 73); 8 rows against 4,096 x 4,096 weights 13 us, of
+// 1,001 x 777 f32 34 us (library 73), its weights' gradient on wide tiles shared by two
+// blocks 29 (64), on tiles of 64 columns 45; 8 rows against 4,096 x 4,096 weights 13 us, of
 // which 5 are memory's, the rest start, joining and finish.
 #include <algorithm>
 
@@ -48,15 +49,19 @@ struct Stages {
   static constexpr uint32_t b_rows = MODE == PAIR ? BN / 2 : BN;  // a block's
   static constexpr uint32_t a_bytes = kTileA * kTileK * 2, b_bytes = b_rows * kTileK * 2;
   static constexpr uint32_t bytes = planes * (a_bytes + b_bytes);
-  // sums that the blocks of a cluster are sent, of a tile in all
-  static constexpr uint32_t sums = MODE == SPLIT ? (BN + 4) * kTileA * 4 : 0;
+  // Sums that the blocks of a cluster are sent, of a tile in all; in the ring's place
+  // where all blocks are done with that first (by_stage: sums are in registers).
+  static constexpr uint32_t sent = MODE == SPLIT ? (BN + 4) * kTileA * 4 : 0;
+  static constexpr uint32_t sums = by_stage ? 0 : sent;
   // pieces of results (32 rows of 128 bytes) on their way out, of each warp
-  static constexpr uint32_t pieces = MODE == SPLIT || BN < 128 ? 0 : MODE == PAIR || sizeof(T) == 2 ? 2 : 1;
+  static constexpr uint32_t pieces =
+      MODE == SPLIT || BN < 128 ? 0 : MODE == PAIR || sizeof(T) == 2 ? 2 : 1;
 
   static constexpr uint32_t out = pieces * kFinishWarps * 4096;
   static constexpr uint32_t most = (kSmem - 2048 - sums - out) / bytes;
   static constexpr uint32_t count = most < 12 ? most : 12;
   static_assert(count >= 2, "copies beside products");
+  static_assert(!by_stage || count * bytes >= sent, "room for sums");
   static constexpr uint32_t smem = count * bytes + out + sums + 1024;  // to a multiple of 1,024
   static constexpr uint32_t columns = 2 * BN < 32 ? 32 : 2 * BN;
 };
@@ -88,7 +93,8 @@ __device__ __forceinline__ void activate(int act, float (&v)[C]) {
   auto all = [&](auto a) {
 #pragma unroll
     for (int i = 0; i < C; ++i)
-      v[i] = sizeof(T) == 2 ? act_value16<decltype(a)::value>(v[i]) : act_value<decltype(a)::value>(v[i]);
+      v[i] = sizeof(T) == 2 ? act_value16<decltype(a)::value>(v[i])
+                            : act_value<decltype(a)::value>(v[i]);
   };
   using std::integral_constant;
   switch (act) {
@@ -198,7 +204,7 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
   extern __shared__ __align__(128) uint8_t product_bytes[];
   uint8_t* ring = product_bytes + (1024 - (smem_addr(product_bytes) & 1023)) % 1024;
   uint8_t* out = ring + S::count * S::bytes;
-  float* sent = reinterpret_cast<float*>(out + S::out);
+  float* sent = reinterpret_cast<float*>(S::by_stage ? ring : out + S::out);
   constexpr int kPieces = S::pieces ? S::pieces : 1;
   __shared__ uint64_t arrived[kFinishWarps][kPieces];  // the residual's piece is there
   __shared__ uint64_t full[S::count], empty[S::count], done[2], taken[2];
@@ -283,9 +289,14 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
   if (warp == 1) tmem_alloc<TWO>(&tmem, S::columns);
   tmem_fence_before();
   __syncthreads();
-  // the others' barriers and memory are there (SPLIT: by the time that sums are sent)
+  // The others' barriers are there; SPLIT: and their memory, by the time that sums are
+  // sent (by_stage: once they have made their sums).
   if constexpr (TWO) cluster_barrier();
-  if constexpr (MODE == SPLIT) cluster_arrive();
+  if constexpr (MODE == SPLIT && !S::by_stage) cluster_arrive();
+  auto others_ready = [&] {
+    if constexpr (S::by_stage) cluster_arrive();
+    cluster_wait();
+  };
   tmem_fence_after();
   const uint32_t sums = *(volatile uint32_t*)&tmem;
 
@@ -430,7 +441,7 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
         }
       };
       constexpr int kUnroll = S::by_stage ? 8 : 1;  // registers have no addresses
-      if constexpr (MODE == SPLIT) cluster_wait();
+      if constexpr (MODE == SPLIT) others_ready();
       if (!sound && MODE != SPLIT) {
         if constexpr (staged)
           if (fetched && lane == 0)  // what is still on its way
@@ -441,7 +452,9 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
       }
       if constexpr (staged) {
         // of this lane's row, the 16-byte chunk k of a piece; and value `col` of a row
-        auto chunk = [&](uint8_t* of, uint32_t k) { return of + lane * 128 + ((k ^ (lane & 7)) << 4); };
+        auto chunk = [&](uint8_t* of, uint32_t k) {
+          return of + lane * 128 + ((k ^ (lane & 7)) << 4);
+        };
         auto value = [&](auto* of, uint32_t row, uint32_t col) {
           using Q = std::remove_pointer_t<decltype(of)>;
           const uint32_t byte = col * sizeof(Q);
@@ -602,7 +615,8 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
     if (S::pieces && lane == 0) bulk_wait_all<0>();
   }
   __syncwarp();
-  if (MODE == SPLIT && warp < 2) cluster_wait();
+  if constexpr (MODE == SPLIT)
+    if (warp < 2) others_ready();
   tmem_fence_before();
   __syncthreads();
   if constexpr (MODE != ONE) cluster_barrier();  // SPLIT: every block's sums are there
@@ -646,7 +660,8 @@ int launch(plx_ctx* ctx, TensorProduct& t, const Product& p, const Operand& a, c
     for (int plane = 0; plane < (int)S::planes; ++plane)
       if (int rc = tensor_map(&m[plane], bf16 ? PLX_BF16 : PLX_F16,
                               (const char*)o.p + plane * o.plane, o.k_major ? t.depth : count,
-                              o.k_major ? count : t.depth, o.ld, 64, o.k_major ? tile : kTileK, true))
+                              o.k_major ? count : t.depth, o.ld, 64,
+                              o.k_major ? tile : kTileK, true))
         return rc;
     return PLX_OK;
   };
@@ -711,13 +726,17 @@ int product_tensor(plx_ctx* ctx, int dtype, const Product& p) {
   // What the tiles of a width take: rounds of blocks, each with its share of k (a unit is
   // the products of 64 values of k by one column). A block waits for its products or
   // for its operands, of 128 + width rows; starting and finishing a tile takes 500
-  // units, sending and joining a shared one's sums another 500.
+  // units, sending and joining a shared one's sums another 500, of wide tiles of 32-bit
+  // values more. Blocks of a cluster are neighbours, so that 33 clusters of 4 and 15 of 8
+  // have room at once; one more waits for a whole round (256 x 1,024 x 1,024 f32 on 16
+  // clusters of 8: 23 us; on tiles of 64 columns 15).
   const bool f32 = dtype == PLX_F32;
   const uint32_t sms = (uint32_t)ctx->num_sms, ks = (p.depth + kTileK - 1) / kTileK;
   // by products; by their operands out of shared memory; by copies into it
   auto step_of = [&](uint32_t width, uint32_t b_rows) {
     const double read = 128 + b_rows;
-    return std::max({(f32 ? 6.3 : 1.05) * width, (f32 ? 3.45 : 0.575) * read, (f32 ? 2.7 : 0.9) * read});
+    return std::max({(f32 ? 6.3 : 1.05) * width, (f32 ? 3.45 : 0.575) * read,
+                     (f32 ? 2.7 : 0.9) * read});
   };
   uint32_t bn = 0, parts = 1;
   bool pair = false;
@@ -729,10 +748,12 @@ int product_tensor(plx_ctx* ctx, int dtype, const Product& p) {
     const uint64_t tiles =
         (uint64_t)((t.rows + kTileA - 1) / kTileA) * ((t.cols + width - 1) / width);
     for (uint32_t s = 1; s <= 8; s *= 2) {
-      if (s > 1 && (tiles * s > sms || s > ks || width > (f32 ? 64 : 128))) break;
+      const uint32_t room = s < 4 ? sms : s == 4 ? sms * 8 / 9 : sms * 4 / 5;
+      if (s > 1 && (tiles * s > room || s > ks || width > 128)) break;
       const double rounds = (double)((tiles * s + sms - 1) / sms);
       const double took =
-          rounds * (step_of(width, width) * ((ks + s - 1) / s) + (s > 1 ? 1000 : 500));
+          rounds * (step_of(width, width) * ((ks + s - 1) / s) +
+                    (s == 1 ? 500 : f32 && width == 128 ? 1300 + 150 * s : 1000));
       if (bn == 0 || took < best) {
         best = took;
         bn = width;
@@ -755,12 +776,14 @@ int product_tensor(plx_ctx* ctx, int dtype, const Product& p) {
     switch (bn) {
       case 256: return launch<T, WIDEST, ONE>(ctx, t, p, a, b, parts, wide);
       case 128:
-        if constexpr (sizeof(T) == 2)
-          if (split) return launch<T, 128, SPLIT>(ctx, t, p, a, b, parts, wide);
-        return launch<T, 128, ONE>(ctx, t, p, a, b, parts, wide);
-      case 64: return (split ? launch<T, 64, SPLIT> : launch<T, 64, ONE>)(ctx, t, p, a, b, parts, wide);
-      case 32: return (split ? launch<T, 32, SPLIT> : launch<T, 32, ONE>)(ctx, t, p, a, b, parts, wide);
-      default: return (split ? launch<T, 16, SPLIT> : launch<T, 16, ONE>)(ctx, t, p, a, b, parts, wide);
+        return (split ? launch<T, 128, SPLIT> : launch<T, 128, ONE>)(ctx, t, p, a, b, parts,
+                                                                     wide);
+      case 64:
+        return (split ? launch<T, 64, SPLIT> : launch<T, 64, ONE>)(ctx, t, p, a, b, parts, wide);
+      case 32:
+        return (split ? launch<T, 32, SPLIT> : launch<T, 32, ONE>)(ctx, t, p, a, b, parts, wide);
+      default:
+        return (split ? launch<T, 16, SPLIT> : launch<T, 16, ONE>)(ctx, t, p, a, b, parts, wide);
     }
   };
   return with_dtype(dtype, go);

@@ -79,6 +79,11 @@ DENSE = [  # rows, n, m, dtype, apply, residual, extra row stride, shift, param
     (3, 1000, 300, "f32", "gelu", True, 1, 1, "f32"),
     (7, 515, 130, "f32", "relu", False, 1, 0, "f32"),
     (65, 1000, 33, "f16", "silu", True, 0, 0, "f32"),
+    # wide tiles of 32-bit values, sums shared by 2, 4 and 8 blocks
+    (1000, 600, 1024, "f32", "silu", True, 0, 0, "f32"),
+    (513, 1001, 1020, "f32", "gelu", True, 1, 1, "f32"),
+    (250, 1023, 1000, "f32", "tanh", False, 0, 0, "f32"),
+    (1000, 1024, 129, "f32", "identity", True, 4, 0, "f32"),
 ]
 
 
