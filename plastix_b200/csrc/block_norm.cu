@@ -308,7 +308,8 @@ extern "C" int plx_block_norm(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype
         auto with = [&](auto bias_c, auto values_c) -> int {
           constexpr bool VALUES = decltype(values_c)::value;
           using R = BlockRing<T, VV, NV, TPR, VALUES ? 3 : 2, kStages<T>>;
-          constexpr auto kernel = k_block_norm<T, VV, NV, TPR, decltype(bias_c)::value, VALUES, EACH>;
+          constexpr auto kernel =
+              k_block_norm<T, VV, NV, TPR, decltype(bias_c)::value, VALUES, EACH>;
           if (R::bytes > 32 * 1024) PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, R::bytes));
           const unsigned grid = (unsigned)std::min<uint64_t>((rows + per_block - 1) / per_block,
                                                              (uint64_t)ctx->num_sms * EACH);

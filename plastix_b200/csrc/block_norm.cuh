@@ -57,7 +57,8 @@ struct Columns {
   using P = Pack<T, V>;
   uint32_t c0;
   int left;  // values from the first column to the row's end
-  __device__ __forceinline__ Columns(uint32_t n, uint32_t first) : c0(first), left((int)n - (int)first) {}
+  __device__ __forceinline__ Columns(uint32_t n, uint32_t first)
+      : c0(first), left((int)n - (int)first) {}
   __device__ __forceinline__ bool in(int group) const { return group * GSTEP < left; }
   // whether the second value of a pair is in the row as well
   __device__ __forceinline__ bool both(int group) const {
@@ -94,7 +95,8 @@ struct Columns {
     for (int g = 0; g < G; ++g) {
       if constexpr (V == 1) {
         const Q* at = w + c0 + g * GSTEP;
-        v[g] = pack2(w && in(g) ? to_f32(at[0]) : none, w && in(g) && both(g) ? to_f32(at[STEP]) : none);
+        v[g] = pack2(w && in(g) ? to_f32(at[0]) : none,
+                     w && in(g) && both(g) ? to_f32(at[STEP]) : none);
       } else if (w && in(g)) {
         const Pack<Q, V> q = load_pack<Q, V>(w + c0 + g * GSTEP);
 #pragma unroll

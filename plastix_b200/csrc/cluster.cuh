@@ -29,7 +29,8 @@ __device__ __forceinline__ uint32_t peer_smem(const void* p, uint32_t rank) {
   return r;
 }
 __device__ __forceinline__ void st_peer(uint32_t at, float2 v) {
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.x), "f"(v.y) : "memory");
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.x), "f"(v.y)
+               : "memory");
 }
 __device__ __forceinline__ void st_peer(uint32_t at, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");

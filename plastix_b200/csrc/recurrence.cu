@@ -395,7 +395,8 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const W zero = all<W>(0.0f);
 
-  if (p.offsets && !LEAVE) {  // offsets that no rows have; streams without steps hand their state on
+  // offsets that no rows have; streams without steps hand their state on
+  if (p.offsets && !LEAVE) {
     for (uint32_t s = blockIdx.x; s < p.streams; s += gridDim.x) {
       const int64_t begin = p.offsets[s], end = p.offsets[s + 1];
       if (threadIdx.x == 0 && (begin < 0 || begin > end || (uint64_t)end > p.rows))
@@ -434,7 +435,8 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
   auto fetch = [&](uint32_t stage) {
     if constexpr (TENSOR) {  // by one thread
       if (fetched < tiles) {
-        const int y = (int)(row0 + (FROM_END ? tiles - 1 - fetched : fetched) * (int64_t)kWalkSteps);
+        const int64_t tile = FROM_END ? tiles - 1 - fetched : fetched;
+        const int y = (int)(row0 + tile * kWalkSteps);
         mbar_arrive_expect_tx(&full[stage], R::stage);
 #pragma unroll
         for (int k = 0; k < ARRAYS; ++k)
@@ -465,7 +467,8 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
         for (uint32_t j = 0; j < before; ++j) {
           const uint32_t q = group * p.parts + (BACK ? p.parts - 1 - j : j);
           const bool s = p.shut[q] != 0;
-          const Pair v = reinterpret_cast<const Pair*>(p.pairs)[((uint64_t)q * p.tiles + across) * 32 + lane];
+          const Pair v =
+              reinterpret_cast<const Pair*>(p.pairs)[((uint64_t)q * p.tiles + across) * 32 + lane];
           given = s ? v.h : fmaw(v.a, given, v.h);
         }
         runs[0][0][lane].h = given;
@@ -478,7 +481,8 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
   P nothing;
 #pragma unroll
   for (int e = 0; e < V; ++e) nothing.v[e] = from_f32<T>(0.0f);
-  int64_t clear0 = 0, clear1 = 0;  // rows in which no stream begins or ends, and all are some stream's
+  // rows in which no stream begins or ends, and all are some stream's
+  int64_t clear0 = 0, clear1 = 0;
   uint32_t stage = 0, half = 0, parity = 0;
   for (int tile = 0; tile < tiles; ++tile, at += tile_dir * (int)kWalkSteps, half ^= 1) {
     const int len = (int)max((int64_t)0, min((int64_t)kRun, row1 - at));
@@ -751,7 +755,8 @@ int check_recurrence(const plx_ctx* ctx, uint32_t streams, uint64_t rows, uint32
   PLX_CHECK_ARG(offsets || streams == 0 || rows % streams == 0,
                 "%llu rows are not the same number of steps for each of %u streams",
                 (unsigned long long)rows, streams);
-  const size_t need = plx_recurrence_scratch_bytes(streams, rows, n, dtype, offsets != nullptr, mix, back);
+  const size_t need =
+      plx_recurrence_scratch_bytes(streams, rows, n, dtype, offsets != nullptr, mix, back);
   PLX_CHECK_ARG(need == 0 || (scratch && scratch_bytes >= need),
                 "%zu bytes of scratch are needed, got %zu", need,
                 scratch ? scratch_bytes : (size_t)0);
@@ -891,8 +896,8 @@ extern "C" int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, u
                               const void* gate, int64_t ldg, int gate_kind, int mix,
                               const float* state, void* h, int64_t ldh, float* final_state,
                               void* scratch, size_t scratch_bytes) {
-  if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, mix, false, scratch,
-                                scratch_bytes))
+  if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, mix, false,
+                                scratch, scratch_bytes))
     return rc;
   if (rows) PLX_CHECK_ARG(x && gate && h, "x, gate and h are required");
   PLX_CHECK_ARG(rows <= 1 || (ldx >= (int64_t)n && ldg >= (int64_t)n && ldh >= (int64_t)n),
@@ -922,8 +927,8 @@ extern "C" int plx_recurrence_backward(plx_ctx* ctx, uint32_t n_streams, uint64_
                                        int64_t ldh, const float* state, const float* dfinal,
                                        void* dx, int64_t lddx, void* dgate, int64_t lddg,
                                        float* dstate, void* scratch, size_t scratch_bytes) {
-  if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, mix, true, scratch,
-                                scratch_bytes))
+  if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, mix, true,
+                                scratch, scratch_bytes))
     return rc;
   if (rows) {
     PLX_CHECK_ARG(dh && gate && h && dx && dgate, "dh, gate, h, dx and dgate are required");
