@@ -619,8 +619,8 @@ size_t plx_layer_norm_scratch_bytes(uint64_t rows, uint32_t n);
 /* Gradients of layer norm: dx [rows, n] and, of type param_dtype, dweight and
  * dbias [n], each written where not NULL (dweight and dbias are the sums over
  * all rows, added in an order that rows, n, the types and the arrays'
- * alignment set: the same bits on every call; zero for rows = 0). scratch is 16-byte aligned and may
- * hold anything; calls that run at once need scratch of their own. */
+ * alignment set: the same bits on every call; zero for rows = 0). scratch is
+ * 16-byte aligned and may hold anything; calls that run at once need scratch of their own. */
 int plx_layer_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* dy,
                             int64_t lddy, const void* x, int64_t ldx, const float* mean,
                             const float* rstd, int param_dtype, const void* weight, void* dx,
@@ -809,10 +809,18 @@ int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n, 
                    int64_t ldg, int gate_kind, int mix, const float* state, void* h, int64_t ldh,
                    float* final_state, void* scratch, size_t scratch_bytes);
 
+/* The same into an h whose values are of no use: its rows of no stream become
+ * zero. */
+int plx_recurrence_new(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n, int dtype,
+                       const int32_t* offsets, const void* x, int64_t ldx, const void* gate,
+                       int64_t ldg, int gate_kind, int mix, const float* state, void* h,
+                       int64_t ldh, float* final_state, void* scratch, size_t scratch_bytes);
+
 /* Gradients of sum(dh * h) + sum(dfinal * final_state): dx, dgate [rows, n] and,
- * where not NULL, dstate [n_streams, n]. h as plx_recurrence wrote it; x is
- * needed with mix alone; state and dfinal may be NULL for 0. dx and dgate may be
- * the arrays of dh, x or gate, not h's; dstate may be dfinal's. */
+ * where not NULL, dstate [n_streams, n]; dx and dgate are zero in rows of no
+ * stream, whatever dh has there. h as plx_recurrence wrote it; x is needed with
+ * mix alone; state and dfinal may be NULL for 0. dx and dgate may be the arrays of
+ * dh, x or gate, not h's; dstate may be dfinal's. */
 int plx_recurrence_backward(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n, int dtype,
                             const int32_t* offsets, const void* dh, int64_t lddh, const void* x,
                             int64_t ldx, const void* gate, int64_t ldg, int gate_kind, int mix,

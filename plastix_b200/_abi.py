@@ -241,6 +241,9 @@ _SIGNATURES = {
     "plx_recurrence": (c_int, [c_void_p, c_uint32, c_uint64, c_uint32, c_int, c_void_p, c_void_p,
                                c_int64, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p,
                                c_int64, c_void_p, c_void_p, ctypes.c_size_t]),
+    "plx_recurrence_new": (c_int, [c_void_p, c_uint32, c_uint64, c_uint32, c_int, c_void_p,
+                                   c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_void_p,
+                                   c_void_p, c_int64, c_void_p, c_void_p, ctypes.c_size_t]),
     "plx_recurrence_backward": (c_int, [c_void_p, c_uint32, c_uint64, c_uint32, c_int, c_void_p,
                                         c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                         c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p,

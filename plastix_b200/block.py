@@ -353,10 +353,11 @@ def recurrence(ctx: Context, x: torch.Tensor, gate: torch.Tensor,
     ``gate`` are [streams, steps, n], [steps, n] for one stream, or with
     ``offsets`` (int32 [streams + 1]) [rows, n] with stream s in the rows from
     offsets[s] to before offsets[s + 1]; rows of no stream are left as they
-    are. a is the gate ("decay") or its sigmoid ("sigmoid"). ``state`` [streams,
-    n] in float32 is h before the first steps (None: 0), ``final`` h after the
-    last ones, what ``state`` was for streams without steps. ``out`` may be x
-    or gate, ``final_out`` state: a step in place."""
+    are in ``out``, and zero in a new h. a is the gate ("decay") or its sigmoid
+    ("sigmoid"). ``state`` [streams, n] in float32 is h before the first steps
+    (None: 0), ``final`` h after the last ones, what ``state`` was for streams
+    without steps. ``out`` may be x or gate, ``final_out`` state: a step in
+    place."""
     rows, n, ldx, dtype = _plain_rows(ctx, x, "x")
     ldg = _same_rows(ctx, gate, x, "gate", "x")
     gate_kind = _one_of(_GATES, kind, "kind")
@@ -378,9 +379,9 @@ def recurrence(ctx: Context, x: torch.Tensor, gate: torch.Tensor,
         size = _abi.lib().plx_recurrence_scratch_bytes(streams, rows, n, dtype,
                                                        offsets is not None, int(mix), 0)
         scratch = x.new_empty(size, dtype=torch.uint8) if size else None
-        _abi.call("plx_recurrence", ctx.handle, streams, rows, n, dtype, offsets_p, x.data_ptr(),
-                  ldx, gate.data_ptr(), ldg, gate_kind, int(mix), state_p, h.data_ptr(), ldh,
-                  final.data_ptr(), _address(scratch), size)
+        _abi.call("plx_recurrence_new" if out is None else "plx_recurrence", ctx.handle, streams,
+                  rows, n, dtype, offsets_p, x.data_ptr(), ldx, gate.data_ptr(), ldg, gate_kind,
+                  int(mix), state_p, h.data_ptr(), ldh, final.data_ptr(), _address(scratch), size)
     return h, final
 
 
@@ -392,7 +393,7 @@ def recurrence_backward(ctx: Context, dh: torch.Tensor, gate: torch.Tensor, h: t
     """(dx, dgate, dstate): gradients of sum(dh * h) + sum(dfinal * final) for
     the arguments of ``recurrence`` and the h that it returned. ``x`` is needed
     with ``mix`` alone; ``dfinal`` may be None. dstate is None without a state.
-    Rows of no stream are left as they are in dx and dgate."""
+    dx and dgate are zero in rows of no stream."""
     rows, n, ldg, dtype = _plain_rows(ctx, gate, "gate")
     lddh = _same_rows(ctx, dh, gate, "dh", "gate")
     ldh = _same_rows(ctx, h, gate, "h", "gate")

@@ -46,6 +46,7 @@ struct Args {
   const float *state, *dfinal;
   void *out, *out2;            // h; or dx and dgate
   int64_t ldo, ldo2;
+  bool clear;                  // rows of no stream become zero (with offsets)
   float* state_out;            // final; or dstate
   float2* pairs;               // of the parts, [group][part][unit]
   uint32_t* shut;              // parts in which a stream begins (ends), [group][part]
@@ -405,6 +406,19 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
       if (begin == end && p.state_out)
         for (uint32_t i = threadIdx.x; i < p.n; i += kWalkWarps * 32)
           p.state_out[(uint64_t)s * p.n + i] = given ? given[(uint64_t)s * p.n + i] : 0.0f;
+    }
+  }
+  // rows before the first stream and behind the last one
+  if (p.clear && !LEAVE) {
+    const int64_t rows = (int64_t)p.rows;
+    const int64_t first = min(max((int64_t)p.offsets[0], (int64_t)0), rows);
+    const int64_t last = min(max((int64_t)p.offsets[p.streams], first), rows);
+    for (int64_t k = blockIdx.x; k < first + rows - last; k += gridDim.x) {
+      const int64_t row = k < first ? k : last + k - first;
+      for (uint32_t i = threadIdx.x; i < p.n; i += kWalkWarps * 32) {
+        ((T*)p.out)[row * p.ldo + i] = from_f32<T>(0.0f);
+        if constexpr (BACK) ((T*)p.out2)[row * p.ldo2 + i] = from_f32<T>(0.0f);
+      }
     }
   }
   const uint32_t across = blockIdx.x % p.tiles, rest = blockIdx.x / p.tiles;
@@ -891,11 +905,11 @@ extern "C" size_t plx_recurrence_scratch_bytes(uint32_t n_streams, uint64_t rows
   return most;
 }
 
-extern "C" int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n,
-                              int dtype, const int32_t* offsets, const void* x, int64_t ldx,
-                              const void* gate, int64_t ldg, int gate_kind, int mix,
-                              const float* state, void* h, int64_t ldh, float* final_state,
-                              void* scratch, size_t scratch_bytes) {
+static int forward(plx_ctx* ctx, bool clear, uint32_t n_streams, uint64_t rows, uint32_t n,
+                   int dtype, const int32_t* offsets, const void* x, int64_t ldx,
+                   const void* gate, int64_t ldg, int gate_kind, int mix, const float* state,
+                   void* h, int64_t ldh, float* final_state, void* scratch,
+                   size_t scratch_bytes) {
   if (int rc = check_recurrence(ctx, n_streams, rows, n, dtype, offsets, gate_kind, mix, false,
                                 scratch, scratch_bytes))
     return rc;
@@ -916,8 +930,27 @@ extern "C" int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, u
   a.state = state;
   a.out = h;
   a.ldo = ldh;
+  a.clear = clear && offsets;
   a.state_out = final_state;
   return launch<false>(ctx, a, dtype, gate_kind, mix != 0, scratch);
+}
+
+extern "C" int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n,
+                              int dtype, const int32_t* offsets, const void* x, int64_t ldx,
+                              const void* gate, int64_t ldg, int gate_kind, int mix,
+                              const float* state, void* h, int64_t ldh, float* final_state,
+                              void* scratch, size_t scratch_bytes) {
+  return forward(ctx, false, n_streams, rows, n, dtype, offsets, x, ldx, gate, ldg, gate_kind,
+                 mix, state, h, ldh, final_state, scratch, scratch_bytes);
+}
+
+extern "C" int plx_recurrence_new(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n,
+                                  int dtype, const int32_t* offsets, const void* x, int64_t ldx,
+                                  const void* gate, int64_t ldg, int gate_kind, int mix,
+                                  const float* state, void* h, int64_t ldh, float* final_state,
+                                  void* scratch, size_t scratch_bytes) {
+  return forward(ctx, true, n_streams, rows, n, dtype, offsets, x, ldx, gate, ldg, gate_kind,
+                 mix, state, h, ldh, final_state, scratch, scratch_bytes);
 }
 
 extern "C" int plx_recurrence_backward(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n,
@@ -958,6 +991,7 @@ extern "C" int plx_recurrence_backward(plx_ctx* ctx, uint32_t n_streams, uint64_
   a.out = dx;
   a.ldo = lddx;
   a.out2 = dgate;
+  a.clear = offsets != nullptr;
   a.ldo2 = lddg;
   a.state_out = dstate;
   return launch<true>(ctx, a, dtype, gate_kind, mix != 0, scratch);

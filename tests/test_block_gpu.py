@@ -579,6 +579,34 @@ def test_recurrence_of_ragged_streams(ctx, cuts, rows, n, dtype, kind, mix):
     check_recurrence(ctx, streams, rows, n, dtype, kind, mix, cuts, offsets, inputs, (rows, n))
 
 
+@pytest.mark.parametrize("cuts, rows, n, dtype", [
+    ([2, 130, 131, 400, 400, 900], 1000, 64, "f32"), ([3, 10], 40, 31, "bf16"), ([5, 5], 9, 8, "f16"),
+    ([0, 3000], 3001, 72, "bf16"), ([9, 2400], 2400, 33, "f32"), ([0, 7, 12], 12, 40, "f32")])
+def test_rows_of_no_stream_are_zero_in_new_results(ctx, cuts, rows, n, dtype):
+    """In memory that held NaN; what a layer's gradients sum over padded rows stays finite."""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    x, gate, dh = (torch.randn(rows, n, device="cuda", generator=g).to(TYPES[dtype]) for _ in range(3))
+    state = torch.zeros(len(cuts) - 1, n, device="cuda")
+    offsets = torch.tensor(cuts, dtype=torch.int32, device="cuda")
+    none = torch.ones(rows, dtype=torch.bool, device="cuda")
+    none[cuts[0]:cuts[-1]] = False
+    for t in (x, gate, dh):
+        t[none] = float("nan")
+    for mix in (False, True):
+        held = [torch.full_like(x, float("nan")) for _ in range(3)]
+        del held
+        h, _ = block.recurrence(ctx, x, gate, state, mix=mix, offsets=offsets)
+        held = [torch.full_like(x, float("nan")) for _ in range(3)]
+        del held
+        dx, dgate, _ = block.recurrence_backward(ctx, dh, gate, h, state, x=x, mix=mix, offsets=offsets)
+        weight = torch.ones(16, n, device="cuda").to(TYPES[dtype])
+        _, dweight, _ = block.dense_backward(ctx, dx @ weight.T, h, weight)
+        ctx.sync()
+        for t in (h, dx, dgate):
+            assert (t[none] == 0).all() and t[~none].isfinite().all()
+        assert dweight.isfinite().all()
+
+
 def test_streams_keep_to_themselves(ctx):
     """NaN and infinity of one stream, and in rows of none, do not reach another."""
     cuts = [2, 130, 131, 400, 400, 900]
