@@ -366,11 +366,13 @@ def recurrence(ctx: Context, x: torch.Tensor, gate: torch.Tensor,
     h, ldh = out, n
     if out is not None:
         ldh = _in_place_of(ctx, out, (x, ldx, "x"), (gate, ldg, "gate"))
+        _check_apart(out, ldh, "out", (state, n, "state"))
     final = final_out
     if final is not None:
         _state(ctx, final, x, streams, "final_out")
         if final.data_ptr() != state_p:
             _check_apart(final, n, "final_out", (state, n, "state"))
+        _check_apart(final, n, "final_out", (x, ldx, "x"), (gate, ldg, "gate"), (out, ldh, "out"))
     with _scope(ctx, x, gate, state, offsets, out, final_out):
         if out is None:
             h = _new(x)

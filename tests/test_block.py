@@ -182,6 +182,19 @@ def test_python_layer_refuses():
             call()
 
 
+def test_states_that_overlap_rows_are_refused():
+    c = FakeContext()
+    flat = torch.zeros(64)
+    rows, x = flat[:32].view(4, 8), torch.zeros(4, 8)
+    for state in (flat[:8].view(1, 8), flat[24:32].view(1, 8)):
+        for call in (lambda: block.recurrence(c, x, x, state, out=rows),
+                     lambda: block.recurrence(c, x, x, out=rows, final_out=state),
+                     lambda: block.recurrence(c, rows, x, final_out=state),
+                     lambda: block.recurrence(c, x, rows, state, final_out=state)):
+            with pytest.raises(ValueError, match="overlaps"):
+                call()
+
+
 def test_results_that_overlap_other_inputs_are_refused():
     c = FakeContext()
     both = torch.zeros(9, 8)
