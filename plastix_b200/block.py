@@ -107,12 +107,11 @@ def _new(like: torch.Tensor) -> torch.Tensor:
 
 def _in_place_of(ctx: Context, out: torch.Tensor, *inputs) -> int:
     """The row stride of ``out``, which may be one of the inputs (tensor, row
-    stride, name) and touches no other. Inputs that are the same tensor count as
-    one."""
+    stride, name) and touches no other. Inputs that are the same rows count as
+    one; rows that only begin where out does are others."""
     ldo = _same_rows(ctx, out, inputs[0][0], "out", inputs[0][2])
-    same = [t for t, ld, _ in inputs if t.data_ptr() == out.data_ptr() and ld == ldo]
-    _check_apart(out, ldo, "out", *((t, ld, name) for t, ld, name in inputs
-                                    if not any(t.data_ptr() == s.data_ptr() for s in same)))
+    _check_apart(out, ldo, "out", *(i for i in inputs
+                                    if i[0].data_ptr() != out.data_ptr() or i[1] != ldo))
     return ldo
 
 
