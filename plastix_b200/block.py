@@ -165,7 +165,7 @@ def dense(ctx: Context, x: torch.Tensor, weight: torch.Tensor,
         ldy = _rows(ctx, out, "out")[2]
         if residual is not None:
             _check_result(out, ldy, residual, ldr, "out")
-        _check_apart(out, ldy, "out", (x, ldx, "x"), (weight, ldw, "weight"))
+        _check_apart(out, ldy, "out", (x, ldx, "x"), (weight, ldw, "weight"), (bias, m, "bias"))
     # aligned rows of 16-bit values need no scratch
     size = 0 if dtype != _abi.F32 and _aligned((x, ldx, rows), (weight, ldw, m)) else \
         _abi.lib().plx_dense_scratch_bytes(rows, n, m, dtype, 0, 0)
@@ -259,7 +259,8 @@ def block_norm(ctx: Context, x: torch.Tensor, o: torch.Tensor,
     as the parameters float32 or x's type), of every unit of every row (like x;
     so is a gate for an x of one dimension), or None for 1; ``gate_apply``
     "sigmoid" takes its sigmoid. With ``stats`` returns (r, u, stats), which
-    ``block_norm_backward`` takes. ``out`` (for r) may be x or o."""
+    ``block_norm_backward`` takes. ``out`` (for r) may be x, o or a gate of
+    every value."""
     rows, n, ldx, dtype = _plain_rows(ctx, x, "x")
     ldo = _same_rows(ctx, o, x, "o", "x")
     p = _block_params(ctx, x, gate, gate_apply, kind, post, scale, eps, post_weight, post_bias,
@@ -270,6 +271,9 @@ def block_norm(ctx: Context, x: torch.Tensor, o: torch.Tensor,
         if p.gate == _abi.BLOCK_GATE_VALUES:
             inputs.append((gate, p.ldg, "gate"))
         ldr = _in_place_of(ctx, out, *inputs)
+        _check_apart(out, ldr, "out", (gate if p.gate == _abi.BLOCK_GATE_UNITS else None, n, "gate"),
+                     (post_weight, n, "post_weight"), (post_bias, n, "post_bias"),
+                     (pre_weight, n, "pre_weight"), (pre_bias, n, "pre_bias"))
     with _scope(ctx, x, o, gate, post_weight, post_bias, pre_weight, pre_bias, out):
         if out is None:
             r = _new(x)
@@ -365,13 +369,14 @@ def recurrence(ctx: Context, x: torch.Tensor, gate: torch.Tensor,
     h, ldh = out, n
     if out is not None:
         ldh = _in_place_of(ctx, out, (x, ldx, "x"), (gate, ldg, "gate"))
-        _check_apart(out, ldh, "out", (state, n, "state"))
+        _check_apart(out, ldh, "out", (state, n, "state"), (offsets, 0, "offsets"))
     final = final_out
     if final is not None:
         _state(ctx, final, x, streams, "final_out")
         if final.data_ptr() != state_p:
             _check_apart(final, n, "final_out", (state, n, "state"))
-        _check_apart(final, n, "final_out", (x, ldx, "x"), (gate, ldg, "gate"), (out, ldh, "out"))
+        _check_apart(final, n, "final_out", (x, ldx, "x"), (gate, ldg, "gate"), (out, ldh, "out"),
+                     (offsets, 0, "offsets"))
     with _scope(ctx, x, gate, state, offsets, out, final_out):
         if out is None:
             h = _new(x)

@@ -20,3 +20,24 @@ def test_inputs_that_begin_where_the_result_does_are_refused_at_another_stride()
                  lambda: block.recurrence(c, apart, rows, out=rows)):
         with pytest.raises(ValueError, match="out overlaps"):
             call()
+
+
+def test_results_over_parameters_are_refused():
+    """Every block reads parameters and offsets while others write results."""
+    c, x = FakeContext(), torch.zeros(4, 16)
+    buf = torch.zeros(6, 16)
+    out, inside = buf[:4], buf[2]
+    w = torch.zeros(16, 16)
+    steps = torch.zeros(4, 16)
+    offsets = steps.view(torch.int32).view(-1)[20:23]
+    held = torch.zeros(2, 16)
+    bad = [lambda: block.dense(c, x, w, inside, out=out),
+           lambda: block.block_norm(c, x, x, inside, out=out),
+           lambda: block.recurrence(c, x, x, offsets=offsets, out=steps),
+           lambda: block.recurrence(c, x, x, offsets=held.view(torch.int32).view(-1)[3:6], final_out=held)]
+    bad += [lambda name=name: block.block_norm(c, x, x, out=out, **{name: inside})
+            for name in ("post_weight", "post_bias", "pre_weight", "pre_bias")]
+    for k, call in enumerate(bad):
+        with pytest.raises(ValueError, match="overlaps"):
+            call()
+            pytest.fail(f"call {k} was not refused")
