@@ -41,3 +41,31 @@ def test_results_over_parameters_are_refused():
         with pytest.raises(ValueError, match="overlaps"):
             call()
             pytest.fail(f"call {k} was not refused")
+
+
+def overlaps(a, b):
+    """Whether two views share an element, by looking at every one."""
+    def touched(t):
+        at = torch.arange(t.untyped_storage().nbytes() // t.element_size())
+        return set(at.as_strided(t.size(), t.stride(), t.storage_offset()).flatten().tolist())
+    return bool(touched(a) & touched(b))
+
+
+def test_rows_side_by_side_are_told_from_rows_that_overlap():
+    """All placements of two tensors of rows in a small buffer: refused where they share an element, and not
+    where one lies beside the other in rows of the same stride."""
+    buf = torch.zeros(80)
+    a = buf.as_strided((3, 4), (11, 1), 15)
+    for n in (1, 3, 5):
+        for ld in (5, 11, 12):
+            for at in range(0, 80 - 2 * ld - n + 1):
+                b = buf.as_strided((3, n), (ld, 1), at)
+                try:
+                    block._check_apart(a, 11, "out", (b, ld, "x"))
+                    refused = False
+                except ValueError:
+                    refused = True
+                if overlaps(a, b):
+                    assert refused, (n, ld, at)
+                elif ld == 11:
+                    assert not refused, (n, at)

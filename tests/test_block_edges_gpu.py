@@ -26,3 +26,24 @@ def test_block_norm_in_place_of_its_gate(ctx, n, dtype):
     r2, u2 = block.block_norm(ctx, x, o, gate, gate_apply="sigmoid", out=gate)
     ctx.sync()
     assert r2 is gate and torch.equal(r2, r) and torch.equal(u2, u)
+
+
+def test_results_beside_their_inputs(ctx):
+    """x and out as the two halves of wider rows."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for n in (64, 77):
+        x, gate = (torch.randn(300, n, device="cuda", generator=g) for _ in range(2))
+        w = torch.randn(n, n, device="cuda", generator=g)
+        want = (block.dense(ctx, x, w), block.block_norm(ctx, x, gate)[0], block.recurrence(ctx, x, gate)[0])
+        for k, call in enumerate((lambda a, b: block.dense(ctx, a, w, out=b),
+                                  lambda a, b: block.block_norm(ctx, a, gate, out=b)[0],
+                                  lambda a, b: block.recurrence(ctx, a, gate, out=b)[0])):
+            wide = torch.zeros(300, 2 * n, device="cuda")
+            wide[:, :n] = x
+            got = call(wide[:, :n], wide[:, n:])
+            ctx.sync()
+            assert torch.equal(wide[:, :n], x)
+            if n == 64:
+                assert torch.equal(got, want[k])
+            else:  # other alignment, and with it another order of sums
+                within(f64(got), f64(want[k]), 1e-4 + 0 * f64(got), "out")
