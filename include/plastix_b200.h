@@ -800,8 +800,10 @@ size_t plx_recurrence_scratch_bytes(uint32_t n_streams, uint64_t rows, uint32_t 
  * or leave [0, rows] make plx_ctx_sync report PLX_ERR_ARG and leave the results
  * unspecified. state [n_streams, n] is h before the first steps (NULL: 0),
  * final_state [n_streams, n] h after the last ones (state where there are none),
- * written where not NULL; it may be state's array. States are in 32 bits, so is
- * h from step to step. h may be x's or gate's array. Sums are folded in an
+ * written where not NULL; it may be state's array. Decays may be of any size and
+ * sign; h is as step by step where that is finite, but for the order of sums (an
+ * error relative to the sum of the magnitudes, which decays above 1 make grow). States
+ * are in 32 bits, so is h from step to step. h may be x's or gate's array. Sums are folded in an
  * order that the arguments set: the same bits on every call. scratch as for
  * plx_dense. */
 int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n, int dtype,

@@ -14,12 +14,20 @@
 // ones before them took 205 us for 65,536 steps of 512 units. Short streams are taken
 // in tiles that hold them whole: values stay in registers between the two walks.
 // Everything is folded in an order that the arguments set.
+// Decays may be of any size, and their product A leaves 32 bits where no h does (200
+// steps of 1.5 before the first x; 1e20, 1e20, 0). Where A h + H is not finite, the run
+// is walked step by step from h instead; where a part's is not, the block before it
+// goes on through it. Units and streams whose pairs are finite keep the same bits. (A
+// product below 2^-149 counts as 0: it would leave less than that of h. Sigmoids are at
+// most 1; behind an infinite x their h may be NaN.)
 // Measured: 8 streams of 2,048 steps of 4,096 units bf16, sigmoid gates, mixed,
 // forwards and backwards 225 us, 5.4 TB/s (205 without the Newton step in a, whose
 // error a long memory shows; 477 with a lane's own copies in place of tensor copies);
 // 65,536 steps of 512 units 72 us, 2.8 TB/s of what has to be read (4.7 of what is);
 // 37 ragged streams of 20,017 steps of 501 units f32 (no multiple of 16 bytes), both
-// ways, 124 us, 2.6 TB/s (3.5 of what is read).
+// ways, 127 us, 2.5 TB/s (3.4 of what is read); 121 without the steps that decays above
+// 1 may need. In the sigmoids' kernels those steps took 88 to 106 us forwards without
+// ever being reached (registers), so that only decays have them.
 #include <type_traits>
 
 #include "norm.cuh"
@@ -72,6 +80,13 @@ template <typename F>
 __device__ __forceinline__ float each(float v, F f) { return f(v); }
 template <typename F>
 __device__ __forceinline__ F2 each(F2 v, F f) { return pack2(f(v.x), f(v.y)); }
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
+__device__ __forceinline__ bool finite(F2 v) { return finite(v.x) && finite(v.y); }
+// Of each unit the first value where that is finite, else the second.
+__device__ __forceinline__ float finite_or(float v, float w) { return finite(v) ? v : w; }
+__device__ __forceinline__ F2 finite_or(F2 v, F2 w) {
+  return pack2(finite_or(v.x, w.x), finite_or(v.y, w.y));
+}
 template <typename T, int V>
 __device__ __forceinline__ Units<V> wide(const Pack<T, V>& q) {
   if constexpr (V == 2) return pair_of(q, 0);
@@ -174,6 +189,10 @@ struct Step {
     if (SIGMOID) slope = mulw(slope, mulw(a, keep));
   }
   __device__ __forceinline__ W dx(W g) const { return MIX ? mulw(g, keep) : g; }
+  // What the step hands on of what it is given.
+  __device__ __forceinline__ W on(W given) const {
+    return BACK ? mulw(a, addw(wide<T, V>(dh), given)) : fmaw(a, given, b);
+  }
 };
 
 // A lane's units of an array: V of them, GAP apart; those there are.
@@ -235,6 +254,7 @@ k_recurrence_tile(const __grid_constant__ Args p) {
     W a, h;
   };
   __shared__ Pair runs[kWarps][32];
+  __shared__ W handed[SIGMOID ? 1 : 32];
   __shared__ uint32_t run_shut[kWarps];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const W zero = all<W>(0.0f);
@@ -329,6 +349,25 @@ k_recurrence_tile(const __grid_constant__ Args p) {
     const Pair v = runs[w][lane];
     carry = run_shut[w] ? v.h : fmaw(v.a, carry, v.h);
   }
+  if (!SIGMOID && __syncthreads_or(!finite(carry))) {  // run after run
+    for (uint32_t w = 0; w < blockDim.x / 32; ++w) {
+      if (w == warp) {
+        carry = w ? handed[lane] : zero;
+        W end = H;
+        if (!stop) {
+          end = carry;
+#pragma unroll
+          for (int k = 0; k < kRun; ++k) {
+            const int i = BACK ? kRun - 1 - k : k;
+            if (i < len) end = steps[i].on(end);
+          }
+          end = finite_or(fmaw(A, carry, H), end);
+        }
+        handed[lane] = end;
+      }
+      __syncthreads();
+    }
+  }
 
   // ---- the run once more, from what it is given
 #pragma unroll
@@ -380,6 +419,7 @@ template <typename T, bool SIGMOID, bool MIX, bool BACK, bool LEAVE, bool TENSOR
 __global__ void __launch_bounds__(kWalkWarps * 32, BACK && !LEAVE ? 2 : 3)
 k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps maps) {
   constexpr int V = 2, GAP = TENSOR ? 1 : 32;
+  constexpr bool SAFE = !SIGMOID && !LEAVE;  // pairs may not be finite
   using W = Units<V>;
   using P = Pack<T, V>;
   constexpr int ARRAYS = LEAVE || !BACK ? 2 : MIX ? 4 : 3;
@@ -392,6 +432,7 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
   __shared__ uint64_t full[S];
   __shared__ uint32_t gave_up;
   __shared__ Pair runs[2][kWalkWarps][32];
+  __shared__ W handed[SAFE ? 32 : 1];
   __shared__ uint32_t run_shut[2][kWalkWarps];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const W zero = all<W>(0.0f);
@@ -426,9 +467,9 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
   const Lane<V, GAP> own(across, p.n);
   const uint32_t unit = own.unit;
   const int64_t g0 = (int64_t)group * p.group_rows, g1 = min(g0 + p.group_rows, (int64_t)p.rows);
-  const int64_t row0 = min(g0 + (int64_t)part * p.part_rows, g1);
-  const int64_t row1 = min(row0 + p.part_rows, g1);
-  const int tiles = (int)((row1 - row0 + kWalkSteps - 1) / kWalkSteps);
+  int64_t row0 = min(g0 + (int64_t)part * p.part_rows, g1);
+  int64_t row1 = min(row0 + p.part_rows, g1);
+  int tiles = (int)((row1 - row0 + kWalkSteps - 1) / kWalkSteps);
   // Steps are walked in the direction `dir`, and so are tiles for results. For a
   // part's pair they are taken the other way round: what is read last is what the
   // next kernel reads first, out of L2.
@@ -472,24 +513,59 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
 
   W A = all<W>(1.0f), given = zero;  // forwards h; backwards what a step hands to the one before
   bool shut = false;
+  // What the part that is walked as the j-th hands on of what it is given.
+  auto part_hands = [&](uint32_t j, W h) {
+    const uint32_t q = group * p.parts + (BACK ? p.parts - 1 - j : j);
+    const bool s = p.shut[q] != 0;
+    const Pair v =
+        reinterpret_cast<const Pair*>(p.pairs)[((uint64_t)q * p.tiles + across) * 32 + lane];
+    return s ? v.h : fmaw(v.a, h, v.h);
+  };
+  const uint32_t before = BACK ? p.parts - 1 - part : part;  // parts walked before this one
+  int next_part = 0x7fffffff;  // the tile at which a part begins that is this block's as well
   if constexpr (!LEAVE) {
-    // what the parts walked before leave
-    const uint32_t before = BACK ? p.parts - 1 - part : part;
-    if (before) {
+    if (SAFE ? p.parts > 1 : before > 0) {
+      // what the parts walked before leave
       if (warp == 0) {
 #pragma unroll 8
-        for (uint32_t j = 0; j < before; ++j) {
-          const uint32_t q = group * p.parts + (BACK ? p.parts - 1 - j : j);
-          const bool s = p.shut[q] != 0;
-          const Pair v =
-              reinterpret_cast<const Pair*>(p.pairs)[((uint64_t)q * p.tiles + across) * 32 + lane];
-          given = s ? v.h : fmaw(v.a, given, v.h);
+        for (uint32_t j = 0; j < before; ++j) given = part_hands(j, given);
+        if constexpr (SAFE) {  // a part that is not given a finite value is left to the block before it
+          uint32_t more = 0;
+          if (__any_sync(~0u, !finite(given))) {
+            more = ~0u;
+          } else if (before + 1 < p.parts) {
+            W h = part_hands(before, given);
+            while (__any_sync(~0u, !finite(h)) && before + ++more + 1 < p.parts)
+              h = part_hands(before + more, h);
+          }
+          if (lane == 0) run_shut[0][0] = more;
         }
         runs[0][0][lane].h = given;
       }
       __syncthreads();
       given = runs[0][0][lane].h;
+      const uint32_t more = SAFE ? run_shut[0][0] : 0;
       __syncthreads();
+      if (more == ~0u) {
+        if constexpr (TENSOR) {
+          if (threadIdx.x == 0)  // what is on its way
+            for (int s = 0; s < min(S, tiles); ++s)
+              mbar_wait_bounded(&full[s], 0, p.timeout_ns);
+        }
+        return;
+      }
+      if (more) {  // parts begin at whole tiles of one another
+        next_part = tiles;
+        if (BACK) row0 -= (int64_t)more * p.part_rows;
+        else row1 = min(row1 + (int64_t)more * p.part_rows, g1);
+        tiles = (int)((row1 - row0 + kWalkSteps - 1) / kWalkSteps);
+        if constexpr (TENSOR) {
+          if (threadIdx.x == 0 && next_part < S) {
+            fetched = next_part;
+            for (int s = next_part; s < S; ++s) fetch(s);
+          }
+        }
+      }
     }
   }
   P nothing;
@@ -498,8 +574,20 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
   // rows in which no stream begins or ends, and all are some stream's
   int64_t clear0 = 0, clear1 = 0;
   uint32_t stage = 0, half = 0, parity = 0;
+  bool tainted = false;  // what is given may not be finite
   for (int tile = 0; tile < tiles; ++tile, at += tile_dir * (int)kWalkSteps, half ^= 1) {
     const int len = (int)max((int64_t)0, min((int64_t)kRun, row1 - at));
+    if constexpr (SAFE) {
+      if (tile == next_part) {  // units that the pairs do for go on from those
+        W h = zero;
+        const uint32_t done = BACK ? p.parts - 1 - (uint32_t)((at - g0) / p.part_rows)
+                                   : (uint32_t)((at - g0) / p.part_rows);
+        for (uint32_t j = 0; j < done; ++j) h = part_hands(j, h);
+        given = finite_or(h, given);
+        tainted = true;
+        next_part += (int)(p.part_rows / kWalkSteps);
+      }
+    }
     P q[4][kRun];
     if constexpr (TENSOR) {
       if (!mbar_try_wait(&full[stage], parity) &&
@@ -558,11 +646,11 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
       }
     }
     W a = all<W>(1.0f), h = zero;
-    if (len == kRun && !stop) {
+    if (len == kRun && !stop && (SIGMOID || valid == 0xff)) {
 #pragma unroll
       for (int k = 0; k < kRun; ++k) {
         const int i = BACK ? kRun - 1 - k : k;
-        h = BACK ? mulw(st[i].a, addw(wide<T, V>(st[i].dh), h)) : fmaw(st[i].a, h, st[i].b);
+        h = st[i].on(h);
         a = mulw(a, st[i].a);
       }
     } else {
@@ -570,18 +658,21 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
       for (int k = 0; k < kRun; ++k) {
         const int i = BACK ? kRun - 1 - k : k;
         if (i >= len) continue;
+        if (!SIGMOID && !(valid >> i & 1)) continue;  // rows of no stream hand on what they get
         if (stop >> i & 1) {  // the same for the whole warp
           h = state_at(BACK ? p.dfinal : p.state, i);
           a = zero;
         }
-        h = BACK ? mulw(st[i].a, addw(wide<T, V>(st[i].dh), h)) : fmaw(st[i].a, h, st[i].b);
+        h = st[i].on(h);
         a = mulw(a, st[i].a);
       }
     }
     runs[half][warp][lane] = {a, h};
     if (lane == 0) run_shut[half][warp] = stop;
     // the half is written again after the next tile's barrier; a stage has been read
-    const bool any = __syncthreads_or(stop != 0);
+    // (any: a stream's border, or what may not be folded)
+    const bool any =
+        __syncthreads_or(stop != 0 || (SAFE && (tainted || !finite(fmaw(a, zero, h)))));
     if constexpr (TENSOR) {
       if (threadIdx.x == 0) fetch(stage);
     }
@@ -612,10 +703,35 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
         given = fmaw(v.a, given, v.h);
       }
     } else if (!LEAVE) {
+      const W was = given;
+      bool fine = finite(was);
       for (uint32_t w = 0; w < kWalkWarps; ++w) {
         const Pair v = runs[half][w][lane];
         if (w == warp) carry = given;
         given = run_shut[half][w] ? v.h : fmaw(v.a, given, v.h);
+        if (SAFE) fine &= finite(given);
+      }
+      if (SAFE) tainted = __any_sync(~0u, !fine);
+      if (SAFE && tainted) {  // so say all warps: run after run
+        for (uint32_t w = 0; w < kWalkWarps; ++w) {
+          if (w == warp) {
+            carry = w ? handed[lane] : was;
+            const Pair v = runs[half][warp][lane];
+            W end = v.h;
+            if (!run_shut[half][warp]) {
+              end = carry;
+#pragma unroll
+              for (int k = 0; k < kRun; ++k) {
+                const int i = BACK ? kRun - 1 - k : k;
+                if (i < len && (valid >> i & 1)) end = st[i].on(end);
+              }
+              end = finite_or(fmaw(v.a, carry, v.h), end);
+            }
+            handed[lane] = end;
+          }
+          __syncthreads();
+        }
+        given = handed[lane];
       }
     }
     if constexpr (!LEAVE) {
@@ -847,7 +963,7 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
       auto walk = [&](auto tensor_c) -> int {
         constexpr bool TENSOR = decltype(tensor_c)::value;
         constexpr int ARRAYS = BACK ? (MIX ? 4 : 3) : 2;
-        Maps maps;
+        Maps maps = {};
         if constexpr (TENSOR) {
           const void* of[4] = {a.gate, BACK ? a.dh : a.x, a.h, a.x};
           const int64_t ld[4] = {a.ldg, BACK ? a.lddh : a.ldx, a.ldh, a.ldx};

@@ -6,7 +6,7 @@ import torch
 import block_formulas as F
 from plastix_b200 import _abi, block
 from plastix_b200.runtime import Context
-from test_block_gpu import made, stored
+from test_block_gpu import gate_bounds, made, stored, walk
 from test_readout_gpu import HALF_STEP, TYPES, U, f64, within
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +43,166 @@ def test_results_beside_their_inputs(ctx):
             got = call(wide[:, :n], wide[:, n:])
             ctx.sync()
             assert torch.equal(wide[:, :n], x) and torch.equal(got, want[k])
+
+
+# ------------------------------------------------------------------- decays of any size
+def placed(a):
+    t, v, _ = made(a, "f32")
+    return t, v
+
+
+def decay_inputs(streams, steps, n, kind, at):
+    """Streams whose decays' product leaves 32 bits though no h or g does, from step `at` on.
+    "grown": decays of 1e5 (or 1.5, over many steps) while h is 0; x begins behind them, dh ends before them.
+    "cut": decays of 1e20, 1e20 and 0 on values of 1e-30."""
+    g = np.random.default_rng([streams, steps, n, at])
+    rows = (streams, steps, n)
+    gate = g.uniform(0.3, 0.95, size=rows) * np.where(g.random(rows) < 0.1, -1, 1)
+    x, dh = g.normal(size=rows), g.normal(size=rows)
+    state, dfinal = g.normal(size=(streams, n)), g.normal(size=(streams, n))
+    if kind == "cut":
+        gate[:, at - 1], x[:, at - 1], dh[:, at] = 0.0, 1e-30, 1e-30
+        gate[:, at], gate[:, at + 1], gate[:, at + 2] = 1e20, 1e20, 0.0
+        x[:, at:at + 2], dh[:, at + 1] = 0.0, 0.0
+    else:
+        value, count = (1e5, 16) if kind == "grown" else (1.5, min(steps - at - 2, 700))
+        gate[:, at:at + count] = value
+        x[:, :at + count], dh[:, at:] = 0.0, 0.0
+        state[:], dfinal[:] = 0.0, 0.0
+    flat = (lambda a: placed(a.reshape(-1, n)))
+    return flat(x), flat(gate), flat(dh), placed(state), placed(dfinal)
+
+
+def check_decays(ctx, streams, n, mix, cuts, offsets, inputs, shape):
+    """Forwards and backwards against the formulas, as test_block_gpu's check, for 1 - a of either sign."""
+    (x, xv), (gate, gv), (dh, dhv), (state, sv), (dfinal, dfv) = inputs
+    how = dict(kind="decay", mix=mix, offsets=offsets)
+    xs, gates, dhs = (t.view(shape) for t in (x, gate, dh))
+    h, final = block.recurrence(ctx, xs, gates, state, **how)
+    again = block.recurrence(ctx, xs, gates, state, **how)
+    ctx.sync()
+    assert torch.equal(h, again[0]) and torch.equal(final, again[1])
+    a, keep, e_a, e_keep = gate_bounds(gv, "decay")
+    b, e_b = (keep * xv, np.abs(xv) * e_keep + U * np.abs(keep * xv)) if mix else (xv, 0 * xv)
+    want, wfinal = F.recurrence(xv, gv, sv, cuts, "decay", mix)
+    tol, ftol = walk(a, b, e_a, e_b, sv, cuts, False)
+    owned = ~np.isnan(want)
+    got = f64(h).reshape(-1, n)
+    within(got[owned], want[owned], stored(want, tol, "f32")[owned], "h")
+    within(f64(final), wfinal, ftol + U * np.abs(wfinal), "final")
+    assert (got[~owned] == 0).all()
+
+    back = dict(x=xs, dfinal=dfinal, **how)
+    dx, dgate, dstate = block.recurrence_backward(ctx, dhs, gates, h, state, **back)
+    again = block.recurrence_backward(ctx, dhs, gates, h, state, **back)
+    ctx.sync()
+    for p, q in zip((dx, dgate, dstate), again):
+        assert torch.equal(p, q)
+    wx, wg, ws = F.recurrence_backward(dhv, xv, gv, got, sv, dfv, cuts, "decay", mix)
+    gtol, stol = walk(a, dhv, e_a, 0 * dhv, dfv, cuts, True)
+    g = F.recurrence_backward(dhv, xv, gv, got, sv, dfv, cuts, "decay", False)[0]
+    before = np.zeros_like(xv)
+    for s in range(streams):
+        lo, hi = cuts[s], cuts[s + 1]
+        if hi > lo:
+            before[lo], before[lo + 1:hi] = sv[s], got[lo:hi - 1]
+    arm = before - xv if mix else before
+    t_dx = np.abs(keep) * gtol + np.abs(g) * e_keep + U * np.abs(wx) if mix else gtol
+    t_da = np.abs(arm) * gtol + np.abs(g) * 3 * U * (np.abs(before) + np.abs(xv))
+    for name, t, w, off in (("dx", dx, wx, t_dx), ("dgate", dgate, wg, t_da)):
+        t = f64(t).reshape(-1, n)
+        within(t[owned], w[owned], stored(w, off, "f32")[owned], name)
+        assert (t[~owned] == 0).all()
+    within(f64(dstate), ws, stol + U * np.abs(ws), "dstate")
+
+
+DECAYS = [  # streams, steps, n, kind, at
+    (5, 24, 40, "grown", 3),     # whole streams in a tile
+    (300, 30, 33, "grown", 9),
+    (4, 20, 64, "cut", 2),
+    (4, 20, 64, "cut", 6),       # over the border of two runs
+    (3, 90, 48, "slow", 0),
+    (600, 200, 64, "grown", 50),  # walks of several streams
+    (3, 500, 4096, "grown", 100),  # a walk a stream
+    (2, 700, 31, "grown", 120),  # over the border of two tiles, or in parts
+    (1, 5000, 64, "slow", 100),  # in parts
+    (1, 5000, 64, "slow", 4200),
+    (1, 4000, 37, "slow", 1900),
+    (1, 4000, 64, "cut", 126),   # over the border of two parts
+    (1, 4000, 64, "cut", 127),
+    (1, 4000, 33, "cut", 63),
+    (2, 3000, 64, "grown", 120),
+    (2, 4000, 1024, "slow", 300),  # in long parts
+]
+
+
+@pytest.mark.parametrize("mix", [False, True])
+@pytest.mark.parametrize("streams, steps, n, kind, at", DECAYS)
+def test_decays_of_any_size(ctx, streams, steps, n, kind, at, mix):
+    cuts = [s * steps for s in range(streams + 1)]
+    inputs = decay_inputs(streams, steps, n, kind, at)
+    with np.errstate(all="ignore"):
+        check_decays(ctx, streams, n, mix, cuts, None, inputs, (streams, steps, n))
+
+
+@pytest.mark.parametrize("cuts, rows", [([0, 5, 1300, 1300, 3000], 3100), ([4, 900, 2600], 2600), ([0, 40, 90, 99], 120)])
+@pytest.mark.parametrize("n", [64, 33])
+def test_decays_of_any_size_in_ragged_streams(ctx, cuts, rows, n):
+    """Products that leave 32 bits in every stream that is long enough, and in rows of no stream."""
+    g = np.random.default_rng([rows, n])
+    gate = g.uniform(0.3, 0.95, size=(rows, n))
+    x, dh = g.normal(size=(rows, n)), g.normal(size=(rows, n))
+    streams = len(cuts) - 1
+    state, dfinal = g.normal(size=(streams, n)), g.normal(size=(streams, n))
+    for s in range(streams):
+        lo, hi = cuts[s], cuts[s + 1]
+        if hi - lo > 30:
+            end = lo + 20 + (hi - lo - 30) // 2
+            gate[lo + 10:end] = 1e5
+            x[lo:end], dh[lo + 10:hi] = 0.0, 0.0
+            state[s], dfinal[s] = 0.0, 0.0
+    gate[:cuts[0]], gate[cuts[-1]:] = 1e30, 1e30
+    inputs = placed(x), placed(gate), placed(dh), placed(state), placed(dfinal)
+    offsets = torch.tensor(cuts, dtype=torch.int32, device="cuda")
+    with np.errstate(all="ignore"):
+        check_decays(ctx, streams, n, True, cuts, offsets, inputs, (rows, n))
+
+
+@pytest.mark.parametrize("steps, n, dtype", [(20, 64, "f32"), (300, 64, "f32"), (5000, 64, "bf16"), (5000, 33, "f32"),
+                                             (4000, 1024, "bf16")])
+@pytest.mark.parametrize("kind", ["decay", "sigmoid"])
+def test_infinity_stays_what_it_is_step_by_step(ctx, steps, n, dtype, kind):
+    """h behind an infinite x is infinite of its sign until a decay of 0 (which makes NaN of it), not NaN because a
+    product of decays is 0 (behind sigmoids it is not finite); other units keep their bits."""
+    g = torch.Generator(device="cuda").manual_seed(steps + n)
+    x = torch.randn(2, steps, n, device="cuda", generator=g).to(TYPES[dtype])
+    gate = (torch.rand(2, steps, n, device="cuda", generator=g) * 0.5 + 0.25).to(TYPES[dtype])
+    want, _ = block.recurrence(ctx, x, gate, kind=kind)
+    bad = x.clone()
+    bad[0, 5, 3], bad[1, 2, 7] = float("inf"), float("-inf")
+    bad_gate = gate.clone()
+    if kind == "decay":
+        bad_gate[1, steps - 4, 7] = 0.0
+    h, final = block.recurrence(ctx, bad, bad_gate, kind=kind)
+    ctx.sync()
+    if kind == "decay":
+        assert (h[0, 5:, 3] == float("inf")).all() and final[0, 3] == float("inf")
+        assert (h[1, 2:steps - 4, 7] == float("-inf")).all() and h[1, steps - 4:, 7].isnan().all()
+    assert not h[0, 5:, 3].isfinite().any() and not h[1, 2:, 7].isfinite().any()
+    assert torch.equal(h[0, :5, 3], want[0, :5, 3]) and torch.equal(h[1, :2, 7], want[1, :2, 7])
+    others = [u for u in range(n) if u not in (3, 7)]
+    assert torch.equal(h[:, :, others], want[:, :, others])
+    assert torch.equal(h[1, :, 3], want[1, :, 3]) and torch.equal(h[0, :, 7], want[0, :, 7])
+
+
+def test_decays_of_any_size_in_place(ctx):
+    """The part that a block goes on into is not written by another one."""
+    inputs = decay_inputs(1, 5000, 64, "slow", 1000)
+    (x, _), (gate, _), _, (state, _), _ = inputs
+    h, final = block.recurrence(ctx, x.view(1, 5000, 64), gate.view(1, 5000, 64), state, kind="decay")
+    for where in (0, 1):
+        t = [x.clone().view(1, 5000, 64), gate.clone().view(1, 5000, 64)]
+        s = state.clone()
+        h2, _ = block.recurrence(ctx, *t, s, kind="decay", out=t[where], final_out=s)
+        ctx.sync()
+        assert h.isfinite().all() and torch.equal(h2, h) and torch.equal(s, final)
