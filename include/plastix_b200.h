@@ -724,7 +724,9 @@ int plx_dense(plx_ctx* ctx, uint64_t rows, uint32_t n, uint32_t m, int dtype, co
               void* scratch, size_t scratch_bytes);
 
 /* Gradients of plx_dense (cf. DoBackwardPass, plastix.hpp:164-211): with
- * dz = dy act'(pre), rounded to dtype for the products,
+ * dz = dy act'(pre), rounded to dtype for the products (as PLX_F16 times a power of
+ * two that puts the largest finite |dy| at 2^13 to 2^14, so that small and large
+ * gradients keep their bits),
  *   dx = dz weight;  dweight = dz^T x;  dbias = sum of dz over the rows
  * each written where not NULL (dweight and dbias are zero for rows = 0); x is
  * not needed without dweight, weight not without dx, pre not for

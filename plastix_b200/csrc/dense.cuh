@@ -90,6 +90,7 @@ struct Operand {
 };
 
 // What becomes of the sums z[i][j] of a product: y = act(z + bias[j]) + residual.
+// factor: of float16 operands, what z is multiplied by before (NULL: nothing).
 struct Finish {
   int param_dtype, act;
   const void* bias;
@@ -98,6 +99,7 @@ struct Finish {
   void* y;
   int64_t ldy;
   float* pre;  // z + bias, [rows][cols]
+  const float* factor;
 };
 
 // y[i][j] for i < rows, j < cols: sums over k < depth of a(i, k) b(j, k).

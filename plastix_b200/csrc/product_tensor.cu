@@ -116,6 +116,7 @@ __device__ __forceinline__ float bias_at(const Finish& f, uint32_t col) {
 template <typename T>
 __device__ __forceinline__ void finish_one(const Finish& f, uint32_t row, uint32_t col,
                                            uint32_t cols, float z) {
+  if (std::is_same_v<T, __half> && f.factor) z *= *f.factor;
   float v[1] = {f.bias ? z + bias_at<T>(f, col) : z};
   if (f.pre) f.pre[(uint64_t)row * cols + col] = v[0];
   activate<T>(f.act, v);
@@ -123,10 +124,15 @@ __device__ __forceinline__ void finish_one(const Finish& f, uint32_t row, uint32
   ((T*)f.y)[(int64_t)row * f.ldy + col] = from_f32<T>(v[0]);
 }
 
-// Adds the bias of C consecutive columns; `wide`: all there, in 16-byte pieces.
+// Applies the factor and adds the bias of C consecutive columns; `wide`: all there, in 16-byte pieces.
 template <typename T, int C>
 __device__ __forceinline__ void add_bias(const Finish& f, uint32_t col, uint32_t cols, bool wide,
                                          float (&v)[C]) {
+  if (std::is_same_v<T, __half> && f.factor) {
+    const float by = *f.factor;
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] *= by;
+  }
   if (!f.bias) return;
   if (!wide) {
 #pragma unroll

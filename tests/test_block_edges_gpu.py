@@ -6,7 +6,7 @@ import torch
 import block_formulas as F
 from plastix_b200 import _abi, block
 from plastix_b200.runtime import Context
-from test_block_gpu import gate_bounds, made, stored, walk
+from test_block_gpu import act_error, gate_bounds, made, product_error, stored, walk
 from test_readout_gpu import HALF_STEP, TYPES, U, f64, within
 
 pytestmark = pytest.mark.gpu
@@ -206,3 +206,53 @@ def test_decays_of_any_size_in_place(ctx):
         h2, _ = block.recurrence(ctx, *t, s, kind="decay", out=t[where], final_out=s)
         ctx.sync()
         assert h.isfinite().all() and torch.equal(h2, h) and torch.equal(s, final)
+
+
+# ------------------------------------------------------------------- float16 gradients
+@pytest.mark.parametrize("rows, n, m, more", [(2000, 72, 136, 0), (2000, 33, 70, 1), (7, 300, 130, 8), (1, 40, 9, 0)])
+@pytest.mark.parametrize("size", [1e-6, 1e-4, 1.0, 3e4])
+@pytest.mark.parametrize("apply", ["tanh", "gelu"])
+def test_dense_gradients_of_small_and_large_float16(ctx, rows, n, m, more, size, apply):
+    """dz of dy that float16 holds, but whose products with a slope it would not: each is off by half a step of its
+    own size and 2^-38 of the largest dy, whatever the gradients' magnitude."""
+    g = np.random.default_rng([rows, n, m])
+    even = min(1.0, 10 / size)  # keeps sums of large gradients in float16
+    x, xv, _ = made((np.abs(g.normal(size=(rows, n))) + 0.5) * even, "f16", n + more)
+    w, wv, _ = made(g.normal(size=(m, n)) * even, "f16", n + more)
+    dy, dyv, _ = made(np.minimum(np.abs(g.normal(size=(rows, m))) + 0.2, 2.1) * size, "f16", m + more)
+    z, zv, _ = made(g.normal(size=(rows, m)) + 1.0, "f32")
+    b, _, _ = made(g.normal(size=(1, m)), "f32")
+    dx, dw, db = block.dense_backward(ctx, dy, x, w, z, apply=apply, bias=b[0])
+    again = block.dense_backward(ctx, dy, x, w, z, apply=apply, bias=b[0])
+    ctx.sync()
+    for p, q in zip((dx, dw, db), again):
+        assert torch.equal(p, q)
+    wx, ww, wb, dz = F.dense_backward(dyv, xv, wv, zv, apply)
+    slope = F.act(zv, apply)[1]
+    off = np.abs(dyv) * (act_error(zv, slope) + 4 * U)
+    dzerr = off + HALF_STEP["f16"] * (np.abs(dz) + off) + 2.0 ** -38 * np.abs(dyv).max()
+    tx = dzerr @ np.abs(wv) + product_error(dz, wv, m)
+    tw = dzerr.T @ np.abs(xv) + product_error(dz.T, xv, rows)
+    assert np.abs(wx).max() < 65000 and np.abs(ww).max() < 65000
+    within(f64(dx), wx, stored(wx, tx, "f16"), "dx")
+    within(f64(dw), ww, stored(ww, tw, "f16"), "dweight")
+    within(f64(db), wb, stored(wb, off.sum(0) + (rows + 64) * U * np.abs(dz).sum(0), "f32"), "dbias")
+
+
+def test_float16_gradients_beside_infinities_and_zeros(ctx):
+    """An infinite dy has no part in the others' scale; gradients of 0 are 0."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(300, 64, device="cuda", generator=g).half()
+    w = torch.randn(80, 64, device="cuda", generator=g).half()
+    z = torch.randn(300, 80, device="cuda", generator=g)
+    dy = (torch.randn(300, 80, device="cuda", generator=g) * 1e-5).half()
+    dy[0, 0] = 0.0
+    dx, dw, _ = block.dense_backward(ctx, dy, x, w, z, apply="tanh")
+    bad = dy.clone()
+    bad[0, 0] = float("inf")
+    dx2, dw2, _ = block.dense_backward(ctx, bad, x, w, z, apply="tanh")
+    none = block.dense_backward(ctx, torch.zeros_like(dy), x, w, z, apply="tanh")
+    ctx.sync()
+    assert torch.equal(dx[1:], dx2[1:]) and torch.equal(dw[1:], dw2[1:])
+    assert not dx2[0].isfinite().any() and not dw2[0].isfinite().any()
+    assert not none[0].any() and not none[1].any()
