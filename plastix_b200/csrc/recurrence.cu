@@ -798,6 +798,13 @@ k_copy_state(uint64_t count, const float* from, float* to) {
     to[i] = from ? from[i] : 0.0f;
 }
 
+// Offsets of streams without any rows: all 0.
+__global__ void __launch_bounds__(256)
+k_check_offsets(uint32_t count, const int32_t* offsets, int32_t* status) {
+  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < count; i += gridDim.x * 256)
+    if (offsets[i] != 0) record_status(status, kStatusBadOffsets);
+}
+
 // How a call is cut, and what it needs of scratch.
 struct Plan {
   bool short_streams, states_apart;
@@ -908,7 +915,14 @@ int launch(plx_ctx* ctx, Args a, int dtype, int gate_kind, bool mix, void* scrat
     PLX_LAUNCH_CHECK("k_copy_state");
     return PLX_OK;
   };
-  if (a.rows == 0) return state_out && state_out != given ? copy_state(given) : PLX_OK;
+  if (a.rows == 0) {
+    if (a.offsets) {
+      k_check_offsets<<<std::min((a.streams + 256) / 256, 1024u), 256, 0, ctx->stream>>>(
+          a.streams + 1, a.offsets, ctx->d_status);
+      PLX_LAUNCH_CHECK("k_check_offsets");
+    }
+    return state_out && state_out != given ? copy_state(given) : PLX_OK;
+  }
   if (a.rows == 1) a.ldx = a.ldg = a.ldh = a.lddh = a.ldo = a.ldo2 = a.n;
   a.steps = a.offsets ? 0 : (uint32_t)(a.rows / a.streams);
   a.status = ctx->d_status;

@@ -256,3 +256,22 @@ def test_float16_gradients_beside_infinities_and_zeros(ctx):
     assert torch.equal(dx[1:], dx2[1:]) and torch.equal(dw[1:], dw2[1:])
     assert not dx2[0].isfinite().any() and not dw2[0].isfinite().any()
     assert not none[0].any() and not none[1].any()
+
+
+# ------------------------------------------------------------------- offsets without rows
+@pytest.mark.parametrize("cuts", [[0, 5], [0, 0, 3, 3], [-1, 0], [2, 2]])
+def test_bad_offsets_are_reported_without_rows(ctx, cuts):
+    x = torch.zeros(0, 32, device="cuda")
+    offsets = torch.tensor(cuts, dtype=torch.int32, device="cuda")
+    block.recurrence(ctx, x, x, offsets=offsets)
+    with pytest.raises(_abi.PlxError, match="offsets"):
+        ctx.sync()
+    block.recurrence_backward(ctx, x, x, x, offsets=offsets)
+    with pytest.raises(_abi.PlxError, match="offsets"):
+        ctx.sync()
+    state = torch.randn(700, 32, device="cuda")
+    none = torch.zeros(701, dtype=torch.int32, device="cuda")
+    h, final = block.recurrence(ctx, x, x, state, offsets=none)
+    _, _, dstate = block.recurrence_backward(ctx, x, x, h, state, dfinal=final, offsets=none)
+    ctx.sync()
+    assert torch.equal(final, state) and torch.equal(dstate, state)
