@@ -774,8 +774,8 @@ size_t plx_block_norm_scratch_bytes(uint64_t rows, uint32_t n);
 /* Gradients of sum(dr * r) + sum(du * u); dr or du may be NULL, not both. dx and
  * d_o are required; dgate ([n] of param_dtype or [rows, n], as the gate) and the
  * parameters' gradients ([n] of param_dtype) are written where not NULL (those
- * of [n] are zero for rows = 0), summed in an order that the arguments set: the
- * same bits on every call. scratch as for plx_dense. */
+ * of [n] are zero for rows = 0; those of post need post), summed in an order that the
+ * arguments set: the same bits on every call. scratch as for plx_dense. */
 int plx_block_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype, const void* dr,
                             int64_t lddr, const void* du, int64_t lddu, const void* x, int64_t ldx,
                             const void* o, int64_t ldo, const float* stats,

@@ -414,6 +414,8 @@ extern "C" int plx_block_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
                 scratch ? scratch_bytes : (size_t)0);
   PLX_CHECK_ARG(aligned16(scratch) && aligned16(stats),
                 "scratch and stats have to be 16-byte aligned");
+  PLX_CHECK_ARG(params->post || (!dpost_weight && !dpost_bias),
+                "dpost_weight and dpost_bias need post");
   const bool units = params->gate == PLX_BLOCK_GATE_UNITS;
   const bool values = params->gate == PLX_BLOCK_GATE_VALUES;
   if (rows) {

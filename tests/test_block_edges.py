@@ -2,8 +2,9 @@
 import pytest
 import torch
 
-from plastix_b200 import block
-from test_readout import FakeContext
+from plastix_b200 import _abi, block
+from test_block import block_bwd_args, params
+from test_readout import FakeContext, refused
 
 
 def test_inputs_that_begin_where_the_result_does_are_refused_at_another_stride():
@@ -69,3 +70,10 @@ def test_rows_side_by_side_are_told_from_rows_that_overlap():
                     assert refused, (n, ld, at)
                 elif ld == 11:
                     assert not refused, (n, at)
+
+
+def test_gradients_of_a_norm_that_is_not_there_are_refused():
+    """They would be left as they were, where every gradient that is given is written."""
+    for name in ("dw1", "db1"):
+        change = {k: None for k in ("dw1", "db1") if k != name}
+        refused(1, b"post", "plx_block_norm_backward", *block_bwd_args(params=params(post=0), **change))
