@@ -26,8 +26,8 @@ namespace {
 
 constexpr int kSums = 5;  // dw2, dw1, dgate of units, db2, db1
 constexpr uint32_t kSms = 148;  // of a B200; fixes the order of the sums
-constexpr uint32_t kMostGroups = kSms * 4;
 constexpr uint32_t kLongGroups = 64;
+constexpr uint32_t kLong = 16384;  // values of the longest row that registers hold
 
 struct SumsOut {
   void* out[kSums];
@@ -389,15 +389,24 @@ uint32_t groups_of(uint64_t rows, uint32_t per_block, uint32_t most) {
       std::min<uint64_t>(by_rows, std::max<uint64_t>(kSms, (by_rows + 7) / 8)), most);
 }
 
+// Column sums of the groups that a call leaves, as many as its launch has blocks (of the
+// ladder in plx_block_norm_backward).
+uint64_t sums_bytes(uint64_t rows, uint32_t n) {
+  const uint32_t most = n <= 1024 ? kSms * 4 : n <= 2048 ? kSms * 2 : n <= 4096 ? kSms
+                        : n <= 8192 ? kSms / 2 : kSms / 4;
+  const uint64_t groups =
+      n > kLong ? std::min<uint64_t>(rows, kLongGroups) : groups_of(rows, 1, most);
+  return (std::max<uint64_t>(1, groups) * kSums * n * 4 + 15) / 16 * 16;
+}
+
 }  // namespace
 }  // namespace plx
 
 using namespace plx;
 
 extern "C" size_t plx_block_norm_scratch_bytes(uint64_t rows, uint32_t n) {
-  // column sums of the groups, and the means of rows that no registers hold
-  const uint64_t sums = (uint64_t)std::max(1u, groups_of(rows, 1, kMostGroups)) * kSums * n * 4;
-  return (size_t)((sums + 15) / 16 * 16 + rows * 16);
+  // and the means of rows that no registers hold
+  return (size_t)(sums_bytes(rows, n) + (n > kLong ? rows * 16 : 0));
 }
 
 extern "C" int plx_block_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, int dtype,
@@ -461,7 +470,7 @@ extern "C" int plx_block_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
     a.lddg = a.dgate ? lddg : 0;
   }
   a.partial = sums ? (float*)scratch : nullptr;
-  float4* means = (float4*)((char*)scratch + need - rows * 16);
+  float4* means = (float4*)((char*)scratch + sums_bytes(rows, n));
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int V = 16 / sizeof(T);
@@ -525,7 +534,7 @@ extern "C" int plx_block_norm_backward(plx_ctx* ctx, uint64_t rows, uint32_t n, 
         else if (n <= 2048) launch(vv, nv, PLX_C(256), PLX_C(1), PLX_C(2));
         else if (n <= 4096) launch(vv, nv, PLX_C(512), PLX_C(1), PLX_C(1));
         else if (n <= 8192) launch(vv, nv, PLX_C(512), PLX_C(2), PLX_C(1));
-        else if (n <= 16384) launch(vv, nv, PLX_C(512), PLX_C(4), PLX_C(1));
+        else if (n <= kLong) launch(vv, nv, PLX_C(512), PLX_C(4), PLX_C(1));
         else loops();
       };
       if (v == V) ladder(PLX_C(V), PLX_C(8 / V));

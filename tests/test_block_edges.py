@@ -77,3 +77,11 @@ def test_gradients_of_a_norm_that_is_not_there_are_refused():
     for name in ("dw1", "db1"):
         change = {k: None for k in ("dw1", "db1") if k != name}
         refused(1, b"post", "plx_block_norm_backward", *block_bwd_args(params=params(post=0), **change))
+
+
+@pytest.mark.parametrize("rows, n, most", [(600, 65536, 64), (1 << 20, 16384, 37), (1 << 20, 8192, 74), (5, 20000, 5),
+                                           (1 << 20, 1024, 592), (1 << 20, 4096, 148), (1, 100, 1), (0, 100, 1)])
+def test_scratch_of_block_norm_is_what_its_launches_leave(rows, n, most):
+    """Five column sums of every group, and the four means of rows that are too long for registers."""
+    size = _abi.lib().plx_block_norm_scratch_bytes(rows, n)
+    assert size == most * 5 * n * 4 + (rows * 16 if n > 16384 else 0)
