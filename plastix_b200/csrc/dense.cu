@@ -12,10 +12,12 @@
 // stays; what the type cuts off is below 2^-38 of the largest dy. (Looking for the
 // largest dy first takes 10 us of 445 forwards and backwards of 8,192 x 4,096 x 2,048.)
 // 32-bit values are cut into three bfloat16 values whose sum they are, toward zero, so
-// that all have one sign; of the nine products of parts six are made, the others are
-// below 2^-24 of the value's. A part that would be 0 is the first one times 2^-30 or
-// 2^-40, so that an infinity beside it stays one (values below 2^-100 have no room for
-// all parts).
+// that all have one sign: up to 2^-7 and 2^-15 of the value beside the first. Of the nine
+// products of parts six are made; what is left out makes a product up to 2^-21 smaller,
+// 4e-8 on average (two more would make that 2^-30, and the tensor cores' work a third
+// longer). A part that would be 0 is the first one times 2^-30 or 2^-40, so that an
+// infinity beside it stays one (values below 2^-100 have no room for all parts, and below
+// 2^-93 an infinity beside them may become NaN).
 #include "dense.cuh"
 
 namespace plx {

@@ -275,3 +275,38 @@ def test_bad_offsets_are_reported_without_rows(ctx, cuts):
     _, _, dstate = block.recurrence_backward(ctx, x, x, h, state, dfinal=final, offsets=none)
     ctx.sync()
     assert torch.equal(final, state) and torch.equal(dstate, state)
+
+
+# ------------------------------------------------------------------- how exact products are
+def pre_of(ctx, a, b):
+    """z of rows and weights as they are, in 64 bits."""
+    _, z = block.dense(ctx, a, b, pre=True)
+    ctx.sync()
+    return z.double()
+
+
+@pytest.mark.parametrize("n", range(1, 9))
+@pytest.mark.parametrize("rows", [9, 64, 300])
+def test_products_of_32_bit_values_with_all_bits_set(ctx, n, rows):
+    """Parts of a value are up to 2^-7 and 2^-15 of it, so that the products that are not made are 8 U of a
+    product. The first parts' products are added last: in that step each of n + 1 terms may be cut by 2 U of the
+    sum, in the five before by 2^-6 of that; one rounding in registers and one of the result."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    a, b = (1 + torch.rand(k, n, device="cuda", generator=g) for k in (rows, 130))
+    a, b = ((t.view(torch.int32) | 0x7fff).view(torch.float32) for t in (a, b))
+    want = a.double() @ b.double().t()
+    tol = (8 + 2 * (n + 1) * (1 + 5 / 64) + 2) * U
+    assert ((pre_of(ctx, a, b) - want).abs() <= tol * want).all()
+
+
+@pytest.mark.parametrize("rows, n, m", [(64, 1001, 130), (300, 1001, 520), (16, 4096, 64), (1000, 2000, 1024)])
+def test_sums_of_32_bit_values_leave_the_tensor_cores(ctx, rows, n, m):
+    """Terms of one sign. In the tensor cores a step is cut by 2 U of its sum; those of 64 terms alone are made
+    there: the four of the first parts with a quarter, two, three and four quarters of it cost 5 U of the 64 terms'
+    sum, the others 2^-6 of as much. Those sums are added with roundings of U of the sum so far, half of the whole
+    on average. (All steps in the tensor cores: 24 for 64 terms, off by 1e-5, 160 U, at 1,001.)"""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    a, b = (torch.rand(k, n, device="cuda", generator=g) + 0.1 for k in (rows, m))
+    want = a.double() @ b.double().t()
+    tol = (8 + 6 + (n // 64 + 1) / 2 + 2) * U
+    assert ((pre_of(ctx, a, b) - want).abs() <= tol * want).all()
