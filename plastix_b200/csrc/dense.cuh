@@ -15,8 +15,9 @@ __device__ __forceinline__ float act_value(float z) {
     return z * (0.5f * erfcf(z * -0.70710678118654752f));
   else return z;
 }
-// The same for results of 16 bits, in fewer instructions: relative errors of a few
-// 2^-22, of GELU's Phi below 4e-6 for |z| < 10 and 1e-4 beyond (where it is below
+// The same for results of 16 bits, in fewer instructions. Relative errors: sigmoids
+// (9 + 1.3 |z|) 2^-24 (the exponent's argument is rounded), tanh 8e-6 (at 0.02, where 1 -
+// e begins to cancel), GELU's Phi 1e-5 for |z| < 10 and 1e-4 beyond (where it is below
 // 1e-23).
 template <int ACT>
 __device__ __forceinline__ float act_value16(float z) {

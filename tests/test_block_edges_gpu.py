@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 import torch
+from scipy.special import erfc
 
 import block_formulas as F
 from plastix_b200 import _abi, block
@@ -310,3 +311,24 @@ def test_sums_of_32_bit_values_leave_the_tensor_cores(ctx, rows, n, m):
     want = a.double() @ b.double().t()
     tol = (8 + 6 + (n // 64 + 1) / 2 + 2) * U
     assert ((pre_of(ctx, a, b) - want).abs() <= tol * want).all()
+
+
+# ------------------------------------------------------------------- 16-bit activations
+@pytest.mark.parametrize("apply", ["sigmoid", "tanh", "silu", "gelu"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_16_bit_activations_within_their_bounds(ctx, dtype, apply):
+    """Off by half a step of the value that is stored, besides what the kernel's header states: sigmoids
+    (9 + 1.3 |z|) U, tanh 8e-6, GELU's factor 1e-5 where |z| < 10 (a 50th of a float16's half step)."""
+    z = np.concatenate([np.linspace(-9.99, 9.99, 60001), np.linspace(-0.1, 0.1, 4001), np.linspace(-85, 10, 4001)])
+    z = z[np.abs(z) < 10] if apply == "gelu" else z
+    x, xv, _ = made(z[:, None], dtype)
+    y = block.dense(ctx, x, torch.ones(1, 1, device="cuda", dtype=TYPES[dtype]), apply=apply)
+    ctx.sync()
+    # (1 + erf, as the formulas have it, is off by 1e-16: all of GELU's factor below z = -8)
+    want = xv * 0.5 * erfc(xv / -np.sqrt(2)) if apply == "gelu" else F.act(xv, apply)[0]
+    rel = {"tanh": 8e-6, "gelu": 1e-5}.get(apply, (9 + 1.3 * np.abs(xv)) * U)
+    size = np.maximum(np.abs(want) * (1 + rel), 2.0 ** -126)
+    half = 2.0 ** (np.floor(np.log2(size)) - (8 if dtype == "bf16" else 11))
+    if dtype == "f16":
+        half = np.maximum(half, 2.0 ** -25)
+    within(f64(y), want, rel * np.abs(want) + half, "y")
