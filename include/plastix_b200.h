@@ -716,7 +716,9 @@ size_t plx_dense_scratch_bytes(uint64_t rows, uint32_t n, uint32_t m, int dtype,
  * type dtype, bias [m] of param_dtype (PLX_F32 or dtype); bias and residual may
  * be NULL. pre [rows, m] (rows of m floats, nothing between them) is z, written
  * where not NULL, for the backward call. y may be residual's array, not x's.
- * Products are summed in 32 bits. scratch is 16-byte aligned and may hold
+ * Products are summed in 32 bits; those of 16-bit rows on the tensor cores, which cut
+ * sums off: of terms of one sign they (and with them pre) come out up to 1e-4 (float16)
+ * or 8e-4 (bfloat16) too small, after 1,000 terms 5e-7. scratch is 16-byte aligned and may hold
  * anything; calls that run at once need scratch of their own. */
 int plx_dense(plx_ctx* ctx, uint64_t rows, uint32_t n, uint32_t m, int dtype, const void* x,
               int64_t ldx, const void* weight, int64_t ldw, int param_dtype, const void* bias,

@@ -3,7 +3,11 @@
 // six products of planes that matter are made of it, the small ones first. The tensor
 // cores cut sums off, they do not round them: a stage's sums are therefore taken to
 // registers and added there, which is as exact as multiply-adds in 32 bits (all in
-// TMEM were off by 1e-5 after 1,000 values of k).
+// TMEM were off by 1e-5 after 1,000 values of k). 16-bit values' sums stay there for up
+// to 16,384 (float16) or 131,072 (bfloat16) values of k: a step of 16 of them costs 3.4 x
+// 2^-24 of the sum so far where terms have one sign (measured), so that it comes out a
+// fifth of the type's half step too small then; longer sums (LONG) leave TMEM as often
+// (weights' gradients of 131,072 rows of 4,096 x 1,024 f16 902 -> 970 us).
 //
 // Bound by the products (large calls) or by reading the weights (few rows). A
 // block makes tiles of 128 x BN sums: one thread has tensor copies fill a ring of
@@ -42,10 +46,13 @@ constexpr uint32_t kSmem = 232448;  // a block can have
 
 enum Mode { ONE, SPLIT, PAIR };
 
-template <typename T, int BN, Mode MODE>
+template <typename T, int BN, Mode MODE, bool LONG>
 struct Stages {
   static constexpr uint32_t planes = sizeof(T) == 4 ? 3 : 1;
-  static constexpr bool by_stage = sizeof(T) == 4;  // sums leave TMEM after every stage
+  // Sums leave TMEM after so many stages, for registers that add them up.
+  static constexpr bool by_stage = sizeof(T) == 4 || LONG;
+  static constexpr uint32_t period =
+      sizeof(T) == 4 ? 1 : std::is_same_v<T, __half> ? 256 : 2048;
   static constexpr uint32_t b_rows = MODE == PAIR ? BN / 2 : BN;  // a block's
   static constexpr uint32_t a_bytes = kTileA * kTileK * 2, b_bytes = b_rows * kTileK * 2;
   static constexpr uint32_t bytes = planes * (a_bytes + b_bytes);
@@ -199,10 +206,10 @@ __device__ __forceinline__ void finish_row(const Finish& f, uint32_t row, uint32
   }
 }
 
-template <typename T, int BN, Mode MODE>
+template <typename T, int BN, Mode MODE, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1)
 k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
-  using S = Stages<T, BN, MODE>;
+  using S = Stages<T, BN, MODE, LONG>;
   constexpr bool TWO = MODE == PAIR;
   constexpr uint32_t C = BN <= 32 ? 16 : 32;  // columns at a time, at most half of a tile's
   static_assert(BN == 16 || BN % (2 * C) == 0, "halves of a tile");
@@ -338,8 +345,9 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
         if (!ok) break;
       }
       for (uint32_t k = k_first; k < k_last; ++k, ++it) {
+        const uint32_t in = S::by_stage ? (k - k_first) % S::period : k - k_first;
         if constexpr (S::by_stage) {
-          to = next_half();
+          if (in == 0) to = next_half();
           if (!ok) break;
         }
         const uint32_t s = it % S::count;
@@ -360,10 +368,12 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
 #pragma unroll
           for (uint32_t j = 0; j < kTileK / 16; ++j)
             tensor_product<TWO>(to, a + j * da, b + j * db, p.kind,
-                                (!S::by_stage && k > k_first) || q > 6 - kProducts || j > 0);
+                                in > 0 || q > 6 - kProducts || j > 0);
         }
         products_arrive<TWO>(&empty[s]);
-        if constexpr (S::by_stage) products_arrive<TWO>(&done[turn++ & 1]);
+        if constexpr (S::by_stage) {
+          if (in + 1 == S::period || k + 1 == k_last) products_arrive<TWO>(&done[turn++ & 1]);
+        }
       }
       if constexpr (!S::by_stage) {
         if (ok) products_arrive<TWO>(&done[turn++ & 1]);
@@ -417,7 +427,7 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
       if constexpr (S::by_stage) {
 #pragma unroll
         for (uint32_t e = 0; e < kMine; ++e) acc[e] = 0.0f;
-        for (uint32_t k = k_first; sound && k < k_last; ++k, ++turn) {
+        for (uint32_t k = k_first; sound && k < k_last; k += S::period, ++turn) {
           sound = __all_sync(~0u, wait(&done[turn & 1], (turn / 2) & 1, &gave_up, p));
           tmem_fence_after();
           if (!sound) break;
@@ -515,7 +525,7 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
             if (lane == 0) bulk_wait_read<0>();
             __syncwarp();
           }
-#pragma unroll 1
+#pragma unroll (S::by_stage ? 2 : 1)
           for (uint32_t h = 0; h < kHalves; ++h) {
             float v[32];
             take(c * kWide + h * 32, v);
@@ -653,10 +663,10 @@ k_product_tensor(const __grid_constant__ TensorProduct p, bool wide) {
   }
 }
 
-template <typename T, int BN, Mode MODE>
+template <typename T, int BN, Mode MODE, bool LONG = false>
 int launch(plx_ctx* ctx, TensorProduct& t, const Product& p, const Operand& a, const Operand& b,
            uint32_t parts, bool wide) {
-  using S = Stages<T, BN, MODE>;
+  using S = Stages<T, BN, MODE, LONG>;
   constexpr bool bf16 = !std::is_same_v<T, __half>;  // what is multiplied
   constexpr uint32_t high = MODE == PAIR ? 2 * kTileA : kTileA;
   t.tiles_a = (t.rows + high - 1) / high;
@@ -687,7 +697,7 @@ int launch(plx_ctx* ctx, TensorProduct& t, const Product& p, const Operand& a, c
   const uint64_t tiles = (uint64_t)t.tiles_a * t.tiles_b;
   if (tiles >= (1ull << 28))
     return set_error(PLX_ERR_CAPACITY, "%u x %u results are too many for one call", p.rows, p.cols);
-  constexpr auto kernel = k_product_tensor<T, BN, MODE>;
+  constexpr auto kernel = k_product_tensor<T, BN, MODE, LONG>;
   PLX_TRY_CUDA(allow_shared<kernel>(ctx->device, S::smem));
   cudaLaunchConfig_t cfg = {};
   const uint32_t sms = (uint32_t)ctx->num_sms;
@@ -778,6 +788,18 @@ int product_tensor(plx_ctx* ctx, int dtype, const Product& p) {
     using T = decltype(v);
     constexpr int WIDEST = sizeof(T) == 4 ? 128 : 256;  // stages of 32-bit values are long
     const bool split = parts > 1;
+    if constexpr (sizeof(T) == 2) {
+      // sums too long for TMEM
+      if ((pair ? ks : (ks + parts - 1) / parts) > Stages<T, 128, ONE, true>::period) {
+        if (pair) return launch<T, 256, PAIR, true>(ctx, t, p, a, b, 1, wide);
+        if (bn == 256) return launch<T, 256, ONE, true>(ctx, t, p, a, b, 1, wide);
+        if (bn == 128)
+          return (split ? launch<T, 128, SPLIT, true> : launch<T, 128, ONE, true>)(ctx, t, p, a, b,
+                                                                                  parts, wide);
+        return (split ? launch<T, 64, SPLIT, true> : launch<T, 64, ONE, true>)(ctx, t, p, a, b,
+                                                                              parts, wide);
+      }
+    }
     if (pair) return launch<T, WIDEST, PAIR>(ctx, t, p, a, b, 1, wide);
     switch (bn) {
       case 256: return launch<T, WIDEST, ONE>(ctx, t, p, a, b, parts, wide);

@@ -332,3 +332,34 @@ def test_16_bit_activations_within_their_bounds(ctx, dtype, apply):
     if dtype == "f16":
         half = np.maximum(half, 2.0 ** -25)
     within(f64(y), want, rel * np.abs(want) + half, "y")
+
+
+# ------------------------------------------------------------------- long sums of 16-bit values
+LONG = [  # terms, rows, units, dtype
+    (16384, 130, 70, "f16"), (40001, 1100, 1032, "f16"), (200000, 5, 100, "f16"), (140000, 2000, 1400, "f16"),
+    (1 << 22, 64, 40, "f16"),  # (kept in one sum by each of eight blocks: 55,000 U)
+    (200000, 300, 520, "bf16"), (700001, 20, 300, "bf16"), (270000, 1000, 1032, "bf16")]
+
+
+@pytest.mark.parametrize("terms, rows, m, dtype", LONG)
+def test_long_sums_leave_the_tensor_cores(ctx, terms, rows, m, dtype):
+    """Terms of one sign. 16 of them are a step there, in which each and the sum so far, half of the whole on average,
+    may be cut by 2 U of that sum; sums of 16,384 (131,072) are added by roundings of U at most."""
+    g = torch.Generator(device="cuda").manual_seed(terms)
+    a, b = ((torch.rand(k, terms, device="cuda", generator=g) + 0.1).to(TYPES[dtype]) for k in (rows, m))
+    got = pre_of(ctx, a, b)
+    want = torch.zeros_like(got)
+    for k in range(0, terms, 65536):
+        want += a[:, k:k + 65536].double() @ b[:, k:k + 65536].double().t()
+    most = 16384 if dtype == "f16" else 131072
+    tol = (17 * min(terms, most) / 16 + terms // most + 2) * U
+    assert ((got - want).abs() <= tol * want).all()
+    print("off by", ((got - want).abs() / want).max().item() / U, "U, allowed", tol / U)
+    dy = (a * 2.0 ** -8).t().contiguous()  # [terms, rows]: dweight = sums over the terms
+    x = b.t().contiguous()
+    weight = torch.zeros(rows, m, device="cuda", dtype=TYPES[dtype])
+    _, dw, _ = block.dense_backward(ctx, dy, x, weight, input_grad=False)
+    ctx.sync()
+    want = want * 2.0 ** -8
+    assert want.max() < 65000
+    assert ((dw.double() - want).abs() <= (tol + HALF_STEP[dtype] * (1 + tol)) * want).all()
