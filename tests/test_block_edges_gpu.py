@@ -7,7 +7,7 @@ from scipy.special import erfc
 import block_formulas as F
 from plastix_b200 import _abi, block
 from plastix_b200.runtime import Context
-from test_block_gpu import act_error, gate_bounds, made, product_error, stored, walk
+from test_block_gpu import act_error, dense_inputs, gate_bounds, made, product_error, stored, walk
 from test_readout_gpu import HALF_STEP, TYPES, U, f64, within
 
 pytestmark = pytest.mark.gpu
@@ -196,17 +196,52 @@ def test_infinity_stays_what_it_is_step_by_step(ctx, steps, n, dtype, kind):
     assert torch.equal(h[1, :, 3], want[1, :, 3]) and torch.equal(h[0, :, 7], want[0, :, 7])
 
 
-def test_decays_of_any_size_in_place(ctx):
-    """The part that a block goes on into is not written by another one."""
-    inputs = decay_inputs(1, 5000, 64, "slow", 1000)
-    (x, _), (gate, _), _, (state, _), _ = inputs
-    h, final = block.recurrence(ctx, x.view(1, 5000, 64), gate.view(1, 5000, 64), state, kind="decay")
+@pytest.mark.parametrize("streams, steps, n, kind, at", [(4, 24, 64, "grown", 3), (2, 3000, 64, "grown", 120),
+                                                         (1, 4000, 33, "cut", 63), (2, 4000, 1024, "slow", 300)])
+def test_decays_of_any_size_in_place(ctx, streams, steps, n, kind, at):
+    """The part that a block goes on into is not written by another one; backwards dx over dh, dgate over gate and
+    dstate over dfinal, as the C interface allows."""
+    (x, _), (gate, _), (dh, _), (state, _), (dfinal, _) = decay_inputs(streams, steps, n, kind, at)
+    shape = (streams, steps, n)
+    x, gate, dh = (t.view(shape) for t in (x, gate, dh))
+    h, final = block.recurrence(ctx, x, gate, state, kind="decay", mix=True)
     for where in (0, 1):
-        t = [x.clone().view(1, 5000, 64), gate.clone().view(1, 5000, 64)]
-        s = state.clone()
-        h2, _ = block.recurrence(ctx, *t, s, kind="decay", out=t[where], final_out=s)
+        t, s = [x.clone(), gate.clone()], state.clone()
+        h2, _ = block.recurrence(ctx, *t, s, kind="decay", mix=True, out=t[where], final_out=s)
         ctx.sync()
         assert h.isfinite().all() and torch.equal(h2, h) and torch.equal(s, final)
+    want = block.recurrence_backward(ctx, dh, gate, h, state, x=x, dfinal=dfinal, kind="decay", mix=True)
+    size = _abi.lib().plx_recurrence_scratch_bytes(streams, streams * steps, n, 0, 0, 1, 1)
+    scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
+    _abi.call("plx_recurrence_backward", ctx.handle, streams, streams * steps, n, 0, None, dh.data_ptr(), n,
+              x.data_ptr(), n, gate.data_ptr(), n, 0, 1, h.data_ptr(), n, state.data_ptr(), dfinal.data_ptr(),
+              dh.data_ptr(), n, gate.data_ptr(), n, dfinal.data_ptr(), scratch.data_ptr(), size)
+    ctx.sync()
+    for a, b in zip((dh, gate, dfinal), want):
+        assert torch.equal(a, b)
+
+
+def test_calls_with_a_flooded_stream_can_be_captured(ctx):
+    """What is done where pairs are not finite is decided on the device: a graph that was captured on ordinary values
+    gives the eager call's on others."""
+    stream = torch.cuda.Stream()
+    other = Context(0, stream)
+    (x, _), (gate, _), _, (state, _), _ = decay_inputs(2, 3000, 64, "grown", 120)
+    x, gate = x.view(2, 3000, 64), gate.view(2, 3000, 64)
+    want, wfinal = block.recurrence(ctx, x, gate, state, kind="decay")
+    ctx.sync()
+    held, held_gate = torch.randn_like(x), torch.full_like(gate, 0.5)
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        h, final = block.recurrence(other, held, held_gate, state, kind="decay")
+    graph.replay()
+    held.copy_(x)
+    held_gate.copy_(gate)
+    graph.replay()
+    torch.cuda.synchronize()
+    other.sync()
+    assert torch.equal(h, want) and torch.equal(final, wfinal)
 
 
 # ------------------------------------------------------------------- float16 gradients
@@ -363,3 +398,18 @@ def test_long_sums_leave_the_tensor_cores(ctx, terms, rows, m, dtype):
     want = want * 2.0 ** -8
     assert want.max() < 65000
     assert ((dw.double() - want).abs() <= (tol + HALF_STEP[dtype] * (1 + tol)) * want).all()
+
+
+@pytest.mark.parametrize("rows, m", [(1100, 1032), (700, 100), (40, 300), (300, 70)])
+def test_long_sums_with_all_that_follows_them(ctx, rows, m):
+    """Bias, activation, residual and z of float16 rows of 17,000 inputs."""
+    (x, xv), (w, wv), (b, bv), (res, resv), _ = dense_inputs(rows, 17000, m, "f16", 0, 0, "f32")
+    y, z = block.dense(ctx, x, w, b, apply="gelu", residual=res, pre=True)
+    only = block.dense(ctx, x, w, b, apply="gelu", residual=res)
+    ctx.sync()
+    want, wz = F.dense(xv, wv, bv, "gelu", resv)
+    ztol = product_error(xv, wv.T, 17000) + 4 * U * (np.abs(wz) + np.abs(bv))
+    within(f64(z), wz, ztol, "z")
+    a = F.act(wz, "gelu")[0]
+    within(f64(y), want, stored(want, 1.2 * ztol + act_error(wz, a) + U * np.abs(want), "f16"), "y")
+    assert torch.equal(y, only)
