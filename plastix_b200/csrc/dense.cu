@@ -227,7 +227,8 @@ k_dense_cut(const __grid_constant__ CutRows first, const __grid_constant__ CutRo
 
 // Few 32-bit rows: R of them against U units a warp, whose lanes share k and add in
 // a fixed order. Reading the weights once bounds it; cutting them would read and write
-// four times as much.
+// four times as much. Measured, weights of 4,096 x 4,096 out of memory (10.3 us at the copy
+// rate): 1 row 21 us, 4 rows 26, 8 rows 29 (9 rows by planes 64; library 17, 54, 51, 61).
 template <typename P, int R, int U, int V>
 __global__ void __launch_bounds__(256)
 k_dense_few(uint32_t rows, uint32_t n, uint32_t m, const float* __restrict__ x, int64_t ldx,

@@ -118,7 +118,7 @@ __device__ __forceinline__ Pack<T, V> at_least_minus_87(Pack<T, V> q) {
 
 // a and 1 - a of a gate, neither by a difference that cancels: with e = exp(-gate),
 // 1 / (1 + e) and e / (1 + e). Gates below -87 count as -87 (which leaves e^-87 of
-// h). The quotient gets one Newton step: what a is off by, a long memory raises to its
+// h). The quotient gets one step of Newton's method (r + r (1 - d r)): what a is off by, a long memory raises to its
 // length.
 template <bool SIGMOID, typename T, int V>
 __device__ __forceinline__ void gate_value(Pack<T, V> gate, Units<V>& a, Units<V>& keep) {
@@ -812,8 +812,9 @@ struct Plan {
   uint64_t pair_bytes, shut_bytes;
 };
 
-// Blocks of a walk for results that all SMs hold at a time (as many parts as that, so
-// that none waits for a second round).
+// Blocks of a walk for results that the 148 SMs of a B200 hold at a time (as many parts
+// as that, so that none waits for a second round). The number is fixed: scratch is asked
+// for without a context, and the order of the sums goes by it.
 uint32_t walks_at_once(int dtype, bool mix, bool back, bool tensor) {
   if (!tensor) return 148u * (back ? 2 : 3);
   return 148u * (dtype == PLX_F32 && back && mix ? 1 : back || dtype == PLX_F32 ? 2 : 3);
