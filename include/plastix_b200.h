@@ -718,8 +718,8 @@ size_t plx_dense_scratch_bytes(uint64_t rows, uint32_t n, uint32_t m, int dtype,
  * where not NULL, for the backward call. y may be residual's array, not x's.
  * Products are summed in 32 bits; those of 16-bit rows on the tensor cores, which cut
  * sums off: of terms of one sign they (and with them pre) come out up to 1e-4 (float16)
- * or 8e-4 (bfloat16) too small, after 1,000 terms 5e-7. scratch is 16-byte aligned and may hold
- * anything; calls that run at once need scratch of their own. */
+ * or 8e-4 (bfloat16) too small, after 1,000 terms 5e-7. scratch is 16-byte aligned and
+ * may hold anything; calls that run at once need scratch of their own. */
 int plx_dense(plx_ctx* ctx, uint64_t rows, uint32_t n, uint32_t m, int dtype, const void* x,
               int64_t ldx, const void* weight, int64_t ldw, int param_dtype, const void* bias,
               int act, const void* residual, int64_t ldr, void* y, int64_t ldy, float* pre,
@@ -807,9 +807,9 @@ size_t plx_recurrence_scratch_bytes(uint32_t n_streams, uint64_t rows, uint32_t 
  * written where not NULL; it may be state's array. Decays may be of any size and
  * sign; h is as step by step where that is finite, but for the order of sums (an
  * error relative to the sum of the magnitudes, which decays above 1 make grow). States
- * are in 32 bits, so is h from step to step. h may be x's or gate's array. Sums are folded in an
- * order that the arguments set: the same bits on every call. scratch as for
- * plx_dense. */
+ * are in 32 bits, so is h from step to step. h may be x's or gate's array. Sums are
+ * folded in an order that the arguments set: the same bits on every call. scratch as
+ * for plx_dense. */
 int plx_recurrence(plx_ctx* ctx, uint32_t n_streams, uint64_t rows, uint32_t n, int dtype,
                    const int32_t* offsets, const void* x, int64_t ldx, const void* gate,
                    int64_t ldg, int gate_kind, int mix, const float* state, void* h, int64_t ldh,

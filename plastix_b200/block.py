@@ -277,7 +277,8 @@ def block_norm(ctx: Context, x: torch.Tensor, o: torch.Tensor,
         if p.gate == _abi.BLOCK_GATE_VALUES:
             inputs.append((gate, p.ldg, "gate"))
         ldr = _in_place_of(ctx, out, *inputs)
-        _check_apart(out, ldr, "out", (gate if p.gate == _abi.BLOCK_GATE_UNITS else None, n, "gate"),
+        units = gate if p.gate == _abi.BLOCK_GATE_UNITS else None
+        _check_apart(out, ldr, "out", (units, n, "gate"),
                      (post_weight, n, "post_weight"), (post_bias, n, "post_bias"),
                      (pre_weight, n, "pre_weight"), (pre_bias, n, "pre_bias"))
     with _scope(ctx, x, o, gate, post_weight, post_bias, pre_weight, pre_bias, out):

@@ -131,7 +131,8 @@ __device__ __forceinline__ void finish_one(const Finish& f, uint32_t row, uint32
   ((T*)f.y)[(int64_t)row * f.ldy + col] = from_f32<T>(v[0]);
 }
 
-// Applies the factor and adds the bias of C consecutive columns; `wide`: all there, in 16-byte pieces.
+// Applies the factor to C consecutive columns and adds their bias; `wide`: all there, in
+// 16-byte pieces.
 template <typename T, int C>
 __device__ __forceinline__ void add_bias(const Finish& f, uint32_t col, uint32_t cols, bool wide,
                                          float (&v)[C]) {

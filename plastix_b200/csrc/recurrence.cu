@@ -118,8 +118,8 @@ __device__ __forceinline__ Pack<T, V> at_least_minus_87(Pack<T, V> q) {
 
 // a and 1 - a of a gate, neither by a difference that cancels: with e = exp(-gate),
 // 1 / (1 + e) and e / (1 + e). Gates below -87 count as -87 (which leaves e^-87 of
-// h). The quotient gets one step of Newton's method (r + r (1 - d r)): what a is off by, a long memory raises to its
-// length.
+// h). The quotient gets one step of Newton's method (r + r (1 - d r)): what a is off by,
+// a long memory raises to its length.
 template <bool SIGMOID, typename T, int V>
 __device__ __forceinline__ void gate_value(Pack<T, V> gate, Units<V>& a, Units<V>& keep) {
   using W = Units<V>;
@@ -529,7 +529,8 @@ k_recurrence_walk(const __grid_constant__ Args p, const __grid_constant__ Maps m
       if (warp == 0) {
 #pragma unroll 8
         for (uint32_t j = 0; j < before; ++j) given = part_hands(j, given);
-        if constexpr (SAFE) {  // a part that is not given a finite value is left to the block before it
+        if constexpr (SAFE) {
+          // a part that is not given a finite value is left to the block before it
           uint32_t more = 0;
           if (__any_sync(~0u, !finite(given))) {
             more = ~0u;
